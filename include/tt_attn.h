@@ -198,6 +198,59 @@ int tt_attn_decode_paged(const tt_attn_desc* desc, const void* q, const void* k_
                          const int32_t* block_table, const int32_t* seq_lens, int32_t page_size, int32_t max_pages,
                          void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- page tables of a paged cache ---------------------------------------------------------
+ * The block table and the slots of new tokens, made on the GPU from the requests' lengths (no counterpart in the reference).
+ * block_table is [B, max_pages]; request b's first seq_lens[b] tokens lie in its columns 0 .. ceil(seq_lens[b] / page_size) - 1.
+ * free_pages holds *n_free page numbers (an array of free_capacity), used from its end.  All arrays are device int32.
+ *
+ * tt_cache_extend: new_lens[b] more tokens for request b.  Requests are served in their order until the next one's tokens
+ * exceed max_tokens in all or its pages exceed *n_free; that one and those behind it get nothing.  A request with a negative
+ * count, or one whose tokens do not fit its max_pages, gets nothing and keeps none from being served.
+ *   block_table   the new pages' columns are written, nothing else
+ *   seq_lens_out  [B] lengths with the new tokens (seq_lens where a request got nothing)
+ *   n_free_out    [1] what is left of *n_free
+ *   cu_new        [B + 1] cumulative counts of the tokens served: request b's are rows [cu_new[b], cu_new[b + 1])
+ *   slots         [max_tokens] page * page_size + row in the page, by packed row; -1 behind the last row
+ *                 (and where block_table holds a negative page for a token of a page that was there before)
+ *   positions     [max_tokens] each row's place in its sequence; 0 behind the last row
+ * free_pages is not written: the pages taken are those at *n_free_out and above.
+ *
+ * tt_cache_release: the pages of the requests with done[b] != 0 (bytes) go back: free_pages[*n_free ..] gets them in order of
+ * request and column (none beyond free_capacity), seq_lens_out is 0 there, n_free_out counts them.  block_table is only read.
+ *
+ * Outputs must not overlap inputs or each other, except block_table and free_pages as said.  B is at most 16384, and slots
+ * fit 32 bits (pages * page_size < 2^31).  Negative lengths of done requests count as 0, ones beyond a row as the whole row. */
+int tt_cache_extend(int32_t* block_table, const int32_t* seq_lens, const int32_t* new_lens, const int32_t* free_pages,
+                    const int32_t* n_free, int32_t B, int32_t page_size, int32_t max_pages, int32_t free_capacity,
+                    int32_t max_tokens, int32_t* seq_lens_out, int32_t* n_free_out, int32_t* cu_new, int32_t* slots,
+                    int32_t* positions, void* stream);
+int tt_cache_release(const int32_t* block_table, const int32_t* seq_lens, const uint8_t* done, int32_t* free_pages,
+                     const int32_t* n_free, int32_t B, int32_t page_size, int32_t max_pages, int32_t free_capacity,
+                     int32_t* seq_lens_out, int32_t* n_free_out, void* stream);
+
+/* ---- rotary positions ------------------------------------------------------------------------
+ * Query and key heads turned by their tokens' positions (no counterpart in the reference).  Of a head's D channels the first
+ * R form R / 2 pairs; pair i of a token at position p on axis a = axes[i] turns by p * inv_freq[i]:
+ *     (x1, x2) -> scale * (x1 cos - x2 sin, x2 cos + x1 sin)
+ * Pairs are halves (channels i and i + R / 2) or, with `interleaved`, neighbours (2i and 2i + 1); channels from R on are copied.
+ * `backward` turns the other way (sin -> -sin): the gradient of the call with the same arguments, which is linear in x.
+ * Angles are taken in 64 bits and reduced to one turn before their sine and cosine, products are 32-bit, outputs rounded once.
+ *   q, k           [B, heads, S, D] at element strides {batch, head, row} of their own, channels next to each other; inputs may
+ *                  repeat (stride 0), outputs may not.  An output may be its input (same pointer and strides), else the two must not
+ *                  overlap.  k and k_out are both null where there is one tensor only.  Packed tokens [T, H, D]: B = 1, S = T.
+ *   positions      int32, [n_axes, B, S] at strides pos_stride {axis, batch}, rows next to each other; any int32 value
+ *   inv_freq       [R / 2] double, angle per position;  axes: [R / 2] int32 in 0 .. n_axes - 1 (others are taken as the nearest),
+ *                  or null: all of axis 0
+ * D at most 256, R even, dtype TT_F32 or TT_BF16.  16-byte loads where pointers and strides allow them, else one value each. */
+typedef struct tt_rotary_desc {
+    int32_t B, S, H, Hkv, D, R, n_axes, dtype, interleaved;
+    float scale;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+    int64_t pos_stride[2];
+} tt_rotary_desc;
+int tt_rotary(const tt_rotary_desc* desc, const void* q, const void* k, const int32_t* positions, const double* inv_freq,
+              const int32_t* axes, int32_t backward, void* q_out, void* k_out, void* stream);
+
 /* ---- row softmax ------------------------------------------------------------------------
  * out[r,:] = softmax(in[r,:]) over `cols`, row maximum subtracted; rows = product of the leading
  * axes.  One launch that reads and writes every element once; replaces SoftmaxForward of

@@ -13,4 +13,5 @@ from .functional import (  # noqa: F401
     attention_forward_host, attention_backward_host, attention_decode_host, attention_step_host,
     check_device_status, softmax_forward, softmax_backward, fc_forward, fc_backward, attention_decode_paged,
     set_backward_deterministic, attention_forward_varlen, attention_backward_varlen,
+    CacheStep, cache_extend, cache_release, rotary_frequencies, rotary_forward, rotary_backward,
 )

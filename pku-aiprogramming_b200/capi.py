@@ -35,6 +35,13 @@ class VarlenDesc(ctypes.Structure):
                 ("total_q", c_int64), ("total_k", c_int64)]
 
 
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [("B", c_int32), ("S", c_int32), ("H", c_int32), ("Hkv", c_int32), ("D", c_int32), ("R", c_int32),
+                ("n_axes", c_int32), ("dtype", c_int32), ("interleaved", c_int32), ("scale", c_float),
+                ("q_stride", c_int64 * 3), ("k_stride", c_int64 * 3), ("q_out_stride", c_int64 * 3),
+                ("k_out_stride", c_int64 * 3), ("pos_stride", c_int64 * 2)]
+
+
 _P = c_void_p
 _DP = POINTER(Desc)
 _VP = POINTER(VarlenDesc)
@@ -52,6 +59,9 @@ SIGNATURES = {
     "tt_attn_decode": (c_int, [_DP, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
     "tt_attn_decode_paged": (c_int, [_DP, _P, _P, _P, _P, _P, c_int32, c_int32, _P, _P, _P, c_size_t, _P]),
     "tt_attn_decode_static": (c_int, [_DP, _P, _P, _P, _P, _P, _P]),
+    "tt_cache_extend": (c_int, [_P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P, _P, _P, _P, _P]),
+    "tt_cache_release": (c_int, [_P, _P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, _P, _P, _P]),
+    "tt_rotary": (c_int, [POINTER(RotaryDesc), _P, _P, _P, _P, _P, c_int32, _P, _P, _P]),
     "tt_softmax_fwd": (c_int, [_P, _P, c_int64, c_int32, c_int32, _P]),
     "tt_softmax_bwd": (c_int, [_P, _P, _P, c_int64, c_int32, c_int32, _P]),
     "tt_fc_fwd": (c_int, [_P, _P, _P, _P, c_int64, c_int32, c_int32, c_int32, _P]),

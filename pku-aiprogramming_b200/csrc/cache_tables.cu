@@ -1,0 +1,214 @@
+// Page tables of a paged cache from the requests' lengths: pages and slots for new tokens, and pages given back.
+//
+// With c(n) = ceil(n / page): request b needs c(len + new) - c(len) pages; its first page and first packed row are exclusive sums
+// over the requests before it, and whether it is served is a comparison of the inclusive sums with what there is, so the
+// served requests are a prefix.  Token t of a request is at position p = len + t, in the row's column p / page.
+//
+// The bytes are few (4 per length, 8 per token and page), so what counts is the number of launches and of dependent loads in
+// one: every CTA sums over all requests itself (a few loads per thread, from L2) instead of waiting for a launch that
+// does, and a token finds its request by a binary search in shared memory.  Nothing is kept between calls, and no CTA waits
+// for another.
+#include <climits>
+
+#include "common.h"
+
+namespace ttk {
+
+constexpr int kMaxRequests = 16384;   // two ints each in shared memory
+int cache_max_requests() { return kMaxRequests; }
+
+// Inclusive sums over the CTA's threads; `red` [2][32] shared, used once per kernel.
+template <int kThreads>
+__device__ __forceinline__ void cta_sums(long long& a, long long& b, long long (*red)[32]) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, a, o), y = __shfl_up_sync(0xffffffffu, b, o);
+        if (lane >= o) {
+            a += x;
+            b += y;
+        }
+    }
+    if (lane == 31) {
+        red[0][w] = a;
+        red[1][w] = b;
+    }
+    __syncthreads();
+    for (int i = 0; i < w; ++i) {
+        a += red[0][i];
+        b += red[1][i];
+    }
+}
+
+struct Need {
+    int tokens, pages, have;   // new tokens, pages to take, columns in use before
+};
+__device__ __forceinline__ Need need_of(int len, int fresh, int page, long long row_tokens) {
+    Need n{0, 0, 0};
+    if (len < 0 || fresh < 0 || (long long)len + fresh > row_tokens) return n;
+    n.have = len / page + (len % page != 0);
+    n.tokens = fresh;
+    n.pages = (len + fresh) / page + ((len + fresh) % page != 0) - n.have;
+    return n;
+}
+
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) cache_extend_kernel(int* __restrict__ table, const int* __restrict__ lens, const int* __restrict__ fresh,
+                                                                const int* __restrict__ free_pages, const int* __restrict__ n_free, int B,
+                                                                int page, int max_pages, int free_capacity, int max_tokens, int* __restrict__ lens_out,
+                                                                int* __restrict__ n_free_out, int* __restrict__ cu_new, int* __restrict__ slots,
+                                                                int* __restrict__ positions) {
+    extern __shared__ int sm[];
+    int* cu = sm;              // [B + 1] packed rows of the requests served
+    int* first = sm + B + 1;   // [B] pages taken by the requests before; -1: not served
+    __shared__ long long red[2][32];
+    __shared__ int total[2];
+    const int tid = threadIdx.x, per = (B + kThreads - 1) / kThreads, b0 = min(B, tid * per), b1 = min(B, b0 + per);
+    const long long row_tokens = min((long long)max_pages * page, (long long)INT_MAX);
+    if (tid < 2) total[tid] = 0;
+    grid_let_next_start();
+    grid_wait_for_previous();
+    const int have_free = min(max(*n_free, 0), free_capacity);
+    long long tok = 0, pg = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Need n = need_of(lens[b], fresh[b], page, row_tokens);
+        tok += n.tokens;
+        pg += n.pages;
+    }
+    const long long own_tok = tok, own_pg = pg;
+    cta_sums<kThreads>(tok, pg, red);   // (its barrier is behind the clearing of `total`)
+    tok -= own_tok;
+    pg -= own_pg;
+    int most_tok = 0, most_pg = 0;
+    for (int b = b0; b < b1; ++b) {
+        const Need n = need_of(lens[b], fresh[b], page, row_tokens);
+        tok += n.tokens;
+        pg += n.pages;
+        const bool ok = tok <= max_tokens && pg <= have_free;
+        cu[b + 1] = ok ? (int)tok : -1;
+        first[b] = ok ? (int)(pg - n.pages) : -1;
+        if (ok) {
+            most_tok = (int)tok;
+            most_pg = (int)pg;
+        }
+    }
+    atomicMax(&total[0], most_tok);
+    atomicMax(&total[1], most_pg);
+    if (tid == 0) cu[0] = 0;
+    __syncthreads();
+    const int served = total[0];
+    for (int b = b0; b < b1; ++b)
+        if (cu[b + 1] < 0) cu[b + 1] = served;
+    __syncthreads();
+    auto from_free = [&](int i) { return free_pages[have_free - 1 - i]; };   // the i-th page taken
+    if (blockIdx.x == 0) {
+        for (int b = tid; b < B; b += kThreads) {
+            lens_out[b] = lens[b] + (cu[b + 1] - cu[b]);
+            cu_new[b + 1] = cu[b + 1];
+        }
+        if (tid == 0) {
+            cu_new[0] = 0;
+            *n_free_out = have_free - total[1];
+        }
+    }
+    // new columns: a warp per request
+    for (int b = blockIdx.x * (kThreads / 32) + (tid >> 5); b < B; b += gridDim.x * (kThreads / 32)) {
+        if (first[b] < 0) continue;
+        const Need n = need_of(lens[b], fresh[b], page, row_tokens);
+        for (int j = tid & 31; j < n.pages; j += 32) table[(long long)b * max_pages + n.have + j] = from_free(first[b] + j);
+    }
+    for (long long t = (long long)blockIdx.x * kThreads + tid; t < max_tokens; t += (long long)gridDim.x * kThreads) {
+        int slot = -1, pos = 0;
+        if (t < served) {
+            int lo = 0, hi = B;   // the last b with cu[b] <= t, behind requests without tokens
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (cu[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            const int len = lens[lo], have = len / page + (len % page != 0);
+            pos = len + (int)(t - cu[lo]);
+            const int col = pos / page;
+            const int p = col < have ? table[(long long)lo * max_pages + col] : from_free(first[lo] + col - have);
+            if (p >= 0) slot = p * page + (pos - col * page);
+        }
+        slots[t] = slot;
+        positions[t] = pos;
+    }
+}
+
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) cache_release_kernel(const int* __restrict__ table, const int* __restrict__ lens, const unsigned char* __restrict__ done,
+                                                                 int* __restrict__ free_pages, const int* __restrict__ n_free, int B, int page,
+                                                                 int max_pages, int free_capacity, int* __restrict__ lens_out, int* __restrict__ n_free_out) {
+    extern __shared__ int sm[];
+    int* first = sm;   // [B] where the request's pages go, behind *n_free
+    __shared__ long long red[2][32];
+    __shared__ long long total;
+    const int tid = threadIdx.x, per = (B + kThreads - 1) / kThreads, b0 = min(B, tid * per), b1 = min(B, b0 + per);
+    grid_let_next_start();
+    grid_wait_for_previous();
+    const int have_free = min(max(*n_free, 0), free_capacity);
+    auto pages_of = [&](int b) {
+        if (!done[b]) return 0;
+        const int len = lens[b];
+        return len <= 0 ? 0 : min(max_pages, len / page + (len % page != 0));
+    };
+    long long pg = 0, zero = 0;
+    for (int b = b0; b < b1; ++b) pg += pages_of(b);
+    const long long own = pg;
+    cta_sums<kThreads>(pg, zero, red);
+    if (tid == kThreads - 1) total = pg;
+    pg -= own;
+    for (int b = b0; b < b1; ++b) {
+        first[b] = (int)min(pg, (long long)INT_MAX);
+        pg += pages_of(b);
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int b = tid; b < B; b += kThreads) lens_out[b] = done[b] ? 0 : lens[b];
+        if (tid == 0) *n_free_out = (int)min(have_free + total, (long long)free_capacity);
+    }
+    for (int b = blockIdx.x * (kThreads / 32) + (tid >> 5); b < B; b += gridDim.x * (kThreads / 32)) {
+        const int n = pages_of(b);
+        for (int j = tid & 31; j < n; j += 32) {
+            const long long to = (long long)have_free + first[b] + j;
+            if (to < free_capacity) free_pages[to] = table[(long long)b * max_pages + j];
+        }
+    }
+}
+
+// Threads: one request each up to 256, four each beyond.
+cudaError_t cache_extend(int* table, const int* lens, const int* fresh, const int* free_pages, const int* n_free, int B, int page, int max_pages,
+                         int free_capacity, int max_tokens, int* lens_out, int* n_free_out, int* cu_new, int* slots, int* positions, cudaStream_t st) {
+    const size_t smem = (2 * (size_t)B + 1) * sizeof(int);
+    auto go = [&](auto kernel, int threads) {
+        if (smem > 48 * 1024 - 1024) {
+            const cudaError_t e = TT_ALLOW_SMEM(kernel, (2 * (size_t)kMaxRequests + 1) * sizeof(int));
+            if (e != cudaSuccess) return e;
+        }
+        const long long rows = (max_tokens + (long long)threads - 1) / threads, reqs = (B + threads / 32 - 1) / (threads / 32);
+        const long long ctas = rows > reqs ? rows : reqs, most = 4LL * sm_count();
+        LaunchScope ls(K_CACHE_TABLES, st);
+        return launch_overlapped(kernel, (unsigned)(ctas < most ? ctas : most), threads, smem, st, table, lens, fresh, free_pages, n_free, B, page,
+                                 max_pages, free_capacity, max_tokens, lens_out, n_free_out, cu_new, slots, positions);
+    };
+    return B <= 1024 ? go(cache_extend_kernel<256>, 256) : go(cache_extend_kernel<1024>, 1024);
+}
+cudaError_t cache_release(const int* table, const int* lens, const unsigned char* done, int* free_pages, const int* n_free, int B, int page, int max_pages,
+                          int free_capacity, int* lens_out, int* n_free_out, cudaStream_t st) {
+    const size_t smem = (size_t)B * sizeof(int);
+    auto go = [&](auto kernel, int threads) {
+        if (smem > 48 * 1024 - 1024) {
+            const cudaError_t e = TT_ALLOW_SMEM(kernel, (size_t)kMaxRequests * sizeof(int));
+            if (e != cudaSuccess) return e;
+        }
+        const long long reqs = (B + threads / 32 - 1) / (threads / 32), most = 4LL * sm_count();
+        LaunchScope ls(K_CACHE_TABLES, st);
+        return launch_overlapped(kernel, (unsigned)(reqs < most ? reqs : most), threads, smem, st, table, lens, done, free_pages, n_free, B, page,
+                                 max_pages, free_capacity, lens_out, n_free_out);
+    };
+    return B <= 1024 ? go(cache_release_kernel<256>, 256) : go(cache_release_kernel<1024>, 1024);
+}
+
+}  // namespace ttk

@@ -144,7 +144,8 @@ int check_device();   // TT_OK, or TT_ERR_BAD_DEVICE when the current device is 
 enum KernelId {
     K_FWD_TC = 0, K_FWD_SIMT, K_BWD_PREP, K_BWD_DKV, K_BWD_DQ, K_BWD_SIMT_DELTA, K_BWD_SIMT_DQ, K_BWD_SIMT_DKV,
     K_DECODE, K_DECODE_MERGE, K_PROBE, K_SOFTMAX_FWD, K_SOFTMAX_BWD, K_FC_GEMM, K_FC_SIMT, K_FC_COLSUM, K_BWD_FUSED,
-    K_BWD_DQ_CONVERT, K_DECODE_GQ, K_FWD_F32, K_BWD_F32, K_BWD_BOTH, K_COUNT
+    K_BWD_DQ_CONVERT, K_DECODE_GQ, K_FWD_F32, K_BWD_F32, K_BWD_BOTH, K_CACHE_TABLES,
+    K_ROTARY, K_COUNT
 };
 // Scoped around ONE kernel launch: counts it and, when timing is enabled, brackets it with
 // CUDA events on the launching stream.
@@ -263,6 +264,29 @@ cudaError_t attn_decode_paged_forward(const AttnArgs& a, const DecodeView& view,
 // *too_big is set when the plan needs more than the array holds (nothing is launched then).
 size_t attn_decode_static_capacity();
 cudaError_t attn_decode_static(const AttnArgs& a, const DecodePlan& plan, cudaStream_t st, bool* too_big);
+
+// --- page tables of a paged cache (cache_tables.cu); see tt_cache_extend and tt_cache_release
+int cache_max_requests();
+cudaError_t cache_extend(int* table, const int* lens, const int* fresh, const int* free_pages, const int* n_free, int B, int page, int max_pages,
+                         int free_capacity, int max_tokens, int* lens_out, int* n_free_out, int* cu_new, int* slots, int* positions, cudaStream_t st);
+cudaError_t cache_release(const int* table, const int* lens, const unsigned char* done, int* free_pages, const int* n_free, int B, int page, int max_pages,
+                          int free_capacity, int* lens_out, int* n_free_out, cudaStream_t st);
+
+// --- rotary positions (rotary.cu)
+struct RotaryArgs {
+    const void* x[2];   // query and key heads; strides {batch, head, row}
+    void* y[2];
+    long long xs[2][3], ys[2][3];
+    int heads[2];
+    int B, S, D, R, n_axes;
+    const int* pos;
+    long long pos_axis, pos_batch;
+    const double* inv_freq;
+    const int* axes;
+    float scale;
+    int back;
+};
+cudaError_t rotary(const RotaryArgs& a, int bf16, int interleaved, cudaStream_t st);
 
 // Builds a 3-D bf16 tensor map over a dense [slices, rows, cols] array, box
 // [1, box_rows, 64] with 128-byte swizzle.  Returns false (and sets `why`) on failure.

@@ -484,11 +484,155 @@ PyObject* fc_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// A CUDA tensor of one type on q's device, whatever its strides.
+const Tensor* on_device(PyObject* o, at::ScalarType type, const Tensor* like = nullptr) {
+    if (!THPVariable_Check(o)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(o);
+    return t.is_cuda() && t.scalar_type() == type && (!like || t.device() == like->device()) ? &t : nullptr;
+}
+// a contiguous vector of n elements (n < 0: any number)
+const Tensor* vector_arg(PyObject* o, at::ScalarType type, int64_t n, const Tensor* like = nullptr) {
+    const Tensor* t = on_device(o, type, like);
+    return t && t->is_contiguous() && t->dim() == 1 && (n < 0 || t->size(0) == n) ? t : nullptr;
+}
+// The k-th of the caller's output vectors, or a new one; null where the caller's does not fit.
+const Tensor* out_vector(PyObject* given, Py_ssize_t k, int64_t n, const Tensor& like, Tensor* made) {
+    if (given != Py_None) return vector_arg(PyTuple_GET_ITEM(given, k), at::kInt, n, &like);
+    *made = make({n}, at::kInt, like);
+    return made;
+}
+PyObject* item_or(PyObject* given, Py_ssize_t k, const Tensor& made) { return wrap_or(given == Py_None ? Py_None : PyTuple_GET_ITEM(given, k), made); }
+bool tuple_arg(PyObject* o, Py_ssize_t n) { return o == Py_None || (PyTuple_Check(o) && PyTuple_GET_SIZE(o) == n); }
+
+// block_table [B, max_pages] and seq_lens [B]
+bool table_args(PyObject* ot, PyObject* ol, const Tensor** table, const Tensor** lens) {
+    *table = on_device(ot, at::kInt);
+    if (!*table || !(*table)->is_contiguous() || (*table)->dim() != 2 || !fits32((*table)->size(1))) return false;
+    *lens = vector_arg(ol, at::kInt, (*table)->size(0), *table);
+    return *lens != nullptr;
+}
+
+// (block_table, seq_lens, new_lens, free_pages, n_free, page_size, max_tokens, out) -> (seq_lens, n_free, cu_new, slots, positions)
+PyObject* cache_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Tensor *table, *lens;
+        if (n != 8 || !table_args(a[0], a[1], &table, &lens) || !tuple_arg(a[7], 5)) Py_RETURN_NONE;
+        const int64_t B = table->size(0);
+        const Tensor *fresh = vector_arg(a[2], at::kInt, B, table), *pages = vector_arg(a[3], at::kInt, -1, table),
+                     *n_free = vector_arg(a[4], at::kInt, 1, table);
+        int64_t page, tokens;
+        if (!fresh || !pages || !n_free || !fits32(pages->numel())) Py_RETURN_NONE;
+        if (!int_arg(a[5], &page) || !int_arg(a[6], &tokens)) return nullptr;
+        if (!fits32(B) || !fits32(page) || !fits32(tokens) || tokens < 0) Py_RETURN_NONE;
+        OnDevice dev(*table);
+        Tensor made[5];
+        const Tensor* out[5];
+        const int64_t sizes[5] = {B, 1, B + 1, tokens, tokens};
+        for (int i = 0; i < 5; ++i)
+            if (!(out[i] = out_vector(a[7], i, sizes[i], *table, &made[i]))) Py_RETURN_NONE;
+        auto at = [&](int i) { return (int32_t*)ptr(out[i]); };
+        TT_CALL(rc, tt_cache_extend((int32_t*)ptr(table), (const int32_t*)ptr(lens), (const int32_t*)ptr(fresh), (const int32_t*)ptr(pages),
+                                    (const int32_t*)ptr(n_free), (int32_t)B, (int32_t)page, (int32_t)table->size(1), (int32_t)pages->numel(),
+                                    (int32_t)tokens, at(0), at(1), at(2), at(3), at(4), dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(item_or(a[7], 0, made[0]), item_or(a[7], 1, made[1]), item_or(a[7], 2, made[2]), item_or(a[7], 3, made[3]), item_or(a[7], 4, made[4]));
+    });
+}
+
+// (block_table, seq_lens, done, free_pages, n_free, page_size, out) -> (seq_lens, n_free)
+PyObject* cache_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Tensor *table, *lens;
+        if (n != 7 || !table_args(a[0], a[1], &table, &lens) || !tuple_arg(a[6], 2)) Py_RETURN_NONE;
+        const int64_t B = table->size(0);
+        const Tensor* done = vector_arg(a[2], at::kBool, B, table);
+        if (!done) done = vector_arg(a[2], at::kByte, B, table);
+        const Tensor *pages = vector_arg(a[3], at::kInt, -1, table), *n_free = vector_arg(a[4], at::kInt, 1, table);
+        int64_t page;
+        if (!done || !pages || !n_free || !fits32(pages->numel())) Py_RETURN_NONE;
+        if (!int_arg(a[5], &page)) return nullptr;
+        if (!fits32(B) || !fits32(page)) Py_RETURN_NONE;
+        OnDevice dev(*table);
+        Tensor made[2];
+        const Tensor* out[2];
+        for (int i = 0; i < 2; ++i)
+            if (!(out[i] = out_vector(a[6], i, i ? 1 : B, *table, &made[i]))) Py_RETURN_NONE;
+        TT_CALL(rc, tt_cache_release((const int32_t*)ptr(table), (const int32_t*)ptr(lens), (const uint8_t*)ptr(done), (int32_t*)ptr(pages),
+                                     (const int32_t*)ptr(n_free), (int32_t)B, (int32_t)page, (int32_t)table->size(1), (int32_t)pages->numel(),
+                                     (int32_t*)ptr(out[0]), (int32_t*)ptr(out[1]), dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(item_or(a[6], 0, made[0]), item_or(a[6], 1, made[1]));
+    });
+}
+
+// Heads to rotate: [T, H, D] or [B, H, S, D], channels next to each other
+bool heads_arg(const Tensor& t, int64_t* B, int64_t* H, int64_t* S, int64_t (&stride)[3]) {
+    if ((t.dim() != 3 && t.dim() != 4) || (t.size(-1) > 1 && t.stride(-1) != 1)) return false;
+    if (t.dim() == 3) {
+        *B = 1, *S = t.size(0), *H = t.size(1);
+        stride[0] = 0, stride[1] = t.stride(1), stride[2] = t.stride(0);
+    } else {
+        *B = t.size(0), *H = t.size(1), *S = t.size(2);
+        for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
+    }
+    return fits32(*B) && fits32(*H) && fits32(*S);
+}
+
+// (q, k, positions, inv_freq, axes, interleaved, scale, backward, out_q, out_k) -> (q, k)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 10 || !THPVariable_Check(a[0])) Py_RETURN_NONE;
+        const Tensor& q = THPVariable_Unpack(a[0]);
+        tt_rotary_desc d = {};
+        int64_t B, H, S, Bk = 0, Hk = 0, Sk = 0;
+        if (!q.is_cuda() || !float_type(q) || !heads_arg(q, &B, &H, &S, d.q_stride)) Py_RETURN_NONE;
+        const Tensor* k = nullptr;
+        if (a[1] != Py_None) {
+            k = on_device(a[1], q.scalar_type(), &q);
+            if (!k || k->dim() != q.dim() || !heads_arg(*k, &Bk, &Hk, &Sk, d.k_stride) || Bk != B || Sk != S || k->size(-1) != q.size(-1)) Py_RETURN_NONE;
+        } else if (a[9] != Py_None) {
+            Py_RETURN_NONE;
+        }
+        const Tensor *pos = on_device(a[2], at::kInt, &q), *freq = vector_arg(a[3], at::kDouble, -1, &q), *axes = nullptr;
+        if (!pos || !freq || pos->dim() < 1 || pos->dim() > q.dim() - 1 || pos->size(-1) != S || (S > 1 && pos->stride(-1) != 1)) Py_RETURN_NONE;
+        const int64_t n_axes = pos->dim() > 1 ? pos->size(0) : 1;
+        if (pos->dim() == 3 && pos->size(1) != B) Py_RETURN_NONE;
+        if (a[4] != Py_None && !(axes = vector_arg(a[4], at::kInt, freq->size(0), &q))) Py_RETURN_NONE;
+        d.pos_stride[0] = pos->dim() > 1 ? pos->stride(0) : 0;
+        d.pos_stride[1] = pos->dim() == 3 ? pos->stride(1) : 0;
+        const int inter = PyObject_IsTrue(a[5]), back = PyObject_IsTrue(a[7]);
+        if (inter < 0 || back < 0 || !scale_arg(a[6], &d.scale)) return nullptr;
+        if (a[6] == Py_None) d.scale = 1.f;
+        if (!fits32(n_axes) || !fits32(2 * freq->size(0)) || !fits32(q.size(-1))) Py_RETURN_NONE;
+        d.B = (int32_t)B, d.S = (int32_t)S, d.H = (int32_t)H, d.Hkv = (int32_t)Hk, d.D = (int32_t)q.size(-1), d.R = (int32_t)(2 * freq->size(0));
+        d.n_axes = (int32_t)n_axes, d.dtype = tt_type(q), d.interleaved = inter;
+        OnDevice dev(q);
+        Tensor made[2];
+        const Tensor* out[2] = {nullptr, nullptr};
+        for (int i = 0; i < (k ? 2 : 1); ++i) {
+            const Tensor& x = i ? *k : q;
+            if (a[8 + i] != Py_None) {
+                out[i] = on_device(a[8 + i], q.scalar_type(), &q);
+                if (!out[i] || !same_shape(*out[i], x)) Py_RETURN_NONE;
+            } else {
+                made[i] = make_like(x);
+                out[i] = &made[i];
+            }
+            if (!heads_arg(*out[i], &Bk, &Hk, &Sk, i ? d.k_out_stride : d.q_out_stride)) Py_RETURN_NONE;
+        }
+        TT_CALL(rc, tt_rotary(&d, ptr(q), ptr(k), (const int32_t*)ptr(pos), (const double*)ptr(freq), (const int32_t*)ptr(axes), back, ptr(out[0]), ptr(out[1]),
+                              dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(wrap_or(a[8], made[0]), wrap_or(a[9], made[1]));
+    });
+}
+
 #define TT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     TT_METHOD(attention_forward), TT_METHOD(attention_backward), TT_METHOD(attention_forward_varlen),
     TT_METHOD(attention_backward_varlen), TT_METHOD(attention_decode), TT_METHOD(attention_decode_paged),
-    TT_METHOD(softmax_forward), TT_METHOD(softmax_backward), TT_METHOD(fc_forward), TT_METHOD(fc_backward),
+    TT_METHOD(softmax_forward), TT_METHOD(softmax_backward), TT_METHOD(fc_forward), TT_METHOD(fc_backward), TT_METHOD(cache_extend), TT_METHOD(cache_release),
+    TT_METHOD(rotary),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ttorch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,128 @@
+// Rotary positions on query and key heads, several axes, forward and backward.
+//
+// Pair i of a token turns by p[axis_i] * f_i.  In 32 bits a position of 10^6 leaves 0.03 of a radian of the product, so
+// it is taken in 64, in turns, less its nearest whole number; the rest, at most half a turn, goes through sincospif.
+//
+// HBM-bound: every value is read and written once.  A CTA takes a few tokens: their R / 2 sines and cosines go to shared memory
+// once (for up to 40 heads that use them), then a thread keeps its place in the head -- 16 bytes of one half and their partners
+// in the other, or 16 bytes of neighbours -- and walks over tokens and heads, so an access of a warp is whole rows.
+#include "common.h"
+
+namespace ttk {
+
+template <typename T> __device__ __forceinline__ float rt_get(T v);
+template <> __device__ __forceinline__ float rt_get(float v) { return v; }
+template <> __device__ __forceinline__ float rt_get(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T rt_put(float v);
+template <> __device__ __forceinline__ float rt_put(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 rt_put(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int kV> struct alignas(sizeof(T) * kV) RtVec { T v[kV]; };
+
+constexpr int kRotaryThreads = 256;
+
+// kV values per access.  A unit of work is `kV` pairs in halves, or kV / 2 neighbouring pairs (one pair at kV = 1), or kV
+// channels behind R; blockDim = {units per head, rows at a time}.
+template <typename T, int kV, bool kNeighbours>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a, int tokens_per_cta, int turned) {
+    extern __shared__ float2 cs[];   // [tokens_per_cta][R / 2] scale * (cos, sin), and behind them each token's batch entry and row
+    using Vec = RtVec<T, kV>;
+    const int half = a.R / 2, tid = threadIdx.y * blockDim.x + threadIdx.x, n_threads = blockDim.x * blockDim.y;
+    const unsigned t0 = blockIdx.x * (unsigned)tokens_per_cta, n_tok = (unsigned)a.B * (unsigned)a.S;
+    const int here = (int)min((unsigned)tokens_per_cta, n_tok - t0);
+    int2* where = reinterpret_cast<int2*>(cs + tokens_per_cta * half);
+    grid_let_next_start();
+    grid_wait_for_previous();
+    for (int i = tid; i < here * half; i += n_threads) {
+        const int t = i / half, pair = i - t * half;
+        const unsigned at = t0 + t, b = at / (unsigned)a.S, s = at - b * (unsigned)a.S;
+        if (pair == 0) where[t] = make_int2((int)b, (int)s);
+        const int axis = a.axes ? min(max(a.axes[pair], 0), a.n_axes - 1) : 0;
+        const int p = a.pos[axis * a.pos_axis + (long long)b * a.pos_batch + s];
+        const double turns = (double)p * a.inv_freq[pair] * 0.15915494309189533576888;   // / 2 pi
+        float sn, co;
+        sincospif((float)(2.0 * (turns - rint(turns))), &sn, &co);
+        cs[i] = make_float2(a.scale * co, a.back ? -a.scale * sn : a.scale * sn);
+    }
+    __syncthreads();
+    const int u = threadIdx.x, heads = a.heads[0] + a.heads[1];
+    const bool turn = u < turned;
+    // the unit's channels: kV at c0, and in halves their partners at c1
+    const int c0 = turn ? (kNeighbours && kV == 1 ? 2 * u : u * kV) : a.R + (u - turned) * kV;
+    const int c1 = kNeighbours ? c0 + 1 : c0 + half;
+    const bool two = turn && (!kNeighbours || kV == 1);
+    int t = 0, h = threadIdx.y;
+    while (h >= heads) {
+        h -= heads;
+        ++t;
+    }
+    while (t < here) {
+        const int which = h >= a.heads[0], head = which ? h - a.heads[0] : h;
+        const int2 w = where[t];
+        const T* x = (const T*)a.x[which] + w.x * a.xs[which][0] + head * a.xs[which][1] + w.y * a.xs[which][2];
+        T* y = (T*)a.y[which] + w.x * a.ys[which][0] + head * a.ys[which][1] + w.y * a.ys[which][2];
+        if (turn) {
+            Vec v0 = *reinterpret_cast<const Vec*>(x + c0), v1;
+            if (two) v1 = *reinterpret_cast<const Vec*>(x + c1);
+            const float2* f = cs + t * half + (kNeighbours && kV > 1 ? u * (kV / 2) : u * kV);
+            if (two) {
+#pragma unroll
+                for (int e = 0; e < kV; ++e) {
+                    const float x1 = rt_get(v0.v[e]), x2 = rt_get(v1.v[e]);
+                    v0.v[e] = rt_put<T>(x1 * f[e].x - x2 * f[e].y);
+                    v1.v[e] = rt_put<T>(x2 * f[e].x + x1 * f[e].y);
+                }
+                *reinterpret_cast<Vec*>(y + c1) = v1;
+            } else {
+#pragma unroll
+                for (int e = 0; e + 1 < kV; e += 2) {
+                    const float x1 = rt_get(v0.v[e]), x2 = rt_get(v0.v[e + 1]);
+                    v0.v[e] = rt_put<T>(x1 * f[e / 2].x - x2 * f[e / 2].y);
+                    v0.v[e + 1] = rt_put<T>(x2 * f[e / 2].x + x1 * f[e / 2].y);
+                }
+            }
+            *reinterpret_cast<Vec*>(y + c0) = v0;
+        } else if (x != y) {
+            *reinterpret_cast<Vec*>(y + c0) = *reinterpret_cast<const Vec*>(x + c0);
+        }
+        h += blockDim.y;
+        while (h >= heads) {
+            h -= heads;
+            ++t;
+        }
+    }
+}
+
+template <typename T, int kV, bool kNeighbours>
+static cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t st) {
+    const int turned = kNeighbours ? (kV == 1 ? a.R / 2 : a.R / kV) : a.R / 2 / kV, copied = (a.D - a.R) / kV, units = turned + copied;
+    const dim3 block(units, kRotaryThreads / units);
+    const long long n_tok = (long long)a.B * a.S, heads = a.heads[0] + a.heads[1];
+    // about eight units per thread and CTA where there are tokens enough for four CTAs per SM
+    long long per = 8LL * block.y / heads, spread = (n_tok + 4LL * sm_count() - 1) / (4LL * sm_count());
+    if (per > spread) per = spread;
+    const long long fits = 40 * 1024 / ((a.R / 2 + 1) * sizeof(float2));   // at most 128 pairs: 40 tokens
+    if (per > fits) per = fits;
+    if (per < 1) per = 1;
+    LaunchScope ls(K_ROTARY, st);
+    return launch_overlapped(rotary_kernel<T, kV, kNeighbours>, (unsigned)((n_tok + per - 1) / per), block, (size_t)per * (a.R / 2 + 1) * sizeof(float2), st, a,
+                             (int)per, turned);
+}
+template <typename T>
+static cudaError_t launch_rotary_type(const RotaryArgs& a, int interleaved, cudaStream_t st) {
+    constexpr int kV = 16 / sizeof(T);
+    bool wide = a.D % kV == 0 && (interleaved ? a.R : a.R / 2) % kV == 0;
+    for (int i = 0; i < 2; ++i) {
+        if (!a.heads[i]) continue;
+        wide = wide && (((uintptr_t)a.x[i] | (uintptr_t)a.y[i]) & 15) == 0;
+        const int n[3] = {a.B, a.heads[i], a.S};
+        for (int d = 0; d < 3; ++d) wide = wide && (n[d] == 1 || (a.xs[i][d] % kV == 0 && a.ys[i][d] % kV == 0));
+    }
+    if (interleaved) return wide ? launch_rotary<T, kV, true>(a, st) : launch_rotary<T, 1, true>(a, st);
+    return wide ? launch_rotary<T, kV, false>(a, st) : launch_rotary<T, 1, false>(a, st);
+}
+cudaError_t rotary(const RotaryArgs& a, int bf16, int interleaved, cudaStream_t st) {
+    return bf16 ? launch_rotary_type<__nv_bfloat16>(a, interleaved, st) : launch_rotary_type<float>(a, interleaved, st);
+}
+
+}  // namespace ttk

@@ -1,0 +1,173 @@
+// C-ABI layer of what stands around a paged cache: page tables and rotary positions.  Argument checks and launches;
+// see include/tt_attn.h.
+#include "../../include/tt_attn.h"
+#include "common.h"
+
+#include <cmath>
+#include <cstdlib>
+
+namespace ttk {
+namespace {
+
+struct Span {
+    const void* p;
+    size_t bytes;
+    const char* name;
+};
+bool overlap(const Span& a, const Span& b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+// Outputs that lie on an input or on each other: some CTAs would read what others have written.
+int check_overlap(const char* who, const Span* out, int n_out, const Span* in, int n_in) {
+    for (int i = 0; i < n_out; ++i) {
+        for (int j = 0; j < n_in; ++j)
+            if (overlap(out[i], in[j])) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].name, in[j].name);
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j])) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].name, out[j].name);
+    }
+    return TT_OK;
+}
+
+int table_args(const char* who, int32_t B, int32_t page_size, int32_t max_pages, int32_t free_capacity) {
+    if (B < 1 || page_size < 1 || max_pages < 1 || free_capacity < 0)
+        return fail(TT_ERR_BAD_SHAPE, "%s: B=%d page_size=%d max_pages=%d must be >= 1, free_capacity=%d >= 0", who, B, page_size, max_pages, free_capacity);
+    if (B > cache_max_requests()) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d, at most %d requests", who, B, cache_max_requests());
+    return TT_OK;
+}
+
+// Whether rows of D elements at strides st over extents n lie apart from each other.
+bool rows_apart(const int64_t* st, const int* n, int D) {
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (st[order[j]] < st[order[i]]) {
+                const int t = order[i];
+                order[i] = order[j];
+                order[j] = t;
+            }
+    int64_t reach = D;   // from the first element to behind the last of the dimensions so far
+    for (int i = 0; i < 3; ++i) {
+        const int d = order[i];
+        if (n[d] == 1) continue;
+        if (st[d] < reach) return false;
+        reach += st[d] * (n[d] - 1);
+    }
+    return true;
+}
+// A tensor of rows at strides st: what it spans, and whether that holds nothing else.
+struct Rows {
+    Span span;
+    bool dense;
+    Rows(const void* p, const int64_t* st, const int* n, int D, size_t size, const char* name) {
+        int64_t last = D, all = D;
+        for (int i = 0; i < 3; ++i) {
+            if (n[i] > 1) last += st[i] * (n[i] - 1);
+            all *= n[i];
+        }
+        span = Span{p, (size_t)last * size, name};
+        dense = last == all;
+    }
+};
+
+}  // namespace
+}  // namespace ttk
+
+using namespace ttk;
+
+extern "C" {
+
+int tt_cache_extend(int32_t* block_table, const int32_t* seq_lens, const int32_t* new_lens, const int32_t* free_pages, const int32_t* n_free, int32_t B,
+                    int32_t page_size, int32_t max_pages, int32_t free_capacity, int32_t max_tokens, int32_t* seq_lens_out, int32_t* n_free_out,
+                    int32_t* cu_new, int32_t* slots, int32_t* positions, void* stream) {
+    const char* who = "tt_cache_extend";
+    int rc = table_args(who, B, page_size, max_pages, free_capacity);
+    if (rc != TT_OK) return rc;
+    if (max_tokens < 0) return fail(TT_ERR_BAD_SHAPE, "%s: max_tokens=%d", who, max_tokens);
+    if (!block_table || !seq_lens || !new_lens || !n_free || !seq_lens_out || !n_free_out || !cu_new || (free_capacity && !free_pages) ||
+        (max_tokens && (!slots || !positions)))
+        return fail(TT_ERR_NULL, "%s: null pointer", who);
+    const size_t n = (size_t)B * 4, t = (size_t)max_tokens * 4;
+    const Span out[] = {{seq_lens_out, n, "seq_lens_out"}, {n_free_out, 4, "n_free_out"}, {cu_new, n + 4, "cu_new"}, {slots, t, "slots"},
+                        {positions, t, "positions"}, {block_table, n * max_pages, "block_table"}};
+    const Span in[] = {{seq_lens, n, "seq_lens"}, {new_lens, n, "new_lens"}, {free_pages, (size_t)free_capacity * 4, "free_pages"}, {n_free, 4, "n_free"}};
+    if ((rc = check_overlap(who, out, 6, in, 4)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
+    const cudaError_t e = cache_extend(block_table, seq_lens, new_lens, free_pages, n_free, B, page_size, max_pages, free_capacity, max_tokens, seq_lens_out,
+                                       n_free_out, cu_new, slots, positions, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_extend: launch");
+}
+
+int tt_cache_release(const int32_t* block_table, const int32_t* seq_lens, const uint8_t* done, int32_t* free_pages, const int32_t* n_free, int32_t B,
+                     int32_t page_size, int32_t max_pages, int32_t free_capacity, int32_t* seq_lens_out, int32_t* n_free_out, void* stream) {
+    const char* who = "tt_cache_release";
+    int rc = table_args(who, B, page_size, max_pages, free_capacity);
+    if (rc != TT_OK) return rc;
+    if (!block_table || !seq_lens || !done || !n_free || !seq_lens_out || !n_free_out || (free_capacity && !free_pages))
+        return fail(TT_ERR_NULL, "%s: null pointer", who);
+    const size_t n = (size_t)B * 4;
+    const Span out[] = {{seq_lens_out, n, "seq_lens_out"}, {n_free_out, 4, "n_free_out"}, {free_pages, (size_t)free_capacity * 4, "free_pages"}};
+    const Span in[] = {{block_table, n * max_pages, "block_table"}, {seq_lens, n, "seq_lens"}, {done, (size_t)B, "done"}, {n_free, 4, "n_free"}};
+    if ((rc = check_overlap(who, out, 3, in, 4)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
+    const cudaError_t e = cache_release(block_table, seq_lens, done, free_pages, n_free, B, page_size, max_pages, free_capacity, seq_lens_out, n_free_out,
+                                        (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_release: launch");
+}
+
+int tt_rotary(const tt_rotary_desc* d, const void* q, const void* k, const int32_t* positions, const double* inv_freq, const int32_t* axes, int32_t backward,
+              void* q_out, void* k_out, void* stream) {
+    const char* who = "tt_rotary";
+    if (!d) return fail(TT_ERR_NULL, "%s: desc is null", who);
+    const int hk = k ? d->Hkv : 0;
+    if (d->B < 0 || d->S < 0 || d->H < 1 || (k && hk < 1)) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d S=%d H=%d Hkv=%d", who, d->B, d->S, d->H, d->Hkv);
+    if (d->D < 2 || d->D > 256 || d->R < 2 || d->R > d->D || d->R % 2)
+        return fail(TT_ERR_BAD_SHAPE, "%s: D=%d must be 2..256 and R=%d even, 2..D", who, d->D, d->R);
+    if (d->n_axes < 1) return fail(TT_ERR_BAD_SHAPE, "%s: n_axes=%d", who, d->n_axes);
+    if (d->dtype != TT_F32 && d->dtype != TT_BF16) return fail(TT_ERR_BAD_DTYPE, "%s: dtype %d unknown", who, d->dtype);
+    if (!std::isfinite(d->scale)) return fail(TT_ERR_BAD_SHAPE, "%s: scale is not finite", who);
+    if ((int64_t)d->B * d->S >= (1LL << 31) || (int64_t)d->H + hk >= (1LL << 24)) return fail(TT_ERR_BAD_SHAPE, "%s: more than 2^31-1 tokens or 2^24 heads", who);
+    if ((k == nullptr) != (k_out == nullptr)) return fail(TT_ERR_NULL, "%s: k and k_out go together", who);
+    if (d->B == 0 || d->S == 0) return TT_OK;
+    if (!q || !q_out || !positions || !inv_freq) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    const size_t size = d->dtype == TT_BF16 ? 2 : 4;
+    const int nq[3] = {d->B, d->H, d->S}, nk[3] = {d->B, hk, d->S};
+    for (int i = 0; i < 3; ++i)
+        if (d->q_stride[i] < 0 || d->q_out_stride[i] < 0 || (k && (d->k_stride[i] < 0 || d->k_out_stride[i] < 0)) || (i < 2 && d->pos_stride[i] < 0))
+            return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
+    if (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
+    if (!rows_apart(d->q_out_stride, nq, d->D) || (k && !rows_apart(d->k_out_stride, nk, d->D)))
+        return fail(TT_ERR_BAD_SHAPE, "%s: rows of an output overlap", who);
+    // An output lies on its own input row by row, or apart from everything.  Slices of one buffer interleave without
+    // meeting, so spans decide only where both tensors fill theirs.
+    auto same = [](const int64_t* x, const int64_t* y, const int* n) {
+        for (int i = 0; i < 3; ++i)
+            if (n[i] > 1 && x[i] != y[i]) return false;
+        return true;
+    };
+    const Rows in[2] = {{q, d->q_stride, nq, d->D, size, "q"}, {k, d->k_stride, nk, d->D, size, "k"}};
+    const Rows out[2] = {{q_out, d->q_out_stride, nq, d->D, size, "q_out"}, {k_out, d->k_out_stride, nk, d->D, size, "k_out"}};
+    for (int i = 0; i < (k ? 2 : 1); ++i) {
+        for (int j = 0; j < (k ? 2 : 1); ++j) {
+            if (i == j && out[i].span.p == in[j].span.p && same(i ? d->k_out_stride : d->q_out_stride, i ? d->k_stride : d->q_stride, i ? nk : nq)) continue;
+            if (out[i].span.p == in[j].span.p || (out[i].dense && in[j].dense && overlap(out[i].span, in[j].span)))
+                return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in[j].span.name);
+        }
+    }
+    if (k && (q_out == k_out || (out[0].dense && out[1].dense && overlap(out[0].span, out[1].span))))
+        return fail(TT_ERR_BAD_SHAPE, "%s: q_out overlaps k_out", who);
+    const int rc = check_device();
+    if (rc != TT_OK) return rc;
+    RotaryArgs a = {};
+    a.x[0] = q; a.x[1] = k; a.y[0] = q_out; a.y[1] = k_out;
+    for (int i = 0; i < 3; ++i) {
+        a.xs[0][i] = d->q_stride[i]; a.xs[1][i] = d->k_stride[i];
+        a.ys[0][i] = d->q_out_stride[i]; a.ys[1][i] = d->k_out_stride[i];
+    }
+    a.heads[0] = d->H; a.heads[1] = hk;
+    a.B = d->B; a.S = d->S; a.D = d->D; a.R = d->R; a.n_axes = d->n_axes;
+    a.pos = positions; a.pos_axis = d->pos_stride[0]; a.pos_batch = d->pos_stride[1];
+    a.inv_freq = inv_freq; a.axes = axes; a.scale = d->scale; a.back = backward != 0;
+    const cudaError_t e = rotary(a, d->dtype == TT_BF16, d->interleaved != 0, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_rotary: launch");
+}
+
+}  // extern "C"

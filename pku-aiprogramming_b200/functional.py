@@ -12,6 +12,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -187,6 +188,127 @@ def attention_decode_paged(q, k_pool, v_pool, block_table=None, seq_lens=None, m
     (default: page_size * max_pages, or L of the dense cache)."""
     r = _native.attention_decode_paged(q, k_pool, v_pool, block_table, seq_lens, max_len, scale, out, lse, workspace, need_lse)
     return r if r.__class__ is tuple else _done(r, _explain_paged, q, k_pool, v_pool, block_table, seq_lens, max_len)
+
+
+class CacheStep(NamedTuple):
+    """What `cache_extend` says of the new tokens: lengths with them, pages left, cumulative counts `[B+1]`, and for
+    each packed row its slot in the cache (-1 behind the last row) and its position."""
+    seq_lens: torch.Tensor
+    n_free: torch.Tensor
+    cu_new: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+
+
+def _explain_tables(block_table, seq_lens, more, out=None, sizes=()):
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2 or block_table.dtype != torch.int32 \
+            or not block_table.is_cuda or not block_table.is_contiguous():
+        raise ValueError("block_table must be a contiguous CUDA int32 tensor [B, max_pages]")
+    B = block_table.shape[0]
+    for name, t, n, types in [("seq_lens", seq_lens, B, (torch.int32,))] + more:
+        if not isinstance(t, torch.Tensor) or t.dtype not in types or t.device != block_table.device \
+                or not t.is_contiguous() or t.dim() != 1 or (n is not None and t.shape[0] != n):
+            raise ValueError(f"{name} must be a contiguous {types[0]} vector" + (f" of {n}" if n is not None else "") +
+                             " on block_table's device")
+    if out is not None:
+        raise ValueError(f"out must be a tuple of contiguous int32 vectors of {sizes} elements on block_table's device")
+    raise ValueError("page_size and max_tokens must be 32-bit integers, max_tokens not negative")
+
+
+def cache_extend(block_table, seq_lens, new_lens, free_pages, n_free, page_size, max_tokens, out=None):
+    """Pages and slots for `new_lens` more tokens of each request, on the GPU -> `CacheStep`.
+
+    `block_table` `[B, max_pages]` gets the new pages' columns; `free_pages` with `n_free` `[1]` page numbers on it is used
+    from its end and not written.  Requests are served in their order until one's tokens exceed `max_tokens` in all or its
+    pages what is free; it and those behind it get nothing (their lengths stay).  All tensors int32, CUDA.  `out`: a
+    `CacheStep` to write into; it must not share memory with the inputs, so a loop keeps two and takes them in turn."""
+    r = _native.cache_extend(block_table, seq_lens, new_lens, free_pages, n_free, page_size, max_tokens, out)
+    if r.__class__ is tuple:
+        return CacheStep._make(r)
+    i32 = (torch.int32,)
+    return _done(r, lambda: _explain_tables(block_table, seq_lens, [
+        ("new_lens", new_lens, block_table.shape[0], i32), ("free_pages", free_pages, None, i32), ("n_free", n_free, 1, i32)], out,
+        "B, 1, B + 1, max_tokens, max_tokens"))
+
+
+def cache_release(block_table, seq_lens, done, free_pages, n_free, page_size, out=None):
+    """The pages of the requests that `done` (bool `[B]`) marks, back on `free_pages` behind its `n_free` -> (seq_lens with
+    0 there, n_free).  `out`: those two tensors, apart from the inputs."""
+    r = _native.cache_release(block_table, seq_lens, done, free_pages, n_free, page_size, out)
+    if r.__class__ is tuple:
+        return r
+    return _done(r, lambda: _explain_tables(block_table, seq_lens, [
+        ("done", done, block_table.shape[0], (torch.bool, torch.uint8)), ("free_pages", free_pages, None, (torch.int32,)),
+        ("n_free", n_free, 1, (torch.int32,))], out, "B, 1"))
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, sections=None, cyclic=False, own_ladder=False, device="cuda"):
+    """(inv_freq `[rotary_dim/2]` float64, axes int32 or None) of `rotary_forward`.
+
+    `sections`: the pairs of each axis, `rotary_dim / 2` in all (None: one axis).  Pairs go to the axes section by section, or
+    with `cyclic` in turn, as long as an axis has some left.  Pair i of n turns by `base ** (-i / n)` per position;
+    with `own_ladder` each axis counts its own pairs, i.e. it has slow and fast ones as an axis alone would."""
+    n = int(rotary_dim) // 2
+    sections = [n] if sections is None else [int(s) for s in sections]
+    if int(rotary_dim) != 2 * n or n < 1:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if any(s < 0 for s in sections) or sum(sections) != n:
+        raise ValueError(f"sections {sections} must add up to rotary_dim / 2 = {n}")
+    if not base > 0:
+        raise ValueError("base must be positive")
+    if cyclic:
+        axes = [a for turn in range(max(sections)) for a, s in enumerate(sections) if turn < s]
+    else:
+        axes = [a for a, s in enumerate(sections) for _ in range(s)]
+    seen = [0] * len(sections)
+    freq = []
+    for i, a in enumerate(axes):
+        freq.append(float(base) ** -((seen[a] / sections[a]) if own_ladder else i / n))
+        seen[a] += 1
+    inv_freq = torch.tensor(freq, dtype=torch.float64, device=device)
+    return inv_freq, (torch.tensor(axes, dtype=torch.int32, device=device) if len(sections) > 1 else None)
+
+
+def _explain_rotary(q, k, positions, inv_freq, axes, out_q, out_k):
+    for name, t in (("q", q), ("k", k), ("out_q", out_q), ("out_k", out_k)):
+        if t is None and name != "q":
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DT or t.dim() not in (3, 4) \
+                or (t.shape[-1] > 1 and t.stride(-1) != 1):
+            raise ValueError(f"{name} must be a CUDA float32/bfloat16 tensor [T,H,D] or [B,H,S,D] whose channels lie next to each other")
+        if t.dtype != q.dtype or t.dim() != q.dim() or t.device != q.device:
+            raise ValueError(f"{name} must have q's type, dimensions and device")
+    for name, t, x in (("out_q", out_q, q), ("out_k", out_k, k)):
+        if t is not None and (x is None or t.shape != x.shape):
+            raise ValueError(f"{name} must have its input's shape")
+    rows = 0 if q.dim() == 3 else 2
+    if k is not None and (k.shape[rows] != q.shape[rows] or k.shape[-1] != q.shape[-1] or (rows and k.shape[0] != q.shape[0])):
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)} k {tuple(k.shape)}")
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != q.device \
+            or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float64 vector on q's device, one frequency per pair")
+    if axes is not None and (not isinstance(axes, torch.Tensor) or axes.dtype != torch.int32 or axes.shape != inv_freq.shape
+                             or axes.device != q.device or not axes.is_contiguous()):
+        raise ValueError("axes must be a contiguous int32 vector on q's device, one axis per pair")
+    want = "[axes, T] or [T]" if q.dim() == 3 else "[axes, B, S], [axes, S] or [S]"
+    raise ValueError(f"positions must be an int32 tensor {want} on q's device, rows next to each other")
+
+
+def rotary_forward(q, k, positions, inv_freq, axes=None, interleaved=False, scale=None, out_q=None, out_k=None):
+    """Query and key heads turned by their positions -> (q, k), inputs `[T,H,D]` (packed) or `[B,H,S,D]`, k may be None.
+
+    Pair i of the first `2 * len(inv_freq)` channels turns by `positions[axes[i]] * inv_freq[i]` (float64 `[R/2]`, int32 `[R/2]` or
+    None, see `rotary_frequencies`): channels i and i + R/2, or with `interleaved` 2i and 2i + 1; the other channels are copied.
+    positions: int32 `[axes, T]` / `[axes, B, S]` / `[axes, S]`, or `[T]` / `[S]` with one axis.  Strided inputs are fine as long
+    as channels lie next to each other; `out_q`, `out_k` may be the inputs themselves.  `scale` (1) multiplies the result."""
+    r = _native.rotary(q, k, positions, inv_freq, axes, interleaved, scale, False, out_q, out_k)
+    return r if r.__class__ is tuple else _done(r, _explain_rotary, q, k, positions, inv_freq, axes, out_q, out_k)
+
+
+def rotary_backward(dq, dk, positions, inv_freq, axes=None, interleaved=False, scale=None, out_q=None, out_k=None):
+    """(dq, dk) with respect to the inputs of `rotary_forward` for upstream gradients `dq`, `dk` of its results."""
+    r = _native.rotary(dq, dk, positions, inv_freq, axes, interleaved, scale, True, out_q, out_k)
+    return r if r.__class__ is tuple else _done(r, _explain_rotary, dq, dk, positions, inv_freq, axes, out_q, out_k)
 
 
 def _explain_softmax_forward(x):

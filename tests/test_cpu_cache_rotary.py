@@ -1,0 +1,138 @@
+"""Argument checks of the page-table and rotary calls (status codes, no GPU needed) and the frequency table."""
+import ctypes
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+def _buffers(n=8, size=4096):
+    raw = (ctypes.c_char * (n * size))()
+    base = ctypes.addressof(raw)
+    base += -base % 256
+    return raw, [ctypes.c_void_p(base + i * size) for i in range(n - 1)]
+
+
+def _extend(tt, **kw):
+    raw, p = _buffers(12)
+    a = dict(table=p[0], lens=p[1], new=p[2], free=p[3], n_free=p[4], B=4, page=16, max_pages=8, cap=10, tokens=20, lens_out=p[5], n_free_out=p[6], cu=p[7],
+             slots=p[8], pos=p[9])
+    a.update({k: (p[v] if isinstance(v, str) and k else v) for k, v in kw.items()})
+    rc = tt.capi.lib.tt_cache_extend(a["table"], a["lens"], a["new"], a["free"], a["n_free"], a["B"], a["page"], a["max_pages"], a["cap"], a["tokens"],
+                                     a["lens_out"], a["n_free_out"], a["cu"], a["slots"], a["pos"], None)
+    del raw
+    return rc
+
+
+def _at(p, offset):
+    return ctypes.c_void_p(p.value + offset)
+
+
+def test_extend_refuses_what_does_not_fit(tt):
+    c = tt.capi
+    for bad in (dict(B=0), dict(B=16385), dict(page=0), dict(max_pages=0), dict(cap=-1), dict(tokens=-1)):
+        assert _extend(tt, **bad) == c.TT_ERR_BAD_SHAPE, bad
+    for null in ("table", "lens", "new", "free", "n_free", "lens_out", "n_free_out", "cu", "slots", "pos"):
+        assert _extend(tt, **{null: None}) == c.TT_ERR_NULL, null
+
+
+def test_extend_and_release_refuse_outputs_on_inputs(tt):
+    lib, c = tt.capi.lib, tt.capi
+    raw, p = _buffers(12)
+    table, lens, new, free, n_free, lens_out, n_out, cu, slots, pos = p[:10]
+
+    def extend(**kw):
+        a = dict(table=table, lens=lens, new=new, free=free, n_free=n_free, lens_out=lens_out, n_out=n_out, cu=cu, slots=slots, pos=pos)
+        a.update(kw)
+        return lib.tt_cache_extend(a["table"], a["lens"], a["new"], a["free"], a["n_free"], 4, 16, 8, 10, 20, a["lens_out"], a["n_out"], a["cu"], a["slots"],
+                                   a["pos"], None)
+
+    for kw in (dict(lens_out=lens), dict(lens_out=_at(lens, 12)), dict(n_out=n_free), dict(cu=_at(new, -4)), dict(slots=pos), dict(pos=_at(free, 36)),
+               dict(lens_out=_at(table, 124)), dict(n_out=_at(cu, 16))):
+        assert extend(**kw) == c.TT_ERR_BAD_SHAPE and "overlaps" in c.last_error(), kw
+
+    def release(**kw):
+        a = dict(table=table, lens=lens, done=new, free=free, n_free=n_free, lens_out=lens_out, n_out=n_out)
+        a.update(kw)
+        return lib.tt_cache_release(a["table"], a["lens"], a["done"], a["free"], a["n_free"], a.get("B", 4), 16, 8, 10, a["lens_out"], a["n_out"], None)
+
+    assert release(B=0) == c.TT_ERR_BAD_SHAPE and release(B=16385) == c.TT_ERR_BAD_SHAPE
+    for null in ("table", "lens", "done", "free", "n_free", "lens_out", "n_out"):
+        assert release(**{null: None}) == c.TT_ERR_NULL, null
+    for kw in (dict(lens_out=lens), dict(n_out=n_free), dict(lens_out=free), dict(free=_at(table, 64)), dict(n_out=_at(lens_out, 12))):
+        assert release(**kw) == c.TT_ERR_BAD_SHAPE and "overlaps" in c.last_error(), kw
+    if not torch.cuda.is_available():
+        assert extend() == c.TT_ERR_BAD_DEVICE and release() == c.TT_ERR_BAD_DEVICE
+    del raw
+
+
+def _rotary_desc(tt, **kw):
+    d = tt.capi.RotaryDesc(B=2, S=4, H=4, Hkv=2, D=16, R=8, n_axes=1, dtype=tt.capi.TT_F32, interleaved=0, scale=1.0)
+    d.q_stride[:] = d.q_out_stride[:] = (4 * 4 * 16, 4 * 16, 16)
+    d.k_stride[:] = d.k_out_stride[:] = (2 * 4 * 16, 4 * 16, 16)
+    d.pos_stride[:] = (8, 4)
+    for name, v in kw.items():
+        if isinstance(v, tuple):
+            getattr(d, name)[:] = v
+        else:
+            setattr(d, name, v)
+    return d
+
+
+def test_rotary_refuses_what_does_not_fit(tt):
+    lib, c = tt.capi.lib, tt.capi
+    raw, p = _buffers(8)
+    q, k, q_out, k_out, pos, freq = p[:6]
+
+    def call(d, q=q, k=k, pos=pos, freq=freq, q_out=q_out, k_out=k_out):
+        return lib.tt_rotary(ctypes.byref(d), q, k, pos, freq, None, 0, q_out, k_out, None)
+
+    assert lib.tt_rotary(None, q, k, pos, freq, None, 0, q_out, k_out, None) == c.TT_ERR_NULL
+    for bad in (dict(H=0), dict(Hkv=0), dict(D=1), dict(D=257), dict(R=0), dict(R=7), dict(R=18), dict(n_axes=0), dict(B=-1), dict(S=-1),
+                dict(scale=math.inf), dict(scale=math.nan), dict(B=1 << 16, S=1 << 15), dict(q_stride=(-1, 64, 16)), dict(pos_stride=(-1, 4))):
+        assert call(_rotary_desc(tt, **bad)) == c.TT_ERR_BAD_SHAPE, bad
+    assert call(_rotary_desc(tt, dtype=7)) == c.TT_ERR_BAD_DTYPE
+    # rows of an output that lie on each other
+    for st in ((0, 64, 16), (256, 0, 16), (256, 64, 15), (64, 64, 16), (63, 256, 16)):
+        assert call(_rotary_desc(tt, q_out_stride=st)) == c.TT_ERR_BAD_SHAPE, st
+    d = _rotary_desc(tt)
+    for kw in (dict(q=None), dict(q_out=None), dict(pos=None), dict(freq=None), dict(k=None), dict(k_out=None)):
+        assert call(d, **kw) == c.TT_ERR_NULL, kw
+    for kw in (dict(q_out=k), dict(q_out=_at(q, 64)), dict(k_out=_at(q, 512)), dict(k_out=q_out), dict(k_out=_at(q_out, 128)), dict(q_out=_at(k, 960)),
+               dict(q=_at(q, 2))):
+        assert call(d, **kw) == c.TT_ERR_BAD_SHAPE, kw
+    assert call(_rotary_desc(tt, q_stride=(16, 32, 128)), q_out=q) == c.TT_ERR_BAD_SHAPE   # in place at other strides
+    for empty in (dict(B=0), dict(S=0)):
+        assert call(_rotary_desc(tt, **empty), q=None, pos=None) == c.TT_OK
+    if not torch.cuda.is_available():
+        assert call(d) == c.TT_ERR_BAD_DEVICE and call(d, q_out=q, k_out=k) == c.TT_ERR_BAD_DEVICE
+    del raw
+
+
+def test_calls_on_cpu_tensors_are_refused(tt):
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    i = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="block_table"):
+        tt.cache_extend(torch.zeros(4, 8, dtype=torch.int32), i, i, i, i[:1], 16, 4)
+    with pytest.raises(ValueError, match="block_table"):
+        tt.cache_release(torch.zeros(4, 8, dtype=torch.int32), i, i.bool(), i, i[:1], 16)
+    freq, _ = tt.rotary_frequencies(8, device="cpu")
+    with pytest.raises(ValueError, match="q must be a CUDA"):
+        tt.rotary_forward(torch.zeros(4, 2, 8), None, i, freq)
+
+
+def test_frequencies(tt):
+    freq, axes = tt.rotary_frequencies(8, base=100.0, device="cpu")
+    assert axes is None and freq.dtype == torch.float64
+    assert torch.allclose(freq, torch.tensor([1.0, 100 ** -0.25, 0.1, 100 ** -0.75], dtype=torch.float64), rtol=1e-15, atol=0)
+    freq, axes = tt.rotary_frequencies(12, sections=(1, 3, 2), device="cpu")
+    assert axes.tolist() == [0, 1, 1, 1, 2, 2]
+    freq, axes = tt.rotary_frequencies(12, sections=(1, 3, 2), cyclic=True, device="cpu")
+    assert axes.tolist() == [0, 1, 2, 1, 2, 1] and freq[1] == 10000.0 ** (-1 / 6)
+    freq, axes = tt.rotary_frequencies(12, sections=(2, 0, 4), own_ladder=True, device="cpu")
+    assert axes.tolist() == [0, 0, 2, 2, 2, 2] and freq.tolist() == [10000.0 ** -(i / n) for n in (2, 4) for i in range(n)]
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, sections=(1, 2)), dict(rotary_dim=8, sections=(5, -1)), dict(rotary_dim=8, base=0.0)):
+        with pytest.raises(ValueError):
+            tt.rotary_frequencies(**bad, device="cpu")
