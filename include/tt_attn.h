@@ -228,6 +228,30 @@ int tt_cache_release(const int32_t* block_table, const int32_t* seq_lens, const 
                      const int32_t* n_free, int32_t B, int32_t page_size, int32_t max_pages, int32_t free_capacity,
                      int32_t* seq_lens_out, int32_t* n_free_out, void* stream);
 
+/* ---- key/value cache in 4 bits --------------------------------------------------------------
+ * k_cache, v_cache: [n_pages, Hkv, tt_cache_q4_page_bytes(page_size, D)] bytes each, 16-byte aligned; D 64 or 128, page_size a
+ * multiple of 16.  A page holds, for one key/value head, [page_size][D / 2] bytes (channel 2j in the low half of byte j) and then
+ * [page_size][D / 32] scale codes, one for 32 channels: 4.25 bits a value.  Code c stands for the scale s = half(c << 7) / 8, i.e. five bits
+ * of exponent and three of mantissa; a value is (n - 8) s with n in 0 .. 15, which bf16 holds exactly.
+ *
+ * tt_cache_append_q4: T new tokens' keys and values [T, Hkv, D] (float or bf16, channels next to each other, element strides
+ * {token, head}) into their slots (page * page_size + row, as from tt_cache_extend).  A slot that is negative or behind the last page is
+ * passed over; no two tokens may have one slot (what such a slot then holds is of either, and may be of both).  Per group: s is
+ * the smallest scale with 7.5 s >= max |x|, n = rint(x / s) (ties to even) held to -8 .. 7, plus 8, so an error is at most s / 2.
+ * The largest scale is 896: values beyond 6720 and infinities become the largest.  A group with a NaN reads as NaN.
+ *
+ * tt_cache_read_q4: the first cu_lens[b + 1] - cu_lens[b] tokens of each sequence as packed bf16 k, v [total, Hkv, D] (what
+ * tt_attn_fwd_varlen takes); sequence b's are rows [cu_lens[b], cu_lens[b + 1]), found by block_table [B, max_pages].  cu_lens
+ * counts up from 0.  Rows from cu_lens[B] on are left as they were; rows whose page is not one of the n_pages, or lies behind the
+ * table's width, are 0. */
+size_t tt_cache_q4_page_bytes(int32_t page_size, int32_t D);   /* 0: not supported */
+int tt_cache_append_q4(const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype,
+                       const int64_t* k_stride, const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages,
+                       int32_t page_size, void* stream);
+int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* cu_lens, int32_t B,
+                     int32_t Hkv, int32_t D, int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t total, void* k, void* v,
+                     void* stream);
+
 /* ---- rotary positions ------------------------------------------------------------------------
  * Query and key heads turned by their tokens' positions (no counterpart in the reference).  Of a head's D channels the first
  * R form R / 2 pairs; pair i of a token at position p on axis a = axes[i] turns by p * inv_freq[i]:

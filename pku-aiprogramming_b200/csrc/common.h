@@ -145,7 +145,7 @@ enum KernelId {
     K_FWD_TC = 0, K_FWD_SIMT, K_BWD_PREP, K_BWD_DKV, K_BWD_DQ, K_BWD_SIMT_DELTA, K_BWD_SIMT_DQ, K_BWD_SIMT_DKV,
     K_DECODE, K_DECODE_MERGE, K_PROBE, K_SOFTMAX_FWD, K_SOFTMAX_BWD, K_FC_GEMM, K_FC_SIMT, K_FC_COLSUM, K_BWD_FUSED,
     K_BWD_DQ_CONVERT, K_DECODE_GQ, K_FWD_F32, K_BWD_F32, K_BWD_BOTH, K_CACHE_TABLES,
-    K_ROTARY, K_COUNT
+    K_ROTARY, K_CACHE_APPEND, K_CACHE_READ, K_COUNT
 };
 // Scoped around ONE kernel launch: counts it and, when timing is enabled, brackets it with
 // CUDA events on the launching stream.
@@ -271,6 +271,15 @@ cudaError_t cache_extend(int* table, const int* lens, const int* fresh, const in
                          int free_capacity, int max_tokens, int* lens_out, int* n_free_out, int* cu_new, int* slots, int* positions, cudaStream_t st);
 cudaError_t cache_release(const int* table, const int* lens, const unsigned char* done, int* free_pages, const int* n_free, int B, int page, int max_pages,
                           int free_capacity, int* lens_out, int* n_free_out, cudaStream_t st);
+
+// --- 4-bit key/value cache (cache_q4.cu); D 64 or 128, page_size a multiple of 16; strides in elements {token, head}
+struct CacheQ4 {
+    void *k, *v;
+    int n_pages, page_size, hkv, D;
+};
+cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, const long long (&ks)[2], const long long (&vs)[2], int bf16, const int* slots,
+                            int T, cudaStream_t st);
+cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st);
 
 // --- rotary positions (rotary.cu)
 struct RotaryArgs {

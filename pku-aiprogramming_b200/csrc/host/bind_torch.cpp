@@ -627,12 +627,83 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// The two pools of a 4-bit cache: contiguous bytes [pages, Hkv, page bytes] of one shape and device.
+bool q4_cache(PyObject* ok, PyObject* ov, const Tensor** k, const Tensor** v) {
+    *k = on_device(ok, at::kByte);
+    *v = *k ? on_device(ov, at::kByte, *k) : nullptr;
+    return *v && (*k)->dim() == 3 && (*k)->is_contiguous() && (*v)->is_contiguous() && same_shape(**k, **v) && fits32((*k)->size(0)) && fits32((*k)->size(1));
+}
+// tokens of a page of `bytes` at head dim D; 0: no page has that size
+int64_t q4_page_size(int64_t bytes, int64_t D) {
+    if (D != 64 && D != 128) return 0;
+    const int64_t row = D / 2 + D / 32;
+    return bytes > 0 && bytes % (16 * row) == 0 && fits32(bytes) ? bytes / row : 0;
+}
+
+// (k, v, slots, k_cache, v_cache) -> (k_cache, v_cache)
+PyObject* cache_append_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Tensor *kc, *vc;
+        if (n != 5 || !q4_cache(a[3], a[4], &kc, &vc) || !THPVariable_Check(a[0])) Py_RETURN_NONE;
+        const Tensor& k = THPVariable_Unpack(a[0]);
+        const Tensor* v = float_type(k) ? on_device(a[1], k.scalar_type(), kc) : nullptr;
+        if (!v || !k.is_cuda() || k.device() != kc->device() || k.dim() != 3 || !same_shape(k, *v) || k.stride(2) != 1 || v->stride(2) != 1 || k.size(1) != kc->size(1) ||
+            !fits32(k.size(0)))
+            Py_RETURN_NONE;
+        const Tensor* slots = vector_arg(a[2], at::kInt, k.size(0), kc);
+        const int64_t page = q4_page_size(kc->size(2), k.size(2));
+        if (!slots || page == 0) Py_RETURN_NONE;
+        const int64_t ks[2] = {k.stride(0), k.stride(1)}, vs[2] = {v->stride(0), v->stride(1)};
+        OnDevice dev(*kc);
+        TT_CALL(rc, tt_cache_append_q4(ptr(k), ptr(v), (const int32_t*)ptr(slots), (int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), tt_type(k), ks, vs,
+                                       ptr(kc), ptr(vc), (int32_t)kc->size(0), (int32_t)page, dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        Py_INCREF(a[3]);
+        Py_INCREF(a[4]);
+        return pack(a[3], a[4]);
+    });
+}
+
+// (k_cache, v_cache, block_table, cu_lens, total, page_size, k, v) -> (k, v)
+PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Tensor *kc, *vc;
+        if (n != 8 || !q4_cache(a[0], a[1], &kc, &vc)) Py_RETURN_NONE;
+        const Tensor* table = on_device(a[2], at::kInt, kc);
+        if (!table || !table->is_contiguous() || table->dim() != 2 || !fits32(table->size(0)) || !fits32(table->size(1))) Py_RETURN_NONE;
+        const Tensor* cu = vector_arg(a[3], at::kInt, table->size(0) + 1, kc);
+        int64_t total, page;
+        if (!cu) Py_RETURN_NONE;
+        if (!int_arg(a[4], &total) || !int_arg(a[5], &page)) return nullptr;
+        if (total < 0 || !fits32(total) || page < 1 || !fits32(page)) Py_RETURN_NONE;
+        const int64_t D = kc->size(2) == page * 34 ? 64 : kc->size(2) == page * 68 ? 128 : 0;
+        if (D == 0 || page % 16) Py_RETURN_NONE;
+        OnDevice dev(*kc);
+        Tensor made[2];
+        const Tensor* out[2];
+        for (int i = 0; i < 2; ++i) {
+            if (a[6 + i] != Py_None) {
+                out[i] = on_device(a[6 + i], at::kBFloat16, kc);
+                if (!out[i] || !out[i]->is_contiguous() || out[i]->dim() != 3 || out[i]->size(0) != total || out[i]->size(1) != kc->size(1) || out[i]->size(2) != D)
+                    Py_RETURN_NONE;
+            } else {
+                made[i] = make({total, kc->size(1), D}, at::kBFloat16, *kc);
+                out[i] = &made[i];
+            }
+        }
+        TT_CALL(rc, tt_cache_read_q4(ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(cu), (int32_t)table->size(0), (int32_t)kc->size(1), (int32_t)D,
+                                     (int32_t)kc->size(0), (int32_t)page, (int32_t)table->size(1), (int32_t)total, ptr(out[0]), ptr(out[1]), dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(wrap_or(a[6], made[0]), wrap_or(a[7], made[1]));
+    });
+}
+
 #define TT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     TT_METHOD(attention_forward), TT_METHOD(attention_backward), TT_METHOD(attention_forward_varlen),
     TT_METHOD(attention_backward_varlen), TT_METHOD(attention_decode), TT_METHOD(attention_decode_paged),
     TT_METHOD(softmax_forward), TT_METHOD(softmax_backward), TT_METHOD(fc_forward), TT_METHOD(fc_backward), TT_METHOD(cache_extend), TT_METHOD(cache_release),
-    TT_METHOD(rotary),
+    TT_METHOD(rotary), TT_METHOD(cache_append_q4), TT_METHOD(cache_read_q4),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ttorch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

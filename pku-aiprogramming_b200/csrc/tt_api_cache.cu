@@ -1,4 +1,4 @@
-// C-ABI layer of what stands around a paged cache: page tables and rotary positions.  Argument checks and launches;
+// C-ABI layer of what stands around a paged cache: page tables, the 4-bit cache, rotary positions.  Argument checks and launches;
 // see include/tt_attn.h.
 #include "../../include/tt_attn.h"
 #include "common.h"
@@ -33,6 +33,17 @@ int table_args(const char* who, int32_t B, int32_t page_size, int32_t max_pages,
     if (B < 1 || page_size < 1 || max_pages < 1 || free_capacity < 0)
         return fail(TT_ERR_BAD_SHAPE, "%s: B=%d page_size=%d max_pages=%d must be >= 1, free_capacity=%d >= 0", who, B, page_size, max_pages, free_capacity);
     if (B > cache_max_requests()) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d, at most %d requests", who, B, cache_max_requests());
+    return TT_OK;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+int q4_args(const char* who, const void* k_cache, const void* v_cache, int32_t Hkv, int32_t D, int32_t n_pages, int32_t page_size) {
+    if (D != 64 && D != 128) return fail(TT_ERR_UNSUPPORTED, "%s: head dim 64 or 128 only, got %d", who, D);
+    if (page_size < 16 || page_size % 16) return fail(TT_ERR_BAD_SHAPE, "%s: page_size=%d must be a multiple of 16", who, page_size);
+    if (Hkv < 1 || n_pages < 0) return fail(TT_ERR_BAD_SHAPE, "%s: Hkv=%d n_pages=%d", who, Hkv, n_pages);
+    if ((int64_t)n_pages * page_size >= (1LL << 31)) return fail(TT_ERR_BAD_SHAPE, "%s: pages of %d x %d tokens, at most 2^31 - 1", who, n_pages, page_size);
+    if (n_pages && (!k_cache || !v_cache)) return fail(TT_ERR_NULL, "%s: null cache", who);
+    if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(TT_ERR_BAD_SHAPE, "%s: the cache must be 16-byte aligned", who);
     return TT_OK;
 }
 
@@ -111,6 +122,48 @@ int tt_cache_release(const int32_t* block_table, const int32_t* seq_lens, const 
     const cudaError_t e = cache_release(block_table, seq_lens, done, free_pages, n_free, B, page_size, max_pages, free_capacity, seq_lens_out, n_free_out,
                                         (cudaStream_t)stream);
     return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_release: launch");
+}
+
+size_t tt_cache_q4_page_bytes(int32_t page_size, int32_t D) {
+    if ((D != 64 && D != 128) || page_size < 16 || page_size % 16) return 0;
+    return (size_t)page_size * (D / 2 + D / 32);
+}
+
+int tt_cache_append_q4(const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype, const int64_t* k_stride,
+                       const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages, int32_t page_size, void* stream) {
+    const char* who = "tt_cache_append_q4";
+    int rc = q4_args(who, k_cache, v_cache, Hkv, D, n_pages, page_size);
+    if (rc != TT_OK) return rc;
+    if (dtype != TT_F32 && dtype != TT_BF16) return fail(TT_ERR_BAD_DTYPE, "%s: dtype %d unknown", who, dtype);
+    if (T < 0 || (int64_t)T * Hkv >= (1LL << 31)) return fail(TT_ERR_BAD_SHAPE, "%s: T=%d Hkv=%d", who, T, Hkv);
+    if (!k_stride || !v_stride) return fail(TT_ERR_NULL, "%s: null strides", who);
+    if (T && (!k || !v || !slots)) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    const size_t size = dtype == TT_BF16 ? 2 : 4;
+    if (((uintptr_t)k | (uintptr_t)v) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
+    const size_t pool = (size_t)n_pages * Hkv * tt_cache_q4_page_bytes(page_size, D);
+    if (overlap({k_cache, pool, ""}, {v_cache, pool, ""})) return fail(TT_ERR_BAD_SHAPE, "%s: k_cache overlaps v_cache", who);
+    if ((rc = check_device()) != TT_OK || T == 0 || n_pages == 0) return rc;
+    const CacheQ4 c{k_cache, v_cache, n_pages, page_size, Hkv, D};
+    const long long ks[2] = {k_stride[0], k_stride[1]}, vs[2] = {v_stride[0], v_stride[1]};
+    const cudaError_t e = cache_append_q4(c, k, v, ks, vs, dtype == TT_BF16, slots, T, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_append_q4: launch");
+}
+
+int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* cu_lens, int32_t B, int32_t Hkv, int32_t D,
+                     int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t total, void* k, void* v, void* stream) {
+    const char* who = "tt_cache_read_q4";
+    int rc = q4_args(who, k_cache, v_cache, Hkv, D, n_pages, page_size);
+    if (rc != TT_OK) return rc;
+    if (B < 1 || max_pages < 1 || total < 0 || (int64_t)total * Hkv >= (1LL << 31))
+        return fail(TT_ERR_BAD_SHAPE, "%s: B=%d max_pages=%d total=%d Hkv=%d", who, B, max_pages, total, Hkv);
+    if (!block_table || !cu_lens || (total && (!k || !v))) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    if (!aligned16(k) || !aligned16(v)) return fail(TT_ERR_BAD_SHAPE, "%s: k and v must be 16-byte aligned", who);
+    const size_t pool = (size_t)n_pages * Hkv * tt_cache_q4_page_bytes(page_size, D), n = (size_t)total * Hkv * D * 2;
+    const Span out[] = {{k, n, "k"}, {v, n, "v"}}, in[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}};
+    if ((rc = check_overlap(who, out, 2, in, 2)) != TT_OK || (rc = check_device()) != TT_OK || total == 0) return rc;
+    const CacheQ4 c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, Hkv, D};
+    const cudaError_t e = cache_read_q4(c, block_table, cu_lens, B, max_pages, total, k, v, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_read_q4: launch");
 }
 
 int tt_rotary(const tt_rotary_desc* d, const void* q, const void* k, const int32_t* positions, const double* inv_freq, const int32_t* axes, int32_t backward,

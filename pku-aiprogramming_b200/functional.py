@@ -242,6 +242,69 @@ def cache_release(block_table, seq_lens, done, free_pages, n_free, page_size, ou
         ("n_free", n_free, 1, (torch.int32,))], out, "B, 1"))
 
 
+def cache_alloc_q4(pages, kv_heads, page_size, head_dim, device="cuda"):
+    """(k_cache, v_cache) of a 4-bit key/value cache: zeroed bytes `[pages, kv_heads, page bytes]`, head dim 64 or 128, pages
+    of a multiple of 16 tokens.  4.25 bits a value: per 32 channels a scale of 8 bits and 4 bits each."""
+    n = int(capi.lib.tt_cache_q4_page_bytes(int(page_size), int(head_dim)))
+    if n == 0:
+        raise ValueError(f"page_size {page_size} must be a multiple of 16 and head_dim {head_dim} 64 or 128")
+    k = torch.zeros((int(pages), int(kv_heads), n), dtype=torch.uint8, device=device)
+    return k, torch.zeros_like(k)
+
+
+def _explain_q4_cache(k_cache, v_cache):
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 3 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous CUDA uint8 tensor [pages, kv_heads, page bytes], see cache_alloc_q4")
+    if k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
+        raise ValueError("k_cache and v_cache must have one shape and device")
+
+
+def _explain_append_q4(k, v, slots, k_cache, v_cache):
+    _explain_q4_cache(k_cache, v_cache)
+    for name, t in (("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dtype not in _DT or t.device != k_cache.device or t.dim() != 3 or t.stride(2) != 1:
+            raise ValueError(f"{name} must be a float32/bfloat16 tensor [T, kv_heads, D] on the cache's device, channels next to each other")
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k and v must have one shape and type")
+    if k.shape[1] != k_cache.shape[1]:
+        raise ValueError(f"k has {k.shape[1]} heads, the cache {k_cache.shape[1]}")
+    if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int32 or slots.device != k_cache.device or tuple(slots.shape) != (k.shape[0],) \
+            or not slots.is_contiguous():
+        raise ValueError(f"slots must be a contiguous int32 vector of {k.shape[0]} on the cache's device")
+    raise ValueError(f"pages of {k_cache.shape[2]} bytes are not a multiple of 16 tokens of head dim {k.shape[2]} (64 or 128)")
+
+
+def cache_append_q4(k, v, slots, k_cache, v_cache):
+    """New keys and values `[T, kv_heads, D]` (float32 or bfloat16, strided) into a 4-bit cache at `slots` (int32 `[T]`, as from
+    `cache_extend`; -1 is passed over, no slot may come twice) -> (k_cache, v_cache), written in place."""
+    r = _native.cache_append_q4(k, v, slots, k_cache, v_cache)
+    return r if r.__class__ is tuple else _done(r, _explain_append_q4, k, v, slots, k_cache, v_cache)
+
+
+def _explain_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size):
+    _explain_q4_cache(k_cache, v_cache)
+    dev = k_cache.device
+    if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or block_table.device != dev or block_table.dim() != 2 \
+            or not block_table.is_contiguous():
+        raise ValueError("block_table must be a contiguous int32 tensor [B, max_pages] on the cache's device")
+    n = block_table.shape[0] + 1
+    if not isinstance(cu_lens, torch.Tensor) or cu_lens.dtype != torch.int32 or cu_lens.device != dev or tuple(cu_lens.shape) != (n,) \
+            or not cu_lens.is_contiguous():
+        raise ValueError(f"cu_lens must be a contiguous int32 vector of {n} cumulative token counts on the cache's device")
+    if int(page_size) < 16 or int(page_size) % 16 or k_cache.shape[2] not in (34 * int(page_size), 68 * int(page_size)):
+        raise ValueError(f"pages of {k_cache.shape[2]} bytes are not {page_size} tokens (a multiple of 16) of head dim 64 or 128")
+    raise ValueError("total must be a 32-bit integer, k and v contiguous bfloat16 [total, kv_heads, D] on the cache's device")
+
+
+def cache_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size, k=None, v=None):
+    """The first `cu_lens[b+1] - cu_lens[b]` tokens of each sequence of a 4-bit cache as packed bfloat16 k, v `[total, kv_heads, D]`:
+    the keys of `attention_forward_varlen` with `cu_k = cu_lens`, for prompt tokens that follow what is cached.  Rows of given
+    `k`, `v` from `cu_lens[B]` on stay as they are."""
+    r = _native.cache_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size, k, v)
+    return r if r.__class__ is tuple else _done(r, _explain_read_q4, k_cache, v_cache, block_table, cu_lens, total, page_size)
+
+
 def rotary_frequencies(rotary_dim, base=10000.0, sections=None, cyclic=False, own_ladder=False, device="cuda"):
     """(inv_freq `[rotary_dim/2]` float64, axes int32 or None) of `rotary_forward`.
 

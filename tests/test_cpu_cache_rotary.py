@@ -136,3 +136,47 @@ def test_frequencies(tt):
     for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, sections=(1, 2)), dict(rotary_dim=8, sections=(5, -1)), dict(rotary_dim=8, base=0.0)):
         with pytest.raises(ValueError):
             tt.rotary_frequencies(**bad, device="cpu")
+
+
+def test_q4_cache_refuses_what_does_not_fit(tt):
+    lib, c = tt.capi.lib, tt.capi
+    raw, p = _buffers(10, 1 << 16)
+    k, v, slots, kc, vc, table, cu, ok, ov = p[:9]
+    st = (ctypes.c_int64 * 2)(128, 64)
+    assert [lib.tt_cache_q4_page_bytes(*a) for a in ((16, 64), (48, 128), (8, 64), (24, 64), (16, 96), (0, 64), (-16, 128))] == [16 * 34, 48 * 68, 0, 0, 0, 0, 0]
+
+    def append(k=k, v=v, slots=slots, T=4, hkv=2, D=64, dtype=0, ks=st, vs=st, kc=kc, vc=vc, pages=3, page=16):
+        return lib.tt_cache_append_q4(k, v, slots, T, hkv, D, dtype, ks, vs, kc, vc, pages, page, None)
+
+    assert append(D=96) == c.TT_ERR_UNSUPPORTED and append(dtype=7) == c.TT_ERR_BAD_DTYPE
+    for kw in (dict(page=8), dict(page=24), dict(page=0), dict(hkv=0), dict(pages=-1), dict(pages=1 << 27, page=16), dict(T=-1), dict(T=1 << 30, hkv=2), dict(kc=_at(kc, 8)), dict(vc=_at(vc, 4)),
+               dict(vc=kc), dict(vc=_at(kc, 16 * 34 * 2)), dict(k=_at(k, 2)), dict(k=_at(k, 1), dtype=1)):
+        assert append(**kw) == c.TT_ERR_BAD_SHAPE, kw
+    for kw in (dict(k=None), dict(v=None), dict(slots=None), dict(kc=None), dict(vc=None), dict(ks=None), dict(vs=None)):
+        assert append(**kw) == c.TT_ERR_NULL, kw
+
+    def read(kc=kc, vc=vc, table=table, cu=cu, B=2, hkv=2, D=64, pages=3, page=16, max_pages=4, total=40, k=ok, v=ov):
+        return lib.tt_cache_read_q4(kc, vc, table, cu, B, hkv, D, pages, page, max_pages, total, k, v, None)
+
+    assert read(D=32) == c.TT_ERR_UNSUPPORTED
+    for kw in (dict(B=0), dict(max_pages=0), dict(total=-1), dict(total=1 << 30), dict(page=12), dict(hkv=0), dict(k=_at(ok, 2)), dict(v=ok), dict(k=kc), dict(v=_at(vc, 3200)), dict(kc=_at(kc, 1))):
+        assert read(**kw) == c.TT_ERR_BAD_SHAPE, kw
+    for kw in (dict(table=None), dict(cu=None), dict(k=None), dict(v=None), dict(kc=None)):
+        assert read(**kw) == c.TT_ERR_NULL, kw
+    if not torch.cuda.is_available():
+        assert append() == c.TT_ERR_BAD_DEVICE and read() == c.TT_ERR_BAD_DEVICE
+    del raw
+
+
+def test_q4_format():
+    """Every code's scale, the smallest scale that reaches a value, and errors of half a step."""
+    import numpy as np
+    import q4_oracle as q4
+    s = q4.scales(np.arange(q4.TOP + 1))
+    assert s[0] == 0 and s[1] == 2.0 ** -20 and s[8] == 2.0 ** -17 and s[q4.TOP] == 896.0 and (np.diff(s) > 0).all() and np.isnan(q4.scales(q4.NAN))
+    x = np.random.default_rng(0).standard_normal((50, 2, 64)) * np.logspace(-4, 3, 50)[:, None, None]
+    nib, codes = q4.encode(x)
+    step = np.repeat(q4.scales(codes), 32, -1)
+    assert (np.abs(q4.decode(nib, codes) - x) <= step / 2 * (1 + 1e-12)).all()
+    top = np.abs(x.reshape(50, 2, 2, 32)).max(-1)
+    assert (7.5 * q4.scales(codes) >= top).all() and (7.5 * q4.scales(codes - 1) < top).all()
