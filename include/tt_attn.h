@@ -252,6 +252,19 @@ int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* bl
                      int32_t Hkv, int32_t D, int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t total, void* k, void* v,
                      void* stream);
 
+/* Decode over a 4-bit cache: tt_attn_decode_paged with q and out bf16 [B, H, 1, D] and the cache as above.
+ *   block_table    [B, max_pages]; key r of batch entry b is row r % page_size of page block_table[b, r / page_size].  Keys of a
+ *                  page that is not one of the n_pages, or of a column behind max_pages, count as absent.
+ *                  NULL: batch entry b has page b to itself (page_size >= desc->L, n_pages >= B).
+ *   seq_lens       [B] or NULL (desc->L each), clamped to 0 .. desc->L; an entry without keys gets out = 0, lse = -inf
+ * desc: dtype TT_BF16, S = 1, D 64 or 128, L the longest sequence there may be, at most 2^30; any group H / Hkv.  `lse` may be NULL.
+ * Products are exact in what the cache holds; probabilities are rounded to 11 bits, sums are 32-bit.  Results repeat to the bit.
+ * Workspace: tt_attn_decode_q4_workspace_bytes(desc) bytes, 256-byte aligned, contents ignored. */
+size_t tt_attn_decode_q4_workspace_bytes(const tt_attn_desc* desc);
+int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                      const int32_t* seq_lens, int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- rotary positions ------------------------------------------------------------------------
  * Query and key heads turned by their tokens' positions (no counterpart in the reference).  Of a head's D channels the first
  * R form R / 2 pairs; pair i of a token at position p on axis a = axes[i] turns by p * inv_freq[i]:

@@ -64,6 +64,8 @@ SIGNATURES = {
     "tt_cache_q4_page_bytes": (c_size_t, [c_int32, c_int32]),
     "tt_cache_append_q4": (c_int, [_P, _P, _P, c_int32, c_int32, c_int32, c_int32, POINTER(c_int64), POINTER(c_int64), _P, _P, c_int32, c_int32, _P]),
     "tt_cache_read_q4": (c_int, [_P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P, _P]),
+    "tt_attn_decode_q4_workspace_bytes": (c_size_t, [_DP]),
+    "tt_attn_decode_q4": (c_int, [_DP, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, _P, _P, _P, c_size_t, _P]),
     "tt_rotary": (c_int, [POINTER(RotaryDesc), _P, _P, _P, _P, _P, c_int32, _P, _P, _P]),
     "tt_softmax_fwd": (c_int, [_P, _P, c_int64, c_int32, c_int32, _P]),
     "tt_softmax_bwd": (c_int, [_P, _P, _P, c_int64, c_int32, c_int32, _P]),

@@ -145,7 +145,7 @@ enum KernelId {
     K_FWD_TC = 0, K_FWD_SIMT, K_BWD_PREP, K_BWD_DKV, K_BWD_DQ, K_BWD_SIMT_DELTA, K_BWD_SIMT_DQ, K_BWD_SIMT_DKV,
     K_DECODE, K_DECODE_MERGE, K_PROBE, K_SOFTMAX_FWD, K_SOFTMAX_BWD, K_FC_GEMM, K_FC_SIMT, K_FC_COLSUM, K_BWD_FUSED,
     K_BWD_DQ_CONVERT, K_DECODE_GQ, K_FWD_F32, K_BWD_F32, K_BWD_BOTH, K_CACHE_TABLES,
-    K_ROTARY, K_CACHE_APPEND, K_CACHE_READ, K_COUNT
+    K_ROTARY, K_CACHE_APPEND, K_CACHE_READ, K_DECODE_Q4, K_COUNT
 };
 // Scoped around ONE kernel launch: counts it and, when timing is enabled, brackets it with
 // CUDA events on the launching stream.
@@ -280,6 +280,12 @@ struct CacheQ4 {
 cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, const long long (&ks)[2], const long long (&vs)[2], int bf16, const int* slots,
                             int T, cudaStream_t st);
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st);
+
+// Decode over it (attn_decode_q4.cu): block_table null: one page per batch entry.
+size_t attn_decode_q4_workspace(const AttnArgs& a);
+cudaError_t attn_decode_q4(const AttnArgs& a, const CacheQ4& c, const int* block_table, const int* seq_lens, int max_pages, void* workspace, cudaStream_t st);
+// Merge of normalised results [slice, splits, group, D] and their log-sum-exps (attn_decode.cu).
+cudaError_t attn_decode_merge(const AttnArgs& a, const float* po, const float* plse, int splits, cudaStream_t st);
 
 // --- rotary positions (rotary.cu)
 struct RotaryArgs {

@@ -698,12 +698,58 @@ PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// (q, k_cache, v_cache, block_table, seq_lens, max_len, scale, out, lse, workspace, need_lse) -> (out, lse)
+PyObject* attention_decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Tensor *kc, *vc;
+        if (n != 11 || !q4_cache(a[1], a[2], &kc, &vc)) Py_RETURN_NONE;
+        const Tensor* q = on_device(a[0], at::kBFloat16, kc);
+        if (!q || !q->is_contiguous() || q->dim() != 4 || q->size(2) != 1) Py_RETURN_NONE;
+        const int64_t B = q->size(0), H = q->size(1), D = q->size(3), hkv = kc->size(1), page = q4_page_size(kc->size(2), D);
+        if (hkv < 1 || H % hkv != 0 || page == 0 || !fits32(B) || !fits32(H)) Py_RETURN_NONE;
+        const Tensor *table = nullptr, *lens = nullptr;
+        int64_t max_pages = 0, L = page;
+        if (a[3] != Py_None) {
+            table = on_device(a[3], at::kInt, kc);
+            if (!table || !table->is_contiguous() || table->dim() != 2 || table->size(0) != B || !fits32(table->size(1))) Py_RETURN_NONE;
+            max_pages = table->size(1);
+            L = page * max_pages;
+        } else if (kc->size(0) != B) {
+            Py_RETURN_NONE;
+        }
+        if (a[4] != Py_None && !(lens = vector_arg(a[4], at::kInt, B, kc))) Py_RETURN_NONE;
+        const int64_t most = L;
+        if (a[5] != Py_None && !int_arg(a[5], &L)) return nullptr;
+        if (L > most || !fits32(L)) Py_RETURN_NONE;
+        const int need_lse = PyObject_IsTrue(a[10]);
+        tt_attn_desc d{(int32_t)B, (int32_t)H, 1, (int32_t)L, (int32_t)D, TT_BF16, 0, 0.f, (int32_t)hkv};
+        if (need_lse < 0 || !scale_arg(a[6], &d.scale)) return nullptr;
+        const Tensor *out = nullptr, *lse = nullptr, *ws = nullptr;
+        if (a[7] != Py_None && (!(out = on_device(a[7], at::kBFloat16, q)) || !out->is_contiguous() || !same_shape(*out, *q))) Py_RETURN_NONE;
+        if (a[8] != Py_None && (!(lse = on_device(a[8], at::kFloat, q)) || !lse->is_contiguous() || lse->dim() != 3 || lse->size(0) != B || lse->size(1) != H || lse->size(2) != 1))
+            Py_RETURN_NONE;
+        if (a[9] != Py_None && (!THPVariable_Check(a[9]) || !(ws = &THPVariable_Unpack(a[9]))->is_contiguous() || ws->device() != q->device())) Py_RETURN_NONE;
+        OnDevice dev(*q);
+        Tensor new_out, new_lse, made;
+        if (!out) new_out = make_like(*q);
+        if (!lse && need_lse) new_lse = make({B, H, 1}, at::kFloat, *q);
+        size_t bytes;
+        ws = workspace_arg(ws, tt_attn_decode_q4_workspace_bytes(&d), 0, *q, &made, &bytes);
+        TT_CALL(rc, tt_attn_decode_q4(&d, ptr(q), ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(lens), (int32_t)kc->size(0), (int32_t)page,
+                                      (int32_t)max_pages, out ? ptr(out) : ptr(new_out),
+                                      (float*)(lse ? ptr(lse) : new_lse.defined() ? ptr(new_lse) : nullptr), ptr(ws), bytes, dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(wrap_or(a[7], new_out), wrap_or(a[8], new_lse));
+    });
+}
+
 #define TT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     TT_METHOD(attention_forward), TT_METHOD(attention_backward), TT_METHOD(attention_forward_varlen),
     TT_METHOD(attention_backward_varlen), TT_METHOD(attention_decode), TT_METHOD(attention_decode_paged),
     TT_METHOD(softmax_forward), TT_METHOD(softmax_backward), TT_METHOD(fc_forward), TT_METHOD(fc_backward), TT_METHOD(cache_extend), TT_METHOD(cache_release),
     TT_METHOD(rotary), TT_METHOD(cache_append_q4), TT_METHOD(cache_read_q4),
+    TT_METHOD(attention_decode_q4),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ttorch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -42,7 +42,7 @@ static const char* const kKernelNames[K_COUNT] = {
     "attn_bwd_simt_delta", "attn_bwd_simt_dq", "attn_bwd_simt_dkv", "attn_decode", "attn_decode_merge",
     "umma_probe", "softmax_rows_fwd", "softmax_rows_bwd", "fc_gemm_sm100", "fc_gemm_simt",
     "fc_colsum", "attn_bwd_fused_sm100", "attn_bwd_dq_convert", "attn_decode_gq_sm100", "attn_fwd_f32_sm100", "attn_bwd_f32_sm100", "attn_bwd_sm100_both", "cache_tables",
-    "rotary", "cache_append_q4", "cache_read_q4"};
+    "rotary", "cache_append_q4", "cache_read_q4", "attn_decode_q4"};
 struct TimedLaunch {
     KernelId id;
     cudaEvent_t start, stop;

@@ -7,6 +7,7 @@
 #include <cstdlib>
 
 namespace ttk {
+int resolve(const tt_attn_desc* d, AttnArgs* a, const char* who);   // tt_api.cu
 namespace {
 
 struct Span {
@@ -164,6 +165,45 @@ int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* bl
     const CacheQ4 c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, Hkv, D};
     const cudaError_t e = cache_read_q4(c, block_table, cu_lens, B, max_pages, total, k, v, (cudaStream_t)stream);
     return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_read_q4: launch");
+}
+
+static int resolve_q4(const char* who, const tt_attn_desc* desc, AttnArgs* a) {
+    const int rc = resolve(desc, a, who);
+    if (rc != TT_OK) return rc;
+    if (a->S != 1) return fail(TT_ERR_BAD_SHAPE, "%s: S must be 1, got %d", who, a->S);
+    if (!a->bf16 || (a->D != 64 && a->D != 128)) return fail(TT_ERR_BAD_DTYPE, "%s: bf16 with D = 64 or 128 only (dtype %d, D %d)", who, desc->dtype, a->D);
+    if (a->L > (1 << 30)) return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds 2^30", who, a->L);
+    a->causal = 0;
+    return TT_OK;
+}
+size_t tt_attn_decode_q4_workspace_bytes(const tt_attn_desc* desc) {
+    AttnArgs a;
+    return resolve_q4("tt_attn_decode_q4_workspace_bytes", desc, &a) == TT_OK ? attn_decode_q4_workspace(a) : 0;
+}
+int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* seq_lens,
+                      int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "tt_attn_decode_q4";
+    AttnArgs a;
+    int rc = resolve_q4(who, desc, &a);
+    if (rc != TT_OK) return rc;
+    const int hkv = desc->H / a.group;
+    if ((rc = q4_args(who, k_cache, v_cache, hkv, a.D, n_pages, page_size)) != TT_OK) return rc;
+    if (!q || !out) return fail(TT_ERR_NULL, "%s: q and out must be non-null", who);
+    if (!aligned16(q) || !aligned16(out)) return fail(TT_ERR_BAD_SHAPE, "%s: q and out must be 16-byte aligned", who);
+    if (block_table) {
+        if (max_pages < 1 || (int64_t)page_size * max_pages < a.L)
+            return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds page_size*max_pages=%lld", who, a.L, (long long)page_size * max_pages);
+    } else if (page_size < a.L || n_pages < desc->B) {
+        return fail(TT_ERR_BAD_SHAPE, "%s: without a block table page_size=%d must hold L=%d and n_pages=%d the batch of %d", who, page_size, a.L, n_pages, desc->B);
+    }
+    const size_t need = attn_decode_q4_workspace(a);
+    if (need && (!workspace || workspace_bytes < need)) return fail(TT_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, workspace_bytes);
+    if (need && ((uintptr_t)workspace & 255)) return fail(TT_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+    if ((rc = check_device()) != TT_OK) return rc;
+    a.q = q; a.out = out; a.lse = lse;
+    const CacheQ4 c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, hkv, a.D};
+    const cudaError_t e = attn_decode_q4(a, c, block_table, seq_lens, max_pages, workspace, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_attn_decode_q4: launch");
 }
 
 int tt_rotary(const tt_rotary_desc* d, const void* q, const void* k, const int32_t* positions, const double* inv_freq, const int32_t* axes, int32_t backward,

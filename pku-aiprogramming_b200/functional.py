@@ -305,6 +305,45 @@ def cache_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size, k=No
     return r if r.__class__ is tuple else _done(r, _explain_read_q4, k_cache, v_cache, block_table, cu_lens, total, page_size)
 
 
+def _explain_decode_q4(q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse):
+    _explain_q4_cache(k_cache, v_cache)
+    dev = k_cache.device
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[2] != 1 or q.dtype != torch.bfloat16 or q.device != dev or not q.is_contiguous():
+        raise ValueError("q must be a contiguous bfloat16 tensor [B,H,1,D] on the cache's device")
+    B, H, _, D = q.shape
+    Hkv = k_cache.shape[1]
+    if Hkv < 1 or H % Hkv != 0:
+        raise ValueError(f"key/value heads {Hkv} must divide query heads {H}")
+    row = D // 2 + D // 32
+    if D not in (64, 128) or k_cache.shape[2] == 0 or k_cache.shape[2] % (16 * row) != 0:
+        raise ValueError(f"pages of {k_cache.shape[2]} bytes are not a multiple of 16 tokens of head dim {D} (64 or 128)")
+    for name, t, shape in (("block_table", block_table, None), ("seq_lens", seq_lens, (B,))):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous()
+                              or (shape is not None and tuple(t.shape) != shape)):
+            raise ValueError(f"{name} must be a contiguous int32 tensor on the cache's device" + (f" of shape {shape}" if shape else ""))
+    if block_table is not None and (block_table.dim() != 2 or block_table.shape[0] != B):
+        raise ValueError("block_table must be [B, max_pages]")
+    if block_table is None and k_cache.shape[0] != B:
+        raise ValueError("a cache without a block table must have one page per batch entry")
+    longest = k_cache.shape[2] // row * (1 if block_table is None else block_table.shape[1])
+    if max_len is not None and int(max_len) > longest:
+        raise ValueError(f"max_len exceeds the {longest} keys that a sequence may have")
+    for name, t, shape, dtype in (("out", out, q.shape, torch.bfloat16), ("lse", lse, (B, H, 1), torch.float32)):
+        if t is not None and (not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on the cache's device")
+    raise ValueError("workspace must be a contiguous tensor on the cache's device, and lengths 32-bit integers")
+
+
+def attention_decode_q4(q, k_cache, v_cache, block_table=None, seq_lens=None, max_len=None, scale=None, out=None, lse=None, workspace=None, need_lse=True):
+    """Single-query attention over a 4-bit cache (see `cache_alloc_q4`) -> (out, lse), as `attention_decode_paged` over a 16-bit one.
+
+    q `[B,H,1,D]` bfloat16, D 64 or 128.  `block_table` (int32 `[B, max_pages]`) names each sequence's pages; None: batch entry b has
+    page b to itself.  `seq_lens` (int32 `[B]`): keys of each sequence.  `max_len`: longest possible sequence (default: what the pages
+    can hold), which decides how the keys are divided.  An empty sequence gives out = 0, lse = -inf."""
+    r = _native.attention_decode_q4(q, k_cache, v_cache, block_table, seq_lens, max_len, scale, out, lse, workspace, need_lse)
+    return r if r.__class__ is tuple else _done(r, _explain_decode_q4, q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse)
+
+
 def rotary_frequencies(rotary_dim, base=10000.0, sections=None, cyclic=False, own_ladder=False, device="cuda"):
     """(inv_freq `[rotary_dim/2]` float64, axes int32 or None) of `rotary_forward`.
 

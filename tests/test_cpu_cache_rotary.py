@@ -180,3 +180,32 @@ def test_q4_format():
     assert (np.abs(q4.decode(nib, codes) - x) <= step / 2 * (1 + 1e-12)).all()
     top = np.abs(x.reshape(50, 2, 2, 32)).max(-1)
     assert (7.5 * q4.scales(codes) >= top).all() and (7.5 * q4.scales(codes - 1) < top).all()
+
+
+def test_q4_decode_refuses_what_does_not_fit(tt):
+    lib, c = tt.capi.lib, tt.capi
+    raw, p = _buffers(10, 1 << 16)
+    q, kc, vc, table, lens, out, ws = p[:7]
+
+    def call(q=q, kc=kc, vc=vc, table=table, pages=9, page=16, max_pages=4, out=out, ws=ws, ws_bytes=1 << 16, desc=None, **kw):
+        a = dict(B=2, H=4, S=1, L=50, D=64, dtype=c.TT_BF16, Hkv=2)
+        a.update(kw)
+        d = c.make_desc(a["B"], a["H"], a["S"], a["L"], a["D"], a["dtype"], False, a.get("scale"), Hkv=a["Hkv"])
+        return lib.tt_attn_decode_q4(ctypes.byref(d), q, kc, vc, table, lens, pages, page, max_pages, out, None, ws, ws_bytes, None)
+
+    for kw in (dict(S=2), dict(L=0), dict(L=65), dict(L=(1 << 30) + 1, max_pages=1 << 27), dict(H=3), dict(B=0), dict(page=8, max_pages=8), dict(page=24), dict(max_pages=3), dict(pages=-1),
+               dict(q=_at(q, 2)), dict(out=_at(out, 8)), dict(kc=_at(kc, 8)), dict(table=None, page=48), dict(table=None, page=64, pages=1), dict(scale=math.inf)):
+        assert call(**kw) == c.TT_ERR_BAD_SHAPE, kw
+    for kw in (dict(D=96), dict(dtype=c.TT_F32)):
+        assert call(**kw) == c.TT_ERR_BAD_DTYPE, kw
+    for kw in (dict(q=None), dict(out=None), dict(kc=None), dict(vc=None)):
+        assert call(**kw) == c.TT_ERR_NULL, kw
+    assert lib.tt_attn_decode_q4(None, q, kc, vc, table, lens, 9, 16, 4, out, None, ws, 1 << 16, None) == c.TT_ERR_NULL
+    long = dict(L=5000, max_pages=313, pages=700)
+    d = c.make_desc(2, 4, 1, 5000, 64, c.TT_BF16, False, None, Hkv=2)
+    need = lib.tt_attn_decode_q4_workspace_bytes(ctypes.byref(d))
+    assert need > 0
+    assert call(**long, ws=None) == c.TT_ERR_WORKSPACE and call(**long, ws_bytes=need - 1) == c.TT_ERR_WORKSPACE and call(**long, ws=_at(ws, 64), ws_bytes=need) == c.TT_ERR_WORKSPACE
+    if not torch.cuda.is_available():
+        assert call() == c.TT_ERR_BAD_DEVICE
+    del raw
