@@ -32,7 +32,7 @@ using namespace sm100;
 namespace {
 
 constexpr int kWarps = 4, kTile = 32, kDepth = 3;   // a step of a warp: 32 keys, two accumulator tiles of 16
-constexpr float kSlack = 5.f, kLift = 10.f;
+constexpr float kSlack = 5.f, kLift = 10.f, kNone = -3e38f;   // (kNone: no score yet; above every finite one that counts as such)
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -48,15 +48,16 @@ __device__ __forceinline__ void copy16(uint32_t saddr, const void* p, bool some)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr), "l"(p), "r"(some ? 16 : 0) : "memory");
 }
 template <int N>
-__device__ __forceinline__ void lds(uint32_t (&w)[N], uint32_t saddr) {
-    if (N == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1 % N]), "=r"(w[2 % N]), "=r"(w[3 % N]) : "r"(saddr) : "memory");
-    else if (N == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1 % N]) : "r"(saddr) : "memory");
-    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(saddr) : "memory");
-}
-__device__ __forceinline__ uint32_t lds_byte(uint32_t saddr) {
-    uint32_t x;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(saddr) : "memory");
-    return x;
+__device__ __forceinline__ void lds(uint32_t (&w)[N], const unsigned char* p) {
+    if (N == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[0] = x.x; w[1 % N] = x.y; w[2 % N] = x.z; w[3 % N] = x.w;
+    } else if (N == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[0] = x.x; w[1 % N] = x.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
 }
 __device__ __forceinline__ half2 as_half2(uint32_t x) { return *reinterpret_cast<half2*>(&x); }
 __device__ __forceinline__ uint32_t bits(half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
@@ -139,25 +140,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
     const int k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
     const long long row0 = (long long)slice * a.group + h0;   // the tile's first query head
 
-    // 16 keys lie in one page.  Lane i looks up the page of the i-th 16 keys of a batch; the page -1 has no keys.
+    // 16 keys lie in one page.  Lane i looks up where the i-th 16 keys of a batch are: the byte of their first row, or -1, and their row in
+    // the page.
     const int n_sub = k1 > k0 ? ((k1 - k0 + kTile - 1) / kTile + kWarps - 1 - warp) / kWarps * 2 : 0;   // this warp's 16-key tiles
     auto first_key = [&](int sub) { return k0 + ((sub >> 1) * kWarps + warp) * kTile + (sub & 1) * 16; };
-    auto look_up = [&](int sub, int& page, int& row) {
+    long long at_now;
+    int row_now;
+    auto look_up = [&](int sub) {
         const int key = first_key(sub);
-        page = -1;
-        row = 0;
+        at_now = -1;
+        row_now = 0;
         if (sub < n_sub && key < k1) {
             const int col = key / a.page;
-            row = key - col * a.page;
-            if (a.table) page = col < a.max_pages ? __ldg(a.table + (long long)b * a.max_pages + col) : -1;
-            else page = b;
-            if (page >= a.n_pages) page = -1;
+            const int page = !a.table ? b : col < a.max_pages ? __ldg(a.table + (long long)b * a.max_pages + col) : -1;
+            if (page >= 0 && page < a.n_pages) {
+                row_now = key - col * a.page;
+                at_now = ((long long)page * a.hkv + hk) * ((long long)a.page * q4_row_bytes(D)) + row_now * (D / 2);
+            }
         }
     };
-    const long long page_bytes = (long long)a.page * q4_row_bytes(D);
-    const int codes_at = a.page * (D / 2);
-    int page_now, row_now;   // of the batch that holds the tiles being loaded
-    look_up(lane, page_now, row_now);
+    look_up(lane);
     // Pieces of a slot are numbered [K rows][V rows]; a lane copies every 32nd, and the first lanes the codes.
     constexpr int kCopies = 16 * S::kPieces / 32, kCodes = D / 32;   // per tensor; 16-byte pieces of codes
     uint32_t to_k[kCopies], to_v[kCopies];
@@ -167,32 +169,34 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
         to_k[i] = S::k_at(piece / S::kPieces, piece % S::kPieces);
         to_v[i] = S::v_at(piece / S::kPieces, piece % S::kPieces);
     }
-    unsigned there = 0;   // bit j of step i: slot 2 (i % kDepth) + j has keys
-    auto fetch = [&](int sub) {   // both tiles of a step
+    const unsigned char *from_k = a.kc + lane * 16, *from_v = a.vc + lane * 16;
+    const unsigned char* from_codes = (lane < kCodes ? a.kc : a.vc) + a.page * (D / 2) + lane % kCodes * 16;
+    // Both tiles of a step into the slots at `slot`: bits of those that have keys.
+    auto fetch = [&](int sub, uint32_t slot) -> unsigned {
+        unsigned has = 0;
         if (sub < n_sub) {
-            if ((sub & 31) == 0 && sub > 0) look_up(sub + lane, page_now, row_now);
-            const int at_slot = sub % (2 * kDepth);
+            if ((sub & 31) == 0 && sub > 0) look_up(sub + lane);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int page = __shfl_sync(0xffffffffu, page_now, (sub + j) & 31), row = __shfl_sync(0xffffffffu, row_now, (sub + j) & 31);
-                const bool some = page >= 0;
-                const long long at = some ? ((long long)page * a.hkv + hk) * page_bytes : 0;
-                const unsigned char *kp = a.kc + at, *vp = a.vc + at;
-                const uint32_t slot = ring + (at_slot + j) * S::kBytes;
+                const long long at = __shfl_sync(0xffffffffu, at_now, (sub + j) & 31);
+                const int row = __shfl_sync(0xffffffffu, row_now, (sub + j) & 31);
+                const bool some = at >= 0;
+                const uint32_t to = slot + j * S::kBytes;
 #pragma unroll
                 for (int i = 0; i < kCopies; ++i) {
-                    copy16(slot + to_k[i], kp + row * (D / 2) + (lane + 32 * i) * 16, some);
-                    copy16(slot + to_v[i], vp + row * (D / 2) + (lane + 32 * i) * 16, some);
+                    copy16(to + to_k[i], from_k + at + 512 * i, some);
+                    copy16(to + to_v[i], from_v + at + 512 * i, some);
                 }
-                if (lane < 2 * kCodes)
-                    copy16(slot + S::kKc + lane * 16, (lane < kCodes ? kp : vp) + codes_at + row * (D / 32) + lane % kCodes * 16, some);
-                there = (there & ~(1u << (at_slot + j))) | (some ? 1u << (at_slot + j) : 0u);
+                if (lane < 2 * kCodes) copy16(to + S::kKc + lane * 16, from_codes + at - row * (D / 2 - D / 32), some);
+                has |= some ? 1u << j : 0u;
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        return has;
     };
+    unsigned has[kDepth];   // of the step at hand and those on their way
 #pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) fetch(2 * i);
+    for (int i = 0; i < kDepth - 1; ++i) has[i] = fetch(2 * i, ring + i * 2 * S::kBytes);
 
     // query heads as the B operand: lane (g, t) has head g's quarter t of the channels, pairs (i, i + 4) of eight
     uint32_t qf[NT][kG][4];
@@ -227,14 +231,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
         for (int j = 0; j < 2; ++j) to_log2[n][j] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
     }
 
-    float o[kMT][NT][4], m[NT][2], l[NT][2];
+    float o[kMT][NT][4], m[NT][2], l[NT][2];   // m: what a score is taken less; 2^-kLift of the reference
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int i = 0; i < kMT; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
-        m[n][0] = m[n][1] = -INFINITY;
+        m[n][0] = m[n][1] = kNone;
         l[n][0] = l[n][1] = 0.f;
     }
     // where this lane reads in a slot
@@ -242,23 +246,27 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_from[i] = S::v_at(2 * t + (i & 1) + (i >> 1) * 8, g * (D / 16) / 16) + g * (D / 16) % 16;
 
+    uint32_t at_slot = 0, free_slot = (kDepth - 1) * 2 * S::kBytes;   // of the step at hand, and of the one before it
     for (int sub = 0; sub < n_sub; sub += 2) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
         __syncwarp();
-        const int at_slot = sub % (2 * kDepth);
-        const uint32_t slot = ring + at_slot * S::kBytes;
-        const unsigned here = there >> at_slot & 3;
-        fetch(sub + 2 * (kDepth - 1));   // into the slots of the step before, which every lane has left
+        const unsigned char* slot = smem + warp * (kDepth * 2 * S::kBytes) + at_slot;
+        const unsigned here = has[0];
+#pragma unroll
+        for (int i = 0; i + 1 < kDepth; ++i) has[i] = has[i + 1];
+        has[kDepth - 2] = fetch(sub + 2 * (kDepth - 1), ring + free_slot);   // every lane has left that slot
+        free_slot = at_slot;
+        at_slot = at_slot == (kDepth - 1) * 2 * S::kBytes ? 0 : at_slot + 2 * S::kBytes;
         // scores
         float s[2][NT][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const uint32_t from = slot + u * S::kBytes;
+            const unsigned char* from = slot + u * S::kBytes;
             uint32_t x[2][kG];
 #pragma unroll
             for (int r = 0; r < 2; ++r) lds(x[r], from + (g + 8 * r) * (D / 2) + t * (D / 8));
-            const Scale2 lo(lds_byte(from + S::kKc + g * (D / 32) + t * (D / 32) / 4) * 0x00800080u),
-                hi(lds_byte(from + S::kKc + (g + 8) * (D / 32) + t * (D / 32) / 4) * 0x00800080u);
+            const Scale2 lo(from[S::kKc + g * (D / 32) + t * (D / 32) / 4] * 0x00800080u),
+                hi(from[S::kKc + (g + 8) * (D / 32) + t * (D / 32) / 4] * 0x00800080u);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -311,7 +319,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 top[n][j] = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2])) * to_log2[n][j];
-                raise = raise || top[n][j] > m[n][j] + kSlack;
+                raise = raise || top[n][j] > m[n][j] + (kLift + kSlack);
             }
         }
         if (__any_sync(0xffffffffu, raise)) {
@@ -322,7 +330,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
                     float x = top[n][j];
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    const float to = fmaxf(m[n][j], x), f = m[n][j] == to ? 1.f : ex2_approx(m[n][j] - to);
+                    const float to = fmaxf(m[n][j], x - kLift), f = ex2_approx(m[n][j] - to);
                     m[n][j] = to;
                     l[n][j] *= f;
 #pragma unroll
@@ -337,12 +345,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
         uint32_t p[2][NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0] - kLift, m1 = m[n][1] == -INFINITY ? 0.f : m[n][1] - kLift;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float x = ex2_approx(fmaf(s[u][n][2 * i], to_log2[n][0], -m0)), y = ex2_approx(fmaf(s[u][n][2 * i + 1], to_log2[n][1], -m1));
+                    const float x = ex2_approx(fmaf(s[u][n][2 * i], to_log2[n][0], -m[n][0])), y = ex2_approx(fmaf(s[u][n][2 * i + 1], to_log2[n][1], -m[n][1]));
                     l[n][0] += x;
                     l[n][1] += y;
                     p[u][n][i] = transposed8x8(bits(__floats2half2_rn(x, y)));
@@ -411,7 +418,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float mw = sm_m[w * kHeads + h], lw = sm_l[w * kHeads + h];
-            if (mw == -INFINITY && lw == 0.f) continue;   // no keys
+            if (lw == 0.f) continue;   // no keys
             const float f = mw == top ? 1.f : ex2_approx(mw - top);
             den = fmaf(f, lw, den);
             const float4 y = *reinterpret_cast<const float4*>(sm_o + (w * kHeads + h) * (D + 4) + c);
@@ -419,7 +426,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
             x[2] = fmaf(f, y.z, x[2]); x[3] = fmaf(f, y.w, x[3]);
         }
         const float inv = den == 0.f ? 0.f : 1.f / den;
-        const float lse = den == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : (top - kLift) * 0.69314718056f) + logf(den);
+        const float lse = den == 0.f ? -INFINITY : top * 0.69314718056f + logf(den);
         if (a.splits == 1) {
             const __nv_bfloat162 y[2] = {__floats2bfloat162_rn(x[0] * inv, x[1] * inv), __floats2bfloat162_rn(x[2] * inv, x[3] * inv)};
             *reinterpret_cast<uint2*>(a.out + (row0 + h) * D + c) = *reinterpret_cast<const uint2*>(y);
