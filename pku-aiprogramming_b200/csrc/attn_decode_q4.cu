@@ -21,8 +21,11 @@
 // 2^kLift higher, up to 2^15: rounded to half it is off by 2^-11 of itself (bf16: 2^-8) down to 2^-24 of the row's largest, and by
 // 2^-35 of that below.  Accumulators are 32-bit.
 //
-// A warp takes every fourth 32 keys of its CTA's range through a ring of its own in shared memory (cp.async, kDepth steps of 32 keys; no
-// barrier between warps until the end); four warps and then the ranges are merged.
+// All slices' keys, in steps of 32, make one sequence that is cut into equal parts, one for each warp on the GPU whatever the lengths are
+// (a launch with a CTA per range of one slice ended on its last wave: 64 sequences of 4096 to 8192 106 us).  A warp sums the lengths,
+// finds its part, and streams it through a ring of its own in shared memory (cp.async, kDepth steps ahead, into the next slice's
+// keys where one ends); no warp waits for another.  A slice that one warp has to itself is written at once; of others each warp leaves
+// a normalised result and its log-sum-exp, which a second kernel merges.  Results do not depend on timing.
 #include "cache_q4.cuh"
 #include "sm100_ptx.cuh"
 
@@ -31,7 +34,16 @@ using namespace sm100;
 
 namespace {
 
-constexpr int kWarps = 4, kTile = 32, kDepth = 3;   // a step of a warp: 32 keys, two accumulator tiles of 16
+#ifndef Q4_DEPTH
+#define Q4_DEPTH 3
+#endif
+#ifndef Q4_CTAS
+#define Q4_CTAS 3
+#endif
+#ifndef Q4_LEAST
+#define Q4_LEAST 2
+#endif
+constexpr int kWarps = 4, kTile = 32, kDepth = Q4_DEPTH;   // a step of a warp: 32 keys, two accumulator tiles of 16
 constexpr float kSlack = 5.f, kLift = 10.f, kNone = -3e38f;   // (kNone: no score yet; above every finite one that counts as such)
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -110,52 +122,132 @@ struct DecodeQ4Args {
     const __nv_bfloat16* q;
     const unsigned char *kc, *vc;
     const int *table, *lens;
-    int L, hkv, group, head_tiles, n_pages, page, max_pages, splits, chunk;
+    int B, L, hkv, group, head_tiles, n_pages, page, max_pages;
     float scale_log2;
-    uint32_t k1024;   // 0x64006400, see Scale2
-    __nv_bfloat16* out;   // splits == 1
-    float* lse;           // may be null then
-    float *po, *plse;     // splits > 1: normalised rows [slice, split, group, D] and log-sum-exps
+    uint32_t k1024;    // 0x64006400, see Scale2
+    __nv_bfloat16* out;
+    float* lse;        // may be null
+    // Workspace: steps before each batch entry [B + 1] (of one slice), and for every part of a slice that a warp does not have to itself the
+    // normalised rows [part][part_rows][D] and log-sum-exps.  Parts are numbered warp + slice: one of the two grows from each to the next.
+    unsigned* before;
+    float *po, *plse;
+    int part_rows;
+};
+
+// Of `total` steps warp w of `parts` has `per`, one more if it is among the first `rest`.  Counts fit 32 bits: the host sees to it.
+constexpr int kLeastSteps = Q4_LEAST;   // of a part
+struct Q4Shares {
+    unsigned parts, per, rest;
+    __host__ __device__ __forceinline__ Q4Shares(unsigned total, unsigned warps) {
+        parts = (total + kLeastSteps - 1) / kLeastSteps;
+        parts = parts < 1 ? 1 : parts < warps ? parts : warps;
+        per = total / parts;
+        rest = total - per * parts;
+    }
+    __host__ __device__ __forceinline__ unsigned begin(unsigned w) const { return w * per + (w < rest ? w : rest); }
+    __host__ __device__ __forceinline__ unsigned warp_of(unsigned x) const {
+        const unsigned longer = rest * (per + 1);
+        return x < longer ? x / (per + 1) : rest + (x - longer) / per;
+    }
+};
+
+__device__ __forceinline__ int q4_len(const DecodeQ4Args& a, int b) { return a.lens ? min(max(__ldg(a.lens + b), 0), a.L) : a.L; }
+__device__ __forceinline__ unsigned q4_steps(int len) { return (unsigned)(len + kTile - 1) / kTile; }
+
+// A place in the sequence of steps: the batch entry it is in and where that one's steps begin.
+struct Q4Cursor {
+    int b, len;
+    unsigned begin;
+    __device__ __forceinline__ void to(const DecodeQ4Args& a, unsigned per_b, unsigned x) {   // x >= begin, below the end
+        unsigned n;
+        while (x - begin >= (n = q4_steps(len) * per_b)) {
+            begin += n;
+            len = q4_len(a, ++b);
+        }
+    }
+    // the slice within the batch entry, and the step within the slice
+    __device__ __forceinline__ int slice(unsigned x, int* step) const {
+        const unsigned steps = q4_steps(len), s = (x - begin) / steps;
+        *step = (int)(x - begin - s * steps);
+        return (int)s;
+    }
 };
 
 template <int D, int NT>
-constexpr int q4_smem() {
-    const int ring = kWarps * kDepth * 2 * Slot<D>::kBytes, merge = kWarps * 8 * NT * (D + 4 + 2) * 4;
-    return ring > merge ? ring : merge;
-}
+constexpr int q4_smem() { return kWarps * kDepth * 2 * Slot<D>::kBytes; }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) attn_decode_q4_kernel(const DecodeQ4Args a) {
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 : 2) attn_decode_q4_kernel(const DecodeQ4Args a) {
     constexpr int kHeads = 8 * NT, kG = D / 32, kVW = D / 64, kMT = D / 16;
     using S = Slot<D>;
     extern __shared__ __align__(128) unsigned char smem[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp_idx(), g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits, tile = item % a.head_tiles, slice = item / a.head_tiles;
-    const int b = slice / a.hkv, hk = slice - b * a.hkv, h0 = tile * kHeads, n_heads = min(kHeads, a.group - h0);
+    const int lane = threadIdx.x & 31, warp = uniform_warp_idx(), g = lane >> 2, t = lane & 3;
     const uint32_t k1024 = a.k1024;
     const uint32_t ring = smem_u32(smem) + warp * (kDepth * 2 * S::kBytes);
+    const unsigned w_all = gridDim.x * kWarps, w = blockIdx.x + gridDim.x * warp, per_b = a.hkv * a.head_tiles;   // few parts: on different SMs
     grid_let_next_start();
     grid_wait_for_previous();
-    const int len = a.lens ? min(max(__ldg(a.lens + b), 0), a.L) : a.L;
-    const int k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
-    const long long row0 = (long long)slice * a.group + h0;   // the tile's first query head
 
-    // 16 keys lie in one page.  Lane i looks up where the i-th 16 keys of a batch are: the byte of their first row, or -1, and their row in
-    // the page.
-    const int n_sub = k1 > k0 ? ((k1 - k0 + kTile - 1) / kTile + kWarps - 1 - warp) / kWarps * 2 : 0;   // this warp's 16-key tiles
-    auto first_key = [&](int sub) { return k0 + ((sub >> 1) * kWarps + warp) * kTile + (sub & 1) * 16; };
+    // the batch's steps, and where this warp's part begins
+    unsigned sum = 0;
+    for (int i = lane; i < a.B; i += 32) sum += q4_steps(q4_len(a, i));
+    const unsigned total = __reduce_add_sync(0xffffffffu, sum) * per_b;
+    const Q4Shares shares(total, w_all);
+    if (w >= shares.parts) return;
+    const unsigned x0 = shares.begin(w);
+    const int n = (int)(shares.begin(w + 1) - x0);
+    Q4Cursor now{0, 0, 0};   // of the step at hand
+    {
+        const unsigned y = x0 / per_b;
+        unsigned done = 0;
+        int found = -1;
+        for (int i = 0; i < a.B && (found < 0 || w == 0); i += 32) {
+            const int len = i + lane < a.B ? q4_len(a, i + lane) : 0;
+            unsigned to = q4_steps(len);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const unsigned x = __shfl_up_sync(0xffffffffu, to, d);
+                if (lane >= d) to += x;
+            }
+            to += done;
+            if (w == 0 && i + lane < a.B) {   // for the merge
+                a.before[i + lane + 1] = to;
+                if (i + lane == 0) a.before[0] = 0;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, to > y);
+            if (found < 0 && past) {
+                const int at = __ffs(past) - 1;
+                found = i + at;
+                now.b = found;
+                now.len = __shfl_sync(0xffffffffu, len, at);
+                now.begin = (__shfl_sync(0xffffffffu, to, at) - q4_steps(now.len)) * per_b;
+            }
+            done = __shfl_sync(0xffffffffu, to, 31);
+        }
+        if (found < 0) return;   // no keys at all
+    }
+
+    // 16 keys lie in one page.  Lane i looks up where the i-th 16 keys of a batch of 32 are: the byte of their first row, or -1, and beside
+    // their row in the page how many keys there are, less one.
+    Q4Cursor ahead = now;
     long long at_now;
     int row_now;
-    auto look_up = [&](int sub) {
-        const int key = first_key(sub);
+    auto look_up = [&](int sub) {   // sub: the lane's, a multiple of 32 for lane 0
         at_now = -1;
         row_now = 0;
-        if (sub < n_sub && key < k1) {
-            const int col = key / a.page;
-            const int page = !a.table ? b : col < a.max_pages ? __ldg(a.table + (long long)b * a.max_pages + col) : -1;
-            if (page >= 0 && page < a.n_pages) {
-                row_now = key - col * a.page;
-                at_now = ((long long)page * a.hkv + hk) * ((long long)a.page * q4_row_bytes(D)) + row_now * (D / 2);
+        if (sub < 2 * n) {
+            const unsigned x = x0 + (sub >> 1);
+            int step;
+            ahead.to(a, per_b, x);
+            const int slice = ahead.slice(x, &step), key = step * kTile + (sub & 1) * 16, left = ahead.len - key;
+            if (left > 0) {
+                const int col = key / a.page;
+                const int page = !a.table ? ahead.b : col < a.max_pages ? __ldg(a.table + (long long)ahead.b * a.max_pages + col) : -1;
+                if (page >= 0 && page < a.n_pages) {
+                    const int row = key - col * a.page;
+                    at_now = ((long long)page * a.hkv + slice / a.head_tiles) * ((long long)a.page * q4_row_bytes(D)) + row * (D / 2);
+                    row_now = row | (min(left, 16) - 1);
+                }
             }
         }
     };
@@ -171,289 +263,395 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : D == 64 ? 3 : 2) at
     }
     const unsigned char *from_k = a.kc + lane * 16, *from_v = a.vc + lane * 16;
     const unsigned char* from_codes = (lane < kCodes ? a.kc : a.vc) + a.page * (D / 2) + lane % kCodes * 16;
-    // Both tiles of a step into the slots at `slot`: bits of those that have keys.
-    auto fetch = [&](int sub, uint32_t slot) -> unsigned {
-        unsigned has = 0;
-        if (sub < n_sub) {
-            if ((sub & 31) == 0 && sub > 0) look_up(sub + lane);
+    // Both tiles of step i into the slots at `slot`: their numbers of keys, 8 bits each.
+    auto fetch = [&](int i, uint32_t slot) -> unsigned {
+        unsigned keys = 0;
+        if (i < n) {
+            if ((i & 15) == 0 && i > 0) look_up(2 * i + lane);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const long long at = __shfl_sync(0xffffffffu, at_now, (sub + j) & 31);
-                const int row = __shfl_sync(0xffffffffu, row_now, (sub + j) & 31);
+                const long long at = __shfl_sync(0xffffffffu, at_now, (2 * i + j) & 31);
+                const int row = __shfl_sync(0xffffffffu, row_now, (2 * i + j) & 31);
                 const bool some = at >= 0;
                 const uint32_t to = slot + j * S::kBytes;
 #pragma unroll
-                for (int i = 0; i < kCopies; ++i) {
-                    copy16(to + to_k[i], from_k + at + 512 * i, some);
-                    copy16(to + to_v[i], from_v + at + 512 * i, some);
+                for (int c = 0; c < kCopies; ++c) {
+                    copy16(to + to_k[c], from_k + at + 512 * c, some);
+                    copy16(to + to_v[c], from_v + at + 512 * c, some);
                 }
-                if (lane < 2 * kCodes) copy16(to + S::kKc + lane * 16, from_codes + at - row * (D / 2 - D / 32), some);
-                has |= some ? 1u << j : 0u;
+                if (lane < 2 * kCodes) copy16(to + S::kKc + lane * 16, from_codes + at - (row & ~15) * (D / 2 - D / 32), some);
+                keys |= some ? (unsigned)((row & 15) + 1) << (8 * j) : 0u;
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        return has;
+        return keys;
     };
-    unsigned has[kDepth];   // of the step at hand and those on their way
+    unsigned keys[kDepth];   // of the step at hand and those on their way
 #pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) has[i] = fetch(2 * i, ring + i * 2 * S::kBytes);
-
-    // query heads as the B operand: lane (g, t) has head g's quarter t of the channels, pairs (i, i + 4) of eight
-    uint32_t qf[NT][kG][4];
-    float to_log2[NT][2];   // the scores' factor of heads 2t and 2t + 1
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        float x[kG][8], top = 0.f;
-#pragma unroll
-        for (int i = 0; i < kG; ++i) {
-            const uint4 w = g + 8 * n < n_heads ? __ldg(reinterpret_cast<const uint4*>(a.q + (row0 + g + 8 * n) * D + t * (D / 4)) + i) : make_uint4(0, 0, 0, 0);
-            const uint32_t y[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[i][2 * j] = __uint_as_float(y[j] << 16);
-                x[i][2 * j + 1] = __uint_as_float(y[j] & 0xffff0000u);
-                top = fmaxf(top, fmaxf(fabsf(x[i][2 * j]), fabsf(x[i][2 * j + 1])));
-            }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the head's largest value to 2^10 .. 2^11 (infinities stay)
-        const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.f && e < 128 ? min(max(10 - e, -100), 100) : 0;
-        const float f = __uint_as_float((unsigned)(up + 127) << 23), back = __uint_as_float((unsigned)(127 - up) << 23);
-#pragma unroll
-        for (int i = 0; i < kG; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float by = j & 1 ? f : 16 * f;
-                qf[n][i][j] = bits(__floats2half2_rn(x[i][j] * by, x[i][j + 4] * by));
-            }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) to_log2[n][j] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
-    }
-
-    float o[kMT][NT][4], m[NT][2], l[NT][2];   // m: what a score is taken less; 2^-kLift of the reference
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < kMT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
-        m[n][0] = m[n][1] = kNone;
-        l[n][0] = l[n][1] = 0.f;
-    }
+    for (int i = 0; i < kDepth - 1; ++i) keys[i] = fetch(i, ring + i * 2 * S::kBytes);
+    uint32_t at_slot = 0, free_slot = (kDepth - 1) * 2 * S::kBytes;   // of the step at hand, and of the one before it
     // where this lane reads in a slot
     uint32_t v_from[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_from[i] = S::v_at(2 * t + (i & 1) + (i >> 1) * 8, g * (D / 16) / 16) + g * (D / 16) % 16;
 
-    uint32_t at_slot = 0, free_slot = (kDepth - 1) * 2 * S::kBytes;   // of the step at hand, and of the one before it
-    for (int sub = 0; sub < n_sub; sub += 2) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
-        __syncwarp();
-        const unsigned char* slot = smem + warp * (kDepth * 2 * S::kBytes) + at_slot;
-        const unsigned here = has[0];
+    for (int i = 0; i < n;) {   // slice by slice
+        int step;
+        now.to(a, per_b, x0 + i);
+        const int slice_b = now.slice(x0 + i, &step), tile = slice_b % a.head_tiles;
+        const long long slice = (long long)now.b * per_b + slice_b;
+        const int h0 = tile * kHeads, n_heads = min(kHeads, a.group - h0), in_slice = (int)q4_steps(now.len), end = min(n, i + in_slice - step);
+        const bool whole = step == 0 && end - i == in_slice;
+        const long long row0 = ((long long)now.b * a.hkv + slice_b / a.head_tiles) * a.group + h0;   // the tile's first query head
+
+        // query heads as the B operand: lane (g, t) has head g's quarter t of the channels, pairs (i, i + 4) of eight
+        uint32_t qf[NT][kG][4];
+        float to_log2[NT][2];   // the scores' factor of heads 2t and 2t + 1
 #pragma unroll
-        for (int i = 0; i + 1 < kDepth; ++i) has[i] = has[i + 1];
-        has[kDepth - 2] = fetch(sub + 2 * (kDepth - 1), ring + free_slot);   // every lane has left that slot
-        free_slot = at_slot;
-        at_slot = at_slot == (kDepth - 1) * 2 * S::kBytes ? 0 : at_slot + 2 * S::kBytes;
-        // scores
-        float s[2][NT][4];
+        for (int n = 0; n < NT; ++n) {
+            float x[kG][8], top = 0.f;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const unsigned char* from = slot + u * S::kBytes;
-            uint32_t x[2][kG];
+            for (int i = 0; i < kG; ++i) {
+                const uint4 w = g + 8 * n < n_heads ? __ldg(reinterpret_cast<const uint4*>(a.q + (row0 + g + 8 * n) * D + t * (D / 4)) + i) : make_uint4(0, 0, 0, 0);
+                const uint32_t y[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int r = 0; r < 2; ++r) lds(x[r], from + (g + 8 * r) * (D / 2) + t * (D / 8));
-            const Scale2 lo(from[S::kKc + g * (D / 32) + t * (D / 32) / 4] * 0x00800080u),
-                hi(from[S::kKc + (g + 8) * (D / 32) + t * (D / 32) / 4] * 0x00800080u);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[u][n][j] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kG; ++w) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {   // channels 0, 4 and 1, 5 of eight, then 2, 6 and 3, 7
-                    const uint32_t y0 = x[0][w] >> 8 * h, y1 = x[1][w] >> 8 * h;
-                    const uint32_t a0 = lo.low(y0, k1024), a1 = hi.low(y1, k1024), a2 = lo.high(y0, k1024), a3 = hi.high(y1, k1024);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(s[u][n], a0, a1, a2, a3, qf[n][w][2 * h], qf[n][w][2 * h + 1]);
+                for (int j = 0; j < 4; ++j) {
+                    x[i][2 * j] = __uint_as_float(y[j] << 16);
+                    x[i][2 * j + 1] = __uint_as_float(y[j] & 0xffff0000u);
+                    top = fmaxf(top, fmaxf(fabsf(x[i][2 * j]), fabsf(x[i][2 * j + 1])));
                 }
             }
-        }
-        // V's codes of keys 2t, 2t + 1 and 2t + 8, 2t + 9
-        uint32_t vc[2][2][kVW];
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // the head's largest value to 2^10 .. 2^11 (infinities stay)
+            const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.f && e < 128 ? min(max(10 - e, -100), 100) : 0;
+            const float f = __uint_as_float((unsigned)(up + 127) << 23), back = __uint_as_float((unsigned)(127 - up) << 23);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+            for (int i = 0; i < kG; ++i)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) lds(vc[u][i], slot + u * S::kBytes + S::kVc + (2 * t + 8 * i) * (D / 32));
-        // keys behind the range, or without a page: no score, and scales of 0 so that what lies there does not meet P = 0
-        if (first_key(sub) + kTile > k1 || here != 3) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int left = here >> u & 1 ? k1 - first_key(sub + u) : 0;   // keys of these 16
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (g + (j >> 1) * 8 >= left) s[u][n][j] = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int key = 2 * t + 8 * i;
-                    if (D == 128) {
-                        if (key >= left) vc[u][i][0] = 0;
-                        if (key + 1 >= left) vc[u][i][kVW - 1] = 0;
-                    } else {
-                        if (key >= left) vc[u][i][0] = 0;
-                        else if (key + 1 >= left) vc[u][i][0] &= 0xffffu;
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const float by = j & 1 ? f : 16 * f;
+                    qf[n][i][j] = bits(__floats2half2_rn(x[i][j] * by, x[i][j + 4] * by));
                 }
-            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) to_log2[n][j] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
         }
-        // the maximum, where a score passes it by 2^kSlack
-        bool raise = false;
-        float top[NT][2];
+        float o[kMT][NT][4], m[NT][2], l[NT][2];   // m: what a score is taken less; 2^-kLift of the reference
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                top[n][j] = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2])) * to_log2[n][j];
-                raise = raise || top[n][j] > m[n][j] + (kLift + kSlack);
-            }
+            for (int i = 0; i < kMT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
+            m[n][0] = m[n][1] = kNone;
+            l[n][0] = l[n][1] = 0.f;
         }
-        if (__any_sync(0xffffffffu, raise)) {
+        for (; i < end; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+            __syncwarp();
+            const unsigned char* slot = smem + warp * (kDepth * 2 * S::kBytes) + at_slot;
+            const unsigned here = keys[0];
+#pragma unroll
+            for (int k = 0; k + 1 < kDepth; ++k) keys[k] = keys[k + 1];
+            keys[kDepth - 2] = fetch(i + kDepth - 1, ring + free_slot);   // every lane has left that slot
+            free_slot = at_slot;
+            at_slot = at_slot == (kDepth - 1) * 2 * S::kBytes ? 0 : at_slot + 2 * S::kBytes;
+            // scores
+            float s[2][NT][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const unsigned char* from = slot + u * S::kBytes;
+                uint32_t x[2][kG];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) lds(x[r], from + (g + 8 * r) * (D / 2) + t * (D / 8));
+                const Scale2 lo(from[S::kKc + g * (D / 32) + t * (D / 32) / 4] * 0x00800080u),
+                    hi(from[S::kKc + (g + 8) * (D / 32) + t * (D / 32) / 4] * 0x00800080u);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[u][n][j] = 0.f;
+#pragma unroll
+                for (int w = 0; w < kG; ++w) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {   // channels 0, 4 and 1, 5 of eight, then 2, 6 and 3, 7
+                        const uint32_t y0 = x[0][w] >> 8 * h, y1 = x[1][w] >> 8 * h;
+                        const uint32_t a0 = lo.low(y0, k1024), a1 = hi.low(y1, k1024), a2 = lo.high(y0, k1024), a3 = hi.high(y1, k1024);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_f16(s[u][n], a0, a1, a2, a3, qf[n][w][2 * h], qf[n][w][2 * h + 1]);
+                    }
+                }
+            }
+            // V's codes of keys 2t, 2t + 1 and 2t + 8, 2t + 9
+            uint32_t vc[2][2][kVW];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) lds(vc[u][i], slot + u * S::kBytes + S::kVc + (2 * t + 8 * i) * (D / 32));
+            // keys behind the range, or without a page: no score, and scales of 0 so that what lies there does not meet P = 0
+            if (here != 0x1010u) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int left = here >> (8 * u) & 31;   // keys of these 16
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (g + (j >> 1) * 8 >= left) s[u][n][j] = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = 2 * t + 8 * i;
+                        if (D == 128) {
+                            if (key >= left) vc[u][i][0] = 0;
+                            if (key + 1 >= left) vc[u][i][kVW - 1] = 0;
+                        } else {
+                            if (key >= left) vc[u][i][0] = 0;
+                            else if (key + 1 >= left) vc[u][i][0] &= 0xffffu;
+                        }
+                    }
+                }
+            }
+            // the maximum, where a score passes it by 2^kSlack
+            bool raise = false;
+            float top[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float x = top[n][j];
+                    top[n][j] = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2])) * to_log2[n][j];
+                    raise = raise || top[n][j] > m[n][j] + (kLift + kSlack);
+                }
+            }
+            if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    const float to = fmaxf(m[n][j], x - kLift), f = ex2_approx(m[n][j] - to);
-                    m[n][j] = to;
-                    l[n][j] *= f;
+                for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int i = 0; i < kMT; ++i) {
-                        o[i][n][j] *= f;
-                        o[i][n][j + 2] *= f;
+                    for (int j = 0; j < 2; ++j) {
+                        float x = top[n][j];
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        const float to = fmaxf(m[n][j], x - kLift), f = ex2_approx(m[n][j] - to);
+                        m[n][j] = to;
+                        l[n][j] *= f;
+#pragma unroll
+                        for (int i = 0; i < kMT; ++i) {
+                            o[i][n][j] *= f;
+                            o[i][n][j + 2] *= f;
+                        }
+                    }
+                }
+            }
+            // P^T as the B operand
+            uint32_t p[2][NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float x = ex2_approx(fmaf(s[u][n][2 * i], to_log2[n][0], -m[n][0])), y = ex2_approx(fmaf(s[u][n][2 * i + 1], to_log2[n][1], -m[n][1]));
+                        l[n][0] += x;
+                        l[n][1] += y;
+                        p[u][n][i] = transposed8x8(bits(__floats2half2_rn(x, y)));
+                    }
+                }
+            }
+            // O^T
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                // the two keys' codes of the lane's group of channels, times 128, in the halves of a word
+                uint32_t c[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (D == 128) c[i] = __byte_perm(vc[u][i][0], vc[u][i][kVW - 1], (g >> 1) | (4 + (g >> 1)) << 8);
+                    else c[i] = vc[u][i][0] >> (8 * (g >> 2));
+                    c[i] = (c[i] & 0x00ff00ffu) * 128u;
+                }
+                const Scale2 first(c[0]), second(c[1]);
+                uint32_t r[4][kVW];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) lds(r[i], slot + u * S::kBytes + v_from[i]);
+#pragma unroll
+                for (int w = 0; w < kVW; ++w) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {   // byte j: channels 2j and 2j + 1 of the word's eight
+                        const uint32_t sel = 0x0400u + 0x0101u * j;
+                        const uint32_t x = __byte_perm(r[0][w], r[1][w], sel), y = __byte_perm(r[2][w], r[3][w], sel);
+                        const uint32_t a0 = first.low(x, k1024), a1 = first.high(x, k1024), a2 = second.low(y, k1024), a3 = second.high(y, k1024);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_f16(o[w * 4 + j][n], a0, a1, a2, a3, p[u][n][0], p[u][n][1]);
                     }
                 }
             }
         }
-        // P^T as the B operand
-        uint32_t p[2][NT][2];
+
+        // the part's result: lane (g, t) has channels g (D / 8) .. of heads 2t and 2t + 1
+        const long long part = (w + slice) * a.part_rows;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int n8 = 0; n8 < NT; ++n8) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int j = 0; j < 2; ++j) {
+                const int h = 8 * n8 + 2 * t + j;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float x = ex2_approx(fmaf(s[u][n][2 * i], to_log2[n][0], -m[n][0])), y = ex2_approx(fmaf(s[u][n][2 * i + 1], to_log2[n][1], -m[n][1]));
-                    l[n][0] += x;
-                    l[n][1] += y;
-                    p[u][n][i] = transposed8x8(bits(__floats2half2_rn(x, y)));
+                for (int d = 4; d < 32; d <<= 1) l[n8][j] += __shfl_xor_sync(0xffffffffu, l[n8][j], d);
+                if (h >= n_heads) continue;
+                const float den = l[n8][j], inv = den == 0.f ? 0.f : 1.f / den;
+                const float lse = den == 0.f ? -INFINITY : m[n8][j] * 0.69314718056f + logf(den);
+                float y[D / 8];
+#pragma unroll
+                for (int c = 0; c < kMT; ++c) {
+                    y[2 * c] = 16.f * o[c][n8][j] * inv;
+                    y[2 * c + 1] = o[c][n8][j + 2] * inv;
                 }
-            }
-        }
-        // O^T
+                if (whole) {
+                    __nv_bfloat16* to = a.out + (row0 + h) * D + g * (D / 8);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            // the two keys' codes of the lane's group of channels, times 128, in the halves of a word
-            uint32_t c[2];
+                    for (int c = 0; c < D / 8; c += 8) {
+                        const __nv_bfloat162 z[4] = {__floats2bfloat162_rn(y[c], y[c + 1]), __floats2bfloat162_rn(y[c + 2], y[c + 3]),
+                                                     __floats2bfloat162_rn(y[c + 4], y[c + 5]), __floats2bfloat162_rn(y[c + 6], y[c + 7])};
+                        *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(z);
+                    }
+                    if (g == 0 && a.lse) a.lse[row0 + h] = lse;
+                } else {
+                    float* to = a.po + (part + h) * D + g * (D / 8);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (D == 128) c[i] = __byte_perm(vc[u][i][0], vc[u][i][kVW - 1], (g >> 1) | (4 + (g >> 1)) << 8);
-                else c[i] = vc[u][i][0] >> (8 * (g >> 2));
-                c[i] = (c[i] & 0x00ff00ffu) * 128u;
-            }
-            const Scale2 first(c[0]), second(c[1]);
-            uint32_t r[4][kVW];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) lds(r[i], slot + u * S::kBytes + v_from[i]);
-#pragma unroll
-            for (int w = 0; w < kVW; ++w) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {   // byte j: channels 2j and 2j + 1 of the word's eight
-                    const uint32_t sel = 0x0400u + 0x0101u * j;
-                    const uint32_t x = __byte_perm(r[0][w], r[1][w], sel), y = __byte_perm(r[2][w], r[3][w], sel);
-                    const uint32_t a0 = first.low(x, k1024), a1 = first.high(x, k1024), a2 = second.low(y, k1024), a3 = second.high(y, k1024);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(o[w * 4 + j][n], a0, a1, a2, a3, p[u][n][0], p[u][n][1]);
+                    for (int c = 0; c < D / 8; c += 4) *reinterpret_cast<float4*>(to + c) = make_float4(y[c], y[c + 1], y[c + 2], y[c + 3]);
+                    if (g == 0) a.plse[part + h] = lse;
                 }
             }
         }
     }
+}
 
-    // the warps' results in shared memory, [head][channel], over the rings
-    float* sm_o = reinterpret_cast<float*>(smem);
-    float* sm_m = sm_o + kWarps * kHeads * (D + 4);
-    float* sm_l = sm_m + kWarps * kHeads;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
+// kT threads per query head: zeros for a sequence without keys, nothing where one warp had the whole slice, else the sum of the parts' rows weighted
+// by exp(log-sum-exp).  What bounds it is latency: the parts' places, then their log-sum-exps and the first rows at once.  A warp (kT = 32) where
+// slices have few parts, 512 threads where they have many.
+constexpr int kMergeParts = 1024;   // weights held at a time
+template <int D, int kT>
+__global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kernel(const DecodeQ4Args a, int heads, int rows_all, int w_all) {
+    constexpr int kLanes = D / 4, kRows = kT / kLanes > 0 ? kT / kLanes : 1, kAhead = 4, kWeights = kT == 32 ? 32 : kMergeParts;
+    static_assert(kT % kLanes == 0, "whole rows");
+    __shared__ float sm_w[kT == 32 ? 4 : 1][kWeights], sm_o[kT == 32 ? 1 : kRows][D], sm_r[2][kT / 32];
+    const int tid = threadIdx.x % kT, lane = tid & 31, mine = kT == 32 ? threadIdx.x / 32 : 0, row = kT == 32 ? blockIdx.x * 4 + mine : blockIdx.x;
+    if (row >= rows_all) return;
+    const int hq = row % heads, b = row / heads, group_tile = hq % a.group / a.part_rows, h = hq % a.group % a.part_rows;
+    const int per_b = a.hkv * a.head_tiles, slice_b = hq / a.group * a.head_tiles + group_tile;
+    auto barrier = [] {
+        if (kT == 32) __syncwarp();
+        else __syncthreads();
+    };
+    grid_let_next_start();
+    grid_wait_for_previous();
+    const unsigned first = a.before[b], steps = a.before[b + 1] - first, total = a.before[a.B] * per_b;
+    __nv_bfloat16* out = a.out + (long long)row * D;
+    if (steps == 0) {
+        for (int c = tid; c < D / 2; c += kT) reinterpret_cast<uint32_t*>(out)[c] = 0;
+        if (tid == 0 && a.lse) a.lse[row] = -INFINITY;
+        return;
+    }
+    const Q4Shares shares(total, w_all);
+    const unsigned x = first * per_b + slice_b * steps;
+    const int w0 = (int)shares.warp_of(x), n = (int)shares.warp_of(x + steps - 1) - w0 + 1;
+    if (n == 1) return;
+    const long long part = w0 + (long long)b * per_b + slice_b;
+    const float* plse = a.plse + part * a.part_rows + h;
+    const int r0 = tid / kLanes, col = tid % kLanes * 4;
+    const float* rows = a.po + (part * a.part_rows + h) * D + col;
+    float4 v[kAhead];
+    auto load = [&](int i0) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + k * kRows;
+            v[k] = i < n ? *reinterpret_cast<const float4*>(rows + (long long)i * a.part_rows * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    load(r0);
+    auto reduced = [&](float y, bool max, int at) {   // over the row's threads, `at` 0 or 1
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int h = 8 * n + 2 * t + j, at = warp * kHeads + h;
+        for (int d = 16; d > 0; d >>= 1) {
+            const float z = __shfl_xor_sync(0xffffffffu, y, d);
+            y = max ? fmaxf(y, z) : y + z;
+        }
+        if (kT == 32) return y;
+        if (lane == 0) sm_r[at][tid >> 5] = y;
+        __syncthreads();
+        y = sm_r[at][0];
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], d);
-            if (g == 0) {
-                sm_m[at] = m[n][j];
-                sm_l[at] = l[n][j];
+        for (int i = 1; i < kT / 32; ++i) y = max ? fmaxf(y, sm_r[at][i]) : y + sm_r[at][i];
+        return y;
+    };
+    float top = -INFINITY, den = 0.f;
+    for (int i = tid; i < n; i += kT) top = fmaxf(top, plse[(long long)i * a.part_rows]);
+    top = reduced(top, true, 0);
+    if (top == -INFINITY) top = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = 0; base < n; base += kWeights) {
+        const int end = min(base + kWeights, n);
+        if (base) barrier();
+        for (int i = base + tid; i < end; i += kT) {
+            const float y = plse[(long long)i * a.part_rows], e = y == -INFINITY ? 0.f : expf(y - top);
+            sm_w[mine][i - base] = e;
+            den += e;
+        }
+        barrier();
+        for (int i0 = base + r0; i0 < end; i0 += kAhead * kRows) {
+            if (i0 != r0) load(i0);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + k * kRows;
+                const float f = i < end ? sm_w[mine][i - base] : 0.f;
+                acc.x = fmaf(f, v[k].x, acc.x); acc.y = fmaf(f, v[k].y, acc.y);
+                acc.z = fmaf(f, v[k].z, acc.z); acc.w = fmaf(f, v[k].w, acc.w);
             }
-#pragma unroll
-            for (int i = 0; i < kMT; ++i)
-                *reinterpret_cast<float2*>(sm_o + at * (D + 4) + g * (D / 8) + 2 * i) = make_float2(16.f * o[i][n][j], o[i][n][j + 2]);
         }
     }
-    __syncthreads();
-    const long long part = ((long long)slice * a.splits + split) * a.group + h0;
-    for (int i = tid; i < n_heads * (D / 4); i += kWarps * 32) {
-        const int h = i / (D / 4), c = (i - h * (D / 4)) * 4;
-        float top = -INFINITY;
+    if (kT != 32) *reinterpret_cast<float4*>(&sm_o[r0][col]) = acc;
+    den = reduced(den, false, 1);   // (its barrier orders sm_o too)
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    if (kT == 32) {
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_m[w * kHeads + h]);
-        float den = 0.f, x[4] = {};
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float mw = sm_m[w * kHeads + h], lw = sm_l[w * kHeads + h];
-            if (lw == 0.f) continue;   // no keys
-            const float f = mw == top ? 1.f : ex2_approx(mw - top);
-            den = fmaf(f, lw, den);
-            const float4 y = *reinterpret_cast<const float4*>(sm_o + (w * kHeads + h) * (D + 4) + c);
-            x[0] = fmaf(f, y.x, x[0]); x[1] = fmaf(f, y.y, x[1]);
-            x[2] = fmaf(f, y.z, x[2]); x[3] = fmaf(f, y.w, x[3]);
+        for (int d = 16; d >= kLanes; d >>= 1) {   // D = 64: two rows to a warp
+            acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d); acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
+            acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
         }
-        const float inv = den == 0.f ? 0.f : 1.f / den;
-        const float lse = den == 0.f ? -INFINITY : top * 0.69314718056f + logf(den);
-        if (a.splits == 1) {
-            const __nv_bfloat162 y[2] = {__floats2bfloat162_rn(x[0] * inv, x[1] * inv), __floats2bfloat162_rn(x[2] * inv, x[3] * inv)};
-            *reinterpret_cast<uint2*>(a.out + (row0 + h) * D + c) = *reinterpret_cast<const uint2*>(y);
-            if (c == 0 && a.lse) a.lse[row0 + h] = lse;
-        } else {
-            if (den != 0.f) *reinterpret_cast<float4*>(a.po + (part + h) * D + c) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-            if (c == 0) a.plse[part + h] = lse;
+        const __nv_bfloat162 z[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+        if (r0 == 0) *reinterpret_cast<uint2*>(out + col) = *reinterpret_cast<const uint2*>(z);
+    } else {
+        for (int c = tid; c < D; c += kT) {
+            float y = 0.f;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) y += sm_o[r][c];
+            out[c] = __float2bfloat16_rn(y * inv);
         }
     }
+    if (tid == 0 && a.lse) a.lse[row] = den == 0.f ? -INFINITY : top + logf(den);
 }
 
-// Key ranges per slice and their length: enough CTAs for four per SM four times over, of at least 128 keys.
-static int q4_ranges(const AttnArgs& a, int* chunk) {
-    const int head_tiles = (a.group + 15) / 16;
-    const long long items = a.BH / a.group * head_tiles, want = (16LL * sm_count() + items - 1) / items;
-    long long c = (a.L + want - 1) / want;
-    if (c < 128) c = 128;
-    if (want > 1 && c < 512 && items * ((a.L + 511) / 512) >= 4LL * sm_count()) c = 512;
-    c = (c + 127) / 128 * 128;
-    *chunk = (int)c;
-    return (int)((a.L + c - 1) / c);
+// CTAs: what an SM holds at once, fewer where there are not steps for them.
+template <int NT>
+static int q4_ctas(const AttnArgs& a, int head_tiles) {
+    const long long most = a.BH / a.group * head_tiles * ((a.L + kTile - 1) / kTile);
+    const Q4Shares shares((unsigned)most, sm_count() * kWarps * (NT == 1 ? Q4_CTAS : a.D == 64 ? 3 : 2));
+    return (int)((shares.parts + kWarps - 1) / kWarps);
 }
-size_t attn_decode_q4_workspace(const AttnArgs& a) {
-    int chunk;
-    const size_t n = (size_t)q4_ranges(a, &chunk);
-    return n > 1 ? align256((size_t)a.BH * n * a.D * 4) + align256((size_t)a.BH * n * 4) : 0;
+template <int NT>
+static size_t q4_layout(const AttnArgs& a, DecodeQ4Args* g, void* ws) {
+    const int tiles = (a.group + 8 * NT - 1) / (8 * NT), rows = a.group < 8 * NT ? a.group : 8 * NT;
+    const size_t B = (size_t)(a.BH / a.H), parts = (size_t)q4_ctas<NT>(a, tiles) * kWarps + (size_t)(a.BH / a.group) * tiles;
+    const size_t before = align256((B + 1) * 4), po = align256(parts * rows * a.D * 4);
+    if (g) {
+        g->before = (unsigned*)ws;
+        g->po = (float*)((unsigned char*)ws + before);
+        g->plse = (float*)((unsigned char*)ws + before + po);
+        g->part_rows = rows;
+        g->head_tiles = tiles;
+    }
+    return before + po + align256(parts * rows * 4);
 }
+bool attn_decode_q4_fits(const AttnArgs& a) {
+    const int tile = a.group <= 8 ? 8 : 16;
+    return a.BH / a.group * ((a.group + tile - 1) / tile) * ((a.L + kTile - 1LL) / kTile) < (1LL << 31);
+}
+size_t attn_decode_q4_workspace(const AttnArgs& a) { return a.group <= 8 ? q4_layout<1>(a, nullptr, nullptr) : q4_layout<2>(a, nullptr, nullptr); }
 
 template <int D, int NT>
 static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* table, const int* lens, int max_pages, void* ws, cudaStream_t st) {
@@ -461,24 +659,25 @@ static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* tab
     g.q = (const __nv_bfloat16*)a.q;
     g.kc = (const unsigned char*)c.k; g.vc = (const unsigned char*)c.v;
     g.table = table; g.lens = lens;
-    g.L = a.L; g.hkv = c.hkv; g.group = a.group; g.head_tiles = (a.group + 8 * NT - 1) / (8 * NT);
+    g.B = (int)(a.BH / a.H); g.L = a.L; g.hkv = c.hkv; g.group = a.group;
     g.n_pages = c.n_pages; g.page = c.page_size; g.max_pages = max_pages;
-    g.splits = q4_ranges(a, &g.chunk);
     g.scale_log2 = a.scale * 1.4426950408889634f;
     g.k1024 = 0x64006400u;
     g.out = (__nv_bfloat16*)a.out; g.lse = a.lse;
-    g.po = (float*)ws;
-    g.plse = (float*)((unsigned char*)ws + align256((size_t)a.BH * g.splits * D * 4));
-    const long long ctas = a.BH / a.group * g.head_tiles * g.splits;
-    if (ctas >= (1LL << 31)) return cudaErrorInvalidValue;
+    q4_layout<NT>(a, &g, ws);
+    const int ctas = q4_ctas<NT>(a, g.head_tiles);
+    cudaError_t e = TT_ALLOW_SMEM((attn_decode_q4_kernel<D, NT>), (q4_smem<D, NT>()));
+    if (e != cudaSuccess) return e;
     {
-        cudaError_t e = TT_ALLOW_SMEM((attn_decode_q4_kernel<D, NT>), (q4_smem<D, NT>()));
-        if (e != cudaSuccess) return e;
         LaunchScope ls(K_DECODE_Q4, st);
         e = launch_overlapped(attn_decode_q4_kernel<D, NT>, (unsigned)ctas, kWarps * 32, q4_smem<D, NT>(), st, g);
         if (e != cudaSuccess) return e;
     }
-    return g.splits > 1 ? attn_decode_merge(a, g.po, g.plse, g.splits, st) : cudaSuccess;
+    LaunchScope ls(K_DECODE_MERGE, st);
+    // parts of a slice if all were of the greatest length: up to a dozen rows are one warp's
+    const bool few = (long long)ctas * kWarps <= 12 * (a.BH / a.group) * g.head_tiles;
+    if (few) return launch_overlapped(attn_decode_q4_merge_kernel<D, 32>, (unsigned)((a.BH + 3) / 4), 128, 0, st, g, a.H, (int)a.BH, ctas * kWarps);
+    return launch_overlapped(attn_decode_q4_merge_kernel<D, 512>, (unsigned)a.BH, 512, 0, st, g, a.H, (int)a.BH, ctas * kWarps);
 }
 cudaError_t attn_decode_q4(const AttnArgs& a, const CacheQ4& c, const int* table, const int* lens, int max_pages, void* ws, cudaStream_t st) {
     if (a.D == 128) return a.group <= 8 ? launch_q4<128, 1>(a, c, table, lens, max_pages, ws, st) : launch_q4<128, 2>(a, c, table, lens, max_pages, ws, st);

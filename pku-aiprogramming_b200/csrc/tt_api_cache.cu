@@ -173,6 +173,7 @@ static int resolve_q4(const char* who, const tt_attn_desc* desc, AttnArgs* a) {
     if (a->S != 1) return fail(TT_ERR_BAD_SHAPE, "%s: S must be 1, got %d", who, a->S);
     if (!a->bf16 || (a->D != 64 && a->D != 128)) return fail(TT_ERR_BAD_DTYPE, "%s: bf16 with D = 64 or 128 only (dtype %d, D %d)", who, desc->dtype, a->D);
     if (a->L > (1 << 30)) return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds 2^30", who, a->L);
+    if (!attn_decode_q4_fits(*a)) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d x %d key/value heads x L=%d is too large", who, desc->B, desc->H / a->group, a->L);
     a->causal = 0;
     return TT_OK;
 }
