@@ -23,8 +23,8 @@
 //
 // All slices' keys, in steps of 32, make one sequence that is cut into equal parts, one for each warp on the GPU whatever the lengths are
 // (a launch with a CTA per range of one slice ended on its last wave: 64 sequences of 4096 to 8192 106 us).  A warp sums the lengths,
-// finds its part, and streams it through a ring of its own in shared memory (cp.async, kDepth steps ahead, into the next slice's
-// keys where one ends); no warp waits for another.  A slice that one warp has to itself is written at once; of others each warp leaves
+// finds its part, and streams it through a ring of its own in shared memory (cp.async, kDepth steps, on into the next slice's keys where
+// one ends; bulk copies of 1024 and 64 bytes were slower, 107 us for 95).  No warp waits for another.  A slice that one warp has to itself is written at once; of others each warp leaves
 // a normalised result and its log-sum-exp, which a second kernel merges.  Results do not depend on timing.
 #include "cache_q4.cuh"
 #include "sm100_ptx.cuh"
@@ -34,16 +34,7 @@ using namespace sm100;
 
 namespace {
 
-#ifndef Q4_DEPTH
-#define Q4_DEPTH 3
-#endif
-#ifndef Q4_CTAS
-#define Q4_CTAS 3
-#endif
-#ifndef Q4_LEAST
-#define Q4_LEAST 2
-#endif
-constexpr int kWarps = 4, kTile = 32, kDepth = Q4_DEPTH;   // a step of a warp: 32 keys, two accumulator tiles of 16
+constexpr int kWarps = 4, kTile = 32, kDepth = 3;   // a step of a warp: 32 keys, two accumulator tiles of 16
 constexpr float kSlack = 5.f, kLift = 10.f, kNone = -3e38f;   // (kNone: no score yet; above every finite one that counts as such)
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -56,9 +47,12 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ void copy16(uint32_t saddr, const void* p, bool some) {   // 16 bytes, or zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr), "l"(p), "r"(some ? 16 : 0) : "memory");
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
+__device__ __forceinline__ void copy16(uint32_t saddr, const void* p) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr), "l"(p) : "memory"); }
 template <int N>
 __device__ __forceinline__ void lds(uint32_t (&w)[N], const unsigned char* p) {
     if (N == 4) {
@@ -98,22 +92,11 @@ struct Scale2 {
     }
 };
 
-// 16 keys in a ring slot: rows of K, rows of V, K's codes, V's codes, 16-byte pieces in an order that keeps the reads off each
-// other's banks.
+// 16 keys in a ring slot, each part as it lies in the page: rows of K, rows of V, K's codes, V's codes.
 template <int D>
 struct Slot {
-    static constexpr int kPieces = D / 32;   // of a row
-    static constexpr int kV = 16 * D / 2, kKc = 2 * kV, kVc = kKc + 16 * (D / 32), kBytes = kVc + 16 * (D / 32);
-    // K is read in whole rows, V as a quarter or half piece of every second row
-    static __device__ __forceinline__ int k_at(int key, int piece) { return key * (D / 2) + piece * 16; }
-    static __device__ __forceinline__ int v_at(int key, int piece) {
-        if (D == 128) {
-            const int line = key >> 1, p = (key & 1) * 4 + piece;
-            return kV + line * 128 + ((p ^ ((line << 1 & 7) | (line >> 2 & 1))) << 4);
-        }
-        const int line = key >> 2, p = (key & 3) * 2 + piece;
-        return kV + line * 128 + ((p ^ (line & 1) << 1) << 4);
-    }
+    static constexpr int kRows = 16 * D / 2, kCodes = 16 * D / 32;
+    static constexpr int kV = kRows, kKc = 2 * kRows, kVc = kKc + kCodes, kBytes = kVc + kCodes;
 };
 
 }  // namespace
@@ -135,7 +118,7 @@ struct DecodeQ4Args {
 };
 
 // Of `total` steps warp w of `parts` has `per`, one more if it is among the first `rest`.  Counts fit 32 bits: the host sees to it.
-constexpr int kLeastSteps = Q4_LEAST;   // of a part
+constexpr int kLeastSteps = 2;   // of a part
 struct Q4Shares {
     unsigned parts, per, rest;
     __host__ __device__ __forceinline__ Q4Shares(unsigned total, unsigned warps) {
@@ -173,17 +156,19 @@ struct Q4Cursor {
     }
 };
 
+// (Four of 128 registers each: 95.7 us for 97.5 with 64 long sequences, but 14.0 for 12.2 with a single one.)
+constexpr int q4_ctas_per_sm(int D, int NT) { return NT == 1 || D == 64 ? 3 : 2; }
 template <int D, int NT>
 constexpr int q4_smem() { return kWarps * kDepth * 2 * Slot<D>::kBytes; }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 : 2) attn_decode_q4_kernel(const DecodeQ4Args a) {
+__global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decode_q4_kernel(const DecodeQ4Args a) {
     constexpr int kHeads = 8 * NT, kG = D / 32, kVW = D / 64, kMT = D / 16;
     using S = Slot<D>;
     extern __shared__ __align__(128) unsigned char smem[];
     const int lane = threadIdx.x & 31, warp = uniform_warp_idx(), g = lane >> 2, t = lane & 3;
     const uint32_t k1024 = a.k1024;
-    const uint32_t ring = smem_u32(smem) + warp * (kDepth * 2 * S::kBytes);
+    const unsigned char* ring = smem + warp * (kDepth * 2 * S::kBytes);
     const unsigned w_all = gridDim.x * kWarps, w = blockIdx.x + gridDim.x * warp, per_b = a.hkv * a.head_tiles;   // few parts: on different SMs
     grid_let_next_start();
     grid_wait_for_previous();
@@ -227,73 +212,65 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
         if (found < 0) return;   // no keys at all
     }
 
-    // 16 keys lie in one page.  Lane i looks up where the i-th 16 keys of a batch of 32 are: the byte of their first row, or -1, and beside
-    // their row in the page how many keys there are, less one.
+    // 16 keys lie in one page.  Lane i looks up where the i-th 16 keys of a batch of 32 are: the first row and its codes, in units of 32 bytes
+    // (of which all of these are multiples), or kNowhere.
+    constexpr unsigned kNowhere = 0xffffffffu;
     Q4Cursor ahead = now;
-    long long at_now;
-    int row_now;
+    unsigned rows_at, codes_at;
     auto look_up = [&](int sub) {   // sub: the lane's, a multiple of 32 for lane 0
-        at_now = -1;
-        row_now = 0;
+        rows_at = codes_at = kNowhere;
         if (sub < 2 * n) {
             const unsigned x = x0 + (sub >> 1);
             int step;
             ahead.to(a, per_b, x);
-            const int slice = ahead.slice(x, &step), key = step * kTile + (sub & 1) * 16, left = ahead.len - key;
-            if (left > 0) {
+            const int slice = ahead.slice(x, &step), key = step * kTile + (sub & 1) * 16;
+            if (key < ahead.len) {
                 const int col = key / a.page;
                 const int page = !a.table ? ahead.b : col < a.max_pages ? __ldg(a.table + (long long)ahead.b * a.max_pages + col) : -1;
                 if (page >= 0 && page < a.n_pages) {
                     const int row = key - col * a.page;
-                    at_now = ((long long)page * a.hkv + slice / a.head_tiles) * ((long long)a.page * q4_row_bytes(D)) + row * (D / 2);
-                    row_now = row | (min(left, 16) - 1);
+                    const long long begin = ((long long)page * a.hkv + slice / a.head_tiles) * ((long long)a.page * q4_row_bytes(D));
+                    rows_at = (unsigned)((begin + (long long)row * (D / 2)) >> 5);
+                    codes_at = (unsigned)((begin + (long long)a.page * (D / 2) + row * (D / 32)) >> 5);
                 }
             }
         }
     };
     look_up(lane);
-    // Pieces of a slot are numbered [K rows][V rows]; a lane copies every 32nd, and the first lanes the codes.
-    constexpr int kCopies = 16 * S::kPieces / 32, kCodes = D / 32;   // per tensor; 16-byte pieces of codes
-    uint32_t to_k[kCopies], to_v[kCopies];
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-        const int piece = lane + 32 * i;
-        to_k[i] = S::k_at(piece / S::kPieces, piece % S::kPieces);
-        to_v[i] = S::v_at(piece / S::kPieces, piece % S::kPieces);
-    }
-    const unsigned char *from_k = a.kc + lane * 16, *from_v = a.vc + lane * 16;
-    const unsigned char* from_codes = (lane < kCodes ? a.kc : a.vc) + a.page * (D / 2) + lane % kCodes * 16;
-    // Both tiles of step i into the slots at `slot`: their numbers of keys, 8 bits each.
-    auto fetch = [&](int i, uint32_t slot) -> unsigned {
-        unsigned keys = 0;
+    constexpr int kCodeCopies = S::kCodes / 16;   // lanes that copy codes of K, and of V
+    const unsigned char *from_k = a.kc + lane * 16, *from_v = a.vc + lane * 16, *from_codes = (lane < kCodeCopies ? a.kc : a.vc) + lane % kCodeCopies * 16;
+    const uint32_t into = smem_u32(ring) + lane * 16;
+    // Both tiles of step i into the ring at byte `to`; two bits: those that have keys.
+    auto fetch = [&](int i, uint32_t to) -> unsigned {
+        unsigned has = 0;
         if (i < n) {
             if ((i & 15) == 0 && i > 0) look_up(2 * i + lane);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const long long at = __shfl_sync(0xffffffffu, at_now, (2 * i + j) & 31);
-                const int row = __shfl_sync(0xffffffffu, row_now, (2 * i + j) & 31);
-                const bool some = at >= 0;
-                const uint32_t to = slot + j * S::kBytes;
+                const unsigned at = __shfl_sync(0xffffffffu, rows_at, (2 * i + j) & 31), codes = __shfl_sync(0xffffffffu, codes_at, (2 * i + j) & 31);
+                if (at != kNowhere) {
+                    const uint32_t slot = into + to + j * S::kBytes;
+                    const unsigned char *k = from_k + (unsigned long long)at * 32, *v = from_v + (unsigned long long)at * 32;
 #pragma unroll
-                for (int c = 0; c < kCopies; ++c) {
-                    copy16(to + to_k[c], from_k + at + 512 * c, some);
-                    copy16(to + to_v[c], from_v + at + 512 * c, some);
+                    for (int c = 0; c < S::kRows; c += 512) {
+                        copy16(slot + c, k + c);
+                        copy16(slot + S::kV + c, v + c);
+                    }
+                    if (lane < 2 * kCodeCopies) copy16(slot + S::kKc, from_codes + (unsigned long long)codes * 32);
+                    has |= 1u << j;
                 }
-                if (lane < 2 * kCodes) copy16(to + S::kKc + lane * 16, from_codes + at - (row & ~15) * (D / 2 - D / 32), some);
-                keys |= some ? (unsigned)((row & 15) + 1) << (8 * j) : 0u;
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        return keys;
+        return has;
     };
-    unsigned keys[kDepth];   // of the step at hand and those on their way
+    unsigned has[kDepth];   // of the step at hand and those on their way
 #pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) keys[i] = fetch(i, ring + i * 2 * S::kBytes);
+    for (int i = 0; i < kDepth - 1; ++i) has[i] = fetch(i, i * 2 * S::kBytes);
     uint32_t at_slot = 0, free_slot = (kDepth - 1) * 2 * S::kBytes;   // of the step at hand, and of the one before it
-    // where this lane reads in a slot
-    uint32_t v_from[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v_from[i] = S::v_at(2 * t + (i & 1) + (i >> 1) * 8, g * (D / 16) / 16) + g * (D / 16) % 16;
+    // where this lane reads in a slot: keys g and g + 8 of K, key 2t of V, codes of key g and of key 2t
+    const int k_from = g * (D / 2) + t * (D / 8), v_from = S::kV + 2 * t * (D / 2) + g * (D / 16), kc_from = S::kKc + g * (D / 32) + t * (D / 32) / 4,
+              vc_from = S::kVc + 2 * t * (D / 32);
 
     for (int i = 0; i < n;) {   // slice by slice
         int step;
@@ -336,7 +313,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
 #pragma unroll
             for (int j = 0; j < 2; ++j) to_log2[n][j] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
         }
-        float o[kMT][NT][4], m[NT][2], l[NT][2];   // m: what a score is taken less; 2^-kLift of the reference
+        float o[kMT][NT][4], m[NT][2], above[NT][2];   // m: what a score is taken less, 2^-kLift of the reference; above: what raises it
+        uint64_t sums[NT];                              // of P, heads 2t and 2t + 1
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -344,16 +322,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[i][n][j] = 0.f;
             m[n][0] = m[n][1] = kNone;
-            l[n][0] = l[n][1] = 0.f;
+            above[n][0] = above[n][1] = -INFINITY;
+            sums[n] = 0;
         }
-        for (; i < end; ++i) {
+        int left = now.len - step * kTile;   // keys from the step at hand on
+        for (; i < end; ++i, left -= kTile) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
             __syncwarp();
-            const unsigned char* slot = smem + warp * (kDepth * 2 * S::kBytes) + at_slot;
-            const unsigned here = keys[0];
+            const unsigned char* slot = ring + at_slot;
+            const unsigned here = has[0];
 #pragma unroll
-            for (int k = 0; k + 1 < kDepth; ++k) keys[k] = keys[k + 1];
-            keys[kDepth - 2] = fetch(i + kDepth - 1, ring + free_slot);   // every lane has left that slot
+            for (int k = 0; k + 1 < kDepth; ++k) has[k] = has[k + 1];
+            has[kDepth - 2] = fetch(i + kDepth - 1, free_slot);   // every lane has left that slot
             free_slot = at_slot;
             at_slot = at_slot == (kDepth - 1) * 2 * S::kBytes ? 0 : at_slot + 2 * S::kBytes;
             // scores
@@ -363,13 +343,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
                 const unsigned char* from = slot + u * S::kBytes;
                 uint32_t x[2][kG];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) lds(x[r], from + (g + 8 * r) * (D / 2) + t * (D / 8));
-                const Scale2 lo(from[S::kKc + g * (D / 32) + t * (D / 32) / 4] * 0x00800080u),
-                    hi(from[S::kKc + (g + 8) * (D / 32) + t * (D / 32) / 4] * 0x00800080u);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[u][n][j] = 0.f;
+                for (int r = 0; r < 2; ++r) lds(x[r], from + k_from + r * 8 * (D / 2));
+                const Scale2 lo(from[kc_from] * 0x00800080u), hi(from[kc_from + 8 * (D / 32)] * 0x00800080u);
 #pragma unroll
                 for (int w = 0; w < kG; ++w) {
 #pragma unroll
@@ -377,7 +352,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
                         const uint32_t y0 = x[0][w] >> 8 * h, y1 = x[1][w] >> 8 * h;
                         const uint32_t a0 = lo.low(y0, k1024), a1 = hi.low(y1, k1024), a2 = lo.high(y0, k1024), a3 = hi.high(y1, k1024);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_f16(s[u][n], a0, a1, a2, a3, qf[n][w][2 * h], qf[n][w][2 * h + 1]);
+                        for (int n = 0; n < NT; ++n) {
+                            if (w + h == 0) mma_f16_first(s[u][n], a0, a1, a2, a3, qf[n][w][2 * h], qf[n][w][2 * h + 1]);
+                            else mma_f16(s[u][n], a0, a1, a2, a3, qf[n][w][2 * h], qf[n][w][2 * h + 1]);
+                        }
                     }
                 }
             }
@@ -386,26 +364,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) lds(vc[u][i], slot + u * S::kBytes + S::kVc + (2 * t + 8 * i) * (D / 32));
+                for (int i = 0; i < 2; ++i) lds(vc[u][i], slot + u * S::kBytes + vc_from + i * 8 * (D / 32));
             // keys behind the range, or without a page: no score, and scales of 0 so that what lies there does not meet P = 0
-            if (here != 0x1010u) {
+            if (here != 3 || left < kTile) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const int left = here >> (8 * u) & 31;   // keys of these 16
+                    const int keys = here >> u & 1 ? left - 16 * u : 0;   // of these 16
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (g + (j >> 1) * 8 >= left) s[u][n][j] = -INFINITY;
+                            if (g + (j >> 1) * 8 >= keys) s[u][n][j] = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int key = 2 * t + 8 * i;
                         if (D == 128) {
-                            if (key >= left) vc[u][i][0] = 0;
-                            if (key + 1 >= left) vc[u][i][kVW - 1] = 0;
+                            if (key >= keys) vc[u][i][0] = 0;
+                            if (key + 1 >= keys) vc[u][i][kVW - 1] = 0;
                         } else {
-                            if (key >= left) vc[u][i][0] = 0;
-                            else if (key + 1 >= left) vc[u][i][0] &= 0xffffu;
+                            if (key >= keys) vc[u][i][0] = 0;
+                            else if (key + 1 >= keys) vc[u][i][0] &= 0xffffu;
                         }
                     }
                 }
@@ -417,41 +395,47 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    top[n][j] = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2])) * to_log2[n][j];
-                    raise = raise || top[n][j] > m[n][j] + (kLift + kSlack);
+                    top[n][j] = fmaxf(fmax3(s[0][n][j], s[0][n][j + 2], s[1][n][j]), s[1][n][j + 2]);
+                    raise = raise || top[n][j] > above[n][j];
                 }
             }
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+                    float f[2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         float x = top[n][j];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        const float to = fmaxf(m[n][j], x - kLift), f = ex2_approx(m[n][j] - to);
+                        const float to = fmaxf(m[n][j], x * to_log2[n][j] - kLift);
+                        f[j] = ex2_approx(m[n][j] - to);
                         m[n][j] = to;
-                        l[n][j] *= f;
+                        above[n][j] = (to + (kLift + kSlack)) / to_log2[n][j];
 #pragma unroll
-                        for (int i = 0; i < kMT; ++i) {
-                            o[i][n][j] *= f;
-                            o[i][n][j + 2] *= f;
+                        for (int c = 0; c < kMT; ++c) {
+                            o[c][n][j] *= f[j];
+                            o[c][n][j + 2] *= f[j];
                         }
                     }
+                    sums[n] = mul_f32x2(sums[n], pack_f32x2(f[0], f[1]));
                 }
             }
             // P^T as the B operand
             uint32_t p[2][NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+                const uint64_t less = pack_f32x2(-m[n][0], -m[n][1]), by = pack_f32x2(to_log2[n][0], to_log2[n][1]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float x = ex2_approx(fmaf(s[u][n][2 * i], to_log2[n][0], -m[n][0])), y = ex2_approx(fmaf(s[u][n][2 * i + 1], to_log2[n][1], -m[n][1]));
-                        l[n][0] += x;
-                        l[n][1] += y;
-                        p[u][n][i] = transposed8x8(bits(__floats2half2_rn(x, y)));
+                    for (int k = 0; k < 2; ++k) {
+                        float x, y;
+                        unpack_f32x2(fma_f32x2(pack_f32x2(s[u][n][2 * k], s[u][n][2 * k + 1]), by, less), x, y);
+                        x = ex2_approx(x);
+                        y = ex2_approx(y);
+                        sums[n] = add_f32x2(sums[n], pack_f32x2(x, y));
+                        p[u][n][k] = transposed8x8(bits(__floats2half2_rn(x, y)));
                     }
                 }
             }
@@ -469,7 +453,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
                 const Scale2 first(c[0]), second(c[1]);
                 uint32_t r[4][kVW];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) lds(r[i], slot + u * S::kBytes + v_from[i]);
+                for (int k = 0; k < 4; ++k) lds(r[k], slot + u * S::kBytes + v_from + ((k & 1) + (k >> 1) * 8) * (D / 2));
 #pragma unroll
                 for (int w = 0; w < kVW; ++w) {
 #pragma unroll
@@ -488,13 +472,15 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? Q4_CTAS : D == 64 ? 3 :
         const long long part = (w + slice) * a.part_rows;
 #pragma unroll
         for (int n8 = 0; n8 < NT; ++n8) {
+            float l[2];
+            unpack_f32x2(sums[n8], l[0], l[1]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int h = 8 * n8 + 2 * t + j;
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) l[n8][j] += __shfl_xor_sync(0xffffffffu, l[n8][j], d);
+                for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
                 if (h >= n_heads) continue;
-                const float den = l[n8][j], inv = den == 0.f ? 0.f : 1.f / den;
+                const float den = l[j], inv = den == 0.f ? 0.f : 1.f / den;
                 const float lse = den == 0.f ? -INFINITY : m[n8][j] * 0.69314718056f + logf(den);
                 float y[D / 8];
 #pragma unroll
@@ -630,7 +616,7 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kern
 template <int NT>
 static int q4_ctas(const AttnArgs& a, int head_tiles) {
     const long long most = a.BH / a.group * head_tiles * ((a.L + kTile - 1) / kTile);
-    const Q4Shares shares((unsigned)most, sm_count() * kWarps * (NT == 1 ? Q4_CTAS : a.D == 64 ? 3 : 2));
+    const Q4Shares shares((unsigned)most, sm_count() * kWarps * (q4_ctas_per_sm(a.D, NT)));
     return (int)((shares.parts + kWarps - 1) / kWarps);
 }
 template <int NT>

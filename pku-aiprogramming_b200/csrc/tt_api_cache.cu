@@ -43,6 +43,7 @@ int q4_args(const char* who, const void* k_cache, const void* v_cache, int32_t H
     if (page_size < 16 || page_size % 16) return fail(TT_ERR_BAD_SHAPE, "%s: page_size=%d must be a multiple of 16", who, page_size);
     if (Hkv < 1 || n_pages < 0) return fail(TT_ERR_BAD_SHAPE, "%s: Hkv=%d n_pages=%d", who, Hkv, n_pages);
     if ((int64_t)n_pages * page_size >= (1LL << 31)) return fail(TT_ERR_BAD_SHAPE, "%s: pages of %d x %d tokens, at most 2^31 - 1", who, n_pages, page_size);
+    if ((double)n_pages * Hkv * page_size * (D / 2 + D / 32) >= 137438953472.0) return fail(TT_ERR_BAD_SHAPE, "%s: a cache of 2^37 bytes or more", who);
     if (n_pages && (!k_cache || !v_cache)) return fail(TT_ERR_NULL, "%s: null cache", who);
     if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(TT_ERR_BAD_SHAPE, "%s: the cache must be 16-byte aligned", who);
     return TT_OK;
