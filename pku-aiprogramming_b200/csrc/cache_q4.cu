@@ -29,7 +29,9 @@ __device__ __forceinline__ void q4_load8(const T* p, float (&x)[8]) {
     }
 }
 
-// Eight channels of a group that four lanes share -> their word and the group's code; whole warps.
+// Eight channels of a group that four lanes share -> their word and the group's code; whole warps.  The levels are added up as they are, four bits
+// apart: each is 1.5 2^23's bits plus -8 .. 7, and what that comes to without the levels' own 8 is a constant.
+template <typename T>
 __device__ __forceinline__ uint32_t q4_encode8(const float (&x)[8], int* code) {
     unsigned top = 0;   // bits of |x|: ordered as the values, with NaN above infinity
 #pragma unroll
@@ -40,12 +42,17 @@ __device__ __forceinline__ uint32_t q4_encode8(const float (&x)[8], int* code) {
         *code = kQ4NaN;
         return 0x88888888u;
     }
-    *code = q4_code(__uint_as_float(top));
-    const float s = 0.125f * q4_scale8(*code), inv = *code ? 1.f / s : 0.f;
+    float s8;
+    *code = q4_code(__uint_as_float(top), &s8);
+    const float s = 0.125f * s8, inv = *code ? q4_reciprocal(s) : 0.f;
+    const bool over = __uint_as_float(top) > 7.5f * s;   // beyond the largest scale
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= q4_level(x[i], s, inv) << (4 * i);
-    return w;
+    for (int i = 7; i >= 0; --i) {
+        const float y = over ? fminf(fmaxf(x[i], -7.5f * s), 7.5f * s) : x[i];
+        w = (w << 4) + (sizeof(T) == 2 ? q4_level_bf16(y, inv) : q4_level_f32(y, s, inv));
+    }
+    return w - kQ4Bits * 0x11111111u + 0x88888888u;
 }
 
 template <typename T, int D, bool kWide>
@@ -65,7 +72,7 @@ __global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __
         q4_load8<T, kWide>(v + t * v_tok + h * v_head + c * 8, y);
     }
     int ck, cv;
-    const uint32_t wk = q4_encode8(x, &ck), wv = q4_encode8(y, &cv);
+    const uint32_t wk = q4_encode8<T>(x, &ck), wv = q4_encode8<T>(y, &cv);
     if (!here) return;
     const int p = slot / page, r = slot - p * page;
     const long long at = ((long long)p * hkv + h) * ((long long)page * q4_row_bytes(D));
@@ -81,7 +88,7 @@ __global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __
 template <int D>
 __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc, const int* __restrict__ table,
                                                                    const int* __restrict__ cu, int B, int hkv, int n_pages, int page, int max_pages, int total,
-                                                                   int tokens_per_cta, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v) {
+                                                                   int tokens_per_cta, uint32_t k128, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v) {   // k128: 0x43004300, in a register
     constexpr int kLanes = D / 8, kRows = kQ4Threads / kLanes;
     __shared__ int2 where[kQ4Threads];   // of each token of the CTA its page and row in it; page -1: zeros, -2: left alone
     const int t0 = blockIdx.x * tokens_per_cta, n = min(tokens_per_cta, total - t0);
@@ -113,20 +120,26 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
         const long long to = ((long long)t0 * hkv + row) * D + c * 8;
         const long long at = ((long long)w.x * hkv + h) * ((long long)page * q4_row_bytes(D));
         const long long word = at + w.y * (D / 2) + c * 4, code = at + (long long)page * (D / 2) + w.y * (D / 32) + c / 4;
+        uint32_t x[2] = {0x88888888u, 0x88888888u}, codes[2] = {0, 0};
+        if (w.x >= 0) {
+            x[0] = *reinterpret_cast<const uint32_t*>(kc + word);
+            x[1] = *reinterpret_cast<const uint32_t*>(vc + word);
+            codes[0] = kc[code];
+            codes[1] = vc[code];
+        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const unsigned char* from = i ? vc : kc;
-            uint32_t x = 0x88888888u;
-            float s = 0.f;
-            if (w.x >= 0) {
-                x = *reinterpret_cast<const uint32_t*>(from + word);
-                s = 0.125f * q4_scale8(from[code]);
-            }
-            __nv_bfloat162 y[4];
+            // 0x4300 | n is 128 + n in bf16; (128 + n) s - 136 s, exactly: 17 times four bits has eight
+            const __nv_bfloat162 s = __float2bfloat162_rn(0.125f * q4_scale8((int)codes[i])), off = __hmul2(s, __float2bfloat162_rn(-136.f));
+            uint32_t y[4];   // channels j and j + 4
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                y[j] = __floats2bfloat162_rn((float)((int)(x >> (8 * j) & 15) - 8) * s, (float)((int)(x >> (8 * j + 4) & 15) - 8) * s);
-            *reinterpret_cast<uint4*>((i ? v : k) + to) = *reinterpret_cast<const uint4*>(y);
+            for (int j = 0; j < 4; ++j) {
+                asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y[j]) : "r"(x[i] >> (4 * j)), "n"(0x000f000f), "r"(k128));
+                const __nv_bfloat162 z = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&y[j]), s, off);
+                y[j] = *reinterpret_cast<const uint32_t*>(&z);
+            }
+            const uint4 out = make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
+            *reinterpret_cast<uint4*>((i ? v : k) + to) = out;
         }
     }
 }
@@ -159,7 +172,7 @@ cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* c
     LaunchScope ls(K_CACHE_READ, st);
     auto go = [&](auto kernel) {
         return launch_overlapped(kernel, grid, kQ4Threads, 0, st, (const unsigned char*)c.k, (const unsigned char*)c.v, block_table, cu, B, c.hkv, c.n_pages, c.page_size,
-                                 max_pages, total, per, (__nv_bfloat16*)k, (__nv_bfloat16*)v);
+                                 max_pages, total, per, 0x43004300u, (__nv_bfloat16*)k, (__nv_bfloat16*)v);
     };
     return c.D == 128 ? go(cache_read_q4_kernel<128>) : go(cache_read_q4_kernel<64>);
 }

@@ -18,24 +18,46 @@ __host__ __device__ constexpr int q4_row_bytes(int D) { return D / 2 + D / 32; }
 // half(code << 7): eight times the scale
 __device__ __forceinline__ float q4_scale8(int code) { return __half2float(__ushort_as_half((unsigned short)(code << 7))); }
 
-// The smallest code whose scale s has 7.5 s >= top (0.9375 times half(c << 7)); `top` finite or infinite.  The product is exact: four bits
-// times four.
-__device__ __forceinline__ int q4_code(float top) {
-    const float u = top * 1.0666666667f;   // top / 0.9375 up to a rounding: the right code or a neighbour
-    const unsigned b = __float_as_uint(u);
-    // round up to four significant bits; below 2^-14 in steps of 2^-17
-    int c = u < 6.103515625e-5f ? (int)ceilf(u * 131072.f) : (int)min((b + 0xfffffu) >> 20, 2047u) - 896;
-    if (c < kQ4Top && 0.9375f * q4_scale8(c) < top) ++c;
-    if (c > 0 && c <= kQ4Top && 0.9375f * q4_scale8(c - 1) >= top) --c;
-    return min(c, kQ4Top);
+// The smallest code whose scale s has 7.5 s >= top, and eight times that scale; `top` finite or infinite.  7.5 s is 0.9375 times half(c << 7),
+// exactly (four bits times four), so a candidate is compared as it is.  The candidate: top / 0.9375 rounded up to four significant bits.
+// The constant is the float below 16 / 15, so a quotient up to a scale does not come out above that scale, and one above it perhaps not above
+// it either: a candidate is too small by one then, never too large.
+__device__ __forceinline__ int q4_code(float top, float* scale8) {
+    const float u = top * 1.0666666f;
+    int c;
+    float b;
+    if (u < 6.103515625e-5f) {   // steps of 2^-17 below 2^-14
+        c = (int)ceilf(u * 131072.f);
+        b = (float)c * (1.f / 131072);
+        if (0.9375f * b < top) b = (float)++c * (1.f / 131072);
+    } else {
+        unsigned bits = min((__float_as_uint(u) + 0xfffffu) >> 20, (unsigned)kQ4Top + 896);
+        if (bits < kQ4Top + 896u && 0.9375f * __uint_as_float(bits << 20) < top) ++bits;
+        c = (int)bits - 896;
+        b = __uint_as_float(bits << 20);
+    }
+    *scale8 = b;
+    return c;
 }
-// x / s to the nearest integer, ties to even, held to -8 .. 7, plus 8.  `inv` is 1 / s (0 for s = 0) to a rounding, which leaves the
-// quotient's nearest integer or the next one; the remainder x - r s is exact (s has four bits, r at most five) and decides.
-__device__ __forceinline__ unsigned q4_level(float x, float s, float inv) {
-    float r = rintf(x * inv);
-    const float rem = fmaf(-r, s, x), far = fabsf(rem), half_step = 0.5f * s;
-    if (far > half_step || (far == half_step && s > 0.f && ((int)fminf(fabsf(r), 64.f) & 1))) r += copysignf(1.f, rem);
-    return (unsigned)((int)fminf(fmaxf(r, -8.f), 7.f) + 8);
+__device__ __forceinline__ float q4_reciprocal(float x) {   // to a unit in the last place or so
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// x / s to the nearest integer, ties to even, held to -8 .. 7, as the bits of 1.5 2^23 plus that: `inv` is 1 / s to 2^-22 or better (0 for s = 0).
+constexpr uint32_t kQ4Bits = 0x4b400000u;   // of 1.5 2^23
+// bf16 x: X 2^c / M with X of eight bits and M of four is either half-way between two integers or at least 2^-5 / 15 away from that, so the quotient
+// is rounded to 2^-10 first, which puts the half-way ones where they belong and lets no other cross.
+__device__ __forceinline__ uint32_t q4_level_bf16(float x, float inv) { return __float_as_uint(fminf(fmaf(x, inv, 12288.f), 12295.f) + (12582912.f - 12288.f)); }
+// float x: the nearest integer by the rounded reciprocal, or the next one; the remainder x - r s is exact (s has four bits, r at most five) and says.
+__device__ __forceinline__ uint32_t q4_level_f32(float x, float s, float inv) {
+    float t = fminf(fmaf(x, inv, 12582912.f), 12582919.f);
+    const float rem = fmaf(12582912.f - t, s, x), far = fabsf(rem), half_step = 0.5f * s;
+    if (far >= half_step && s > 0.f) {
+        if (far > half_step || (__float_as_uint(t) & 1)) t += copysignf(1.f, rem);
+        t = fminf(fmaxf(t, 12582904.f), 12582919.f);
+    }
+    return __float_as_uint(t);
 }
 
 }  // namespace ttk
