@@ -1,102 +1,149 @@
 // Writing new keys and values into the 4-bit cache, and reading sequences back as packed bf16.
 //
-// Both are bound by HBM: D = 128 in bf16 is 256 bytes a token and head, its codes are 68.  A thread has eight channels -- one
-// 16-byte access of bf16, one 4-byte word of the cache -- so a warp's accesses are whole rows on either side, and a group's
-// maximum is over four neighbouring lanes.
+// Both are bound by HBM -- D = 128 in bf16 is 256 bytes a token and head, its codes are 68 -- once the arithmetic is out of the way.  In writing
+// that is the work per group, so a thread has a whole one (32 channels, K and V apart): 20,000 tokens of 8 heads 34.8 us with four lanes to a
+// group, which meet for its maximum.  In reading a thread has 16 channels, the most whose stores are whole sectors.
 #include "cache_q4.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ttk {
 
 constexpr int kQ4Threads = 256;
 
-template <typename T, bool kWide>
-__device__ __forceinline__ void q4_load8(const T* p, float (&x)[8]) {
-    if (!kWide) {
+// 32 channels of a group, and the bits of the largest |x|: ordered as the values, with NaN above infinity.
+template <bool kWide>
+__device__ __forceinline__ unsigned q4_load32(const __nv_bfloat16* p, float (&x)[32]) {
+    uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
-    } else if (sizeof(T) == 2) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
-        const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < 4; ++i) {
+        if (kWide) {
+            const uint4 r = *reinterpret_cast<const uint4*>(p + 8 * i);
+            w[4 * i] = r.x; w[4 * i + 1] = r.y; w[4 * i + 2] = r.z; w[4 * i + 3] = r.w;
+        } else {
+            const unsigned short* q = reinterpret_cast<const unsigned short*>(p) + 8 * i;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(a[i] << 16);
-            x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+            for (int j = 0; j < 4; ++j) w[4 * i + j] = q[2 * j] | (uint32_t)q[2 * j + 1] << 16;
         }
-    } else {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+    return max(top << 16, top & 0xffff0000u);
+}
+template <bool kWide>
+__device__ __forceinline__ unsigned q4_load32(const float* p, float (&x)[32]) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (kWide) {
+            const float4 r = *reinterpret_cast<const float4*>(p + 4 * i);
+            x[4 * i] = r.x; x[4 * i + 1] = r.y; x[4 * i + 2] = r.z; x[4 * i + 3] = r.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = p[4 * i + j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[4 * i + j]) & 0x7fffffffu);
+    }
+    return top;
 }
 
-// Eight channels of a group that four lanes share -> their word and the group's code; whole warps.  The levels are added up as they are, four bits
-// apart: each is 1.5 2^23's bits plus -8 .. 7, and what that comes to without the levels' own 8 is a constant.
+// A group's four words and its code.  The levels are added up as they are, four bits apart: each is 1.5 2^23's bits plus -8 .. 7, and what that comes
+// to without the levels' own 8 is a constant.
 template <typename T>
-__device__ __forceinline__ uint32_t q4_encode8(const float (&x)[8], int* code) {
-    unsigned top = 0;   // bits of |x|: ordered as the values, with NaN above infinity
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (top > 0x7f800000u) {
-        *code = kQ4NaN;
-        return 0x88888888u;
-    }
+__device__ __forceinline__ uint4 q4_encode(float (&x)[32], unsigned top, int* code) {
     float s8;
-    *code = q4_code(__uint_as_float(top), &s8);
+    *code = q4_code(__uint_as_float(min(top, 0x7f800000u)), &s8);
     const float s = 0.125f * s8, inv = *code ? q4_reciprocal(s) : 0.f;
-    const bool over = __uint_as_float(top) > 7.5f * s;   // beyond the largest scale
-    uint32_t w = 0;
+    if (!(__uint_as_float(top) <= 7.5f * s)) {   // beyond the largest scale, or no number
+        if (top > 0x7f800000u) *code = kQ4NaN;
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-        const float y = over ? fminf(fmaxf(x[i], -7.5f * s), 7.5f * s) : x[i];
-        w = (w << 4) + (sizeof(T) == 2 ? q4_level_bf16(y, inv) : q4_level_f32(y, s, inv));
+        for (int i = 0; i < 32; ++i) x[i] = top > 0x7f800000u ? 0.f : fminf(fmaxf(x[i], -7.5f * s), 7.5f * s);
     }
-    return w - kQ4Bits * 0x11111111u + 0x88888888u;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        w[j] = 0;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) w[j] = (w[j] << 4) + (sizeof(T) == 2 ? q4_level_bf16(x[8 * j + i], inv) : q4_level_f32(x[8 * j + i], s, inv));
+        w[j] += 0x88888888u - kQ4Bits * 0x11111111u;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// Where a token's rows are: those of head 0 of its page, and its row in the page; or one of
+constexpr long long kQ4None = -1, kQ4Skip = -2;
+struct Q4Place {
+    long long begin;
+    int row;
+};
+// A thread's walk over (token, head) rows, kRows apart.
+struct Q4Walk {
+    int t, h, dt, dh, hkv;
+    __device__ __forceinline__ Q4Walk(int row, int rows_apart, int heads) : t(row / heads), dt(rows_apart / heads), hkv(heads) {
+        h = row - t * heads;
+        dh = rows_apart - dt * heads;
+    }
+    __device__ __forceinline__ void next() {
+        t += dt;
+        h += dh;
+        if (h >= hkv) {
+            h -= hkv;
+            ++t;
+        }
+    }
+};
 
 template <typename T, int D, bool kWide>
-__global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ slots, unsigned rows,
+__global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ slots, int n_tok, int tokens_per_cta,
                                                                      int hkv, long long k_tok, long long k_head, long long v_tok, long long v_head,
                                                                      unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, int n_slots, int page) {
-    constexpr int kLanes = D / 8, kRows = kQ4Threads / kLanes;
-    const unsigned row = blockIdx.x * (unsigned)kRows + threadIdx.x / kLanes, t = row / (unsigned)hkv, h = row - t * (unsigned)hkv;
-    const int c = threadIdx.x % kLanes;
+    constexpr int kLanes = D / 32, kRows = kQ4Threads / kLanes;
+    __shared__ Q4Place where[kQ4Threads];
+    const int t0 = blockIdx.x * tokens_per_cta, n = min(tokens_per_cta, n_tok - t0), c = threadIdx.x % kLanes;
+    const long long page_bytes = (long long)page * q4_row_bytes(D);
+    const bool second = blockIdx.y != 0;   // V
+    const T* from = (second ? v : k) + t0 * (second ? v_tok : k_tok) + c * 32;
+    const long long tok = second ? v_tok : k_tok, head = second ? v_head : k_head;
+    unsigned char* into = second ? vc : kc;
     grid_let_next_start();
     grid_wait_for_previous();
-    const int slot = row < rows ? slots[t] : -1;
-    const bool here = slot >= 0 && slot < n_slots;
-    float x[8] = {}, y[8] = {};
-    if (here) {
-        q4_load8<T, kWide>(k + t * k_tok + h * k_head + c * 8, x);
-        q4_load8<T, kWide>(v + t * v_tok + h * v_head + c * 8, y);
+    if (threadIdx.x < n) {
+        const int slot = slots[t0 + threadIdx.x], p = slot / page;
+        where[threadIdx.x] = Q4Place{slot >= 0 && slot < n_slots ? p * (hkv * page_bytes) : kQ4Skip, slot - p * page};
     }
-    int ck, cv;
-    const uint32_t wk = q4_encode8<T>(x, &ck), wv = q4_encode8<T>(y, &cv);
-    if (!here) return;
-    const int p = slot / page, r = slot - p * page;
-    const long long at = ((long long)p * hkv + h) * ((long long)page * q4_row_bytes(D));
-    const long long word = at + r * (D / 2) + c * 4, code = at + (long long)page * (D / 2) + r * (D / 32) + c / 4;
-    *reinterpret_cast<uint32_t*>(kc + word) = wk;
-    *reinterpret_cast<uint32_t*>(vc + word) = wv;
-    if (c % 4 == 0) {
-        kc[code] = (unsigned char)ck;
-        vc[code] = (unsigned char)cv;
+    __syncthreads();
+    for (Q4Walk at(threadIdx.x / kLanes, kRows, hkv); at.t < n; at.next()) {
+        const Q4Place w = where[at.t];
+        if (w.begin == kQ4Skip) continue;
+        float x[32];
+        const unsigned top = q4_load32<kWide>(from + at.t * tok + at.h * head, x);
+        int code;
+        const uint4 words = q4_encode<T>(x, top, &code);
+        unsigned char* to = into + w.begin + at.h * page_bytes;
+        *reinterpret_cast<uint4*>(to + w.row * (D / 2) + c * 16) = words;
+        to[(long long)page * (D / 2) + w.row * (D / 32) + c] = (unsigned char)code;
     }
 }
 
-template <int D>
+// kSectors: k and v start on 32 bytes
+template <int D, bool kSectors>
 __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc, const int* __restrict__ table,
                                                                    const int* __restrict__ cu, int B, int hkv, int n_pages, int page, int max_pages, int total,
                                                                    int tokens_per_cta, uint32_t k128, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v) {   // k128: 0x43004300, in a register
-    constexpr int kLanes = D / 8, kRows = kQ4Threads / kLanes;
-    __shared__ int2 where[kQ4Threads];   // of each token of the CTA its page and row in it; page -1: zeros, -2: left alone
+    constexpr int kLanes = D / 16, kRows = kQ4Threads / kLanes, kAhead = 4;
+    __shared__ Q4Place where[kQ4Threads];
     const int t0 = blockIdx.x * tokens_per_cta, n = min(tokens_per_cta, total - t0);
+    const long long page_bytes = (long long)page * q4_row_bytes(D);
     grid_let_next_start();
     grid_wait_for_previous();
     if (threadIdx.x < n) {
         const int t = t0 + threadIdx.x;
-        int2 w = make_int2(-2, 0);
+        Q4Place w{kQ4Skip, 0};
         if (t < cu[B]) {
             int lo = 0, hi = B;   // the last b with cu[b] <= t
             while (hi - lo > 1) {
@@ -106,54 +153,83 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
             }
             const int pos = t - cu[lo], col = pos / page;
             const int p = pos >= 0 && col < max_pages ? table[(long long)lo * max_pages + col] : -1;
-            w = make_int2(p >= 0 && p < n_pages ? p : -1, pos - col * page);
+            w = Q4Place{p >= 0 && p < n_pages ? p * (hkv * page_bytes) : kQ4None, pos - col * page};
         }
         where[threadIdx.x] = w;
     }
     __syncthreads();
     const int c = threadIdx.x % kLanes;
-    const unsigned rows = (unsigned)n * (unsigned)hkv;
-    for (unsigned row = threadIdx.x / kLanes; row < rows; row += kRows) {
-        const unsigned t = row / (unsigned)hkv, h = row - t * (unsigned)hkv;
-        const int2 w = where[t];
-        if (w.x == -2) continue;
-        const long long to = ((long long)t0 * hkv + row) * D + c * 8;
-        const long long at = ((long long)w.x * hkv + h) * ((long long)page * q4_row_bytes(D));
-        const long long word = at + w.y * (D / 2) + c * 4, code = at + (long long)page * (D / 2) + w.y * (D / 32) + c / 4;
-        uint32_t x[2] = {0x88888888u, 0x88888888u}, codes[2] = {0, 0};
-        if (w.x >= 0) {
-            x[0] = *reinterpret_cast<const uint32_t*>(kc + word);
-            x[1] = *reinterpret_cast<const uint32_t*>(vc + word);
-            codes[0] = kc[code];
-            codes[1] = vc[code];
+    long long to = ((long long)t0 * hkv + threadIdx.x / kLanes) * D + c * 16;
+    Q4Walk at(threadIdx.x / kLanes, kRows, hkv);
+    while (at.t < n) {   // kAhead rows' loads, then their values
+        uint2 x[kAhead][2];
+        uint32_t codes[kAhead][2];
+        unsigned there = 0;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i, at.next()) {
+            x[i][0] = x[i][1] = make_uint2(0x88888888u, 0x88888888u);
+            codes[i][0] = codes[i][1] = 0;
+            const Q4Place w = at.t < n ? where[at.t] : Q4Place{kQ4Skip, 0};
+            if (w.begin != kQ4Skip) there |= 1u << i;
+            if (w.begin >= 0) {
+                const long long begin = w.begin + at.h * page_bytes, word = begin + w.row * (D / 2) + c * 8, code = begin + (long long)page * (D / 2) + w.row * (D / 32) + c / 2;
+                x[i][0] = *reinterpret_cast<const uint2*>(kc + word);
+                x[i][1] = *reinterpret_cast<const uint2*>(vc + word);
+                codes[i][0] = kc[code];
+                codes[i][1] = vc[code];
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            // 0x4300 | n is 128 + n in bf16; (128 + n) s - 136 s, exactly: 17 times four bits has eight
-            const __nv_bfloat162 s = __float2bfloat162_rn(0.125f * q4_scale8((int)codes[i])), off = __hmul2(s, __float2bfloat162_rn(-136.f));
-            uint32_t y[4];   // channels j and j + 4
+        for (int i = 0; i < kAhead; ++i, to += kRows * D) {
+            if (!(there >> i & 1)) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y[j]) : "r"(x[i] >> (4 * j)), "n"(0x000f000f), "r"(k128));
-                const __nv_bfloat162 z = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&y[j]), s, off);
-                y[j] = *reinterpret_cast<const uint32_t*>(&z);
+            for (int j = 0; j < 2; ++j) {
+                // 0x4300 | n is 128 + n in bf16; (128 + n) s - 136 s, exactly: 17 times four bits has eight
+                const __nv_bfloat162 s = __float2bfloat162_rn(0.125f * q4_scale8((int)codes[i][j])), off = __hmul2(s, __float2bfloat162_rn(-136.f));
+                uint32_t out[8];
+#pragma unroll
+                for (int word = 0; word < 2; ++word) {
+                    uint32_t y[4];   // channels m and m + 4
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y[m]) : "r"((word ? x[i][j].y : x[i][j].x) >> (4 * m)), "n"(0x000f000f), "r"(k128));
+                        const __nv_bfloat162 z = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&y[m]), s, off);
+                        y[m] = *reinterpret_cast<const uint32_t*>(&z);
+                    }
+                    out[4 * word] = __byte_perm(y[0], y[1], 0x5410);
+                    out[4 * word + 1] = __byte_perm(y[2], y[3], 0x5410);
+                    out[4 * word + 2] = __byte_perm(y[0], y[1], 0x7632);
+                    out[4 * word + 3] = __byte_perm(y[2], y[3], 0x7632);
+                }
+                if (kSectors) {
+                    sm100::st_global_32B((j ? v : k) + to, out);
+                } else {
+                    *reinterpret_cast<uint4*>((j ? v : k) + to) = make_uint4(out[0], out[1], out[2], out[3]);
+                    *reinterpret_cast<uint4*>((j ? v : k) + to + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+                }
             }
-            const uint4 out = make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632), __byte_perm(y[2], y[3], 0x7632));
-            *reinterpret_cast<uint4*>((i ? v : k) + to) = out;
         }
     }
+}
+
+// Tokens per CTA: about 128 rows, so that look-ups are few beside the rows, fewer where that leaves SMs without a CTA.
+static int q4_tokens_per_cta(int tokens, int hkv) {
+    int per = 128 / hkv;
+    const int spread = (tokens + 4 * sm_count() - 1) / (4 * sm_count());
+    if (per > spread) per = spread;
+    return per < 1 ? 1 : per;
 }
 
 template <typename T, int D>
 static cudaError_t launch_append(const CacheQ4& c, const void* k, const void* v, const long long (&ks)[2], const long long (&vs)[2], const int* slots, int T_,
                                  cudaStream_t st) {
-    constexpr int kRows = kQ4Threads / (D / 8), kV = 16 / sizeof(T);
-    const unsigned rows = (unsigned)T_ * (unsigned)c.hkv;
+    constexpr int kV = 16 / sizeof(T);
     bool wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
     for (const long long* s : {ks, vs}) wide = wide && (T_ == 1 || s[0] % kV == 0) && (c.hkv == 1 || s[1] % kV == 0);
+    const int per = q4_tokens_per_cta(T_, c.hkv);
     auto go = [&](auto kernel) {
         LaunchScope ls(K_CACHE_APPEND, st);
-        return launch_overlapped(kernel, (rows + kRows - 1) / kRows, kQ4Threads, 0, st, (const T*)k, (const T*)v, slots, rows, c.hkv, ks[0], ks[1], vs[0], vs[1],
+        return launch_overlapped(kernel, dim3((unsigned)((T_ + per - 1) / per), 2), kQ4Threads, 0, st, (const T*)k, (const T*)v, slots, T_, per, c.hkv, ks[0], ks[1], vs[0], vs[1],
                                  (unsigned char*)c.k, (unsigned char*)c.v, c.n_pages * c.page_size, c.page_size);
     };
     return wide ? go(cache_append_q4_kernel<T, D, true>) : go(cache_append_q4_kernel<T, D, false>);
@@ -164,17 +240,16 @@ cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, cons
     return bf16 ? launch_append<__nv_bfloat16, 64>(c, k, v, ks, vs, slots, T, st) : launch_append<float, 64>(c, k, v, ks, vs, slots, T, st);
 }
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st) {
-    // about 128 rows per CTA, so that its look-ups are few and its loads many; fewer where that leaves SMs without one
-    int per = 128 / c.hkv, spread = (total + 4 * sm_count() - 1) / (4 * sm_count());
-    if (per > spread) per = spread;
-    if (per < 1) per = 1;
+    const int per = q4_tokens_per_cta(total, c.hkv);
     const unsigned grid = (unsigned)((total + per - 1) / per);
     LaunchScope ls(K_CACHE_READ, st);
     auto go = [&](auto kernel) {
         return launch_overlapped(kernel, grid, kQ4Threads, 0, st, (const unsigned char*)c.k, (const unsigned char*)c.v, block_table, cu, B, c.hkv, c.n_pages, c.page_size,
                                  max_pages, total, per, 0x43004300u, (__nv_bfloat16*)k, (__nv_bfloat16*)v);
     };
-    return c.D == 128 ? go(cache_read_q4_kernel<128>) : go(cache_read_q4_kernel<64>);
+    const bool sectors = (((uintptr_t)k | (uintptr_t)v) & 31) == 0;
+    if (c.D == 128) return sectors ? go(cache_read_q4_kernel<128, true>) : go(cache_read_q4_kernel<128, false>);
+    return sectors ? go(cache_read_q4_kernel<64, true>) : go(cache_read_q4_kernel<64, false>);
 }
 
 }  // namespace ttk
