@@ -2,7 +2,8 @@
 //
 // Both are bound by HBM -- D = 128 in bf16 is 256 bytes a token and head, its codes are 68 -- once the arithmetic is out of the way.  In writing
 // that is the work per group, so a thread has a whole one (32 channels, K and V apart): 20,000 tokens of 8 heads 34.8 us with four lanes to a
-// group, which meet for its maximum.  In reading a thread has 16 channels, the most whose stores are whole sectors.
+// group, which meet for its maximum, 21.5 so.  In reading it is the number of memory instructions: a whole group to a thread there too, as 16 bytes
+// and one, and four stores of a sector each.
 #include "cache_q4.cuh"
 #include "sm100_ptx.cuh"
 
@@ -135,23 +136,28 @@ template <int D, bool kSectors>
 __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigned char* __restrict__ kc, const unsigned char* __restrict__ vc, const int* __restrict__ table,
                                                                    const int* __restrict__ cu, int B, int hkv, int n_pages, int page, int max_pages, int total,
                                                                    int tokens_per_cta, uint32_t k128, __nv_bfloat16* __restrict__ k, __nv_bfloat16* __restrict__ v) {   // k128: 0x43004300, in a register
-    constexpr int kLanes = D / 16, kRows = kQ4Threads / kLanes, kAhead = 4;
+    constexpr int kLanes = D / 32, kRows = kQ4Threads / kLanes, kAhead = 2;
     __shared__ Q4Place where[kQ4Threads];
+    __shared__ int near[kQ4Threads];   // the counts of a small batch: a search step from memory takes as long as all of them
     const int t0 = blockIdx.x * tokens_per_cta, n = min(tokens_per_cta, total - t0);
     const long long page_bytes = (long long)page * q4_row_bytes(D);
     grid_let_next_start();
     grid_wait_for_previous();
+    const bool small = B < kQ4Threads;
+    if (small && threadIdx.x <= B) near[threadIdx.x] = cu[threadIdx.x];
+    __syncthreads();
     if (threadIdx.x < n) {
         const int t = t0 + threadIdx.x;
+        auto count = [&](int b) { return small ? near[b] : cu[b]; };
         Q4Place w{kQ4Skip, 0};
-        if (t < cu[B]) {
+        if (t < count(B)) {
             int lo = 0, hi = B;   // the last b with cu[b] <= t
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (cu[mid] <= t) lo = mid;
+                if (count(mid) <= t) lo = mid;
                 else hi = mid;
             }
-            const int pos = t - cu[lo], col = pos / page;
+            const int pos = t - count(lo), col = pos / page;
             const int p = pos >= 0 && col < max_pages ? table[(long long)lo * max_pages + col] : -1;
             w = Q4Place{p >= 0 && p < n_pages ? p * (hkv * page_bytes) : kQ4None, pos - col * page};
         }
@@ -159,22 +165,22 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
     }
     __syncthreads();
     const int c = threadIdx.x % kLanes;
-    long long to = ((long long)t0 * hkv + threadIdx.x / kLanes) * D + c * 16;
+    long long to = ((long long)t0 * hkv + threadIdx.x / kLanes) * D + c * 32;
     Q4Walk at(threadIdx.x / kLanes, kRows, hkv);
     while (at.t < n) {   // kAhead rows' loads, then their values
-        uint2 x[kAhead][2];
+        uint4 x[kAhead][2];
         uint32_t codes[kAhead][2];
         unsigned there = 0;
 #pragma unroll
         for (int i = 0; i < kAhead; ++i, at.next()) {
-            x[i][0] = x[i][1] = make_uint2(0x88888888u, 0x88888888u);
+            x[i][0] = x[i][1] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
             codes[i][0] = codes[i][1] = 0;
             const Q4Place w = at.t < n ? where[at.t] : Q4Place{kQ4Skip, 0};
             if (w.begin != kQ4Skip) there |= 1u << i;
             if (w.begin >= 0) {
-                const long long begin = w.begin + at.h * page_bytes, word = begin + w.row * (D / 2) + c * 8, code = begin + (long long)page * (D / 2) + w.row * (D / 32) + c / 2;
-                x[i][0] = *reinterpret_cast<const uint2*>(kc + word);
-                x[i][1] = *reinterpret_cast<const uint2*>(vc + word);
+                const long long begin = w.begin + at.h * page_bytes, word = begin + w.row * (D / 2) + c * 16, code = begin + (long long)page * (D / 2) + w.row * (D / 32) + c;
+                x[i][0] = *reinterpret_cast<const uint4*>(kc + word);
+                x[i][1] = *reinterpret_cast<const uint4*>(vc + word);
                 codes[i][0] = kc[code];
                 codes[i][1] = vc[code];
             }
@@ -186,38 +192,42 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
             for (int j = 0; j < 2; ++j) {
                 // 0x4300 | n is 128 + n in bf16; (128 + n) s - 136 s, exactly: 17 times four bits has eight
                 const __nv_bfloat162 s = __float2bfloat162_rn(0.125f * q4_scale8((int)codes[i][j])), off = __hmul2(s, __float2bfloat162_rn(-136.f));
-                uint32_t out[8];
+                const uint32_t in[4] = {x[i][j].x, x[i][j].y, x[i][j].z, x[i][j].w};
 #pragma unroll
-                for (int word = 0; word < 2; ++word) {
-                    uint32_t y[4];   // channels m and m + 4
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t out[8];
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) {
-                        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y[m]) : "r"((word ? x[i][j].y : x[i][j].x) >> (4 * m)), "n"(0x000f000f), "r"(k128));
-                        const __nv_bfloat162 z = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&y[m]), s, off);
-                        y[m] = *reinterpret_cast<const uint32_t*>(&z);
+                    for (int word = 0; word < 2; ++word) {
+                        uint32_t y[4];   // channels m and m + 4
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y[m]) : "r"(in[2 * half + word] >> (4 * m)), "n"(0x000f000f), "r"(k128));
+                            const __nv_bfloat162 z = __hfma2(*reinterpret_cast<__nv_bfloat162*>(&y[m]), s, off);
+                            y[m] = *reinterpret_cast<const uint32_t*>(&z);
+                        }
+                        out[4 * word] = __byte_perm(y[0], y[1], 0x5410);
+                        out[4 * word + 1] = __byte_perm(y[2], y[3], 0x5410);
+                        out[4 * word + 2] = __byte_perm(y[0], y[1], 0x7632);
+                        out[4 * word + 3] = __byte_perm(y[2], y[3], 0x7632);
                     }
-                    out[4 * word] = __byte_perm(y[0], y[1], 0x5410);
-                    out[4 * word + 1] = __byte_perm(y[2], y[3], 0x5410);
-                    out[4 * word + 2] = __byte_perm(y[0], y[1], 0x7632);
-                    out[4 * word + 3] = __byte_perm(y[2], y[3], 0x7632);
-                }
-                if (kSectors) {
-                    sm100::st_global_32B((j ? v : k) + to, out);
-                } else {
-                    *reinterpret_cast<uint4*>((j ? v : k) + to) = make_uint4(out[0], out[1], out[2], out[3]);
-                    *reinterpret_cast<uint4*>((j ? v : k) + to + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+                    __nv_bfloat16* p = (j ? v : k) + to + 16 * half;
+                    if (kSectors) {
+                        sm100::st_global_32B(p, out);
+                    } else {
+                        *reinterpret_cast<uint4*>(p) = make_uint4(out[0], out[1], out[2], out[3]);
+                        *reinterpret_cast<uint4*>(p + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+                    }
                 }
             }
         }
     }
 }
 
-// Tokens per CTA: about 128 rows, so that look-ups are few beside the rows, fewer where that leaves SMs without a CTA.
-static int q4_tokens_per_cta(int tokens, int hkv) {
-    int per = 128 / hkv;
-    const int spread = (tokens + 4 * sm_count() - 1) / (4 * sm_count());
-    if (per > spread) per = spread;
-    return per < 1 ? 1 : per;
+// Tokens per CTA: whole waves of CTAs of about 512 rows each, so that look-ups are few beside the rows and the last wave is as full as the others.
+static int q4_tokens_per_cta(int tokens, int hkv, int at_once) {
+    const long long waves = ((long long)tokens * hkv / 512 + at_once / 2) / at_once;
+    const long long ctas = at_once * (waves > 1 ? waves : 1), per = (tokens + ctas - 1) / ctas;
+    return (int)(per < kQ4Threads ? per : kQ4Threads);
 }
 
 template <typename T, int D>
@@ -226,7 +236,7 @@ static cudaError_t launch_append(const CacheQ4& c, const void* k, const void* v,
     constexpr int kV = 16 / sizeof(T);
     bool wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
     for (const long long* s : {ks, vs}) wide = wide && (T_ == 1 || s[0] % kV == 0) && (c.hkv == 1 || s[1] % kV == 0);
-    const int per = q4_tokens_per_cta(T_, c.hkv);
+    const int per = q4_tokens_per_cta(T_, c.hkv, 2 * sm_count());   // four CTAs to an SM, for two tensors
     auto go = [&](auto kernel) {
         LaunchScope ls(K_CACHE_APPEND, st);
         return launch_overlapped(kernel, dim3((unsigned)((T_ + per - 1) / per), 2), kQ4Threads, 0, st, (const T*)k, (const T*)v, slots, T_, per, c.hkv, ks[0], ks[1], vs[0], vs[1],
@@ -240,7 +250,7 @@ cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, cons
     return bf16 ? launch_append<__nv_bfloat16, 64>(c, k, v, ks, vs, slots, T, st) : launch_append<float, 64>(c, k, v, ks, vs, slots, T, st);
 }
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st) {
-    const int per = q4_tokens_per_cta(total, c.hkv);
+    const int per = q4_tokens_per_cta(total, c.hkv, 5 * sm_count());
     const unsigned grid = (unsigned)((total + per - 1) / per);
     LaunchScope ls(K_CACHE_READ, st);
     auto go = [&](auto kernel) {
