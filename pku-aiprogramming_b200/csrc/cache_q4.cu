@@ -223,11 +223,13 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
     }
 }
 
-// Tokens per CTA: whole waves of CTAs of about 512 rows each, so that look-ups are few beside the rows and the last wave is as full as the others.
-static int q4_tokens_per_cta(int tokens, int hkv, int at_once) {
-    const long long waves = ((long long)tokens * hkv / 512 + at_once / 2) / at_once;
-    const long long ctas = at_once * (waves > 1 ? waves : 1), per = (tokens + ctas - 1) / ctas;
-    return (int)(per < kQ4Threads ? per : kQ4Threads);
+// Tokens per CTA: about `rows` rows, so that look-ups are few beside them, fewer where that leaves SMs without a CTA.  47,000 tokens of 8 heads:
+// writing 47 / 45 / 46 us at 128 / 256 / 512 rows, reading 39.5 / 43.6 / 46.3.
+static int q4_tokens_per_cta(int tokens, int hkv, int rows) {
+    int per = rows / hkv;
+    const int spread = (tokens + 4 * sm_count() - 1) / (4 * sm_count());
+    if (per > spread) per = spread;
+    return per < 1 ? 1 : per;
 }
 
 template <typename T, int D>
@@ -236,7 +238,7 @@ static cudaError_t launch_append(const CacheQ4& c, const void* k, const void* v,
     constexpr int kV = 16 / sizeof(T);
     bool wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
     for (const long long* s : {ks, vs}) wide = wide && (T_ == 1 || s[0] % kV == 0) && (c.hkv == 1 || s[1] % kV == 0);
-    const int per = q4_tokens_per_cta(T_, c.hkv, 2 * sm_count());   // four CTAs to an SM, for two tensors
+    const int per = q4_tokens_per_cta(T_, c.hkv, 256);
     auto go = [&](auto kernel) {
         LaunchScope ls(K_CACHE_APPEND, st);
         return launch_overlapped(kernel, dim3((unsigned)((T_ + per - 1) / per), 2), kQ4Threads, 0, st, (const T*)k, (const T*)v, slots, T_, per, c.hkv, ks[0], ks[1], vs[0], vs[1],
@@ -250,7 +252,7 @@ cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, cons
     return bf16 ? launch_append<__nv_bfloat16, 64>(c, k, v, ks, vs, slots, T, st) : launch_append<float, 64>(c, k, v, ks, vs, slots, T, st);
 }
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st) {
-    const int per = q4_tokens_per_cta(total, c.hkv, 5 * sm_count());
+    const int per = q4_tokens_per_cta(total, c.hkv, 128);
     const unsigned grid = (unsigned)((total + per - 1) / per);
     LaunchScope ls(K_CACHE_READ, st);
     auto go = [&](auto kernel) {
