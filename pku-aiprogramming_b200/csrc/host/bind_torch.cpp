@@ -495,11 +495,12 @@ const Tensor* vector_arg(PyObject* o, at::ScalarType type, int64_t n, const Tens
     const Tensor* t = on_device(o, type, like);
     return t && t->is_contiguous() && t->dim() == 1 && (n < 0 || t->size(0) == n) ? t : nullptr;
 }
-// The k-th of the caller's output vectors, or a new one; null where the caller's does not fit.
-const Tensor* out_vector(PyObject* given, Py_ssize_t k, int64_t n, const Tensor& like, Tensor* made) {
-    if (given != Py_None) return vector_arg(PyTuple_GET_ITEM(given, k), at::kInt, n, &like);
-    *made = make({n}, at::kInt, like);
-    return made;
+// n elements of a vector from `at` on, on its storage: a few short results cost one allocation (0.9 us each)
+Tensor part_of(const Tensor& whole, int64_t at, int64_t n) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    t.unsafeGetTensorImpl()->set_storage_offset(at);
+    return t;
 }
 PyObject* item_or(PyObject* given, Py_ssize_t k, const Tensor& made) { return wrap_or(given == Py_None ? Py_None : PyTuple_GET_ITEM(given, k), made); }
 bool tuple_arg(PyObject* o, Py_ssize_t n) { return o == Py_None || (PyTuple_Check(o) && PyTuple_GET_SIZE(o) == n); }
@@ -528,8 +529,13 @@ PyObject* cache_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Tensor made[5];
         const Tensor* out[5];
         const int64_t sizes[5] = {B, 1, B + 1, tokens, tokens};
-        for (int i = 0; i < 5; ++i)
-            if (!(out[i] = out_vector(a[7], i, sizes[i], *table, &made[i]))) Py_RETURN_NONE;
+        if (a[7] == Py_None) {
+            const Tensor all = make({2 * (B + 1 + tokens)}, at::kInt, *table);
+            for (int64_t i = 0, at = 0; i < 5; at += sizes[i++]) out[i] = &(made[i] = part_of(all, at, sizes[i]));
+        } else {
+            for (int i = 0; i < 5; ++i)
+                if (!(out[i] = vector_arg(PyTuple_GET_ITEM(a[7], i), at::kInt, sizes[i], table))) Py_RETURN_NONE;
+        }
         auto at = [&](int i) { return (int32_t*)ptr(out[i]); };
         TT_CALL(rc, tt_cache_extend((int32_t*)ptr(table), (const int32_t*)ptr(lens), (const int32_t*)ptr(fresh), (const int32_t*)ptr(pages),
                                     (const int32_t*)ptr(n_free), (int32_t)B, (int32_t)page, (int32_t)table->size(1), (int32_t)pages->numel(),
@@ -555,8 +561,11 @@ PyObject* cache_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
         OnDevice dev(*table);
         Tensor made[2];
         const Tensor* out[2];
-        for (int i = 0; i < 2; ++i)
-            if (!(out[i] = out_vector(a[6], i, i ? 1 : B, *table, &made[i]))) Py_RETURN_NONE;
+        const Tensor all = a[6] == Py_None ? make({B + 1}, at::kInt, *table) : Tensor();
+        for (int i = 0; i < 2; ++i) {
+            if (a[6] == Py_None) out[i] = &(made[i] = part_of(all, i ? B : 0, i ? 1 : B));
+            else if (!(out[i] = vector_arg(PyTuple_GET_ITEM(a[6], i), at::kInt, i ? 1 : B, table))) Py_RETURN_NONE;
+        }
         TT_CALL(rc, tt_cache_release((const int32_t*)ptr(table), (const int32_t*)ptr(lens), (const uint8_t*)ptr(done), (int32_t*)ptr(pages),
                                      (const int32_t*)ptr(n_free), (int32_t)B, (int32_t)page, (int32_t)table->size(1), (int32_t)pages->numel(),
                                      (int32_t*)ptr(out[0]), (int32_t*)ptr(out[1]), dev.stream));

@@ -98,8 +98,10 @@ static cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t st) {
     const int turned = kNeighbours ? (kV == 1 ? a.R / 2 : a.R / kV) : a.R / 2 / kV, copied = (a.D - a.R) / kV, units = turned + copied;
     const dim3 block(units, kRotaryThreads / units);
     const long long n_tok = (long long)a.B * a.S, heads = a.heads[0] + a.heads[1];
-    // about eight units per thread and CTA where there are tokens enough for four CTAs per SM
-    long long per = 8LL * block.y / heads, spread = (n_tok + 4LL * sm_count() - 1) / (4LL * sm_count());
+    // About four units per thread and CTA where there are tokens enough for twelve CTAs per SM: the sines of one run under the rows of others.
+    // 16384 tokens of 40 heads, bf16: 60.1 / 58.2 / 59.6 / 75 us at 2 / 3 / 6 / 24 tokens per CTA; gradients of 4096 tokens of 16 heads, D = 64,
+    // float: 8.9 / 9.1 / 13.0 / 26.6.  (Two rows loaded ahead of the sines, 80 registers: 85 us.)
+    long long per = 4LL * block.y / heads, spread = (n_tok + 12LL * sm_count() - 1) / (12LL * sm_count());
     if (per > spread) per = spread;
     const long long fits = 40 * 1024 / ((a.R / 2 + 1) * sizeof(float2));   // at most 128 pairs: 40 tokens
     if (per > fits) per = fits;

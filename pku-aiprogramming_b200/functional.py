@@ -224,7 +224,7 @@ def cache_extend(block_table, seq_lens, new_lens, free_pages, n_free, page_size,
     `CacheStep` to write into; it must not share memory with the inputs, so a loop keeps two and takes them in turn."""
     r = _native.cache_extend(block_table, seq_lens, new_lens, free_pages, n_free, page_size, max_tokens, out)
     if r.__class__ is tuple:
-        return CacheStep._make(r)
+        return tuple.__new__(CacheStep, r)
     i32 = (torch.int32,)
     return _done(r, lambda: _explain_tables(block_table, seq_lens, [
         ("new_lens", new_lens, block_table.shape[0], i32), ("free_pages", free_pages, None, i32), ("n_free", n_free, 1, i32)], out,
