@@ -133,6 +133,57 @@ void SoftmaxBackward(const TinyTensor<T>& output, const TinyTensor<T>& grad_outp
 
 namespace {
 template <typename T>
+void rotate(const char* who, const TinyTensor<T>& x, TinyTensor<T>& y, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
+            const TinyTensor<int>& axes, bool interleaved, float scale, int backward) {
+    require_gpu(x, who, "input"); require_gpu(positions, who, "positions"); require_gpu(inv_freq, who, "inv_freq"); require_gpu(axes, who, "axes");
+    if (x.shape.size() != 4) throw std::invalid_argument(std::string(who) + ": input must be 4-D [B,H,S,D]");
+    const int B = x.shape[0], H = x.shape[1], S = x.shape[2], D = x.shape[3];
+    const std::vector<int>& p = positions.shape;
+    if ((p.size() != 2 && p.size() != 3) || p.back() != S || (p.size() == 3 && p[1] != B))
+        throw std::invalid_argument(std::string(who) + ": positions must be [axes,S] or [axes,B,S]");
+    if (axes.size != inv_freq.size) throw std::invalid_argument(std::string(who) + ": inv_freq and axes must hold one value per pair");
+    if (y.device != "gpu") y.gpu();
+    y.resize(x.shape);
+    tt_rotary_desc d = {};
+    d.B = B; d.S = S; d.H = H; d.D = D;
+    d.R = (int)(2 * inv_freq.size);
+    d.n_axes = p[0];
+    d.dtype = std::is_same<T, float>::value ? TT_F32 : TT_BF16;
+    d.interleaved = interleaved ? 1 : 0;
+    d.scale = scale;
+    const int64_t stride[3] = {(int64_t)H * S * D, (int64_t)S * D, D};
+    for (int i = 0; i < 3; ++i) d.q_stride[i] = d.q_out_stride[i] = stride[i];
+    d.pos_stride[0] = p.size() == 3 ? (int64_t)B * S : S;
+    d.pos_stride[1] = p.size() == 3 ? S : 0;
+    int rc = tt_rotary(&d, x.p_data, nullptr, positions.p_data, inv_freq.p_data, axes.p_data, backward, y.p_data, nullptr, nullptr);
+    if (rc == TT_OK) rc = tt_check_device_status(nullptr);
+    raise(rc, who);
+}
+}  // namespace
+
+template <typename T>
+void RotaryForward(const TinyTensor<T>& input, TinyTensor<T>& output, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
+                   const TinyTensor<int>& axes, bool interleaved, float scale) {
+    rotate("RotaryForward", input, output, positions, inv_freq, axes, interleaved, scale, 0);
+}
+
+template <typename T>
+void RotaryBackward(const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
+                    const TinyTensor<int>& axes, bool interleaved, float scale) {
+    rotate("RotaryBackward", grad_output, grad_input, positions, inv_freq, axes, interleaved, scale, 1);
+}
+
+#define TT_INSTANTIATE_ROTARY(T)                                                                                                                   \
+    template void RotaryForward<T>(const TinyTensor<T>&, TinyTensor<T>&, const TinyTensor<int>&, const TinyTensor<double>&, const TinyTensor<int>&, \
+                                   bool, float);                                                                                                   \
+    template void RotaryBackward<T>(const TinyTensor<T>&, TinyTensor<T>&, const TinyTensor<int>&, const TinyTensor<double>&,                        \
+                                    const TinyTensor<int>&, bool, float);
+TT_INSTANTIATE_ROTARY(float)
+TT_INSTANTIATE_ROTARY(__nv_bfloat16)
+#undef TT_INSTANTIATE_ROTARY
+
+namespace {
+template <typename T>
 void fc_dims(const TinyTensor<T>& input, const TinyTensor<T>& weight, const TinyTensor<T>& bias, const char* who,
              long long& rows, int& fin, int& fout, bool& scalar_bias) {
     require_gpu(input, who, "input"); require_gpu(weight, who, "weight"); require_gpu(bias, who, "bias");

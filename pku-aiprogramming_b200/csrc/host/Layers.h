@@ -33,6 +33,17 @@ void SoftmaxForward(const TinyTensor<T>& input, TinyTensor<T>& output);
 template <typename T>
 void SoftmaxBackward(const TinyTensor<T>& output, const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input);
 
+// output = input [B,H,S,D] turned by positions [axes,S] or [axes,B,S]: pair i of the first 2 * inv_freq.size channels by
+// positions[axes[i]] * inv_freq[i], channels i and i + inv_freq.size or, interleaved, 2i and 2i + 1, times scale; the
+// other channels are copied.  inv_freq and axes hold one value per pair.
+template <typename T>
+void RotaryForward(const TinyTensor<T>& input, TinyTensor<T>& output, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
+                   const TinyTensor<int>& axes, bool interleaved, float scale);
+// grad_input of sum(output * grad_output): turned the other way.
+template <typename T>
+void RotaryBackward(const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
+                    const TinyTensor<int>& axes, bool interleaved, float scale);
+
 // output[..., out] = input[..., in] . weight[in, out] + bias, bias of shape [out] or [1] (one value
 // for every output) -- signature and semantics of the reference's FcForward (src/Layers.cu:9-40).
 // T = float (fp32 arithmetic) or __nv_bfloat16 (tcgen05 kernel, fp32 accumulation).

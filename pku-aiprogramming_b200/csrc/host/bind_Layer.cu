@@ -26,6 +26,17 @@ PYBIND11_MODULE(myLayer, m) {
           py::arg("scale") = 0.0f);
     m.def("SoftmaxForward", &SoftmaxForward<float>, py::call_guard<py::gil_scoped_release>());
     m.def("SoftmaxBackward", &SoftmaxBackward<float>, py::call_guard<py::gil_scoped_release>());
+    m.def("RotaryForward", &RotaryForward<float>, py::call_guard<py::gil_scoped_release>(), py::arg("input"), py::arg("output"),
+          py::arg("positions"), py::arg("inv_freq"), py::arg("axes"), py::arg("interleaved") = false, py::arg("scale") = 1.0f);
+    m.def("RotaryBackward", &RotaryBackward<float>, py::call_guard<py::gil_scoped_release>(), py::arg("grad_output"),
+          py::arg("grad_input"), py::arg("positions"), py::arg("inv_freq"), py::arg("axes"), py::arg("interleaved") = false,
+          py::arg("scale") = 1.0f);
+    m.def("RotaryForward_bf16", &RotaryForward<__nv_bfloat16>, py::call_guard<py::gil_scoped_release>(), py::arg("input"),
+          py::arg("output"), py::arg("positions"), py::arg("inv_freq"), py::arg("axes"), py::arg("interleaved") = false,
+          py::arg("scale") = 1.0f);
+    m.def("RotaryBackward_bf16", &RotaryBackward<__nv_bfloat16>, py::call_guard<py::gil_scoped_release>(), py::arg("grad_output"),
+          py::arg("grad_input"), py::arg("positions"), py::arg("inv_freq"), py::arg("axes"), py::arg("interleaved") = false,
+          py::arg("scale") = 1.0f);
     // argument orders of the reference's FcForward / FcBackward (src/bind_Layer.cpp:12-13 there)
     m.def("FcForward", &FcForward<float>, py::call_guard<py::gil_scoped_release>());
     m.def("FcBackward", &FcBackward<float>, py::call_guard<py::gil_scoped_release>());

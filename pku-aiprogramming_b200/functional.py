@@ -17,6 +17,7 @@ from typing import NamedTuple
 import torch
 
 from . import capi
+from .rotary_table import rotary_table
 
 
 def _load_binding():
@@ -350,25 +351,9 @@ def rotary_frequencies(rotary_dim, base=10000.0, sections=None, cyclic=False, ow
     `sections`: the pairs of each axis, `rotary_dim / 2` in all (None: one axis).  Pairs go to the axes section by section, or
     with `cyclic` in turn, as long as an axis has some left.  Pair i of n turns by `base ** (-i / n)` per position;
     with `own_ladder` each axis counts its own pairs, i.e. it has slow and fast ones as an axis alone would."""
-    n = int(rotary_dim) // 2
-    sections = [n] if sections is None else [int(s) for s in sections]
-    if int(rotary_dim) != 2 * n or n < 1:
-        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
-    if any(s < 0 for s in sections) or sum(sections) != n:
-        raise ValueError(f"sections {sections} must add up to rotary_dim / 2 = {n}")
-    if not base > 0:
-        raise ValueError("base must be positive")
-    if cyclic:
-        axes = [a for turn in range(max(sections)) for a, s in enumerate(sections) if turn < s]
-    else:
-        axes = [a for a, s in enumerate(sections) for _ in range(s)]
-    seen = [0] * len(sections)
-    freq = []
-    for i, a in enumerate(axes):
-        freq.append(float(base) ** -((seen[a] / sections[a]) if own_ladder else i / n))
-        seen[a] += 1
-    inv_freq = torch.tensor(freq, dtype=torch.float64, device=device)
-    return inv_freq, (torch.tensor(axes, dtype=torch.int32, device=device) if len(sections) > 1 else None)
+    freq, axes, n_axes = rotary_table(rotary_dim, base, sections, cyclic, own_ladder)
+    return (torch.tensor(freq, dtype=torch.float64, device=device),
+            torch.tensor(axes, dtype=torch.int32, device=device) if n_axes > 1 else None)
 
 
 def _explain_rotary(q, k, positions, inv_freq, axes, out_q, out_k):

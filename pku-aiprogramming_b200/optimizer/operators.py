@@ -9,7 +9,7 @@ from this module gives the same numbers on the CPU (that composition is what the
 the kernels against).
 
 Device-resident nodes: `Tensor(x, device="gpu")` keeps a `myTensor` tensor as the node's data
-instead of a NumPy array, so a chain of device-capable ops (`Attention`, `Softmax`, `+`, `-`,
+instead of a NumPy array, so a chain of device-capable ops (`Attention`, `Rotary`, `Softmax`, `+`, `-`,
 scalar `*`, unary `-`, and the reverse sweep's adjoint sums) never leaves the GPU -- the
 reference's GPU ops go through `get_data()` -> Python list -> `np.array` on every call
 (operators.py:56-58, 511 there).  Ops without a device implementation refuse device inputs
@@ -24,6 +24,7 @@ from typing import Optional
 
 import numpy as np
 
+from ..rotary_table import rotary_table
 from .engine import Op, Value, backward_pass
 
 _HOST = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "host_modules")
@@ -514,6 +515,70 @@ class Softmax(TensorOp):
 
 def softmax(x):
     return Softmax()(x)
+
+
+class Rotary(TensorOp):
+    """Heads `[B,H,S,D]` turned by their positions on the GPU (`myLayer.RotaryForward` / `RotaryBackward`): queries and keys
+    ahead of `Attention`.  `positions`: whole numbers `[axes,S]`, `[axes,B,S]` or, with one axis, `[S]`; `rotary_dim` (D), `base`,
+    `sections`, `cyclic` and `own_ladder` say which axis and frequency each pair of channels has (see `rotary_table`);
+    pairs are channels i and i + rotary_dim / 2, or `interleaved` 2i and 2i + 1; `scale` multiplies the result.
+    NumPy-backed input is uploaded (`dtype` picks float32 or bf16 kernels), device-resident input stays, as does its gradient."""
+    device_ok = True
+
+    def __init__(self, positions, rotary_dim: Optional[int] = None, base: float = 10000.0, sections=None, cyclic: bool = False,
+                 own_ladder: bool = False, interleaved: bool = False, scale: float = 1.0, dtype: str = "float32"):
+        if dtype not in ("float32", "bfloat16"):
+            raise ValueError("dtype must be 'float32' or 'bfloat16'")
+        p = np.asarray(positions)
+        if p.dtype.kind not in "iu" or p.ndim not in (1, 2, 3):
+            raise ValueError("positions must be whole numbers [S], [axes,S] or [axes,B,S]")
+        if p.size and (int(p.min()) < -2 ** 31 or int(p.max()) >= 2 ** 31):
+            raise ValueError("positions must fit 32 bits")
+        self.positions = p.astype(np.int32).reshape((1,) * (2 - p.ndim) + p.shape)
+        self.table = lambda D: rotary_table(D if rotary_dim is None else rotary_dim, base, sections, cyclic, own_ladder)
+        self.interleaved, self.scale, self.dtype = bool(interleaved), float(scale), dtype
+        self._saved = None
+
+    @staticmethod
+    def _names(bf16: bool):
+        mt, ml = _native()
+        return (mt.Tensor_bf16, ml.RotaryForward_bf16, ml.RotaryBackward_bf16) if bf16 else (mt.Tensor_float, ml.RotaryForward, ml.RotaryBackward)
+
+    def compute(self, x):
+        resident = _on_device(x)
+        if resident and type(x).__name__ not in ("Tensor_float", "Tensor_bf16"):
+            raise TypeError("device-resident input must be Tensor_float or Tensor_bf16")
+        T, fwd, _ = self._names(type(x).__name__ == "Tensor_bf16" if resident else self.dtype == "bfloat16")
+        tx = x if resident else T(np.ascontiguousarray(x, dtype=np.float32), "gpu")
+        freq, axes, n_axes = self.table(tx.get_shape()[-1])
+        if n_axes != self.positions.shape[0]:
+            raise ValueError(f"positions have {self.positions.shape[0]} axes, sections {n_axes}")
+        mt, _ = _native()
+        rest = (mt.Tensor_int(np.ascontiguousarray(self.positions), "gpu"), mt.Tensor_double(np.array(freq, dtype=np.float64), "gpu"),
+                mt.Tensor_int(np.array(axes, dtype=np.int32), "gpu"), self.interleaved, self.scale)
+        out = T([1], "gpu")
+        fwd(tx, out, *rest)
+        self._saved = (rest, T, resident)
+        return out if resident else out.numpy().astype(x.dtype, copy=False)
+
+    def gradient(self, out_grad, node):
+        if self._saved is None:
+            node.realize_cached_data()
+        rest, T, resident = self._saved
+        _, _, bwd = self._names(T.__name__ == "Tensor_bf16")
+        g = out_grad.realize_cached_data()
+        if _on_device(g) and type(g) is not T:
+            raise TypeError(f"upstream gradient is {type(g).__name__}, the op ran on {T.__name__}")
+        tg = g if _on_device(g) else T(np.ascontiguousarray(g, dtype=np.float32), "gpu")
+        gx = T([1], "gpu")
+        bwd(tg, gx, *rest)
+        if resident:
+            return Tensor(gx, device="gpu", requires_grad=False)
+        return Tensor(gx.numpy().astype(node.inputs[0].dtype, copy=False), requires_grad=False)
+
+
+def rotary(x, positions, **kwargs):
+    return Rotary(positions, **kwargs)(x)
 
 
 class FC(TensorOp):
