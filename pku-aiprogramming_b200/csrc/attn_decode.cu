@@ -501,9 +501,6 @@ template <typename T>
 static cudaError_t launch_tc_merge(const AttnArgs& a, const T* po, const float* plse, int splits, cudaStream_t st) {
     return a.D == 128 ? launch_tc_merge_d<128>(a, po, plse, splits, st) : launch_tc_merge_d<64>(a, po, plse, splits, st);
 }
-cudaError_t attn_decode_merge(const AttnArgs& a, const float* po, const float* plse, int splits, cudaStream_t st) {
-    return launch_tc_merge(a, po, plse, splits, st);
-}
 // Runs the forward view `g` of decode `a`, several key ranges per slice, and merges their results.
 static cudaError_t run_ranges(const AttnArgs& a, AttnArgs g, int splits, void* ws, cudaStream_t st) {
     float* plse = (float*)((unsigned char*)ws + partial_bytes(a, splits));

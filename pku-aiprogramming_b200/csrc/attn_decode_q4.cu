@@ -156,8 +156,10 @@ struct Q4Cursor {
     }
 };
 
-// (Four of 128 registers each: 95.7 us for 97.5 with 64 long sequences, but 14.0 for 12.2 with a single one.)
-constexpr int q4_ctas_per_sm(int D, int NT) { return NT == 1 || D == 64 ? 3 : 2; }
+// What the registers hold.  D = 64, up to eight heads: 140.8 / 112.2 / 113.9 us for 64 sequences of 4096 to 8192 with three / four / five.  D = 128: four
+// of 128 registers are no faster with 64 sequences (95.7 us for 97.5) and slower with one (14.0 for 12.2); up to 16 heads with their queries in shared
+// memory, three of 162 registers: 33.8 for 33.0 with two of 131072, 29.0 for 27.3 with four of 7400.
+constexpr int q4_ctas_per_sm(int D, int NT) { return NT == 1 ? (D == 64 ? 4 : 3) : D == 64 ? 3 : 2; }
 template <int D, int NT>
 constexpr int q4_smem() { return kWarps * kDepth * 2 * Slot<D>::kBytes; }
 
@@ -509,8 +511,9 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
 }
 
 // kT threads per query head: zeros for a sequence without keys, nothing where one warp had the whole slice, else the sum of the parts' rows weighted
-// by exp(log-sum-exp).  What bounds it is latency: the parts' places, then their log-sum-exps and the first rows at once.  A warp (kT = 32) where
-// slices have few parts, 512 threads where they have many.
+// by exp(log-sum-exp).  What bounds it is latency: the parts' places, then their log-sum-exps and the first rows at once; 3 to 6 us behind the other
+// kernel.  Both kernels, with 32 / 128 / 256 / 512 threads a row: 7 parts of 3840 rows 18.3 / 22.8 / 31.2 / 51.3 us, 15 of 1280 rows 28.3 / 27.3 /
+// 30.5 / 37.5, 28 of 512 rows 19.0 / 19.4 / 16.2 / 19.1, 222 of 32 rows 16.9 / 10.7 / 10.1 / 9.9, 1776 of 8 rows 116 / 36 / 24 / 17.5.
 constexpr int kMergeParts = 1024;   // weights held at a time
 template <int D, int kT>
 __global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kernel(const DecodeQ4Args a, int heads, int rows_all, int w_all) {
@@ -525,8 +528,8 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kern
         if (kT == 32) __syncwarp();
         else __syncthreads();
     };
-    grid_let_next_start();
     grid_wait_for_previous();
+    grid_let_next_start();   // (before the wait the next call's CTAs crowd in among the first kernel's: 34.4 us for 27.7 with 32 sequences of up to 4000)
     const unsigned first = a.before[b], steps = a.before[b + 1] - first, total = a.before[a.B] * per_b;
     __nv_bfloat16* out = a.out + (long long)row * D;
     if (steps == 0) {
@@ -639,6 +642,12 @@ bool attn_decode_q4_fits(const AttnArgs& a) {
 }
 size_t attn_decode_q4_workspace(const AttnArgs& a) { return a.group <= 8 ? q4_layout<1>(a, nullptr, nullptr) : q4_layout<2>(a, nullptr, nullptr); }
 
+template <int D, int kT>
+static cudaError_t launch_q4_merge(const DecodeQ4Args& g, const AttnArgs& a, int n_warps, cudaStream_t st) {
+    constexpr int kRows = kT == 32 ? 4 : 1;
+    LaunchScope ls(K_DECODE_MERGE, st);
+    return launch_overlapped(attn_decode_q4_merge_kernel<D, kT>, (unsigned)((a.BH + kRows - 1) / kRows), kT * kRows, 0, st, g, a.H, (int)a.BH, n_warps);
+}
 template <int D, int NT>
 static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* table, const int* lens, int max_pages, void* ws, cudaStream_t st) {
     DecodeQ4Args g = {};
@@ -659,11 +668,12 @@ static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* tab
         e = launch_overlapped(attn_decode_q4_kernel<D, NT>, (unsigned)ctas, kWarps * 32, q4_smem<D, NT>(), st, g);
         if (e != cudaSuccess) return e;
     }
-    LaunchScope ls(K_DECODE_MERGE, st);
-    // parts of a slice if all were of the greatest length: up to a dozen rows are one warp's
-    const bool few = (long long)ctas * kWarps <= 12 * (a.BH / a.group) * g.head_tiles;
-    if (few) return launch_overlapped(attn_decode_q4_merge_kernel<D, 32>, (unsigned)((a.BH + 3) / 4), 128, 0, st, g, a.H, (int)a.BH, ctas * kWarps);
-    return launch_overlapped(attn_decode_q4_merge_kernel<D, 512>, (unsigned)a.BH, 512, 0, st, g, a.H, (int)a.BH, ctas * kWarps);
+    // A warp for a row of up to a dozen parts, if all slices were of the greatest length; else as many threads as leave all rows in one wave.
+    const int n_warps = ctas * kWarps;
+    if (n_warps <= 12 * (a.BH / a.group) * g.head_tiles) return launch_q4_merge<D, 32>(g, a, n_warps, st);
+    const long long room = sm_count() * 1024LL;
+    if (a.BH * 512 <= room) return launch_q4_merge<D, 512>(g, a, n_warps, st);
+    return a.BH * 256 <= room ? launch_q4_merge<D, 256>(g, a, n_warps, st) : launch_q4_merge<D, 128>(g, a, n_warps, st);
 }
 cudaError_t attn_decode_q4(const AttnArgs& a, const CacheQ4& c, const int* table, const int* lens, int max_pages, void* ws, cudaStream_t st) {
     if (a.D == 128) return a.group <= 8 ? launch_q4<128, 1>(a, c, table, lens, max_pages, ws, st) : launch_q4<128, 2>(a, c, table, lens, max_pages, ws, st);

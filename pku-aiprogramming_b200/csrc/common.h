@@ -285,8 +285,6 @@ cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* c
 bool attn_decode_q4_fits(const AttnArgs& a);   // its work counts in 32 bits
 size_t attn_decode_q4_workspace(const AttnArgs& a);
 cudaError_t attn_decode_q4(const AttnArgs& a, const CacheQ4& c, const int* block_table, const int* seq_lens, int max_pages, void* workspace, cudaStream_t st);
-// Merge of normalised results [slice, splits, group, D] and their log-sum-exps (attn_decode.cu).
-cudaError_t attn_decode_merge(const AttnArgs& a, const float* po, const float* plse, int splits, cudaStream_t st);
 
 // --- rotary positions (rotary.cu)
 struct RotaryArgs {
