@@ -232,11 +232,13 @@ int tt_cache_release(const int32_t* block_table, const int32_t* seq_lens, const 
  * k_cache, v_cache: [n_pages, Hkv, tt_cache_q4_page_bytes(page_size, D)] bytes each, 16-byte aligned; D 64 or 128, page_size a
  * multiple of 16.  A page holds, for one key/value head, [page_size][D / 2] bytes (channel 2j in the low half of byte j) and then
  * [page_size][D / 32] scale codes, one for 32 channels: 4.25 bits a value.  Code c stands for the scale s = half(c << 7) / 8, i.e. five bits
- * of exponent and three of mantissa; a value is (n - 8) s with n in 0 .. 15, which bf16 holds exactly.
+ * of exponent and three of mantissa; a value is (n - 8) s with n in 0 .. 15, which bf16 holds exactly.  A cache is below 2^37 bytes,
+ * and has less than 2^31 tokens.
  *
  * tt_cache_append_q4: T new tokens' keys and values [T, Hkv, D] (float or bf16, channels next to each other, element strides
  * {token, head}) into their slots (page * page_size + row, as from tt_cache_extend).  A slot that is negative or behind the last page is
- * passed over; no two tokens may have one slot (what such a slot then holds is of either, and may be of both).  Per group: s is
+ * passed over; no two tokens may have one slot (what such a slot then holds is of either, and may be of both).  k and v must not lie
+ * in the cache.  Per group: s is
  * the smallest scale with 7.5 s >= max |x|, n = rint(x / s) (ties to even) held to -8 .. 7, plus 8, so an error is at most s / 2.
  * The largest scale is 896: values beyond 6720 and infinities become the largest.  A group with a NaN reads as NaN.
  *
@@ -258,6 +260,7 @@ int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* bl
  *                  NULL: batch entry b has page b to itself (page_size >= desc->L, n_pages >= B).
  *   seq_lens       [B] or NULL (desc->L each), clamped to 0 .. desc->L; an entry without keys gets out = 0, lse = -inf
  * desc: dtype TT_BF16, S = 1, D 64 or 128, L the longest sequence there may be, at most 2^30; any group H / Hkv.  `lse` may be NULL.
+ * out, lse and the workspace must not overlap each other or an input, so `out` cannot be `q`.
  * Products are exact in what the cache holds; probabilities are rounded to 11 bits, sums are 32-bit.  Results repeat to the bit.
  * Workspace: tt_attn_decode_q4_workspace_bytes(desc) bytes, 256-byte aligned, contents ignored. */
 size_t tt_attn_decode_q4_workspace_bytes(const tt_attn_desc* desc);

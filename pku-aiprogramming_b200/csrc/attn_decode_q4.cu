@@ -117,7 +117,8 @@ struct DecodeQ4Args {
     int part_rows;
 };
 
-// Of `total` steps warp w of `parts` has `per`, one more if it is among the first `rest`.  Counts fit 32 bits: the host sees to it.
+// Of `total` steps warp w of `parts` has `per`, one more if it is among the first `rest`.  The host has batch x heads x L / 32 below 2^31, so counts
+// fit 32 bits.
 constexpr int kLeastSteps = 2;   // of a part
 struct Q4Shares {
     unsigned parts, per, rest;
@@ -635,10 +636,6 @@ static size_t q4_layout(const AttnArgs& a, DecodeQ4Args* g, void* ws) {
         g->head_tiles = tiles;
     }
     return before + po + align256(parts * rows * 4);
-}
-bool attn_decode_q4_fits(const AttnArgs& a) {
-    const int tile = a.group <= 8 ? 8 : 16;
-    return a.BH / a.group * ((a.group + tile - 1) / tile) * ((a.L + kTile - 1LL) / kTile) < (1LL << 31);
 }
 size_t attn_decode_q4_workspace(const AttnArgs& a) { return a.group <= 8 ? q4_layout<1>(a, nullptr, nullptr) : q4_layout<2>(a, nullptr, nullptr); }
 

@@ -282,7 +282,6 @@ cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, cons
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st);
 
 // Decode over it (attn_decode_q4.cu): block_table null: one page per batch entry.
-bool attn_decode_q4_fits(const AttnArgs& a);   // its work counts in 32 bits
 size_t attn_decode_q4_workspace(const AttnArgs& a);
 cudaError_t attn_decode_q4(const AttnArgs& a, const CacheQ4& c, const int* block_table, const int* seq_lens, int max_pages, void* workspace, cudaStream_t st);
 

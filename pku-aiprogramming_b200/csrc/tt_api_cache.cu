@@ -68,20 +68,55 @@ bool rows_apart(const int64_t* st, const int* n, int D) {
     }
     return true;
 }
-// A tensor of rows at strides st: what it spans, and whether that holds nothing else.
+// A tensor of rows of D elements at strides st over extents n, and what it spans.
 struct Rows {
+    const int64_t* st;
+    const int* n;
     Span span;
-    bool dense;
-    Rows(const void* p, const int64_t* st, const int* n, int D, size_t size, const char* name) {
-        int64_t last = D, all = D;
-        for (int i = 0; i < 3; ++i) {
-            if (n[i] > 1) last += st[i] * (n[i] - 1);
-            all *= n[i];
-        }
+    Rows(const void* p, const int64_t* strides, const int* extents, int D, size_t size, const char* name) : st(strides), n(extents) {
+        int64_t last = D;
+        for (int i = 0; i < 3; ++i) last += st[i] * (n[i] - 1);
         span = Span{p, (size_t)last * size, name};
-        dense = last == all;
     }
 };
+// Whether some row of x and some row of y share an element.  Slices of one buffer interleave without meeting: exact where x and y have the same strides
+// and rows apart from each other, else by what they span.
+bool rows_meet(const Rows& x, const Rows& y, int D, size_t size) {
+    if (!overlap(x.span, y.span)) return false;
+    int64_t st[3];
+    int n[3];
+    for (int i = 0; i < 3; ++i) {
+        if (x.n[i] > 1 && y.n[i] > 1 && x.st[i] != y.st[i]) return true;
+        st[i] = x.n[i] > 1 ? x.st[i] : y.st[i];
+        n[i] = x.n[i] > y.n[i] ? x.n[i] : y.n[i];
+    }
+    if (!rows_apart(st, n, D)) return true;
+    // rows i of x and j of y are delta + sum (i - j) st apart; from the largest stride down the rest is less than a stride, so two i - j can cancel it
+    const int64_t delta = ((const char*)x.span.p - (const char*)y.span.p) / (int64_t)size;
+    bool used[3] = {n[0] == 1, n[1] == 1, n[2] == 1};
+    int64_t left[8] = {delta};
+    int count = 1;
+    for (int k = 0; k < 3; ++k) {
+        int d = -1;
+        for (int i = 0; i < 3; ++i)
+            if (!used[i] && (d < 0 || st[i] > st[d])) d = i;
+        if (d < 0) break;
+        used[d] = true;
+        for (int i = count - 1; i >= 0; --i) {
+            const int64_t r = left[i], down = r >= 0 ? r / st[d] : -((-r + st[d] - 1) / st[d]);   // floor
+            for (int e = 0; e < 2; ++e) {
+                int64_t m = -down - e;   // i - j
+                if (m > x.n[d] - 1) m = x.n[d] - 1;
+                if (m < 1 - y.n[d]) m = 1 - y.n[d];
+                left[e ? count + i : i] = r + m * st[d];
+            }
+        }
+        count *= 2;
+    }
+    for (int i = 0; i < count; ++i)
+        if (left[i] < D && left[i] > -D) return true;
+    return false;
+}
 
 }  // namespace
 }  // namespace ttk
@@ -142,8 +177,11 @@ int tt_cache_append_q4(const void* k, const void* v, const int32_t* slots, int32
     if (T && (!k || !v || !slots)) return fail(TT_ERR_NULL, "%s: null pointer", who);
     const size_t size = dtype == TT_BF16 ? 2 : 4;
     if (((uintptr_t)k | (uintptr_t)v) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
+    if (k_stride[0] < 0 || k_stride[1] < 0 || v_stride[0] < 0 || v_stride[1] < 0) return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
     const size_t pool = (size_t)n_pages * Hkv * tt_cache_q4_page_bytes(page_size, D);
-    if (overlap({k_cache, pool, ""}, {v_cache, pool, ""})) return fail(TT_ERR_BAD_SHAPE, "%s: k_cache overlaps v_cache", who);
+    auto bytes = [&](const int64_t* st) { return T ? (size_t)((T - 1) * st[0] + (Hkv - 1) * st[1] + D) * size : 0; };
+    const Span out[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}}, in[] = {{k, bytes(k_stride), "k"}, {v, bytes(v_stride), "v"}, {slots, (size_t)T * 4, "slots"}};
+    if ((rc = check_overlap(who, out, 2, in, 3)) != TT_OK) return rc;
     if ((rc = check_device()) != TT_OK || T == 0 || n_pages == 0) return rc;
     const CacheQ4 c{k_cache, v_cache, n_pages, page_size, Hkv, D};
     const long long ks[2] = {k_stride[0], k_stride[1]}, vs[2] = {v_stride[0], v_stride[1]};
@@ -174,7 +212,6 @@ static int resolve_q4(const char* who, const tt_attn_desc* desc, AttnArgs* a) {
     if (a->S != 1) return fail(TT_ERR_BAD_SHAPE, "%s: S must be 1, got %d", who, a->S);
     if (!a->bf16 || (a->D != 64 && a->D != 128)) return fail(TT_ERR_BAD_DTYPE, "%s: bf16 with D = 64 or 128 only (dtype %d, D %d)", who, desc->dtype, a->D);
     if (a->L > (1 << 30)) return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds 2^30", who, a->L);
-    if (!attn_decode_q4_fits(*a)) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d x %d key/value heads x L=%d is too large", who, desc->B, desc->H / a->group, a->L);
     a->causal = 0;
     return TT_OK;
 }
@@ -201,7 +238,11 @@ int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cac
     const size_t need = attn_decode_q4_workspace(a);
     if (need && (!workspace || workspace_bytes < need)) return fail(TT_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, workspace_bytes);
     if (need && ((uintptr_t)workspace & 255)) return fail(TT_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
-    if ((rc = check_device()) != TT_OK) return rc;
+    const size_t rows = (size_t)a.BH * a.D * 2, pool = (size_t)n_pages * hkv * tt_cache_q4_page_bytes(page_size, a.D);
+    const Span outs[] = {{out, rows, "out"}, {lse, (size_t)a.BH * 4, "lse"}, {workspace, need, "workspace"}};
+    const Span ins[] = {{q, rows, "q"}, {k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}, {seq_lens, (size_t)desc->B * 4, "seq_lens"},
+                        {block_table, block_table ? (size_t)desc->B * max_pages * 4 : 0, "block_table"}};
+    if ((rc = check_overlap(who, outs, 3, ins, 5)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
     a.q = q; a.out = out; a.lse = lse;
     const CacheQ4 c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, hkv, a.D};
     const cudaError_t e = attn_decode_q4(a, c, block_table, seq_lens, max_pages, workspace, (cudaStream_t)stream);
@@ -231,24 +272,19 @@ int tt_rotary(const tt_rotary_desc* d, const void* q, const void* k, const int32
     if (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
     if (!rows_apart(d->q_out_stride, nq, d->D) || (k && !rows_apart(d->k_out_stride, nk, d->D)))
         return fail(TT_ERR_BAD_SHAPE, "%s: rows of an output overlap", who);
-    // An output lies on its own input row by row, or apart from everything.  Slices of one buffer interleave without
-    // meeting, so spans decide only where both tensors fill theirs.
-    auto same = [](const int64_t* x, const int64_t* y, const int* n) {
-        for (int i = 0; i < 3; ++i)
-            if (n[i] > 1 && x[i] != y[i]) return false;
-        return true;
-    };
+    // An output lies on its own input row by row, or apart from everything.
     const Rows in[2] = {{q, d->q_stride, nq, d->D, size, "q"}, {k, d->k_stride, nk, d->D, size, "k"}};
     const Rows out[2] = {{q_out, d->q_out_stride, nq, d->D, size, "q_out"}, {k_out, d->k_out_stride, nk, d->D, size, "k_out"}};
-    for (int i = 0; i < (k ? 2 : 1); ++i) {
-        for (int j = 0; j < (k ? 2 : 1); ++j) {
-            if (i == j && out[i].span.p == in[j].span.p && same(i ? d->k_out_stride : d->q_out_stride, i ? d->k_stride : d->q_stride, i ? nk : nq)) continue;
-            if (out[i].span.p == in[j].span.p || (out[i].dense && in[j].dense && overlap(out[i].span, in[j].span)))
+    auto in_place = [](const Rows& x, const Rows& y) {
+        for (int i = 0; i < 3; ++i)
+            if (x.n[i] > 1 && x.st[i] != y.st[i]) return false;
+        return x.span.p == y.span.p;
+    };
+    for (int i = 0; i < (k ? 2 : 1); ++i)
+        for (int j = 0; j < (k ? 2 : 1); ++j)
+            if (!(i == j && in_place(out[i], in[j])) && rows_meet(out[i], in[j], d->D, size))
                 return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in[j].span.name);
-        }
-    }
-    if (k && (q_out == k_out || (out[0].dense && out[1].dense && overlap(out[0].span, out[1].span))))
-        return fail(TT_ERR_BAD_SHAPE, "%s: q_out overlaps k_out", who);
+    if (k && rows_meet(out[0], out[1], d->D, size)) return fail(TT_ERR_BAD_SHAPE, "%s: q_out overlaps k_out", who);
     const int rc = check_device();
     if (rc != TT_OK) return rc;
     RotaryArgs a = {};

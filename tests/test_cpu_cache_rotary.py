@@ -110,6 +110,46 @@ def test_rotary_refuses_what_does_not_fit(tt):
     del raw
 
 
+def _elements(at, st, n, D):
+    import numpy as np
+    i = np.indices(n).reshape(3, -1)
+    return set(((at + (i * np.array(st)[:, None]).sum(0))[:, None] + np.arange(D)).reshape(-1).tolist())
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_rotary_outputs_among_the_rows_of_one_buffer(tt, seed):
+    """Slices of one buffer at the same strides, shifted by rows, heads and odd numbers of elements: refused where they share an element, and only there."""
+    import random
+    if torch.cuda.is_available():
+        pytest.skip("the accepted ones would run")
+    lib, c, rng = tt.capi.lib, tt.capi, random.Random(seed)
+    raw, (base,) = _buffers(2, 1 << 16)
+    seen = {True: 0, False: 0}
+    for _ in range(400):
+        D, H, S, B, Hkv = rng.choice([2, 6, 16]), rng.randint(1, 4), rng.randint(1, 5), rng.randint(1, 3), rng.randint(1, 3)
+        width = H + rng.randint(0, 6)
+        st = [(width * S * D, D, width * D), (width * S * D, S * D, D), (D, S * B * D, B * D)][rng.randrange(3)]
+        places = [rng.randrange(0, 8) * D + rng.choice([0, 0, 0, 1, -1]) + 8 for _ in range(2)] + [rng.choice([8, 8 + 4 * D, 8 + S * D]) + 4096 for _ in range(2)]
+        d = _rotary_desc(tt, B=B, H=H, Hkv=Hkv, S=S, D=D, R=2, q_stride=st, q_out_stride=st, k_stride=st, k_out_stride=st)
+        n = ((B, H, S), (B, Hkv, S))
+        q, q_out, k, k_out = [_elements(at, st, n[i // 2], D) for i, at in enumerate(places)]
+        meet = bool((q & q_out and places[0] != places[1]) or (k & k_out and places[2] != places[3]) or q & k_out or k & q_out or q_out & k_out)
+        apart = all(len(e) == B * h * S * D for e, h in ((q_out, H), (k_out, Hkv)))
+        rc = lib.tt_rotary(ctypes.byref(d), *[_at(base, 4 * at) for at in (places[0], places[2])], _at(base, 60000), _at(base, 60000), None, 0,
+                           *[_at(base, 4 * at) for at in (places[1], places[3])], None)
+        if apart:
+            assert rc == (c.TT_ERR_BAD_SHAPE if meet else c.TT_ERR_BAD_DEVICE), (st, places, n, c.last_error())
+            seen[meet] += 1
+        else:
+            assert rc == c.TT_ERR_BAD_SHAPE
+    assert min(seen.values()) > 40
+    # at strides of their own: refused where what they span overlaps
+    d = _rotary_desc(tt, q_out_stride=(4 * 4 * 32, 4 * 32, 32))
+    assert lib.tt_rotary(ctypes.byref(d), base, None, _at(base, 60000), _at(base, 60000), None, 0, _at(base, 4 * 64), None, None) == c.TT_ERR_BAD_SHAPE
+    assert lib.tt_rotary(ctypes.byref(d), base, None, _at(base, 60000), _at(base, 60000), None, 0, _at(base, 4 * 512), None, None) == c.TT_ERR_BAD_DEVICE
+    del raw
+
+
 def test_calls_on_cpu_tensors_are_refused(tt):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present")
@@ -150,7 +190,8 @@ def test_q4_cache_refuses_what_does_not_fit(tt):
 
     assert append(D=96) == c.TT_ERR_UNSUPPORTED and append(dtype=7) == c.TT_ERR_BAD_DTYPE
     for kw in (dict(page=8), dict(page=24), dict(page=0), dict(hkv=0), dict(pages=-1), dict(pages=1 << 27, page=16), dict(T=-1), dict(T=1 << 30, hkv=2), dict(kc=_at(kc, 8)), dict(vc=_at(vc, 4)),
-               dict(vc=kc), dict(vc=_at(kc, 16 * 34 * 2)), dict(k=_at(k, 2)), dict(k=_at(k, 1), dtype=1)):
+               dict(vc=kc), dict(vc=_at(kc, 16 * 34 * 2)), dict(k=_at(k, 2)), dict(k=_at(k, 1), dtype=1), dict(ks=(ctypes.c_int64 * 2)(-128, 64)),
+               dict(k=kc), dict(v=_at(kc, 3200)), dict(k=_at(vc, -4 * (3 * 128 + 127))), dict(slots=_at(vc, 3200)), dict(pages=2 ** 26, page=16, hkv=256)):
         assert append(**kw) == c.TT_ERR_BAD_SHAPE, kw
     for kw in (dict(k=None), dict(v=None), dict(slots=None), dict(kc=None), dict(vc=None), dict(ks=None), dict(vs=None)):
         assert append(**kw) == c.TT_ERR_NULL, kw
@@ -187,14 +228,16 @@ def test_q4_decode_refuses_what_does_not_fit(tt):
     raw, p = _buffers(10, 1 << 16)
     q, kc, vc, table, lens, out, ws = p[:7]
 
-    def call(q=q, kc=kc, vc=vc, table=table, pages=9, page=16, max_pages=4, out=out, ws=ws, ws_bytes=1 << 16, desc=None, **kw):
+    def call(q=q, kc=kc, vc=vc, table=table, pages=9, page=16, max_pages=4, out=out, lse=None, ws=ws, ws_bytes=1 << 16, **kw):
         a = dict(B=2, H=4, S=1, L=50, D=64, dtype=c.TT_BF16, Hkv=2)
         a.update(kw)
         d = c.make_desc(a["B"], a["H"], a["S"], a["L"], a["D"], a["dtype"], False, a.get("scale"), Hkv=a["Hkv"])
-        return lib.tt_attn_decode_q4(ctypes.byref(d), q, kc, vc, table, lens, pages, page, max_pages, out, None, ws, ws_bytes, None)
+        return lib.tt_attn_decode_q4(ctypes.byref(d), q, kc, vc, table, lens, pages, page, max_pages, out, lse, ws, ws_bytes, None)
 
     for kw in (dict(S=2), dict(L=0), dict(L=65), dict(L=(1 << 30) + 1, max_pages=1 << 27), dict(H=3), dict(B=0), dict(page=8, max_pages=8), dict(page=24), dict(max_pages=3), dict(pages=-1),
-               dict(q=_at(q, 2)), dict(out=_at(out, 8)), dict(kc=_at(kc, 8)), dict(table=None, page=48), dict(table=None, page=64, pages=1), dict(scale=math.inf)):
+               dict(q=_at(q, 2)), dict(out=_at(out, 8)), dict(kc=_at(kc, 8)), dict(table=None, page=48), dict(table=None, page=64, pages=1), dict(scale=math.inf),
+               dict(out=q), dict(out=_at(q, 16)), dict(out=_at(kc, 256)), dict(out=vc), dict(out=ws), dict(ws=kc), dict(lse=out), dict(lse=_at(q, 64)), dict(lse=lens),
+               dict(lse=table), dict(pages=2 ** 26, Hkv=128, H=128), dict(B=1 << 20, H=1 << 12)):
         assert call(**kw) == c.TT_ERR_BAD_SHAPE, kw
     for kw in (dict(D=96), dict(dtype=c.TT_F32)):
         assert call(**kw) == c.TT_ERR_BAD_DTYPE, kw

@@ -117,6 +117,20 @@ def test_many_slices_and_one_long_sequence(tt):
         c.check(*tt.attention_decode_q4(**c.args()))
 
 
+@pytest.mark.parametrize("B,H,hkv,D,longest", [(16, 32, 4, 128, 900), (10, 128, 8, 128, 700), (12, 64, 4, 64, 900), (20, 64, 4, 64, 700), (3, 300, 1, 64, 2500), (700, 2, 1, 64, 70)])
+def test_many_rows_of_many_parts(tt, B, H, hkv, D, longest):
+    """Every width of the merge, with a short and an empty sequence among the others; and nothing but empty ones."""
+    rng = np.random.default_rng(B)
+    lens = rng.integers(longest // 2, longest + 1, B).tolist()
+    lens[B // 2], lens[-1] = 0, 1
+    c = Case(lens, H, hkv, D, 16)
+    a = c.args()
+    c.check(*tt.attention_decode_q4(**a))
+    a["seq_lens"].zero_()
+    out, lse = tt.attention_decode_q4(**a)
+    assert not out.any() and (lse == -np.inf).all()
+
+
 @pytest.mark.parametrize("G", [1, 8, 16])
 def test_scores_that_rise(tt, G):
     """Every tile's scores pass the ones before: the reference is raised again and again, in every warp and range."""
@@ -312,7 +326,7 @@ def test_refusals(tt):
     for kw in (dict(q=q.float()), dict(q=q[:, :, 0]), dict(q=q.expand(2, 4, 2, 64)), dict(q=q.cpu()), dict(q=q[:, :3].contiguous()), dict(q=torch.zeros(2, 4, 1, 128, device="cuda").bfloat16()),
                dict(q=torch.zeros(2, 4, 1, 32, device="cuda").bfloat16()), dict(k_cache=a["k_cache"].int()), dict(v_cache=a["v_cache"][:1]), dict(k_cache=a["k_cache"].cpu()),
                dict(block_table=t.long()), dict(block_table=t[:1]), dict(block_table=t[0]), dict(block_table=None), dict(seq_lens=n.long()), dict(seq_lens=n[:1]), dict(max_len=10 ** 6),
-               dict(max_len=2 ** 32 + 16), dict(max_len=0), dict(out=torch.zeros(2, 4, 1, 64, device="cuda")), dict(out=q[:1]), dict(lse=torch.zeros(2, 4, device="cuda")), dict(workspace=5),
+               dict(max_len=2 ** 32 + 16), dict(max_len=0), dict(out=torch.zeros(2, 4, 1, 64, device="cuda")), dict(out=q[:1]), dict(out=q), dict(lse=torch.zeros(2, 4, device="cuda")), dict(workspace=5),
                dict(scale=float("nan"))):
         with pytest.raises(ValueError):
             tt.attention_decode_q4(**{**a, **kw})
