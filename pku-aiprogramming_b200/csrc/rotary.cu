@@ -21,28 +21,55 @@ template <typename T, int kV> struct alignas(sizeof(T) * kV) RtVec { T v[kV]; };
 
 constexpr int kRotaryThreads = 256;
 
+// A token's rows of one of the two tensors: of head 0 in the input and the output.
+template <typename T> struct alignas(16) RtRows {
+    const T* x;
+    T* y;
+};
+
 // kV values per access.  A unit of work is `kV` pairs in halves, or kV / 2 neighbouring pairs (one pair at kV = 1), or kV
 // channels behind R; blockDim = {units per head, rows at a time}.
 template <typename T, int kV, bool kNeighbours>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a, int tokens_per_cta, int turned) {
-    extern __shared__ float2 cs[];   // [tokens_per_cta][R / 2] scale * (cos, sin), and behind them each token's batch entry and row
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a, int tokens_per_cta, int turned, float per_half) {
     using Vec = RtVec<T, kV>;
+    constexpr int kPairs = kNeighbours && kV > 1 ? kV / 2 : kV;   // of a unit
+    extern __shared__ float4 sm[];
+    RtRows<T>* rows = reinterpret_cast<RtRows<T>*>(sm);   // [tokens_per_cta][2]
+    // [tokens_per_cta][R / 2] scale * (cos, sin), two pairs of a unit beside each other and then the same two of the next unit, so that what a
+    // warp reads at a time is whole banks
+    float2* cs = reinterpret_cast<float2*>(rows + 2 * tokens_per_cta);
     const int half = a.R / 2, tid = threadIdx.y * blockDim.x + threadIdx.x, n_threads = blockDim.x * blockDim.y;
     const unsigned t0 = blockIdx.x * (unsigned)tokens_per_cta, n_tok = (unsigned)a.B * (unsigned)a.S;
     const int here = (int)min((unsigned)tokens_per_cta, n_tok - t0);
-    int2* where = reinterpret_cast<int2*>(cs + tokens_per_cta * half);
+    const unsigned b0 = a.B > 1 ? t0 / (unsigned)a.S : 0;
+    auto place = [&](int t, int* b, int* s) {
+        unsigned x = t0 - b0 * (unsigned)a.S + t, y = b0;
+        while (x >= (unsigned)a.S) {
+            x -= (unsigned)a.S;
+            ++y;
+        }
+        *b = (int)y;
+        *s = (int)x;
+    };
     grid_let_next_start();
     grid_wait_for_previous();
     for (int i = tid; i < here * half; i += n_threads) {
-        const int t = i / half, pair = i - t * half;
-        const unsigned at = t0 + t, b = at / (unsigned)a.S, s = at - b * (unsigned)a.S;
-        if (pair == 0) where[t] = make_int2((int)b, (int)s);
+        const int t = (int)(((float)i + 0.5f) * per_half), pair = i - t * half;   // i < 2^13: exact
+        int b, s;
+        place(t, &b, &s);
         const int axis = a.axes ? min(max(a.axes[pair], 0), a.n_axes - 1) : 0;
-        const int p = a.pos[axis * a.pos_axis + (long long)b * a.pos_batch + s];
+        const int p = a.pos[axis * a.pos_axis + b * a.pos_batch + s];
         const double turns = (double)p * a.inv_freq[pair] * 0.15915494309189533576888;   // / 2 pi
         float sn, co;
         sincospif((float)(2.0 * (turns - rint(turns))), &sn, &co);
-        cs[i] = make_float2(a.scale * co, a.back ? -a.scale * sn : a.scale * sn);
+        const int u = pair / kPairs, e = pair % kPairs;
+        cs[t * half + (kPairs == 1 ? u : 2 * ((e >> 1) * turned + u) + (e & 1))] = make_float2(a.scale * co, a.back ? -a.scale * sn : a.scale * sn);
+    }
+    for (int i = n_threads - 1 - tid; i < 2 * here; i += n_threads) {
+        int b, s;
+        place(i >> 1, &b, &s);
+        const int w = i & 1;
+        rows[i] = RtRows<T>{(const T*)a.x[w] + b * a.xs[w][0] + s * a.xs[w][2], (T*)a.y[w] + b * a.ys[w][0] + s * a.ys[w][2]};
     }
     __syncthreads();
     const int u = threadIdx.x, heads = a.heads[0] + a.heads[1];
@@ -57,20 +84,32 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
         ++t;
     }
     while (t < here) {
-        const int which = h >= a.heads[0], head = which ? h - a.heads[0] : h;
-        const int2 w = where[t];
-        const T* x = (const T*)a.x[which] + w.x * a.xs[which][0] + head * a.xs[which][1] + w.y * a.xs[which][2];
-        T* y = (T*)a.y[which] + w.x * a.ys[which][0] + head * a.ys[which][1] + w.y * a.ys[which][2];
+        const bool second = h >= a.heads[0];
+        const int head = second ? h - a.heads[0] : h;
+        const RtRows<T> r = rows[2 * t + second];
+        const T* x = r.x + head * (second ? a.xs[1][1] : a.xs[0][1]);
+        T* y = r.y + head * (second ? a.ys[1][1] : a.ys[0][1]);
         if (turn) {
             Vec v0 = *reinterpret_cast<const Vec*>(x + c0), v1;
             if (two) v1 = *reinterpret_cast<const Vec*>(x + c1);
-            const float2* f = cs + t * half + (kNeighbours && kV > 1 ? u * (kV / 2) : u * kV);
+            const float2* from = cs + t * half + (kPairs == 1 ? u : 2 * u);
+            float2 f[kPairs];
+            if (kPairs == 1) {
+                f[0] = *from;
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPairs; e += 2) {
+                    const float4 z = *reinterpret_cast<const float4*>(from + e * turned);
+                    f[e] = make_float2(z.x, z.y);
+                    f[(e + 1) % kPairs] = make_float2(z.z, z.w);
+                }
+            }
             if (two) {
 #pragma unroll
                 for (int e = 0; e < kV; ++e) {
                     const float x1 = rt_get(v0.v[e]), x2 = rt_get(v1.v[e]);
-                    v0.v[e] = rt_put<T>(x1 * f[e].x - x2 * f[e].y);
-                    v1.v[e] = rt_put<T>(x2 * f[e].x + x1 * f[e].y);
+                    v0.v[e] = rt_put<T>(x1 * f[e % kPairs].x - x2 * f[e % kPairs].y);
+                    v1.v[e] = rt_put<T>(x2 * f[e % kPairs].x + x1 * f[e % kPairs].y);
                 }
                 *reinterpret_cast<Vec*>(y + c1) = v1;
             } else {
@@ -103,12 +142,13 @@ static cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t st) {
     // float: 8.9 / 9.1 / 13.0 / 26.6.  (Two rows loaded ahead of the sines, 80 registers: 85 us.)
     long long per = 4LL * block.y / heads, spread = (n_tok + 12LL * sm_count() - 1) / (12LL * sm_count());
     if (per > spread) per = spread;
-    const long long fits = 40 * 1024 / ((a.R / 2 + 1) * sizeof(float2));   // at most 128 pairs: 40 tokens
+    const size_t token = (size_t)a.R / 2 * sizeof(float2) + 2 * sizeof(RtRows<T>);
+    const long long fits = 40 * 1024 / (long long)token;   // at most 128 pairs: 38 tokens
     if (per > fits) per = fits;
     if (per < 1) per = 1;
     LaunchScope ls(K_ROTARY, st);
-    return launch_overlapped(rotary_kernel<T, kV, kNeighbours>, (unsigned)((n_tok + per - 1) / per), block, (size_t)per * (a.R / 2 + 1) * sizeof(float2), st, a,
-                             (int)per, turned);
+    return launch_overlapped(rotary_kernel<T, kV, kNeighbours>, (unsigned)((n_tok + per - 1) / per), block, (size_t)per * token, st, a, (int)per, turned,
+                             2.f / (float)a.R);
 }
 template <typename T>
 static cudaError_t launch_rotary_type(const RotaryArgs& a, int interleaved, cudaStream_t st) {
