@@ -138,8 +138,10 @@ static cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t st) {
     const dim3 block(units, kRotaryThreads / units);
     const long long n_tok = (long long)a.B * a.S, heads = a.heads[0] + a.heads[1];
     // About four units per thread and CTA where there are tokens enough for twelve CTAs per SM: the sines of one run under the rows of others.
-    // 16384 tokens of 40 heads, bf16: 60.1 / 58.2 / 59.6 / 75 us at 2 / 3 / 6 / 24 tokens per CTA; gradients of 4096 tokens of 16 heads, D = 64,
-    // float: 8.9 / 9.1 / 13.0 / 26.6.  (Two rows loaded ahead of the sines, 80 registers: 85 us.)
+    // 16384 tokens of 40 heads, bf16: 55.1 / 53.3 / 53.5 / 55.8 / 59.6 us at 1 / 2 / 3 / 6 / 12 tokens per CTA (5.9 to 6.3 TB/s); gradients of 4096 tokens
+    // of 16 heads, D = 64, float: 7.7 / 6.4 / 6.7 / 7.9 / 12.0.  Fewer tokens and heads are bound by the sines: 15240 tokens of three heads, R = 256: 13.6
+    // where the rows take 7.3.  (Two rows loaded ahead of the sines, 80 registers: 85 us.  Angles as products of 64-bit integers: 0.5 us slower, but 12.5
+    // with three heads.)
     long long per = 4LL * block.y / heads, spread = (n_tok + 12LL * sm_count() - 1) / (12LL * sm_count());
     if (per > spread) per = spread;
     const size_t token = (size_t)a.R / 2 * sizeof(float2) + 2 * sizeof(RtRows<T>);

@@ -204,3 +204,13 @@ def test_neighbouring_memory_stays(tt):
             tt.rotary_forward(q.t, None, torch.arange(T, dtype=torch.int32, device="cuda"), freq, out_q=out.t)
             torch.cuda.synchronize()
             assert q.intact() and out.intact()
+
+
+def test_frequencies_beyond_a_turn_and_not_finite(tt):
+    """Several turns a position, half a turn exactly, both signs; a frequency that is no number makes its pair so and no other."""
+    freq = torch.tensor([100.0, -7.0, np.pi, -np.pi, 1e-30, 2e5, float("nan"), float("inf")], dtype=torch.float64, device="cuda")
+    pos = torch.tensor([0, 1, 3, -5, 123456, -99999], dtype=torch.int32, device="cuda")
+    x = torch.randn(6, 2, 20, device="cuda")
+    got, _ = tt.rotary_forward(x, None, pos, freq, interleaved=True)
+    assert got[..., 12:16].isnan().all() and torch.equal(got[..., 16:], x[..., 16:])
+    check(torch.cat([got[..., :12], got[..., 16:]], -1), torch.cat([x[..., :12], x[..., 16:]], -1), pos.cpu().numpy()[None, :, None], freq[:6], None, True)
