@@ -2,7 +2,7 @@
 //
 // Both are bound by HBM -- D = 128 in bf16 is 256 bytes a token and head, its codes are 68 -- once the arithmetic is out of the way.  In writing
 // that is the work per group, so a thread has a whole one (32 channels, K and V apart): 20,000 tokens of 8 heads 34.8 us with four lanes to a
-// group, which meet for its maximum, 21.5 so.  In reading it is the number of memory instructions: a whole group to a thread there too, as 16 bytes
+// group, which meet for its maximum, 21.5 so, 19.8 with bf16 kept in pairs (40 registers for 64).  In reading it is the number of memory instructions: a whole group to a thread there too, as 16 bytes
 // and one, and four stores of a sector each.
 #include "cache_q4.cuh"
 #include "sm100_ptx.cuh"
@@ -11,66 +11,78 @@ namespace ttk {
 
 constexpr int kQ4Threads = 256;
 
-// 32 channels of a group, and the bits of the largest |x|: ordered as the values, with NaN above infinity.
-template <bool kWide>
-__device__ __forceinline__ unsigned q4_load32(const __nv_bfloat16* p, float (&x)[32]) {
+// 32 channels of a group as they come, bf16 in pairs.
+template <typename T> struct Q4Group;
+template <> struct Q4Group<__nv_bfloat16> {
     uint32_t w[16];
+    template <bool kWide> __device__ __forceinline__ void load(const __nv_bfloat16* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (kWide) {
-            const uint4 r = *reinterpret_cast<const uint4*>(p + 8 * i);
-            w[4 * i] = r.x; w[4 * i + 1] = r.y; w[4 * i + 2] = r.z; w[4 * i + 3] = r.w;
-        } else {
-            const unsigned short* q = reinterpret_cast<const unsigned short*>(p) + 8 * i;
+        for (int i = 0; i < 4; ++i) {
+            if (kWide) {
+                const uint4 r = *reinterpret_cast<const uint4*>(p + 8 * i);
+                w[4 * i] = r.x; w[4 * i + 1] = r.y; w[4 * i + 2] = r.z; w[4 * i + 3] = r.w;
+            } else {
+                const unsigned short* q = reinterpret_cast<const unsigned short*>(p) + 8 * i;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[4 * i + j] = q[2 * j] | (uint32_t)q[2 * j + 1] << 16;
+                for (int j = 0; j < 4; ++j) w[4 * i + j] = q[2 * j] | (uint32_t)q[2 * j + 1] << 16;
+            }
         }
     }
-    uint32_t top = 0;
+    __device__ __forceinline__ unsigned top() const {   // the bits of the largest |x|: ordered as the values, with NaN above infinity
+        uint32_t y = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        top = __vmaxu2(top, w[i] & 0x7fff7fffu);
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < 16; ++i) y = __vmaxu2(y, w[i] & 0x7fff7fffu);
+        return max(y << 16, y & 0xffff0000u);
     }
-    return max(top << 16, top & 0xffff0000u);
-}
-template <bool kWide>
-__device__ __forceinline__ unsigned q4_load32(const float* p, float (&x)[32]) {
-    unsigned top = 0;
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+    __device__ __forceinline__ void put(int i, float x) {   // x exact in bf16
+        const uint32_t y = __float_as_uint(x);
+        w[i >> 1] = i & 1 ? (w[i >> 1] & 0xffffu) | y : (w[i >> 1] & 0xffff0000u) | y >> 16;
+    }
+};
+template <> struct Q4Group<float> {
+    float x[32];
+    template <bool kWide> __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (kWide) {
-            const float4 r = *reinterpret_cast<const float4*>(p + 4 * i);
-            x[4 * i] = r.x; x[4 * i + 1] = r.y; x[4 * i + 2] = r.z; x[4 * i + 3] = r.w;
-        } else {
+        for (int i = 0; i < 8; ++i) {
+            if (kWide) {
+                const float4 r = *reinterpret_cast<const float4*>(p + 4 * i);
+                x[4 * i] = r.x; x[4 * i + 1] = r.y; x[4 * i + 2] = r.z; x[4 * i + 3] = r.w;
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[4 * i + j] = p[4 * i + j];
+                for (int j = 0; j < 4; ++j) x[4 * i + j] = p[4 * i + j];
+            }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[4 * i + j]) & 0x7fffffffu);
     }
-    return top;
-}
+    __device__ __forceinline__ unsigned top() const {
+        unsigned y = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y = max(y, __float_as_uint(x[i]) & 0x7fffffffu);
+        return y;
+    }
+    __device__ __forceinline__ float get(int i) const { return x[i]; }
+    __device__ __forceinline__ void put(int i, float y) { x[i] = y; }
+};
 
 // A group's four words and its code.  The levels are added up as they are, four bits apart: each is 1.5 2^23's bits plus -8 .. 7, and what that comes
 // to without the levels' own 8 is a constant.
 template <typename T>
-__device__ __forceinline__ uint4 q4_encode(float (&x)[32], unsigned top, int* code) {
+__device__ __forceinline__ uint4 q4_encode(Q4Group<T>& x, int* code) {
+    const unsigned top = x.top();
     float s8;
     *code = q4_code(__uint_as_float(min(top, 0x7f800000u)), &s8);
     const float s = 0.125f * s8, inv = *code ? q4_reciprocal(s) : 0.f;
-    if (!(__uint_as_float(top) <= 7.5f * s)) {   // beyond the largest scale, or no number
+    if (!(__uint_as_float(top) <= 7.5f * s)) {   // beyond the largest scale (7.5 of which, 6720, bf16 holds), or no number
         if (top > 0x7f800000u) *code = kQ4NaN;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = top > 0x7f800000u ? 0.f : fminf(fmaxf(x[i], -7.5f * s), 7.5f * s);
+        for (int i = 0; i < 32; ++i) x.put(i, top > 0x7f800000u ? 0.f : fminf(fmaxf(x.get(i), -7.5f * s), 7.5f * s));
     }
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         w[j] = 0;
 #pragma unroll
-        for (int i = 7; i >= 0; --i) w[j] = (w[j] << 4) + (sizeof(T) == 2 ? q4_level_bf16(x[8 * j + i], inv) : q4_level_f32(x[8 * j + i], s, inv));
+        for (int i = 7; i >= 0; --i) w[j] = (w[j] << 4) + (sizeof(T) == 2 ? q4_level_bf16(x.get(8 * j + i), inv) : q4_level_f32(x.get(8 * j + i), s, inv));
         w[j] += 0x88888888u - kQ4Bits * 0x11111111u;
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
@@ -121,10 +133,10 @@ __global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __
     for (Q4Walk at(threadIdx.x / kLanes, kRows, hkv); at.t < n; at.next()) {
         const Q4Place w = where[at.t];
         if (w.begin == kQ4Skip) continue;
-        float x[32];
-        const unsigned top = q4_load32<kWide>(from + at.t * tok + at.h * head, x);
+        Q4Group<T> x;
+        x.template load<kWide>(from + at.t * tok + at.h * head);
         int code;
-        const uint4 words = q4_encode<T>(x, top, &code);
+        const uint4 words = q4_encode<T>(x, &code);
         unsigned char* to = into + w.begin + at.h * page_bytes;
         *reinterpret_cast<uint4*>(to + w.row * (D / 2) + c * 16) = words;
         to[(long long)page * (D / 2) + w.row * (D / 32) + c] = (unsigned char)code;
@@ -223,10 +235,11 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
     }
 }
 
-// Tokens per CTA: about `rows` rows, so that look-ups are few beside them, fewer where that leaves SMs without a CTA.  47,000 tokens of 8 heads:
-// writing 47 / 45 / 46 us at 128 / 256 / 512 rows, reading 39.5 / 43.6 / 46.3.
-static int q4_tokens_per_cta(int tokens, int hkv, int rows) {
-    int per = rows / hkv;
+// Tokens per CTA: about 128 rows, so that look-ups are few beside them, fewer where that leaves SMs without a CTA.  20,000 tokens of 8 heads, D = 128:
+// writing bf16 20.8 / 19.8 / 21.9 / 22.8 us at 64 / 128 / 256 / 512 rows (5.3 TB/s at 128), float 46.0 / 46.1 / 48.9 / 46.8 (bound by the arithmetic of
+// its ties); 47,000 tokens: reading 39.5 / 43.6 / 46.3 at 128 / 256 / 512 (6.0 TB/s at 128).
+static int q4_tokens_per_cta(int tokens, int hkv) {
+    int per = 128 / hkv;
     const int spread = (tokens + 4 * sm_count() - 1) / (4 * sm_count());
     if (per > spread) per = spread;
     return per < 1 ? 1 : per;
@@ -238,7 +251,7 @@ static cudaError_t launch_append(const CacheQ4& c, const void* k, const void* v,
     constexpr int kV = 16 / sizeof(T);
     bool wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
     for (const long long* s : {ks, vs}) wide = wide && (T_ == 1 || s[0] % kV == 0) && (c.hkv == 1 || s[1] % kV == 0);
-    const int per = q4_tokens_per_cta(T_, c.hkv, 256);
+    const int per = q4_tokens_per_cta(T_, c.hkv);
     auto go = [&](auto kernel) {
         LaunchScope ls(K_CACHE_APPEND, st);
         return launch_overlapped(kernel, dim3((unsigned)((T_ + per - 1) / per), 2), kQ4Threads, 0, st, (const T*)k, (const T*)v, slots, T_, per, c.hkv, ks[0], ks[1], vs[0], vs[1],
@@ -252,7 +265,7 @@ cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, cons
     return bf16 ? launch_append<__nv_bfloat16, 64>(c, k, v, ks, vs, slots, T, st) : launch_append<float, 64>(c, k, v, ks, vs, slots, T, st);
 }
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st) {
-    const int per = q4_tokens_per_cta(total, c.hkv, 128);
+    const int per = q4_tokens_per_cta(total, c.hkv);
     const unsigned grid = (unsigned)((total + per - 1) / per);
     LaunchScope ls(K_CACHE_READ, st);
     auto go = [&](auto kernel) {
