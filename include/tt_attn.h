@@ -281,7 +281,7 @@ int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cac
  *   positions      int32, [n_axes, B, S] at strides pos_stride {axis, batch}, rows next to each other; any int32 value
  *   inv_freq       [R / 2] double, angle per position;  axes: [R / 2] int32 in 0 .. n_axes - 1 (others are taken as the nearest),
  *                  or null: all of axis 0
- * D at most 256, R even, dtype TT_F32 or TT_BF16.  16-byte loads where pointers and strides allow them, else one value each. */
+ * D at most 256, R even, dtype TT_F32 or TT_BF16.  Accesses are of up to 16 bytes, as pointers, strides and R allow. */
 typedef struct tt_rotary_desc {
     int32_t B, S, H, Hkv, D, R, n_axes, dtype, interleaved;
     float scale;

@@ -4,8 +4,8 @@
 // it is taken in 64, in turns, less its nearest whole number; the rest, at most half a turn, goes through sincospif.
 //
 // HBM-bound: every value is read and written once.  A CTA takes a few tokens: their R / 2 sines and cosines go to shared memory
-// once (for up to 40 heads that use them), then a thread keeps its place in the head -- 16 bytes of one half and their partners
-// in the other, or 16 bytes of neighbours -- and walks over tokens and heads, so an access of a warp is whole rows.
+// once (for up to 40 heads that use them), then a thread keeps its place in the head -- up to 16 bytes of one half and their partners
+// in the other, or of neighbours -- and walks over tokens and heads, so an access of a warp is whole rows.
 #include "common.h"
 
 namespace ttk {
@@ -27,10 +27,10 @@ template <typename T> struct alignas(16) RtRows {
     T* y;
 };
 
-// kV values per access.  A unit of work is `kV` pairs in halves, or kV / 2 neighbouring pairs (one pair at kV = 1), or kV
-// channels behind R; blockDim = {units per head, rows at a time}.
+// kV values per access.  A unit of work is `kV` pairs in halves, or kV / 2 neighbouring pairs (one pair at kV = 1), or `copied`
+// bytes of the channels behind R; blockDim = {units per head, rows at a time}.
 template <typename T, int kV, bool kNeighbours>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a, int tokens_per_cta, int turned, float per_half) {
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a, int tokens_per_cta, int turned, int copied, float per_half) {
     using Vec = RtVec<T, kV>;
     constexpr int kPairs = kNeighbours && kV > 1 ? kV / 2 : kV;   // of a unit
     extern __shared__ float4 sm[];
@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
     __syncthreads();
     const int u = threadIdx.x, heads = a.heads[0] + a.heads[1];
     const bool turn = u < turned;
-    // the unit's channels: kV at c0, and in halves their partners at c1
-    const int c0 = turn ? (kNeighbours && kV == 1 ? 2 * u : u * kV) : a.R + (u - turned) * kV;
+    // the unit's channels: kV at c0, and in halves their partners at c1; or `copied` bytes behind R
+    const int c0 = kNeighbours && kV == 1 ? 2 * u : u * kV, copy_at = (u - turned) * copied;
     const int c1 = kNeighbours ? c0 + 1 : c0 + half;
     const bool two = turn && (!kNeighbours || kV == 1);
     int t = 0, h = threadIdx.y;
@@ -122,7 +122,12 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
             }
             *reinterpret_cast<Vec*>(y + c0) = v0;
         } else if (x != y) {
-            *reinterpret_cast<Vec*>(y + c0) = *reinterpret_cast<const Vec*>(x + c0);
+            const char* from = reinterpret_cast<const char*>(x + a.R) + copy_at;
+            char* to = reinterpret_cast<char*>(y + a.R) + copy_at;
+            if (copied == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+            else if (copied == 8) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(from);
+            else if (copied == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+            else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
         }
         h += blockDim.y;
         while (h >= heads) {
@@ -133,8 +138,11 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
 }
 
 template <typename T, int kV, bool kNeighbours>
-static cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t st) {
-    const int turned = kNeighbours ? (kV == 1 ? a.R / 2 : a.R / kV) : a.R / 2 / kV, copied = (a.D - a.R) / kV, units = turned + copied;
+static cudaError_t launch_rotary(const RotaryArgs& a, int aligned, cudaStream_t st) {
+    const int behind = (a.D - a.R) * (int)sizeof(T);
+    int copied = aligned;   // the widest copies that begin and end where these channels do
+    while ((a.R * (int)sizeof(T)) % copied || behind % copied) copied /= 2;
+    const int turned = kNeighbours ? (kV == 1 ? a.R / 2 : a.R / kV) : a.R / 2 / kV, units = turned + behind / copied;
     const dim3 block(units, kRotaryThreads / units);
     const long long n_tok = (long long)a.B * a.S, heads = a.heads[0] + a.heads[1];
     // About four units per thread and CTA where there are tokens enough for twelve CTAs per SM: the sines of one run under the rows of others.
@@ -149,21 +157,30 @@ static cudaError_t launch_rotary(const RotaryArgs& a, cudaStream_t st) {
     if (per > fits) per = fits;
     if (per < 1) per = 1;
     LaunchScope ls(K_ROTARY, st);
-    return launch_overlapped(rotary_kernel<T, kV, kNeighbours>, (unsigned)((n_tok + per - 1) / per), block, (size_t)per * token, st, a, (int)per, turned,
+    return launch_overlapped(rotary_kernel<T, kV, kNeighbours>, (unsigned)((n_tok + per - 1) / per), block, (size_t)per * token, st, a, (int)per, turned, copied,
                              2.f / (float)a.R);
+}
+// kV: the most values that can be turned at a time, from rows that lie at multiples of `aligned` bytes.  10,356 tokens of 40 heads of 80 bf16 channels,
+// R = 20 and 40 in halves (2 and 4 values), 20.5 us of bytes: 53.5 and 37.4 us, 68.5 and 45.1 with copies as narrow, 88.9 and 92.0 with one value at
+// a time.  Bound by the instructions per access.
+template <typename T, int kV>
+static cudaError_t launch_rotary_width(const RotaryArgs& a, int interleaved, int aligned, cudaStream_t st) {
+    if constexpr (kV > 1) {
+        if ((int)(kV * sizeof(T)) > aligned || (interleaved ? a.R : a.R / 2) % kV) return launch_rotary_width<T, kV / 2>(a, interleaved, aligned, st);
+    }
+    return interleaved ? launch_rotary<T, kV, true>(a, aligned, st) : launch_rotary<T, kV, false>(a, aligned, st);
 }
 template <typename T>
 static cudaError_t launch_rotary_type(const RotaryArgs& a, int interleaved, cudaStream_t st) {
-    constexpr int kV = 16 / sizeof(T);
-    bool wide = a.D % kV == 0 && (interleaved ? a.R : a.R / 2) % kV == 0;
+    unsigned long long places = 16;   // or-ed: the lowest bit set is what all are multiples of
     for (int i = 0; i < 2; ++i) {
         if (!a.heads[i]) continue;
-        wide = wide && (((uintptr_t)a.x[i] | (uintptr_t)a.y[i]) & 15) == 0;
+        places |= (uintptr_t)a.x[i] | (uintptr_t)a.y[i];
         const int n[3] = {a.B, a.heads[i], a.S};
-        for (int d = 0; d < 3; ++d) wide = wide && (n[d] == 1 || (a.xs[i][d] % kV == 0 && a.ys[i][d] % kV == 0));
+        for (int d = 0; d < 3; ++d)
+            if (n[d] > 1) places |= (unsigned long long)(a.xs[i][d] | a.ys[i][d]) * sizeof(T);
     }
-    if (interleaved) return wide ? launch_rotary<T, kV, true>(a, st) : launch_rotary<T, 1, true>(a, st);
-    return wide ? launch_rotary<T, kV, false>(a, st) : launch_rotary<T, 1, false>(a, st);
+    return launch_rotary_width<T, 16 / sizeof(T)>(a, interleaved, (int)(places & (0 - places)), st);
 }
 cudaError_t rotary(const RotaryArgs& a, int bf16, int interleaved, cudaStream_t st) {
     return bf16 ? launch_rotary_type<__nv_bfloat16>(a, interleaved, st) : launch_rotary_type<float>(a, interleaved, st);

@@ -115,6 +115,25 @@ def test_in_place_and_into_slices(tt, dtype, R):
     assert got[0].data_ptr() == rows.data_ptr()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,R,shift,gap", [(80, 20, 0, 0), (80, 40, 0, 0), (64, 12, 0, 0), (128, 128, 4, 0), (128, 64, 2, 4), (96, 96, 0, 2), (128, 128, 0, 4), (82, 82, 0, 0), (64, 64, 1, 0)])
+def test_every_width_of_access(tt, D, R, shift, gap, dtype, interleaved):
+    """Rows that begin, end or halve at 2, 4 or 8 bytes; the output's rows too, with what lies between them left as it was."""
+    T, H = 29, 3
+    whole = torch.randn(T * H * (D + gap) + shift, device="cuda").to(dtype)
+    x = whole[shift:].view(T, H, D + gap)[..., :D]
+    freq, _ = tt.rotary_frequencies(R)
+    pos = positions(np.random.default_rng(D + R), (1, T), 3000)
+    p = pos.cpu().numpy()[:, :, None]
+    check(tt.rotary_forward(x, None, pos, freq, interleaved=interleaved)[0], x, p, freq, None, interleaved)
+    into = torch.full_like(whole, 7)
+    y = into[shift:].view(T, H, D + gap)
+    got, _ = tt.rotary_backward(x, None, pos, freq, interleaved=interleaved, out_q=y[..., :D])
+    check(got, x, p, freq, None, interleaved, back=True)
+    assert got.data_ptr() == y.data_ptr() and (y[..., D:] == 7).all() and (into[:shift] == 7).all()
+
+
 def test_far_and_negative_positions(tt):
     pos = torch.tensor([0, 1, -1, 2 ** 20 + 1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda")
     x = torch.randn(6, 2, 128, device="cuda")
