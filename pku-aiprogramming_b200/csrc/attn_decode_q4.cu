@@ -7,8 +7,8 @@
 //
 // Both products are m16n8k16 in halves with 32-bit sums (2.0 cycles per SM each; the 8-bit forms of mma.sync are made of these).  A lane
 // reads exactly the nibbles that are its elements of the operand, and the order of channels within a product is chosen so that they are
-// neighbours of one scale.  With 0x6400 above it a nibble is the half 1024 + n, or 1024 + 16 n four bits up, so a mask makes two halves and
-// one fused multiply-add by the scale's multiples (n - 8) s / 16, or (n - 8) s, of them: exactly, for s has four significant bits and
+// neighbours of one scale.  With 0x4800 above it a nibble is the half (1024 + n) / 128, or (1024 + 16 n) / 128 four bits up, so a mask makes two halves and
+// one fused multiply-add by 8 s, which is the scale code's own bit pattern, (n - 8) s / 16, or (n - 8) s, of them: exactly, for s has four significant bits and
 // n - 8 four.  (Masks alone, without that, give n: for q with an outlier the -8 sum q then cancels in the tensor core's sums.)
 //   S^T [16 keys x 8 heads] += K [16 keys x 16 channels] Q^T: lane (g, t) of a warp (g = lane / 4, t = lane % 4) has of keys g and g + 8 the
 //     quarter t of the channels; q, its exponent moved so that a bf16 value down to 2^-27 of the head's largest is exact in half, is 16 times
@@ -74,25 +74,24 @@ __device__ __forceinline__ half2 as_half2(uint32_t x) { return *reinterpret_cast
 __device__ __forceinline__ uint32_t bits(half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
 // What two codes, times 128 in the halves of a word, make of nibbles: s8 = half(code << 7) = 8 s.  The codes that are written (and NaN) leave
-// every constant finite and exact: 9 s8 <= 64512, and 129 / 16 times four significant bits has eleven.
+// every constant finite and exact: 9 s8 <= 8064, and 129 / 16 times four significant bits has eleven.
 struct Scale2 {
-    half2 mul, even, odd;
+    half2 s8, even, odd;
     __device__ __forceinline__ explicit Scale2(uint32_t codes_times_128) {
-        const half2 s8 = as_half2(codes_times_128);
-        mul = __hmul2(s8, __float2half2_rn(1.f / 128));
+        s8 = as_half2(codes_times_128);
         even = __hmul2(s8, __float2half2_rn(-129.f / 16));
         odd = __hmul2(s8, __float2half2_rn(-9.f));
     }
-    // nibbles in the lowest bits of x's halves: (1024 + n) s8 / 128 - 129 s8 / 16 = (n - 8) s / 16
-    __device__ __forceinline__ uint32_t low(uint32_t x, uint32_t k1024) const { return bits(__hfma2(as_half2(masked<0x000f000fu>(x, k1024)), mul, even)); }
-    // four bits higher: (1024 + 16 n) s8 / 128 - 9 s8 = (n - 8) s
-    __device__ __forceinline__ uint32_t high(uint32_t x, uint32_t k1024) const { return bits(__hfma2(as_half2(masked<0x00f000f0u>(x, k1024)), mul, odd)); }
-    // (x & kMask) | k1024 in one instruction, which takes one constant: the other, 0x64006400, comes in a register that the compiler does not
+    // nibbles in the lowest bits of x's halves: (1024 + n) / 128 s8 - 129 / 16 s8 = (n - 8) s / 16
+    __device__ __forceinline__ uint32_t low(uint32_t x, uint32_t k8) const { return bits(__hfma2(as_half2(masked<0x000f000fu>(x, k8)), s8, even)); }
+    // four bits higher: (1024 + 16 n) / 128 s8 - 9 s8 = (n - 8) s
+    __device__ __forceinline__ uint32_t high(uint32_t x, uint32_t k8) const { return bits(__hfma2(as_half2(masked<0x00f000f0u>(x, k8)), s8, odd)); }
+    // (x & kMask) | k8 in one instruction, which takes one constant: the other, 0x48004800, comes in a register that the compiler does not
     // see through
     template <uint32_t kMask>
-    static __device__ __forceinline__ uint32_t masked(uint32_t x, uint32_t k1024) {
+    static __device__ __forceinline__ uint32_t masked(uint32_t x, uint32_t k8) {
         uint32_t y;
-        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(kMask), "r"(k1024));
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "n"(kMask), "r"(k8));
         return y;
     }
 };
@@ -112,7 +111,7 @@ struct DecodeQ4Args {
     const int *table, *lens;
     int B, L, hkv, group, head_tiles, n_pages, page, max_pages;
     float scale_log2;
-    uint32_t k1024;    // 0x64006400, see Scale2
+    uint32_t k8;    // 0x48004800, see Scale2
     __nv_bfloat16* out;
     float* lse;        // may be null
     // Workspace: steps before each batch entry [B + 1] (of one slice), and for every part of a slice that a warp does not have to itself the
@@ -176,7 +175,7 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
     using S = Slot<D>;
     extern __shared__ __align__(128) unsigned char smem[];
     const int lane = threadIdx.x & 31, warp = uniform_warp_idx(), g = lane >> 2, t = lane & 3;
-    const uint32_t k1024 = a.k1024;
+    const uint32_t k8 = a.k8;
     const unsigned char* ring = smem + warp * (kDepth * 2 * S::kBytes);
     const unsigned w_all = gridDim.x * kWarps, w = blockIdx.x + gridDim.x * warp, per_b = a.hkv * a.head_tiles;   // few parts: on different SMs
     grid_let_next_start();
@@ -359,7 +358,7 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {   // channels 0, 4 and 1, 5 of eight, then 2, 6 and 3, 7
                         const uint32_t y0 = x[0][w] >> 8 * h, y1 = x[1][w] >> 8 * h;
-                        const uint32_t a0 = lo.low(y0, k1024), a1 = hi.low(y1, k1024), a2 = lo.high(y0, k1024), a3 = hi.high(y1, k1024);
+                        const uint32_t a0 = lo.low(y0, k8), a1 = hi.low(y1, k8), a2 = lo.high(y0, k8), a3 = hi.high(y1, k8);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             if (w + h == 0) mma_f16_first(s[u][n], a0, a1, a2, a3, qf[n][w][2 * h], qf[n][w][2 * h + 1]);
@@ -469,7 +468,7 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
                     for (int j = 0; j < 4; ++j) {   // byte j: channels 2j and 2j + 1 of the word's eight
                         const uint32_t sel = 0x0400u + 0x0101u * j;
                         const uint32_t x = __byte_perm(r[0][w], r[1][w], sel), y = __byte_perm(r[2][w], r[3][w], sel);
-                        const uint32_t a0 = first.low(x, k1024), a1 = first.high(x, k1024), a2 = second.low(y, k1024), a3 = second.high(y, k1024);
+                        const uint32_t a0 = first.low(x, k8), a1 = first.high(x, k8), a2 = second.low(y, k8), a3 = second.high(y, k8);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) mma_f16(o[w * 4 + j][n], a0, a1, a2, a3, p[u][n][0], p[u][n][1]);
                     }
@@ -660,7 +659,7 @@ static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* tab
     g.B = (int)(a.BH / a.H); g.L = a.L; g.hkv = c.hkv; g.group = a.group;
     g.n_pages = c.n_pages; g.page = c.page_size; g.max_pages = max_pages;
     g.scale_log2 = a.scale * 1.4426950408889634f;
-    g.k1024 = 0x64006400u;
+    g.k8 = 0x48004800u;
     g.out = (__nv_bfloat16*)a.out; g.lse = a.lse;
     q4_layout<NT>(a, &g, ws);
     const int ctas = q4_ctas<NT>(a, g.head_tiles);
