@@ -28,6 +28,7 @@ template <> struct Q4Group<__nv_bfloat16> {
             }
         }
     }
+    __device__ __forceinline__ void chunk(int i, uint4 r) { w[4 * i] = r.x; w[4 * i + 1] = r.y; w[4 * i + 2] = r.z; w[4 * i + 3] = r.w; }
     __device__ __forceinline__ unsigned top() const {   // the bits of the largest |x|: ordered as the values, with NaN above infinity
         uint32_t y = 0;
 #pragma unroll
@@ -53,6 +54,9 @@ template <> struct Q4Group<float> {
                 for (int j = 0; j < 4; ++j) x[4 * i + j] = p[4 * i + j];
             }
         }
+    }
+    __device__ __forceinline__ void chunk(int i, uint4 r) {
+        x[4 * i] = __uint_as_float(r.x); x[4 * i + 1] = __uint_as_float(r.y); x[4 * i + 2] = __uint_as_float(r.z); x[4 * i + 3] = __uint_as_float(r.w);
     }
     __device__ __forceinline__ unsigned top() const {
         unsigned y = 0;
@@ -115,12 +119,19 @@ template <typename T, int D, bool kWide>
 __global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ slots, int n_tok, int tokens_per_cta,
                                                                      int hkv, long long k_tok, long long k_head, long long v_tok, long long v_head,
                                                                      unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, int n_slots, int page) {
-    constexpr int kLanes = D / 32, kRows = kQ4Threads / kLanes;
+    constexpr int kLanes = D / 32, kRows = kQ4Threads / kLanes, kChunks = 2 * sizeof(T);   // 16 bytes each, of a group
+    // A group of floats is a whole line of 128 bytes, so a load of 16 bytes by a thread for itself would touch as many lines as lanes: the lanes of a row
+    // load it together and exchange through shared memory, chunks moved about by the group so that both ways are without bank conflicts (a line has two
+    // groups of bf16, where this costs more than it gives: 22.5 us for 19.9).
+    constexpr bool kStaged = kWide && sizeof(T) == 4;
     __shared__ Q4Place where[kQ4Threads];
+    __shared__ uint4 stage[kStaged ? kRows : 1][kLanes * kChunks + kLanes];
     const int t0 = blockIdx.x * tokens_per_cta, n = min(tokens_per_cta, n_tok - t0), c = threadIdx.x % kLanes;
+    uint4* staged = stage[kStaged ? threadIdx.x / kLanes : 0];
+    const unsigned row_lanes = ((1u << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes);
     const long long page_bytes = (long long)page * q4_row_bytes(D);
     const bool second = blockIdx.y != 0;   // V
-    const T* from = (second ? v : k) + t0 * (second ? v_tok : k_tok) + c * 32;
+    const T* from = (second ? v : k) + t0 * (second ? v_tok : k_tok) + (kStaged ? 0 : c * 32);
     const long long tok = second ? v_tok : k_tok, head = second ? v_head : k_head;
     unsigned char* into = second ? vc : kc;
     grid_let_next_start();
@@ -134,7 +145,20 @@ __global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __
         const Q4Place w = where[at.t];
         if (w.begin == kQ4Skip) continue;
         Q4Group<T> x;
-        x.template load<kWide>(from + at.t * tok + at.h * head);
+        if constexpr (kStaged) {
+            uint4 y[kChunks];
+            const uint4* p = reinterpret_cast<const uint4*>(from + at.t * tok + at.h * head);
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) y[i] = p[i * kLanes + c];
+            __syncwarp(row_lanes);   // (the row before has been read)
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) staged[(i * kLanes + c) ^ ((i * kLanes + c) / kChunks)] = y[i];
+            __syncwarp(row_lanes);
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i) x.chunk(i, staged[(c * kChunks + i) ^ c]);
+        } else {
+            x.template load<kWide>(from + at.t * tok + at.h * head);
+        }
         int code;
         const uint4 words = q4_encode<T>(x, &code);
         unsigned char* to = into + w.begin + at.h * page_bytes;
@@ -236,8 +260,8 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
 }
 
 // Tokens per CTA: about 128 rows, so that look-ups are few beside them, fewer where that leaves SMs without a CTA.  20,000 tokens of 8 heads, D = 128:
-// writing bf16 20.8 / 19.8 / 21.9 / 22.8 us at 64 / 128 / 256 / 512 rows (5.3 TB/s at 128), float 46.0 / 46.1 / 48.9 / 46.8 (bound by the arithmetic of
-// its ties); 47,000 tokens: reading 39.5 / 43.6 / 46.3 at 128 / 256 / 512 (6.0 TB/s at 128).
+// writing bf16 20.8 / 19.8 / 21.9 / 22.8 us at 64 / 128 / 256 / 512 rows (5.3 TB/s at 128), float 37.0 at 128
+// (46.1 with every lane's loads its own; 5.1 TB/s); 47,000 tokens: reading 39.5 / 43.6 / 46.3 at 128 / 256 / 512 (6.0 TB/s at 128).
 static int q4_tokens_per_cta(int tokens, int hkv) {
     int per = 128 / hkv;
     const int spread = (tokens + 4 * sm_count() - 1) / (4 * sm_count());
