@@ -75,7 +75,7 @@ __device__ __forceinline__ uint4 q4_encode(Q4Group<T>& x, int* code) {
     const unsigned top = x.top();
     float s8;
     *code = q4_code(__uint_as_float(min(top, 0x7f800000u)), &s8);
-    const float s = 0.125f * s8, inv = *code ? q4_reciprocal(s) : 0.f;
+    const float s = 0.125f * s8, inv = !*code ? 0.f : sizeof(T) == 2 ? q4_reciprocal(s) : __frcp_rn(s);
     if (!(__uint_as_float(top) <= 7.5f * s)) {   // beyond the largest scale (7.5 of which, 6720, bf16 holds), or no number
         if (top > 0x7f800000u) *code = kQ4NaN;
 #pragma unroll
@@ -115,8 +115,9 @@ struct Q4Walk {
     }
 };
 
+// (Four CTAs per SM with floats: 36.0 us for 38.9 at 20,000 tokens of 8 heads of 128, where the compiler would take 79 registers.)
 template <typename T, int D, bool kWide>
-__global__ void __launch_bounds__(kQ4Threads) cache_append_q4_kernel(const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ slots, int n_tok, int tokens_per_cta,
+__global__ void __launch_bounds__(kQ4Threads, kWide && sizeof(T) == 4 ? 4 : 0) cache_append_q4_kernel(const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ slots, int n_tok, int tokens_per_cta,
                                                                      int hkv, long long k_tok, long long k_head, long long v_tok, long long v_head,
                                                                      unsigned char* __restrict__ kc, unsigned char* __restrict__ vc, int n_slots, int page) {
     constexpr int kLanes = D / 32, kRows = kQ4Threads / kLanes, kChunks = 2 * sizeof(T);   // 16 bytes each, of a group
@@ -260,8 +261,8 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
 }
 
 // Tokens per CTA: about 128 rows, so that look-ups are few beside them, fewer where that leaves SMs without a CTA.  20,000 tokens of 8 heads, D = 128:
-// writing bf16 20.8 / 19.8 / 21.9 / 22.8 us at 64 / 128 / 256 / 512 rows (5.3 TB/s at 128), float 37.0 at 128
-// (46.1 with every lane's loads its own; 5.1 TB/s); 47,000 tokens: reading 39.5 / 43.6 / 46.3 at 128 / 256 / 512 (6.0 TB/s at 128).
+// writing bf16 20.8 / 19.8 / 21.9 / 22.8 us at 64 / 128 / 256 / 512 rows (5.3 TB/s at 128), float 36.0 at 128
+// (46.1 with every lane's loads its own; 5.2 TB/s); 47,000 tokens: reading 39.5 / 43.6 / 46.3 at 128 / 256 / 512 (6.0 TB/s at 128).
 static int q4_tokens_per_cta(int tokens, int hkv) {
     int per = 128 / hkv;
     const int spread = (tokens + 4 * sm_count() - 1) / (4 * sm_count());

@@ -49,15 +49,14 @@ constexpr uint32_t kQ4Bits = 0x4b400000u;   // of 1.5 2^23
 // bf16 x: X 2^c / M with X of eight bits and M of four is either half-way between two integers or at least 2^-5 / 15 away from that, so the quotient
 // is rounded to 2^-10 first, which puts the half-way ones where they belong and lets no other cross.
 __device__ __forceinline__ uint32_t q4_level_bf16(float x, float inv) { return __float_as_uint(fminf(fmaf(x, inv, 12288.f), 12295.f) + (12582912.f - 12288.f)); }
-// float x: the nearest integer by the rounded reciprocal, or the next one; the remainder x - r s is exact (s has four bits, r at most five) and says.
+// float x, `inv` the float nearest to 1 / s.  A quotient that is not half-way between two integers is rounded as it should be: half-way is h s with
+// h s of eight bits, x is at least an ulp away from that, relatively 2^-24 (1 + 2^-8) or more, and inv is off by less than 2^-24 -- or by nothing,
+// where h s is a power of two, below which floats are denser.  Half-way ones may go either way; the remainder x - r s is exact and says.
 __device__ __forceinline__ uint32_t q4_level_f32(float x, float s, float inv) {
-    float t = fminf(fmaf(x, inv, 12582912.f), 12582919.f);
-    const float rem = fmaf(12582912.f - t, s, x), far = fabsf(rem), half_step = 0.5f * s;
-    if (far >= half_step && s > 0.f) {
-        if (far > half_step || (__float_as_uint(t) & 1)) t += copysignf(1.f, rem);
-        t = fminf(fmaxf(t, 12582904.f), 12582919.f);
-    }
-    return __float_as_uint(t);
+    float t = fmaf(x, inv, 12582912.f);
+    const float rem = fmaf(12582912.f - t, s, x);
+    if (fabsf(rem) == 0.5f * s && (__float_as_uint(t) & 1)) t += copysignf(1.f, rem);
+    return __float_as_uint(fminf(t, 12582919.f));
 }
 
 }  // namespace ttk
