@@ -145,15 +145,17 @@ static cudaError_t launch_rotary(const RotaryArgs& a, int aligned, cudaStream_t 
     const int turned = kNeighbours ? (kV == 1 ? a.R / 2 : a.R / kV) : a.R / 2 / kV, units = turned + behind / copied;
     const dim3 block(units, kRotaryThreads / units);
     const long long n_tok = (long long)a.B * a.S, heads = a.heads[0] + a.heads[1];
-    // About four units per thread and CTA where there are tokens enough for twelve CTAs per SM: the sines of one run under the rows of others.
-    // 16384 tokens of 40 heads, bf16: 55.1 / 53.3 / 53.5 / 55.8 / 59.6 us at 1 / 2 / 3 / 6 / 12 tokens per CTA (5.9 to 6.3 TB/s); gradients of 4096 tokens
-    // of 16 heads, D = 64, float: 7.7 / 6.4 / 6.7 / 7.9 / 12.0.  Fewer tokens and heads are bound by the sines: 15240 tokens of three heads, R = 256: 13.6
-    // where the rows take 7.3.  (Two rows loaded ahead of the sines, 80 registers: 85 us.  Angles as products of 64-bit integers: 0.5 us slower, but 12.5
-    // with three heads.)
-    long long per = 4LL * block.y / heads, spread = (n_tok + 12LL * sm_count() - 1) / (12LL * sm_count());
-    if (per > spread) per = spread;
+    // Tokens per CTA: up to four units per thread, the sines of one CTA run under the rows of others; fewer where all CTAs are resident at once then (eight
+    // per SM), and more, up to half as many again, where that leaves no second wave.  With inputs from memory, us at 2 / 3 / 4 / 5 / 7 / 9 tokens: 4096 tokens
+    // of 16 heads of 64 floats 9.7 / 11.8 / 8.5 / 9.9 / 12.2 / 15.3 (4 are one wave); 5000 of 20 heads of 80 bf16 8.7 / 9.7 / 9.4 / 7.7 / 10.0 / 11.7 (5 are);
+    // 8192 of 9 heads of 128 9.9 / 8.6 / 8.9 / 8.9 / 7.9 / 9.6 (7 are); 16384 of 40 heads of 128 53.3 / 53.6 / 53.9 / 55.2 / 56.8 / 58.3, 6.3 TB/s.  Few tokens and
+    // heads are bound by the sines: 15240 tokens of three heads, R = 256: 14 where the rows take 7.3.  (Two rows loaded ahead of the sines, 80 registers: 85 us for
+    // 58.  Angles as products of 64-bit integers: 0.5 us slower, but 12.5 for 13.6 with three heads.)
+    const long long resident = 8LL * sm_count(), one_wave = (n_tok + resident - 1) / resident;
+    long long per = 4LL * block.y / heads;
+    if (per > one_wave || 3 * per >= 2 * one_wave) per = one_wave;
     const size_t token = (size_t)a.R / 2 * sizeof(float2) + 2 * sizeof(RtRows<T>);
-    const long long fits = 40 * 1024 / (long long)token;   // at most 128 pairs: 38 tokens
+    const long long fits = 27 * 1024 / (long long)token;   // eight CTAs' on an SM; at most 128 pairs: 26 tokens
     if (per > fits) per = fits;
     if (per < 1) per = 1;
     LaunchScope ls(K_ROTARY, st);
