@@ -260,13 +260,15 @@ __global__ void __launch_bounds__(kQ4Threads) cache_read_q4_kernel(const unsigne
     }
 }
 
-// Tokens per CTA: about 128 rows, so that look-ups are few beside them, fewer where that leaves SMs without a CTA.  20,000 tokens of 8 heads, D = 128:
-// writing bf16 20.8 / 19.8 / 21.9 / 22.8 us at 64 / 128 / 256 / 512 rows (5.3 TB/s at 128), float 36.0 at 128
-// (46.1 with every lane's loads its own; 5.2 TB/s); 47,000 tokens: reading 39.5 / 43.6 / 46.3 at 128 / 256 / 512 (6.0 TB/s at 128).
-static int q4_tokens_per_cta(int tokens, int hkv) {
+// Tokens per CTA: about 128 rows, so that look-ups are few beside them; fewer where all CTAs are resident at once then (`resident` of them), and more, up
+// to half as many again, where that leaves no second wave.  20,000 tokens of 8 heads, D = 128: writing bf16 20.8 / 19.8 / 21.9 / 22.8 us at 64 / 128 /
+// 256 / 512 rows (5.3 TB/s at 128), float 35.7 at 128 (46.1 with every lane's loads its own; 5.2 TB/s); 47,000 tokens: reading 39.5 / 43.6 / 46.3 at 128 /
+// 256 / 512 (6.0 TB/s at 128).  One wave, for what 128 rows and four CTAs per SM take: writing 8628 tokens of one head 3.2 for 4.4, 6801 of four 4.9 for
+// 5.7, 1000 of two of 64 floats 2.2 for 3.8; reading 25,070 of four heads 12.1 for 13.8.
+static int q4_tokens_per_cta(int tokens, int hkv, int resident) {
     int per = 128 / hkv;
-    const int spread = (tokens + 4 * sm_count() - 1) / (4 * sm_count());
-    if (per > spread) per = spread;
+    const int one_wave = (tokens + resident - 1) / resident;
+    if (per > one_wave || 3 * per >= 2 * one_wave) per = one_wave;
     return per < 1 ? 1 : per;
 }
 
@@ -276,7 +278,7 @@ static cudaError_t launch_append(const CacheQ4& c, const void* k, const void* v,
     constexpr int kV = 16 / sizeof(T);
     bool wide = (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
     for (const long long* s : {ks, vs}) wide = wide && (T_ == 1 || s[0] % kV == 0) && (c.hkv == 1 || s[1] % kV == 0);
-    const int per = q4_tokens_per_cta(T_, c.hkv);
+    const int per = q4_tokens_per_cta(T_, c.hkv, (wide && sizeof(T) == 2 ? 6 : wide ? 4 : 3) * sm_count() / 2);
     auto go = [&](auto kernel) {
         LaunchScope ls(K_CACHE_APPEND, st);
         return launch_overlapped(kernel, dim3((unsigned)((T_ + per - 1) / per), 2), kQ4Threads, 0, st, (const T*)k, (const T*)v, slots, T_, per, c.hkv, ks[0], ks[1], vs[0], vs[1],
@@ -290,7 +292,7 @@ cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, cons
     return bf16 ? launch_append<__nv_bfloat16, 64>(c, k, v, ks, vs, slots, T, st) : launch_append<float, 64>(c, k, v, ks, vs, slots, T, st);
 }
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st) {
-    const int per = q4_tokens_per_cta(total, c.hkv);
+    const int per = q4_tokens_per_cta(total, c.hkv, 5 * sm_count());
     const unsigned grid = (unsigned)((total + per - 1) / per);
     LaunchScope ls(K_CACHE_READ, st);
     auto go = [&](auto kernel) {
