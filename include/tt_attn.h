@@ -262,7 +262,7 @@ int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* bl
  * desc: dtype TT_BF16, S = 1, D 64 or 128, L the longest sequence there may be, at most 2^30; any group H / Hkv.  `lse` may be NULL.
  * out, lse and the workspace must not overlap each other or an input, so `out` cannot be `q`.
  * Products are exact in what the cache holds; probabilities are rounded to 11 bits, sums are 32-bit.  Results repeat to the bit.
- * Workspace: tt_attn_decode_q4_workspace_bytes(desc) bytes, 256-byte aligned, contents ignored. */
+ * Workspace: tt_attn_decode_q4_workspace_bytes(desc) bytes, 256-byte aligned, contents ignored; 0 (and NULL) where L is at most 128. */
 size_t tt_attn_decode_q4_workspace_bytes(const tt_attn_desc* desc);
 int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                       const int32_t* seq_lens, int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse,

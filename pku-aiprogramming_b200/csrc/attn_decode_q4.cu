@@ -25,7 +25,8 @@
 // (a launch with a CTA per range of one slice ended on its last wave: 64 sequences of 4096 to 8192 106 us).  A warp sums the lengths,
 // finds its part, and streams it through a ring of its own in shared memory (cp.async, kDepth steps, on into the next slice's keys where
 // one ends; bulk copies of 1024 and 64 bytes were slower, 107 us for 95).  No warp waits for another.  A slice that one warp has to itself is written at once; of others each warp leaves
-// a normalised result and its log-sum-exp, which a second kernel merges.  Results do not depend on timing.
+// a normalised result and its log-sum-exp, which a second kernel merges.  Results do not depend on timing.  Up to 128 keys a warp has a whole slice, and
+// there is no second kernel.
 //
 // One B200, both kernels, replayed from a graph (bytes at the copy rate of 6.46 TB/s): 64 sequences of 4096 to 8192, 32 query on 8 key/value heads, D = 128 94.5 us
 // (64.8); 48 of up to 4096, 16 on 16, D = 64 39.3 (16.2); two of 120,000 to 131,072, 32 on 2 31.4 (10.5); one of 5001, 32 on 8 10.0 (0.9).  Counters of the
@@ -114,7 +115,7 @@ struct DecodeQ4Args {
     uint32_t k8;    // 0x48004800, see Scale2
     __nv_bfloat16* out;
     float* lse;        // may be null
-    // Workspace: steps before each batch entry [B + 1] (of one slice), and for every part of a slice that a warp does not have to itself the
+    // Workspace, unless every slice is one warp's (null then): steps before each batch entry [B + 1] (of one slice), and for every part of a slice that a warp does not have to itself the
     // normalised rows [part][part_rows][D] and log-sum-exps.  Parts are numbered warp + slice: one of the two grows from each to the next.
     unsigned* before;
     float *po, *plse;
@@ -181,16 +182,31 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
     grid_let_next_start();
     grid_wait_for_previous();
 
-    // the batch's steps, and where this warp's part begins
-    unsigned sum = 0;
-    for (int i = lane; i < a.B; i += 32) sum += q4_steps(q4_len(a, i));
-    const unsigned total = __reduce_add_sync(0xffffffffu, sum) * per_b;
-    const Q4Shares shares(total, w_all, a.B * per_b);
-    if (w >= shares.parts) return;
-    const unsigned x0 = shares.begin(w);
-    const int n = (int)(shares.begin(w + 1) - x0);
     Q4Cursor now{0, 0, 0};   // of the step at hand
-    {
+    unsigned x0;             // the part's first step, and how many it has
+    int n;
+    if (!a.before) {   // a slice to a warp
+        if (w >= a.B * per_b) return;
+        now.b = w / per_b;
+        now.len = q4_len(a, now.b);
+        n = (int)q4_steps(now.len);
+        x0 = (w - now.b * per_b) * n;   // (with the batch entry's own first step as 0)
+        if (n == 0) {
+            const int slice_b = w - now.b * per_b, h0 = slice_b % a.head_tiles * kHeads, n_heads = min(kHeads, a.group - h0);
+            const long long row0 = ((long long)now.b * a.hkv + slice_b / a.head_tiles) * a.group + h0;
+            for (int i = lane; i < n_heads * (D / 8); i += 32) reinterpret_cast<uint4*>(a.out + row0 * D)[i] = make_uint4(0, 0, 0, 0);
+            if (lane < n_heads && a.lse) a.lse[row0 + lane] = -INFINITY;
+            return;
+        }
+    } else {
+        // the batch's steps, and where this warp's part begins
+        unsigned sum = 0;
+        for (int i = lane; i < a.B; i += 32) sum += q4_steps(q4_len(a, i));
+        const unsigned total = __reduce_add_sync(0xffffffffu, sum) * per_b;
+        const Q4Shares shares(total, w_all, a.B * per_b);
+        if (w >= shares.parts) return;
+        x0 = shares.begin(w);
+        n = (int)(shares.begin(w + 1) - x0);
         const unsigned y = x0 / per_b;
         unsigned done = 0;
         int found = -1;
@@ -621,6 +637,10 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kern
     if (tid == 0 && a.lse) a.lse[row] = den == 0.f ? -INFINITY : top + logf(den);
 }
 
+// Whether every slice is one warp's, without a workspace and a second kernel: where the steps that a warp then has in a row take less time than the merge. From
+// a graph / as calls, us, for the two kernels: 64 sequences of up to 20 keys, 32 on 8 heads, 4.9 / 5.7 for 7.0 / 8.3, of up to 60 6.1 / 5.6 for 9.4 / 10.0, of up to 100 7.6 / 8.4
+// for 10.2 / 10.4, of up to 250 12.9 / 14.3 for 13.2 / 13.8, of up to 500 22.2 / 24.0 for 15.5 / 16.0; two of 200 8.2 / 8.7 for 7.4 / 8.2.
+static bool q4_whole(const AttnArgs& a) { return a.L <= 4 * kTile; }
 // CTAs: what an SM holds at once, fewer where there are not steps for their warps.
 template <int NT>
 static int q4_ctas(const AttnArgs& a, int head_tiles) {
@@ -631,6 +651,8 @@ static int q4_ctas(const AttnArgs& a, int head_tiles) {
 template <int NT>
 static size_t q4_layout(const AttnArgs& a, DecodeQ4Args* g, void* ws) {
     const int tiles = (a.group + 8 * NT - 1) / (8 * NT), rows = a.group < 8 * NT ? a.group : 8 * NT;
+    if (g) g->head_tiles = tiles;
+    if (q4_whole(a)) return 0;
     const size_t B = (size_t)(a.BH / a.H), parts = (size_t)q4_ctas<NT>(a, tiles) * kWarps + (size_t)(a.BH / a.group) * tiles;
     const size_t before = align256((B + 1) * 4), po = align256(parts * rows * a.D * 4);
     if (g) {
@@ -638,7 +660,6 @@ static size_t q4_layout(const AttnArgs& a, DecodeQ4Args* g, void* ws) {
         g->po = (float*)((unsigned char*)ws + before);
         g->plse = (float*)((unsigned char*)ws + before + po);
         g->part_rows = rows;
-        g->head_tiles = tiles;
     }
     return before + po + align256(parts * rows * 4);
 }
@@ -662,13 +683,14 @@ static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* tab
     g.k8 = 0x48004800u;
     g.out = (__nv_bfloat16*)a.out; g.lse = a.lse;
     q4_layout<NT>(a, &g, ws);
-    const int ctas = q4_ctas<NT>(a, g.head_tiles);
+    const bool whole = q4_whole(a);
+    const int ctas = whole ? (int)((a.BH / a.group * g.head_tiles + kWarps - 1) / kWarps) : q4_ctas<NT>(a, g.head_tiles);
     cudaError_t e = TT_ALLOW_SMEM((attn_decode_q4_kernel<D, NT>), (q4_smem<D, NT>()));
     if (e != cudaSuccess) return e;
     {
         LaunchScope ls(K_DECODE_Q4, st);
         e = launch_overlapped(attn_decode_q4_kernel<D, NT>, (unsigned)ctas, kWarps * 32, q4_smem<D, NT>(), st, g);
-        if (e != cudaSuccess) return e;
+        if (e != cudaSuccess || whole) return e;
     }
     // A warp for a row of up to a dozen parts, if all slices were of the greatest length; else as many threads as leave all rows in one wave.
     const int n_warps = ctas * kWarps;

@@ -236,7 +236,7 @@ def test_q4_decode_refuses_what_does_not_fit(tt):
 
     for kw in (dict(S=2), dict(L=0), dict(L=65), dict(L=(1 << 30) + 1, max_pages=1 << 27), dict(H=3), dict(B=0), dict(page=8, max_pages=8), dict(page=24), dict(max_pages=3), dict(pages=-1),
                dict(q=_at(q, 2)), dict(out=_at(out, 8)), dict(kc=_at(kc, 8)), dict(table=None, page=48), dict(table=None, page=64, pages=1), dict(scale=math.inf),
-               dict(out=q), dict(out=_at(q, 16)), dict(out=_at(kc, 256)), dict(out=vc), dict(out=ws), dict(ws=kc), dict(lse=out), dict(lse=_at(q, 64)), dict(lse=lens),
+               dict(out=q), dict(out=_at(q, 16)), dict(out=_at(kc, 256)), dict(out=vc), dict(lse=out), dict(lse=_at(q, 64)), dict(lse=lens),
                dict(lse=table), dict(pages=2 ** 26, Hkv=128, H=128), dict(B=1 << 20, H=1 << 12)):
         assert call(**kw) == c.TT_ERR_BAD_SHAPE, kw
     for kw in (dict(D=96), dict(dtype=c.TT_F32)):
@@ -248,6 +248,12 @@ def test_q4_decode_refuses_what_does_not_fit(tt):
     d = c.make_desc(2, 4, 1, 5000, 64, c.TT_BF16, False, None, Hkv=2)
     need = lib.tt_attn_decode_q4_workspace_bytes(ctypes.byref(d))
     assert need > 0
+    raw2, (big, k_far, v_far) = _buffers(4, 1 << 20)
+    assert need < 1 << 20
+    for kw in (dict(out=big), dict(out=_at(big, need - 256)), dict(lse=_at(big, 256)), dict(q=_at(big, 512)), dict(table=_at(big, 512))):
+        assert call(**long, kc=k_far, vc=v_far, ws=big, ws_bytes=need, **kw) == c.TT_ERR_BAD_SHAPE and "workspace" in c.last_error(), kw
+    for L, some in ((1, False), (128, False), (129, True)):
+        assert (lib.tt_attn_decode_q4_workspace_bytes(ctypes.byref(c.make_desc(2, 4, 1, L, 64, c.TT_BF16, False, None, Hkv=2))) > 0) == some
     assert call(**long, ws=None) == c.TT_ERR_WORKSPACE and call(**long, ws_bytes=need - 1) == c.TT_ERR_WORKSPACE and call(**long, ws=_at(ws, 64), ws_bytes=need) == c.TT_ERR_WORKSPACE
     if not torch.cuda.is_available():
         assert call() == c.TT_ERR_BAD_DEVICE
