@@ -28,8 +28,8 @@
 // a normalised result and its log-sum-exp, which a second kernel merges.  Results do not depend on timing.  Up to 128 keys a warp has a whole slice, and
 // there is no second kernel.
 //
-// One B200, both kernels, replayed from a graph (bytes at the copy rate of 6.46 TB/s): 64 sequences of 4096 to 8192, 32 query on 8 key/value heads, D = 128 94.5 us
-// (64.8); 48 of up to 4096, 16 on 16, D = 64 39.3 (16.2); two of 120,000 to 131,072, 32 on 2 31.4 (10.5); one of 5001, 32 on 8 10.0 (0.9).  Counters of the
+// One B200, both kernels, replayed from a graph (bytes at the copy rate of 6.46 TB/s): 64 sequences of 4096 to 8192, 32 query on 8 key/value heads, D = 128 94.0 us
+// (64.8); 48 of up to 4096, 16 on 16, D = 64 37.9 (16.2); two of 120,000 to 131,072, 32 on 2 31.0 (10.5); one of 5001, 32 on 8 10.0 (0.9).  Counters of the
 // first: 553 instructions per step of a warp, 336 of them unpacking and products; issue slots 56 % busy, ALU 47 %, half-precision multiply-adds 30 %, tensor
 // pipe 26 %, at 1.75 GHz (power).  The pipes add up more than they overlap: without the loads 80.6 us, the loads alone 67.
 #include "cache_q4.cuh"
