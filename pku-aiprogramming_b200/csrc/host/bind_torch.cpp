@@ -495,10 +495,10 @@ const Tensor* vector_arg(PyObject* o, at::ScalarType type, int64_t n, const Tens
     const Tensor* t = on_device(o, type, like);
     return t && t->is_contiguous() && t->dim() == 1 && (n < 0 || t->size(0) == n) ? t : nullptr;
 }
-// n elements of a vector from `at` on, on its storage: a few short results cost one allocation (0.9 us each)
-Tensor part_of(const Tensor& whole, int64_t at, int64_t n) {
-    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
-    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+// A contiguous tensor on another one's storage, `at` of its elements from the start: a few short results cost one allocation (0.9 us each).
+Tensor part_of(const Tensor& whole, int64_t at, at::IntArrayRef sizes, caffe2::TypeMeta type) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), type);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
     t.unsafeGetTensorImpl()->set_storage_offset(at);
     return t;
 }
@@ -531,7 +531,7 @@ PyObject* cache_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t sizes[5] = {B, 1, B + 1, tokens, tokens};
         if (a[7] == Py_None) {
             const Tensor all = make({2 * (B + 1 + tokens)}, at::kInt, *table);
-            for (int64_t i = 0, at = 0; i < 5; at += sizes[i++]) out[i] = &(made[i] = part_of(all, at, sizes[i]));
+            for (int64_t i = 0, at = 0; i < 5; at += sizes[i++]) out[i] = &(made[i] = part_of(all, at, sizes[i], all.dtype()));
         } else {
             for (int i = 0; i < 5; ++i)
                 if (!(out[i] = vector_arg(PyTuple_GET_ITEM(a[7], i), at::kInt, sizes[i], table))) Py_RETURN_NONE;
@@ -563,7 +563,7 @@ PyObject* cache_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor* out[2];
         const Tensor all = a[6] == Py_None ? make({B + 1}, at::kInt, *table) : Tensor();
         for (int i = 0; i < 2; ++i) {
-            if (a[6] == Py_None) out[i] = &(made[i] = part_of(all, i ? B : 0, i ? 1 : B));
+            if (a[6] == Py_None) out[i] = &(made[i] = part_of(all, i ? B : 0, i ? 1 : B, all.dtype()));
             else if (!(out[i] = vector_arg(PyTuple_GET_ITEM(a[6], i), at::kInt, i ? 1 : B, table))) Py_RETURN_NONE;
         }
         TT_CALL(rc, tt_cache_release((const int32_t*)ptr(table), (const int32_t*)ptr(lens), (const uint8_t*)ptr(done), (int32_t*)ptr(pages),
@@ -618,13 +618,20 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         OnDevice dev(q);
         Tensor made[2];
         const Tensor* out[2] = {nullptr, nullptr};
+        // Short results share an allocation; long ones have their own, which each gives back by itself.
+        const int64_t k_at = (q.numel() + 127) / 128 * 128, all = k ? k_at + k->numel() : 0;
+        if (k && k_at && all <= 1 << 19 && a[8] == Py_None && a[9] == Py_None) {
+            const Tensor whole = make({all}, q.scalar_type(), q);
+            made[0] = part_of(whole, 0, q.sizes(), whole.dtype());
+            made[1] = part_of(whole, k_at, k->sizes(), whole.dtype());
+        }
         for (int i = 0; i < (k ? 2 : 1); ++i) {
             const Tensor& x = i ? *k : q;
             if (a[8 + i] != Py_None) {
                 out[i] = on_device(a[8 + i], q.scalar_type(), &q);
                 if (!out[i] || !same_shape(*out[i], x)) Py_RETURN_NONE;
             } else {
-                made[i] = make_like(x);
+                if (!made[i].defined()) made[i] = make_like(x);
                 out[i] = &made[i];
             }
             if (!heads_arg(*out[i], &Bk, &Hk, &Sk, i ? d.k_out_stride : d.q_out_stride)) Py_RETURN_NONE;
@@ -740,8 +747,15 @@ PyObject* attention_decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[9] != Py_None && (!THPVariable_Check(a[9]) || !(ws = &THPVariable_Unpack(a[9]))->is_contiguous() || ws->device() != q->device())) Py_RETURN_NONE;
         OnDevice dev(*q);
         Tensor new_out, new_lse, made;
-        if (!out) new_out = make_like(*q);
-        if (!lse && need_lse) new_lse = make({B, H, 1}, at::kFloat, *q);
+        if (!out && !lse && need_lse) {
+            const int64_t n = q->numel() / 2;   // in floats
+            const Tensor whole = make({n + B * H}, at::kFloat, *q);
+            new_out = part_of(whole, 0, q->sizes(), q->dtype());
+            new_lse = part_of(whole, n, {B, H, 1}, whole.dtype());
+        } else {
+            if (!out) new_out = make_like(*q);
+            if (!lse && need_lse) new_lse = make({B, H, 1}, at::kFloat, *q);
+        }
         size_t bytes;
         ws = workspace_arg(ws, tt_attn_decode_q4_workspace_bytes(&d), 0, *q, &made, &bytes);
         TT_CALL(rc, tt_attn_decode_q4(&d, ptr(q), ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(lens), (int32_t)kc->size(0), (int32_t)page,

@@ -129,3 +129,34 @@ def test_captured_token_step(tt):
         assert all(torch.equal(a, b) for a, b in zip(want, got))
         assert all(torch.equal(a, b) for a, b in zip(eager, captured))
     assert eager[1].tolist() == [40] * B
+
+
+def test_results_that_share_an_allocation(tt):
+    """Short results may lie in one allocation: apart from each other, contiguous, and each usable when the other is gone."""
+    import gc
+    for T, D in ((1, 64), (3, 50), (40, 128), (5000, 128)):
+        q, k = torch.randn(T, 3, D, device="cuda").bfloat16(), torch.randn(T, 1, D, device="cuda").bfloat16()
+        freq, _ = tt.rotary_frequencies(D)
+        pos = torch.arange(T, dtype=torch.int32, device="cuda")
+        a, b = tt.rotary_forward(q, k, pos, freq)
+        assert a.is_contiguous() and b.is_contiguous() and a.shape == q.shape and b.shape == k.shape and a.data_ptr() % 16 == b.data_ptr() % 16 == 0
+        want = tt.rotary_forward(k, None, pos, freq)[0]
+        a.fill_(7)
+        assert torch.equal(b, want)
+        del a
+        gc.collect()
+        other = torch.full((T * 4, D), 3.0, device="cuda").bfloat16()
+        assert torch.equal(b, want) and (other == 3).all()
+    kc, vc = tt.cache_alloc_q4(3, 1, 16, 64)
+    x = torch.randn(20, 1, 64, device="cuda").bfloat16()
+    tt.cache_append_q4(x, x, torch.arange(20, dtype=torch.int32, device="cuda"), kc, vc)
+    table, lens = torch.arange(3, dtype=torch.int32, device="cuda")[None], torch.tensor([20], dtype=torch.int32, device="cuda")
+    for H in (1, 3, 17):
+        q = torch.randn(1, H, 1, 64, device="cuda").bfloat16()
+        out, lse = tt.attention_decode_q4(q, kc, vc, block_table=table, seq_lens=lens)
+        mine, mine_lse = tt.attention_decode_q4(q, kc, vc, block_table=table, seq_lens=lens, out=torch.empty_like(q), lse=torch.empty(1, H, 1, device="cuda"))
+        assert torch.equal(out, mine) and torch.equal(lse, mine_lse) and lse.shape == (1, H, 1) and lse.dtype == torch.float32
+        out.fill_(5)
+        assert torch.equal(lse, mine_lse)
+        lse.fill_(5)
+        assert (out == 5).all()
