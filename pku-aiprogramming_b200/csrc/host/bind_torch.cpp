@@ -697,13 +697,18 @@ PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         OnDevice dev(*kc);
         Tensor made[2];
         const Tensor* out[2];
+        const int64_t one = total * kc->size(1) * D;
+        if (one && 2 * one <= 1 << 19 && a[6] == Py_None && a[7] == Py_None) {   // short results, see part_of
+            const Tensor whole = make({2 * one}, at::kBFloat16, *kc);
+            for (int i = 0; i < 2; ++i) made[i] = part_of(whole, i * one, {total, kc->size(1), D}, whole.dtype());
+        }
         for (int i = 0; i < 2; ++i) {
             if (a[6 + i] != Py_None) {
                 out[i] = on_device(a[6 + i], at::kBFloat16, kc);
                 if (!out[i] || !out[i]->is_contiguous() || out[i]->dim() != 3 || out[i]->size(0) != total || out[i]->size(1) != kc->size(1) || out[i]->size(2) != D)
                     Py_RETURN_NONE;
             } else {
-                made[i] = make({total, kc->size(1), D}, at::kBFloat16, *kc);
+                if (!made[i].defined()) made[i] = make({total, kc->size(1), D}, at::kBFloat16, *kc);
                 out[i] = &made[i];
             }
         }

@@ -151,6 +151,11 @@ def test_results_that_share_an_allocation(tt):
     x = torch.randn(20, 1, 64, device="cuda").bfloat16()
     tt.cache_append_q4(x, x, torch.arange(20, dtype=torch.int32, device="cuda"), kc, vc)
     table, lens = torch.arange(3, dtype=torch.int32, device="cuda")[None], torch.tensor([20], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+    k, v = tt.cache_read_q4(kc, vc, table, cu, 20, 16)
+    assert torch.equal(k, v) and k.is_contiguous() and v.is_contiguous()
+    k.fill_(7)
+    assert torch.equal(v, tt.cache_read_q4(kc, vc, table, cu, 20, 16)[0]) and not (v == 7).all()
     for H in (1, 3, 17):
         q = torch.randn(1, H, 1, 64, device="cuda").bfloat16()
         out, lse = tt.attention_decode_q4(q, kc, vc, block_table=table, seq_lens=lens)
