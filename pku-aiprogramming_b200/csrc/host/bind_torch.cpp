@@ -698,7 +698,7 @@ PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Tensor made[2];
         const Tensor* out[2];
         const int64_t one = total * kc->size(1) * D;
-        if (one && 2 * one <= 1 << 19 && a[6] == Py_None && a[7] == Py_None) {   // short results, see part_of
+        if (one > 0 && one <= 1 << 18 && a[6] == Py_None && a[7] == Py_None) {   // short results, see part_of
             const Tensor whole = make({2 * one}, at::kBFloat16, *kc);
             for (int i = 0; i < 2; ++i) made[i] = part_of(whole, i * one, {total, kc->size(1), D}, whole.dtype());
         }
