@@ -324,8 +324,9 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // the head's largest value to 2^10 .. 2^11 (infinities stay)
-            const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.f && e < 128 ? min(max(10 - e, -100), 100) : 0;
+            // The head's largest value to 2^10 .. 2^11 (infinities stay).  e is -127 .. 127, so the move is -117 or more; it ends at 123, where a value of
+            // bf16, subnormal ones too, is a multiple of 2^-10.  All of f, 16 f and back are normal floats.
+            const int e = (int)(__float_as_uint(top) >> 23) - 127, up = top > 0.f && e < 128 ? min(10 - e, 123) : 0;
             const float f = __uint_as_float((unsigned)(up + 127) << 23), back = __uint_as_float((unsigned)(127 - up) << 23);
 #pragma unroll
             for (int i = 0; i < kG; ++i)
@@ -335,7 +336,8 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
                     qf[n][i][j] = bits(__floats2half2_rn(x[i][j] * by, x[i][j + 4] * by));
                 }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) to_log2[n][j] = a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
+            for (int j = 0; j < 2; ++j)   // (not 0, which times the -inf of absent keys is no number; sums are below 2^31, so what it is held from is 0)
+                to_log2[n][j] = fmaxf(a.scale_log2 * __shfl_sync(0xffffffffu, back, (2 * t + j) * 4), 1.1754944e-38f);
         }
         float o[kMT][NT][4], m[NT][2], above[NT][2];   // m: what a score is taken less, 2^-kLift of the reference; above: what raises it
         uint64_t sums[NT];                              // of P, heads 2t and 2t + 1
