@@ -42,6 +42,10 @@ namespace {
 
 constexpr int kWarps = 4, kTile = 32, kDepth = 3;   // a step of a warp: 32 keys, two accumulator tiles of 16
 constexpr float kSlack = 5.f, kLift = 10.f, kNone = -3e38f;   // (kNone: no score yet; above every finite one that counts as such)
+// References from here on (2^20): a score's last bit is 1/8 or more, so that adding a lift may round it to anything, and a fused multiply-add of it leaves what
+// the reference's own product rounded off, which may be more than the exponential can take.  There is no lift then, the products are rounded first, and every
+// step goes the way of those that raise the reference, where that is done, with 0 and 1 in its and the factor's place for the code behind.
+constexpr float kFar = 1048576.f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -351,6 +355,8 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
             above[n][0] = above[n][1] = -INFINITY;
             sums[n] = 0;
         }
+        bool far = false;                    // whether a head's reference is kFar or more, the true ones and the factors in `kept` then (in local memory: rare)
+        volatile float kept[NT][4];
         int left = now.len - step * kTile;   // keys from the step at hand on
         for (; i < end; ++i, left -= kTile) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
@@ -426,6 +432,16 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
                 }
             }
             if (__any_sync(0xffffffffu, raise)) {
+                if (far) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            m[n][j] = kept[n][j];
+                            to_log2[n][j] = kept[n][2 + j];
+                        }
+                }
+                bool here_far = false;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float f[2];
@@ -434,10 +450,11 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
                         float x = top[n][j];
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        const float to = fmaxf(m[n][j], x * to_log2[n][j] - kLift);
+                        const float y = __fmul_rn(x, to_log2[n][j]), to = fmaxf(m[n][j], fabsf(y) < kFar ? y - kLift : y);
                         f[j] = ex2_approx(m[n][j] - to);
                         m[n][j] = to;
                         above[n][j] = (to + (kLift + kSlack)) / to_log2[n][j];
+                        here_far = here_far || (fabsf(to) >= kFar - 2 * kLift && to != kNone);
 #pragma unroll
                         for (int c = 0; c < kMT; ++c) {
                             o[c][n][j] *= f[j];
@@ -445,6 +462,23 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
                         }
                     }
                     sums[n] = mul_f32x2(sums[n], pack_f32x2(f[0], f[1]));
+                }
+                far = __any_sync(0xffffffffu, here_far);
+                if (far) {   // see kFar
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                for (int k = j; k < 4; k += 2) s[u][n][k] = __fadd_rn(__fmul_rn(s[u][n][k], to_log2[n][j]), -m[n][j]);
+                            kept[n][j] = m[n][j];
+                            kept[n][2 + j] = to_log2[n][j];
+                            m[n][j] = 0.f;
+                            to_log2[n][j] = 1.f;
+                            above[n][j] = -INFINITY;
+                        }
                 }
             }
             // P^T as the B operand
@@ -494,6 +528,12 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
             }
         }
 
+        if (far) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) m[n][j] = kept[n][j];
+        }
         // the part's result: lane (g, t) has channels g (D / 8) .. of heads 2t and 2t + 1
         const long long part = (w + slice) * a.part_rows;
 #pragma unroll
