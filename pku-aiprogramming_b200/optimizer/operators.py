@@ -537,35 +537,43 @@ class Rotary(TensorOp):
         self.positions = p.astype(np.int32).reshape((1,) * (2 - p.ndim) + p.shape)
         self.table = lambda D: rotary_table(D if rotary_dim is None else rotary_dim, base, sections, cyclic, own_ladder)
         self.interleaved, self.scale, self.dtype = bool(interleaved), float(scale), dtype
-        self._saved = None
+        self._saved = {}   # by head dim: one op may turn several inputs, and each one's gradient needs its own
 
-    @staticmethod
-    def _names(bf16: bool):
+    def _kernels(self, x):
+        """(tensor type, forward, backward, whether x stays on the device) for the data x of an input."""
         mt, ml = _native()
-        return (mt.Tensor_bf16, ml.RotaryForward_bf16, ml.RotaryBackward_bf16) if bf16 else (mt.Tensor_float, ml.RotaryForward, ml.RotaryBackward)
-
-    def compute(self, x):
         resident = _on_device(x)
         if resident and type(x).__name__ not in ("Tensor_float", "Tensor_bf16"):
             raise TypeError("device-resident input must be Tensor_float or Tensor_bf16")
-        T, fwd, _ = self._names(type(x).__name__ == "Tensor_bf16" if resident else self.dtype == "bfloat16")
-        tx = x if resident else T(np.ascontiguousarray(x, dtype=np.float32), "gpu")
-        freq, axes, n_axes = self.table(tx.get_shape()[-1])
+        if (type(x).__name__ == "Tensor_bf16") if resident else self.dtype == "bfloat16":
+            return mt.Tensor_bf16, ml.RotaryForward_bf16, ml.RotaryBackward_bf16, resident
+        return mt.Tensor_float, ml.RotaryForward, ml.RotaryBackward, resident
+
+    def _arguments(self, D):
+        """What the kernels take beside the heads, for heads of D channels."""
+        mt, _ = _native()
+        freq, axes, n_axes = self.table(D)
         if n_axes != self.positions.shape[0]:
             raise ValueError(f"positions have {self.positions.shape[0]} axes, sections {n_axes}")
-        mt, _ = _native()
-        rest = (mt.Tensor_int(np.ascontiguousarray(self.positions), "gpu"), mt.Tensor_double(np.array(freq, dtype=np.float64), "gpu"),
+        return (mt.Tensor_int(np.ascontiguousarray(self.positions), "gpu"), mt.Tensor_double(np.array(freq, dtype=np.float64), "gpu"),
                 mt.Tensor_int(np.array(axes, dtype=np.int32), "gpu"), self.interleaved, self.scale)
+
+    def compute(self, x):
+        T, fwd, _, resident = self._kernels(x)
+        tx = x if resident else T(np.ascontiguousarray(x, dtype=np.float32), "gpu")
+        D = tx.get_shape()[-1]
+        rest = self._saved[D] = self._arguments(D)
         out = T([1], "gpu")
         fwd(tx, out, *rest)
-        self._saved = (rest, T, resident)
         return out if resident else out.numpy().astype(x.dtype, copy=False)
 
     def gradient(self, out_grad, node):
-        if self._saved is None:
-            node.realize_cached_data()
-        rest, T, resident = self._saved
-        _, _, bwd = self._names(T.__name__ == "Tensor_bf16")
+        x = node.inputs[0].realize_cached_data()
+        T, _, bwd, resident = self._kernels(x)
+        D = node.inputs[0].shape[-1]
+        if D not in self._saved:
+            self._saved[D] = self._arguments(D)
+        rest = self._saved[D]
         g = out_grad.realize_cached_data()
         if _on_device(g) and type(g) is not T:
             raise TypeError(f"upstream gradient is {type(g).__name__}, the op ran on {T.__name__}")
@@ -574,7 +582,7 @@ class Rotary(TensorOp):
         bwd(tg, gx, *rest)
         if resident:
             return Tensor(gx, device="gpu", requires_grad=False)
-        return Tensor(gx.numpy().astype(node.inputs[0].dtype, copy=False), requires_grad=False)
+        return Tensor(gx.numpy().astype(x.dtype, copy=False), requires_grad=False)
 
 
 def rotary(x, positions, **kwargs):
