@@ -217,6 +217,7 @@ int tt_attn_decode_paged(const tt_attn_desc* desc, const void* q, const void* k_
  *
  * tt_cache_release: the pages of the requests with done[b] != 0 (bytes) go back: free_pages[*n_free ..] gets them in order of
  * request and column (none beyond free_capacity), seq_lens_out is 0 there, n_free_out counts them.  block_table is only read.
+ * Negative entries are no pages and are left out; as many places of free_pages behind n_free_out may then have been written.
  *
  * Outputs must not overlap inputs or each other, except block_table and free_pages as said.  B is at most 16384, and slots
  * fit 32 bits (pages * page_size < 2^31).  Negative lengths of done requests count as 0, ones beyond a row as the whole row. */

@@ -6,11 +6,12 @@
 //
 // The bytes are few (4 per length, 8 per token and page), so what counts is the number of launches and of dependent loads in
 // one: every CTA sums over all requests itself (a few loads per thread, from L2) instead of waiting for a launch that
-// does, and a token finds its request by a binary search in shared memory.  Nothing is kept between calls, and no CTA waits
-// for another.
+// does, and a token finds its request by a binary search in shared memory.  Nothing is kept between calls.  Giving pages back
+// is the work of one CTA or cluster where an entry is no page, since where a page goes depends on how many before it are.
 #include <climits>
 
 #include "common.h"
+#include "sm100_ptx.cuh"
 
 namespace ttk {
 
@@ -139,16 +140,20 @@ __global__ void __launch_bounds__(kThreads) cache_extend_kernel(int* __restrict_
     }
 }
 
+// Pages given back.  Entries of done requests that are no pages (negative) are left out, so a page's place behind *n_free is the number of pages among all
+// entries before it.  Two kernels where there may be many: the first copies all entries to where they belong if there are no such holes, and leaves kHoles in
+// the last of lens_out if it meets one; the second then does all of it anew, or else writes that length.  (What lens_out held before cannot mislead it: with
+// kHoles there it does the work in vain.)
+constexpr int kHoles = INT_MIN;
 constexpr int kCopied = 128;
 template <int kThreads>
-__global__ void __launch_bounds__(kThreads) cache_release_kernel(const int* __restrict__ table, const int* __restrict__ lens, const unsigned char* __restrict__ done,
-                                                                 int* __restrict__ free_pages, const int* __restrict__ n_free, int B, int page,
-                                                                 int max_pages, int free_capacity, int* __restrict__ lens_out, int* __restrict__ n_free_out) {
+__global__ void __launch_bounds__(kThreads) cache_copy_kernel(const int* __restrict__ table, const int* __restrict__ lens, const unsigned char* __restrict__ done,
+                                                              int* __restrict__ free_pages, const int* __restrict__ n_free, int B, int page, int max_pages,
+                                                              int free_capacity, int* __restrict__ lens_out, int* __restrict__ n_free_out) {
     extern __shared__ int sm[];
     int* first = sm;      // [B] where the request's pages go, behind *n_free
     int* count = sm + B;   // [B] how many there are
     __shared__ long long red[2][32];
-    __shared__ long long total;
     const int tid = threadIdx.x, per = (B + kThreads - 1) / kThreads, b0 = min(B, tid * per), b1 = min(B, b0 + per);
     grid_let_next_start();
     grid_wait_for_previous();
@@ -161,23 +166,22 @@ __global__ void __launch_bounds__(kThreads) cache_release_kernel(const int* __re
     }
     const long long own = pg;
     cta_sums<kThreads>(pg, zero, red);
-    if (tid == kThreads - 1) total = pg;
+    if (blockIdx.x == 0 && tid == kThreads - 1) *n_free_out = (int)min(have_free + pg, (long long)free_capacity);
     pg -= own;
     for (int b = b0; b < b1; ++b) {
         first[b] = (int)min(pg, (long long)INT_MAX);
         pg += count[b];
     }
     __syncthreads();
-    if (blockIdx.x == 0) {
-        for (int b = tid; b < B; b += kThreads) lens_out[b] = done[b] ? 0 : lens[b];
-        if (tid == 0) *n_free_out = (int)min(have_free + total, (long long)free_capacity);
-    }
+    if (blockIdx.x == 0)
+        for (int b = tid; b < B - 1; b += kThreads) lens_out[b] = done[b] ? 0 : lens[b];
     // a warp per kCopied columns of a request, all loads of a lane before its stores
-    const unsigned pieces = (max_pages + kCopied - 1) / kCopied;
+    const unsigned pieces = (max_pages - 1) / kCopied + 1;
     for (long long item = blockIdx.x * (kThreads / 32) + (tid >> 5); item < (long long)B * pieces; item += gridDim.x * (kThreads / 32)) {
         const int b = (int)(item / pieces), j0 = (int)(item - (long long)b * pieces) * kCopied, n = count[b];
         if (j0 >= n) continue;
         int x[kCopied / 32];
+        bool hole = false;
 #pragma unroll
         for (int i = 0; i < kCopied / 32; ++i) {
             const int j = j0 + 32 * i + (tid & 31);
@@ -188,12 +192,109 @@ __global__ void __launch_bounds__(kThreads) cache_release_kernel(const int* __re
             const int j = j0 + 32 * i + (tid & 31);
             const long long to = (long long)have_free + first[b] + j;
             if (j < n && to < free_capacity) free_pages[to] = x[i];
+            hole = hole || (j < n && x[i] < 0);
+        }
+        if (hole) lens_out[B - 1] = kHoles;
+    }
+}
+
+// One cluster, or one CTA.  Columns in use are cut into pieces of `width`, `pieces` to a row; a warp counts the pages of a piece and tells every CTA, each sums
+// over all pieces, and the warp writes its piece's pages, which it still holds where it has one piece of kPiece entries, and else finds in its SM's cache.
+constexpr int kGiveThreads = 1024, kGiveCtas = 8, kLoads = 16, kPiece = 32 * kLoads, kMaxPieces = 2 * kMaxRequests;
+__global__ void __launch_bounds__(kGiveThreads) cache_release_kernel(const int* __restrict__ table, const int* __restrict__ lens, const unsigned char* __restrict__ done,
+                                                                     int* __restrict__ free_pages, const int* __restrict__ n_free, int B, int page, int max_pages,
+                                                                     int free_capacity, int width, int pieces, bool copied, int* lens_out, int* __restrict__ n_free_out) {
+    extern __shared__ int sm[];
+    int* count = sm;      // [B] columns in use
+    int* first = sm + B;   // [B * pieces] pages of a piece, and then of those before it
+    __shared__ long long red[2][32];
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, items = B * pieces, n_cta = gridDim.x, cta = blockIdx.x;   // (the grid is one cluster)
+    const int item0 = cta * (threads / 32) + (tid >> 5), apart = n_cta * (threads / 32);
+    grid_let_next_start();
+    grid_wait_for_previous();
+    if (copied) {
+        // Every CTA finds the same: where this is not kHoles, it becomes a length that is not, either, and else it stays until all are at the cluster's barrier.
+        const int last = *(volatile int*)(lens_out + B - 1), held = lens[B - 1], len = done[B - 1] ? 0 : held;
+        if (last != kHoles && len != kHoles) {
+            if (cta == 0 && tid == 0) lens_out[B - 1] = len;
+            return;
+        }
+    }
+    if (n_cta > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    const int have_free = min(max(*n_free, 0), free_capacity);
+    for (int b = tid; b < B; b += threads) {
+        const int held = lens[b], len = done[b] ? held : 0;
+        count[b] = len <= 0 ? 0 : min(max_pages, len / page + (len % page != 0));
+    }
+    __syncthreads();
+    if (n_cta > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // all CTAs have begun: their shared memory may be written
+    int x[kLoads];
+    auto load = [&](const int* from, int n) {   // kPiece entries, of which n are there
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) x[i] = 32 * i + lane < n ? from[32 * i + lane] : -1;
+    };
+    auto piece = [&](int item, const int** from) {   // its number of entries, and the first
+        const int b = item / pieces, j0 = (item - b * pieces) * width;
+        *from = table + (long long)b * max_pages + j0;
+        return min(count[b] - j0, width);
+    };
+    for (int item = item0; item < items; item += apart) {
+        const int* from;
+        const int n = piece(item, &from);
+        int here = 0;
+        for (int j0 = 0; j0 < n; j0 += kPiece) {
+            load(from + j0, n - j0);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) here += x[i] >= 0;
+        }
+        here = __reduce_add_sync(0xffffffffu, here);
+        if (n_cta == 1) {
+            if (lane == 0) first[item] = here;
+        } else if (lane < n_cta) {
+            sm100::st_shared_cluster_u32(sm100::map_to_cta(sm100::smem_u32(first + item), lane), here);
+        }
+    }
+    __syncthreads();
+    if (n_cta > 1) sm100::cluster_sync_all();
+    const int per = (items + threads - 1) / threads, i0 = min(items, tid * per), i1 = min(items, i0 + per);
+    long long pg = 0, zero = 0;
+    for (int i = i0; i < i1; ++i) pg += first[i];
+    const long long own = pg;
+    cta_sums<kGiveThreads>(pg, zero, red);
+    if (cta == 0) {
+        for (int b = tid; b < B; b += threads) {
+            const int held = lens[b];
+            lens_out[b] = done[b] ? 0 : held;
+        }
+        if (tid == threads - 1) *n_free_out = (int)min(have_free + pg, (long long)free_capacity);
+    }
+    pg -= own;
+    for (int i = i0; i < i1; ++i) {
+        const int n = first[i];
+        first[i] = (int)min(pg, (long long)INT_MAX);
+        pg += n;
+    }
+    __syncthreads();
+    const bool held = items <= apart && width == kPiece;
+    for (int item = item0; item < items; item += apart) {
+        const int* from;
+        const int n = piece(item, &from);
+        long long to = (long long)have_free + first[item];
+        for (int j0 = 0; j0 < n; j0 += kPiece) {
+            if (!held) load(from + j0, n - j0);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const unsigned there = __ballot_sync(0xffffffffu, x[i] >= 0);
+                const long long at = to + __popc(there & ((1u << lane) - 1));
+                if (x[i] >= 0 && at < free_capacity) free_pages[at] = x[i];
+                to += __popc(there);
+            }
         }
     }
 }
 
 // Threads: one request each up to 256, four each beyond.  CTAs: every one sums over all requests, so not more than three to an SM (270,000 tokens of 256
-// requests: 6.5 / 5.7 / 8.1 us at two, three and four).  Pages given back: 65,000 of 512 requests 6.0 us with a warp per request, 3.7 with one per 128 columns.
+// requests: 6.5 / 5.7 / 8.1 us at two, three and four).
 cudaError_t cache_extend(int* table, const int* lens, const int* fresh, const int* free_pages, const int* n_free, int B, int page, int max_pages,
                          int free_capacity, int max_tokens, int* lens_out, int* n_free_out, int* cu_new, int* slots, int* positions, cudaStream_t st) {
     const size_t smem = (3 * (size_t)B + 1) * sizeof(int);
@@ -210,20 +311,40 @@ cudaError_t cache_extend(int* table, const int* lens, const int* fresh, const in
     };
     return B <= 1024 ? go(cache_extend_kernel<256>, 256) : go(cache_extend_kernel<1024>, 1024);
 }
+// Pages given back, us from a graph / as calls, by one kernel and by both: 4 requests 3.1 / 5.0 and 3.3 / 7.8; 64 of up to 256 pages 5.8 / 6.1 and 3.5 / 7.4; 512 of
+// up to 512, 65,000 pages, 8.5 / 8.6 and 4.6 / 7.3 (6.0 in the first kernel with a warp per request for one per 128 columns); all 260,000 of them 15.8 / 16.0 and
+// 4.4 / 7.3.  With holes both take as long as one alone and the copying together.
 cudaError_t cache_release(const int* table, const int* lens, const unsigned char* done, int* free_pages, const int* n_free, int B, int page, int max_pages,
                           int free_capacity, int* lens_out, int* n_free_out, cudaStream_t st) {
-    const size_t smem = 2 * (size_t)B * sizeof(int);
-    auto go = [&](auto kernel, int threads) {
-        if (smem > 48 * 1024 - 1024) {
-            const cudaError_t e = TT_ALLOW_SMEM(kernel, 2 * (size_t)kMaxRequests * sizeof(int));
-            if (e != cudaSuccess) return e;
-        }
-        const long long warps = (long long)B * ((max_pages + kCopied - 1) / kCopied), reqs = (warps + threads / 32 - 1) / (threads / 32), most = (threads == 256 ? 8LL : 1LL) * sm_count();
-        LaunchScope ls(K_CACHE_TABLES, st);
-        return launch_overlapped(kernel, (unsigned)(reqs < most ? reqs : most), threads, smem, st, table, lens, done, free_pages, n_free, B, page,
-                                 max_pages, free_capacity, lens_out, n_free_out);
-    };
-    return B <= 1024 ? go(cache_release_kernel<256>, 256) : go(cache_release_kernel<1024>, 1024);
+    int width = kPiece, pieces;
+    while ((long long)B * (pieces = (max_pages - 1) / width + 1) > kMaxPieces) width *= 2;
+    const bool copied = B * pieces > kGiveThreads / 32;
+    if (copied) {
+        const size_t smem = 2 * (size_t)B * sizeof(int);
+        auto go = [&](auto kernel, int threads) {
+            if (smem > 48 * 1024 - 1024) {
+                const cudaError_t e = TT_ALLOW_SMEM(kernel, 2 * (size_t)kMaxRequests * sizeof(int));
+                if (e != cudaSuccess) return e;
+            }
+            const long long warps = B * ((max_pages - 1LL) / kCopied + 1), ctas = (warps + threads / 32 - 1) / (threads / 32), most = (threads == 256 ? 8LL : 1LL) * sm_count();
+            LaunchScope ls(K_CACHE_TABLES, st);
+            return launch_overlapped(kernel, (unsigned)(ctas < most ? ctas : most), threads, smem, st, table, lens, done, free_pages, n_free, B, page, max_pages, free_capacity,
+                                     lens_out, n_free_out);
+        };
+        const cudaError_t e = B <= 1024 ? go(cache_copy_kernel<256>, 256) : go(cache_copy_kernel<1024>, 1024);
+        if (e != cudaSuccess) return e;
+    }
+    const size_t smem = (size_t)B * (1 + pieces) * sizeof(int);
+    if (smem > 48 * 1024 - 1024) {
+        const cudaError_t e = TT_ALLOW_SMEM(cache_release_kernel, (kMaxRequests + (size_t)kMaxPieces) * sizeof(int));
+        if (e != cudaSuccess) return e;
+    }
+    const int threads = B * pieces <= 8 ? 256 : kGiveThreads;
+    int n_cta = 1;
+    while (n_cta < kGiveCtas && n_cta * (threads / 32) < B * pieces) n_cta *= 2;
+    LaunchScope ls(K_CACHE_TABLES, st);
+    return launch_overlapped_cluster(cache_release_kernel, n_cta, threads, smem, st, n_cta, table, lens, done, free_pages, n_free, B, page, max_pages, free_capacity, width,
+                                     pieces, copied, lens_out, n_free_out);
 }
 
 }  // namespace ttk
