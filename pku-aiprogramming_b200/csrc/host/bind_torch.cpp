@@ -606,7 +606,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!pos || !freq || pos->dim() < 1 || pos->dim() > q.dim() - 1 || pos->size(-1) != S || (S > 1 && pos->stride(-1) != 1)) Py_RETURN_NONE;
         const int64_t n_axes = pos->dim() > 1 ? pos->size(0) : 1;
         if (pos->dim() == 3 && pos->size(1) != B) Py_RETURN_NONE;
-        if (a[4] != Py_None && !(axes = vector_arg(a[4], at::kInt, freq->size(0), &q))) Py_RETURN_NONE;
+        if (a[4] != Py_None ? !(axes = vector_arg(a[4], at::kInt, freq->size(0), &q)) : n_axes != 1) Py_RETURN_NONE;   // (rows that nothing would read)
         d.pos_stride[0] = pos->dim() > 1 ? pos->stride(0) : 0;
         d.pos_stride[1] = pos->dim() == 3 ? pos->stride(1) : 0;
         const int inter = PyObject_IsTrue(a[5]), back = PyObject_IsTrue(a[7]);

@@ -377,6 +377,8 @@ def _explain_rotary(q, k, positions, inv_freq, axes, out_q, out_k):
     if axes is not None and (not isinstance(axes, torch.Tensor) or axes.dtype != torch.int32 or axes.shape != inv_freq.shape
                              or axes.device != q.device or not axes.is_contiguous()):
         raise ValueError("axes must be a contiguous int32 vector on q's device, one axis per pair")
+    if axes is None and isinstance(positions, torch.Tensor) and positions.dim() > 1 and positions.shape[0] != 1:
+        raise ValueError(f"positions {tuple(positions.shape)} are of {positions.shape[0]} axes, without `axes` there is one: [1, B, S] for positions of each batch entry")
     want = "[axes, T] or [T]" if q.dim() == 3 else "[axes, B, S], [axes, S] or [S]"
     raise ValueError(f"positions must be an int32 tensor {want} on q's device, rows next to each other")
 
@@ -386,7 +388,8 @@ def rotary_forward(q, k, positions, inv_freq, axes=None, interleaved=False, scal
 
     Pair i of the first `2 * len(inv_freq)` channels turns by `positions[axes[i]] * inv_freq[i]` (float64 `[R/2]`, int32 `[R/2]` or
     None, see `rotary_frequencies`): channels i and i + R/2, or with `interleaved` 2i and 2i + 1; the other channels are copied.
-    positions: int32 `[axes, T]` / `[axes, B, S]` / `[axes, S]`, or `[T]` / `[S]` with one axis.  Strided inputs are fine as long
+    positions: int32 `[axes, T]` / `[axes, B, S]` / `[axes, S]`, or `[T]` / `[S]` with one axis; without `axes` there is one, and more
+    rows are refused (position ids `[B, S]` are `[1, B, S]` here).  Strided inputs are fine as long
     as channels lie next to each other; `out_q`, `out_k` may be the inputs themselves.  `scale` (1) multiplies the result."""
     r = _native.rotary(q, k, positions, inv_freq, axes, interleaved, scale, False, out_q, out_k)
     return r if r.__class__ is tuple else _done(r, _explain_rotary, q, k, positions, inv_freq, axes, out_q, out_k)
