@@ -246,7 +246,7 @@ int tt_cache_release(const int32_t* block_table, const int32_t* seq_lens, const 
  * tt_cache_read_q4: the first cu_lens[b + 1] - cu_lens[b] tokens of each sequence as packed bf16 k, v [total, Hkv, D] (what
  * tt_attn_fwd_varlen takes); sequence b's are rows [cu_lens[b], cu_lens[b + 1]), found by block_table [B, max_pages].  cu_lens
  * counts up from 0.  Rows from cu_lens[B] on are left as they were; rows whose page is not one of the n_pages, or lies behind the
- * table's width, are 0. */
+ * table's width, are 0.  k and v must not overlap each other or an input. */
 size_t tt_cache_q4_page_bytes(int32_t page_size, int32_t D);   /* 0: not supported */
 int tt_cache_append_q4(const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype,
                        const int64_t* k_stride, const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages,
@@ -279,7 +279,8 @@ int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cac
  * Angles are taken in 64 bits and reduced to one turn before their sine and cosine, products are 32-bit, outputs rounded once.
  *   q, k           [B, heads, S, D] at element strides {batch, head, row} of their own, channels next to each other; inputs may
  *                  repeat (stride 0), outputs may not.  An output may be its input (same pointer and strides), else the two must not
- *                  overlap.  k and k_out are both null where there is one tensor only.  Packed tokens [T, H, D]: B = 1, S = T.
+ *                  overlap, and no output what positions, inv_freq and axes span.  k and k_out are both null where there is one
+ *                  tensor only.  Packed tokens [T, H, D]: B = 1, S = T.
  *   positions      int32, [n_axes, B, S] at strides pos_stride {axis, batch}, rows next to each other; any int32 value
  *   inv_freq       [R / 2] double, angle per position;  axes: [R / 2] int32 in 0 .. n_axes - 1 (others are taken as the nearest),
  *                  or null: all of axis 0

@@ -199,8 +199,9 @@ int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* bl
     if (!block_table || !cu_lens || (total && (!k || !v))) return fail(TT_ERR_NULL, "%s: null pointer", who);
     if (!aligned16(k) || !aligned16(v)) return fail(TT_ERR_BAD_SHAPE, "%s: k and v must be 16-byte aligned", who);
     const size_t pool = (size_t)n_pages * Hkv * tt_cache_q4_page_bytes(page_size, D), n = (size_t)total * Hkv * D * 2;
-    const Span out[] = {{k, n, "k"}, {v, n, "v"}}, in[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}};
-    if ((rc = check_overlap(who, out, 2, in, 2)) != TT_OK || (rc = check_device()) != TT_OK || total == 0) return rc;
+    const Span out[] = {{k, n, "k"}, {v, n, "v"}};
+    const Span in[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}, {block_table, (size_t)B * max_pages * 4, "block_table"}, {cu_lens, ((size_t)B + 1) * 4, "cu_lens"}};
+    if ((rc = check_overlap(who, out, 2, in, 4)) != TT_OK || (rc = check_device()) != TT_OK || total == 0) return rc;
     const CacheQ4 c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, Hkv, D};
     const cudaError_t e = cache_read_q4(c, block_table, cu_lens, B, max_pages, total, k, v, (cudaStream_t)stream);
     return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_read_q4: launch");
@@ -285,6 +286,11 @@ int tt_rotary(const tt_rotary_desc* d, const void* q, const void* k, const int32
             if (!(i == j && in_place(out[i], in[j])) && rows_meet(out[i], in[j], d->D, size))
                 return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in[j].span.name);
     if (k && rows_meet(out[0], out[1], d->D, size)) return fail(TT_ERR_BAD_SHAPE, "%s: q_out overlaps k_out", who);
+    const size_t n_pos = (size_t)((d->n_axes - 1) * d->pos_stride[0] + (d->B - 1) * d->pos_stride[1] + d->S);
+    const Span angles[] = {{positions, n_pos * 4, "positions"}, {inv_freq, (size_t)d->R / 2 * 8, "inv_freq"}, {axes, (size_t)d->R / 2 * 4, "axes"}};
+    for (int i = 0; i < (k ? 2 : 1); ++i)
+        for (const Span& in : angles)
+            if (overlap(out[i].span, in)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in.name);
     const int rc = check_device();
     if (rc != TT_OK) return rc;
     RotaryArgs a = {};
