@@ -495,7 +495,8 @@ const Tensor* vector_arg(PyObject* o, at::ScalarType type, int64_t n, const Tens
     const Tensor* t = on_device(o, type, like);
     return t && t->is_contiguous() && t->dim() == 1 && (n < 0 || t->size(0) == n) ? t : nullptr;
 }
-// A contiguous tensor on another one's storage, `at` of its elements from the start: a few short results cost one allocation (0.9 us each).
+// A contiguous tensor on another one's storage, `at` of its elements from the start: a few short results of one type cost one allocation
+// (0.4 us of the host each).  Not results of two types: torch.save refuses those on one storage.
 Tensor part_of(const Tensor& whole, int64_t at, at::IntArrayRef sizes, caffe2::TypeMeta type) {
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), type);
     t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
@@ -752,15 +753,8 @@ PyObject* attention_decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (a[9] != Py_None && (!THPVariable_Check(a[9]) || !(ws = &THPVariable_Unpack(a[9]))->is_contiguous() || ws->device() != q->device())) Py_RETURN_NONE;
         OnDevice dev(*q);
         Tensor new_out, new_lse, made;
-        if (!out && !lse && need_lse) {
-            const int64_t n = q->numel() / 2;   // in floats
-            const Tensor whole = make({n + B * H}, at::kFloat, *q);
-            new_out = part_of(whole, 0, q->sizes(), q->dtype());
-            new_lse = part_of(whole, n, {B, H, 1}, whole.dtype());
-        } else {
-            if (!out) new_out = make_like(*q);
-            if (!lse && need_lse) new_lse = make({B, H, 1}, at::kFloat, *q);
-        }
+        if (!out) new_out = make_like(*q);
+        if (!lse && need_lse) new_lse = make({B, H, 1}, at::kFloat, *q);
         size_t bytes;
         ws = workspace_arg(ws, tt_attn_decode_q4_workspace_bytes(&d), 0, *q, &made, &bytes);
         TT_CALL(rc, tt_attn_decode_q4(&d, ptr(q), ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(lens), (int32_t)kc->size(0), (int32_t)page,
