@@ -496,7 +496,7 @@ const Tensor* vector_arg(PyObject* o, at::ScalarType type, int64_t n, const Tens
     return t && t->is_contiguous() && t->dim() == 1 && (n < 0 || t->size(0) == n) ? t : nullptr;
 }
 // A contiguous tensor on another one's storage, `at` of its elements from the start: a few short results of one type cost one allocation
-// (0.4 us of the host each).  Not results of two types: torch.save refuses those on one storage.
+// (0.5 us of the host each, below what the kernels take of a large call).  Not results of two types: torch.save refuses those on one storage.
 Tensor part_of(const Tensor& whole, int64_t at, at::IntArrayRef sizes, caffe2::TypeMeta type) {
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), type);
     t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
@@ -514,6 +514,7 @@ bool table_args(PyObject* ot, PyObject* ol, const Tensor** table, const Tensor**
     return *lens != nullptr;
 }
 
+constexpr int64_t kSharedTokens = 4096;   // 32 KB of slots and positions, which kept lengths keep; a call 5.0 us up to it, 5.5 beyond
 // (block_table, seq_lens, new_lens, free_pages, n_free, page_size, max_tokens, out) -> (seq_lens, n_free, cu_new, slots, positions)
 PyObject* cache_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -531,8 +532,14 @@ PyObject* cache_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor* out[5];
         const int64_t sizes[5] = {B, 1, B + 1, tokens, tokens};
         if (a[7] == Py_None) {
-            const Tensor all = make({2 * (B + 1 + tokens)}, at::kInt, *table);
-            for (int64_t i = 0, at = 0; i < 5; at += sizes[i++]) out[i] = &(made[i] = part_of(all, at, sizes[i], all.dtype()));
+            // One allocation while it is short.  Lengths and the free count are kept from step to step, the others are not, so beyond that each group has its own.
+            const bool one = tokens <= kSharedTokens;
+            const int64_t kept = B + 1, dropped = B + 1 + 2 * tokens;
+            const Tensor first = make({one ? kept + dropped : kept}, at::kInt, *table), second = one ? first : make({dropped}, at::kInt, *table);
+            for (int64_t i = 0, at = 0; i < 5; at += sizes[i++]) {
+                if (i == 2 && !one) at = 0;
+                out[i] = &(made[i] = part_of(i < 2 ? first : second, at, sizes[i], first.dtype()));
+            }
         } else {
             for (int i = 0; i < 5; ++i)
                 if (!(out[i] = vector_arg(PyTuple_GET_ITEM(a[7], i), at::kInt, sizes[i], table))) Py_RETURN_NONE;
@@ -619,7 +626,8 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         OnDevice dev(q);
         Tensor made[2];
         const Tensor* out[2] = {nullptr, nullptr};
-        // Short results share an allocation; long ones have their own, which each gives back by itself.
+        // Short results, up to 2^19 values (1 MB of bf16), share an allocation: a call 3.9 us up to it, 4.4 beyond.  Long ones have their own, which each gives back
+        // by itself.
         const int64_t k_at = (q.numel() + 127) / 128 * 128, all = k ? k_at + k->numel() : 0;
         if (k && k_at && all <= 1 << 19 && a[8] == Py_None && a[9] == Py_None) {
             const Tensor whole = make({all}, q.scalar_type(), q);
@@ -699,7 +707,7 @@ PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         Tensor made[2];
         const Tensor* out[2];
         const int64_t one = total * kc->size(1) * D;
-        if (one > 0 && one <= 1 << 18 && a[6] == Py_None && a[7] == Py_None) {   // short results, see part_of
+        if (one > 0 && one <= 1 << 18 && a[6] == Py_None && a[7] == Py_None) {   // short results, 1 MB in all: a call 4.0 us up to it, 4.5 beyond
             const Tensor whole = make({2 * one}, at::kBFloat16, *kc);
             for (int i = 0; i < 2; ++i) made[i] = part_of(whole, i * one, {total, kc->size(1), D}, whole.dtype());
         }
