@@ -79,7 +79,8 @@ __device__ __forceinline__ half2 as_half2(uint32_t x) { return *reinterpret_cast
 __device__ __forceinline__ uint32_t bits(half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
 // What two codes, times 128 in the halves of a word, make of nibbles: s8 = half(code << 7) = 8 s.  The codes that are written (and NaN) leave
-// every constant finite and exact: 9 s8 <= 8064, and 129 / 16 times four significant bits has eleven.
+// every constant finite and exact: 9 s8 is at most 9 * 7168 = 64512 (half ends at 65504; the next code's 69120 would be infinite), and 129 / 16 times four significant bits has eleven.
+static_assert(9 * ((8 + kQ4Top % 8) << (kQ4Top / 8 - 18)) <= 65504, "the largest code's constants are finite");
 struct Scale2 {
     half2 s8, even, odd;
     __device__ __forceinline__ explicit Scale2(uint32_t codes_times_128) {
