@@ -7,11 +7,10 @@
 // The bytes are few (4 per length, 8 per token and page), so what counts is the number of launches and of dependent loads in
 // one: every CTA sums over all requests itself (a few loads per thread, from L2) instead of waiting for a launch that
 // does, and a token finds its request by a binary search in shared memory.  Nothing is kept between calls.  Giving pages back
-// is the work of one CTA or cluster where an entry is no page, since where a page goes depends on how many before it are.
+// is the work of one CTA where an entry is no page, since where a page goes depends on how many before it are.
 #include <climits>
 
 #include "common.h"
-#include "sm100_ptx.cuh"
 
 namespace ttk {
 
@@ -198,9 +197,9 @@ __global__ void __launch_bounds__(kThreads) cache_copy_kernel(const int* __restr
     }
 }
 
-// One cluster, or one CTA.  Columns in use are cut into pieces of `width`, `pieces` to a row; a warp counts the pages of a piece and tells every CTA, each sums
-// over all pieces, and the warp writes its piece's pages, which it still holds where it has one piece of kPiece entries, and else finds in its SM's cache.
-constexpr int kGiveThreads = 1024, kGiveCtas = 8, kLoads = 16, kPiece = 32 * kLoads, kMaxPieces = 2 * kMaxRequests;
+// One CTA.  Columns in use are cut into pieces of `width`, `pieces` to a row; a warp counts the pages of a piece, all sum over all pieces, and the warp writes its
+// piece's pages, which it still holds where it has one piece of kPiece entries, and else finds in the SM's cache.
+constexpr int kGiveThreads = 1024, kLoads = 16, kPiece = 32 * kLoads, kMaxPieces = 2 * kMaxRequests;
 __global__ void __launch_bounds__(kGiveThreads) cache_release_kernel(const int* __restrict__ table, const int* __restrict__ lens, const unsigned char* __restrict__ done,
                                                                      int* __restrict__ free_pages, const int* __restrict__ n_free, int B, int page, int max_pages,
                                                                      int free_capacity, int width, int pieces, bool copied, int* lens_out, int* __restrict__ n_free_out) {
@@ -208,26 +207,19 @@ __global__ void __launch_bounds__(kGiveThreads) cache_release_kernel(const int* 
     int* count = sm;      // [B] columns in use
     int* first = sm + B;   // [B * pieces] pages of a piece, and then of those before it
     __shared__ long long red[2][32];
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, items = B * pieces, n_cta = gridDim.x, cta = blockIdx.x;   // (the grid is one cluster)
-    const int item0 = cta * (threads / 32) + (tid >> 5), apart = n_cta * (threads / 32);
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, items = B * pieces;
     grid_let_next_start();
     grid_wait_for_previous();
-    if (copied) {
-        // Every CTA finds the same: where this is not kHoles, it becomes a length that is not, either, and else it stays until all are at the cluster's barrier.
-        const int last = *(volatile int*)(lens_out + B - 1), held = lens[B - 1], len = done[B - 1] ? 0 : held;
-        if (last != kHoles && len != kHoles) {
-            if (cta == 0 && tid == 0) lens_out[B - 1] = len;
-            return;
-        }
+    if (copied && !__syncthreads_or(tid == 0 && lens_out[B - 1] == kHoles)) {
+        if (tid == 0) lens_out[B - 1] = done[B - 1] ? 0 : lens[B - 1];
+        return;
     }
-    if (n_cta > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const int have_free = min(max(*n_free, 0), free_capacity);
     for (int b = tid; b < B; b += threads) {
         const int held = lens[b], len = done[b] ? held : 0;
         count[b] = len <= 0 ? 0 : min(max_pages, len / page + (len % page != 0));
     }
     __syncthreads();
-    if (n_cta > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // all CTAs have begun: their shared memory may be written
     int x[kLoads];
     auto load = [&](const int* from, int n) {   // kPiece entries, of which n are there
 #pragma unroll
@@ -238,7 +230,7 @@ __global__ void __launch_bounds__(kGiveThreads) cache_release_kernel(const int* 
         *from = table + (long long)b * max_pages + j0;
         return min(count[b] - j0, width);
     };
-    for (int item = item0; item < items; item += apart) {
+    for (int item = tid >> 5; item < items; item += threads / 32) {
         const int* from;
         const int n = piece(item, &from);
         int here = 0;
@@ -248,25 +240,18 @@ __global__ void __launch_bounds__(kGiveThreads) cache_release_kernel(const int* 
             for (int i = 0; i < kLoads; ++i) here += x[i] >= 0;
         }
         here = __reduce_add_sync(0xffffffffu, here);
-        if (n_cta == 1) {
-            if (lane == 0) first[item] = here;
-        } else if (lane < n_cta) {
-            sm100::st_shared_cluster_u32(sm100::map_to_cta(sm100::smem_u32(first + item), lane), here);
-        }
+        if (lane == 0) first[item] = here;
     }
     __syncthreads();
-    if (n_cta > 1) sm100::cluster_sync_all();
     const int per = (items + threads - 1) / threads, i0 = min(items, tid * per), i1 = min(items, i0 + per);
     long long pg = 0, zero = 0;
     for (int i = i0; i < i1; ++i) pg += first[i];
     const long long own = pg;
     cta_sums<kGiveThreads>(pg, zero, red);
-    if (cta == 0) {
-        for (int b = tid; b < B; b += threads) {
-            const int held = lens[b];
-            lens_out[b] = done[b] ? 0 : held;
-        }
-        if (tid == threads - 1) *n_free_out = (int)min(have_free + pg, (long long)free_capacity);
+    if (tid == threads - 1) *n_free_out = (int)min(have_free + pg, (long long)free_capacity);
+    for (int b = tid; b < B; b += threads) {
+        const int held = lens[b];
+        lens_out[b] = done[b] ? 0 : held;
     }
     pg -= own;
     for (int i = i0; i < i1; ++i) {
@@ -275,8 +260,8 @@ __global__ void __launch_bounds__(kGiveThreads) cache_release_kernel(const int* 
         pg += n;
     }
     __syncthreads();
-    const bool held = items <= apart && width == kPiece;
-    for (int item = item0; item < items; item += apart) {
+    const bool held = items <= threads / 32 && width == kPiece;
+    for (int item = tid >> 5; item < items; item += threads / 32) {
         const int* from;
         const int n = piece(item, &from);
         long long to = (long long)have_free + first[item];
@@ -311,9 +296,10 @@ cudaError_t cache_extend(int* table, const int* lens, const int* fresh, const in
     };
     return B <= 1024 ? go(cache_extend_kernel<256>, 256) : go(cache_extend_kernel<1024>, 1024);
 }
-// Pages given back, us from a graph / as calls, by one kernel and by both: 4 requests 3.1 / 5.0 and 3.3 / 7.8; 64 of up to 256 pages 5.8 / 6.1 and 3.5 / 7.4; 512 of
-// up to 512, 65,000 pages, 8.5 / 8.6 and 4.6 / 7.3 (6.0 in the first kernel with a warp per request for one per 128 columns); all 260,000 of them 15.8 / 16.0 and
-// 4.4 / 7.3.  With holes both take as long as one alone and the copying together.
+// Pages given back, us from a graph / as calls: 4 requests 3.1 / 5.0 by the one kernel, 3.3 / 7.8 by both; one with 8192 columns 4.6 / 5.0 and 3.4 / 7.4.  By both: 64 of
+// up to 256 pages 3.7 / 7.1, 512 of up to 512 of which half are done, 65,000 pages, 4.6 / 7.0 (copying with a warp per request for one per 128 columns takes 2.3 more);
+// all 260,000 of them 4.7 / 7.2.  With a hole the 65,000 take 33 us, those of 26 requests 18: one SM does it then, since CTAs that count together would wait for
+// each other in every call to learn whether there is one (0.8 us).
 cudaError_t cache_release(const int* table, const int* lens, const unsigned char* done, int* free_pages, const int* n_free, int B, int page, int max_pages,
                           int free_capacity, int* lens_out, int* n_free_out, cudaStream_t st) {
     int width = kPiece, pieces;
@@ -339,12 +325,9 @@ cudaError_t cache_release(const int* table, const int* lens, const unsigned char
         const cudaError_t e = TT_ALLOW_SMEM(cache_release_kernel, (kMaxRequests + (size_t)kMaxPieces) * sizeof(int));
         if (e != cudaSuccess) return e;
     }
-    const int threads = B * pieces <= 8 ? 256 : kGiveThreads;
-    int n_cta = 1;
-    while (n_cta < kGiveCtas && n_cta * (threads / 32) < B * pieces) n_cta *= 2;
     LaunchScope ls(K_CACHE_TABLES, st);
-    return launch_overlapped_cluster(cache_release_kernel, n_cta, threads, smem, st, n_cta, table, lens, done, free_pages, n_free, B, page, max_pages, free_capacity, width,
-                                     pieces, copied, lens_out, n_free_out);
+    return launch_overlapped(cache_release_kernel, 1, B * pieces <= 8 ? 256 : kGiveThreads, smem, st, table, lens, done, free_pages, n_free, B, page, max_pages, free_capacity,
+                             width, pieces, copied, lens_out, n_free_out);
 }
 
 }  // namespace ttk
