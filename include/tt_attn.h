@@ -262,7 +262,8 @@ int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* bl
  *   seq_lens       [B] or NULL (desc->L each), clamped to 0 .. desc->L; an entry without keys gets out = 0, lse = -inf
  * desc: dtype TT_BF16, S = 1, D 64 or 128, L the longest sequence there may be, at most 2^30; any group H / Hkv.  `lse` may be NULL.
  * q may be of any finite size, as long as scale * q is finite in 32 bits and scores stay below 2^127.
- * out, lse and the workspace must not overlap each other or an input, so `out` cannot be `q`.
+ * out, lse and the workspace must not overlap each other or an input, so `out` cannot be `q`.  A group of more than 16 query heads
+ * reads the cache once for each 16 of them.
  * Products are exact in what the cache holds; probabilities are rounded to 11 bits, sums are 32-bit.  Results repeat to the bit.
  * Workspace: tt_attn_decode_q4_workspace_bytes(desc) bytes, 256-byte aligned, contents ignored; 0 (and NULL) where L is at most 128. */
 size_t tt_attn_decode_q4_workspace_bytes(const tt_attn_desc* desc);

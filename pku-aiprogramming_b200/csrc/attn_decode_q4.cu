@@ -1,9 +1,10 @@
 // Single-query attention over the 4-bit key/value cache: out = softmax(scale q K^T) V with K, V = (n - 8) s.
 //
 // A key and key/value head are 2 (D / 2 + D / 32) bytes, at D = 128 136 of them for 256 values.  At the measured copy rate an SM
-// gets 23 bytes a cycle, so it has 5.9 cycles for those 256 values: what bounds this next to HBM is the instructions that turn
+// gets 23 bytes a cycle, so it has 5.9 cycles for those 256 values: next to HBM what counts is the instructions that turn
 // nibbles into operands.  Operands that are made in registers go to mma.sync, whose accumulators (16 x 8) a group of up to eight
-// query heads fills; tcgen05 would want them in shared or tensor memory, 512 more bytes a key.
+// query heads fills; tcgen05 would want them in shared or tensor memory, 512 more bytes a key.  A warp takes up to 16 query heads; a larger group reads and
+// unpacks the cache once for each 16.
 //
 // Both products are m16n8k16 in halves with 32-bit sums (2.0 cycles per SM each; the 8-bit forms of mma.sync are made of these).  A lane
 // reads exactly the nibbles that are its elements of the operand, and the order of channels within a product is chosen so that they are
@@ -28,10 +29,11 @@
 // a normalised result and its log-sum-exp, which a second kernel merges.  Results do not depend on timing.  Up to 128 keys a warp has a whole slice, and
 // there is no second kernel.
 //
-// One B200, both kernels, replayed from a graph (bytes at the copy rate of 6.46 TB/s): 64 sequences of 4096 to 8192, 32 query on 8 key/value heads, D = 128 94.0 us
-// (64.8); 48 of up to 4096, 16 on 16, D = 64 37.9 (16.2); two of 120,000 to 131,072, 32 on 2 31.0 (10.5); one of 5001, 32 on 8 10.0 (0.9).  Counters of the
-// first: 553 instructions per step of a warp, 336 of them unpacking and products; issue slots 56 % busy, ALU 47 %, half-precision multiply-adds 30 %, tensor
-// pipe 26 %, at 1.75 GHz (power).  The pipes add up more than they overlap: without the loads 80.6 us, the loads alone 67.
+// One B200, both kernels, replayed from a graph, three inputs in turn (bytes at the copy rate of 6.46 TB/s): 64 sequences of 4096 to 8192, 32 query on 8 key/value
+// heads, D = 128 97.4 us (67.6); 48 of up to 4096, 16 on 16, D = 64 39.3 (16.2); two of 120,000 to 131,072, 32 on 2 32.4 (10.5); one of 5001, 32 on 8 10.0 (0.9).
+// Counters of the first: 553 instructions per step of a warp, 336 of them unpacking and products, 138 cycles at four issues each where the bytes take 175;
+// issue slots 56 % busy, ALU 47 %, half-precision multiply-adds 29 %, tensor pipe 26 %, at 1.75 GHz (power).  So no pipe bounds it but the order within a warp: it waits
+// on its own arithmetic, and the loads do not run under all of it (without them 80.6 us, the loads alone 67, of 94).
 #include "cache_q4.cuh"
 #include "sm100_ptx.cuh"
 

@@ -234,7 +234,7 @@ def cache_extend(block_table, seq_lens, new_lens, free_pages, n_free, page_size,
 
 def cache_release(block_table, seq_lens, done, free_pages, n_free, page_size, out=None):
     """The pages of the requests that `done` (bool `[B]`) marks, back on `free_pages` behind its `n_free` -> (seq_lens with
-    0 there, n_free).  `out`: those two tensors, apart from the inputs."""
+    0 there, n_free).  Negative entries of their rows are no pages and are left out.  `out`: those two tensors, apart from the inputs."""
     r = _native.cache_release(block_table, seq_lens, done, free_pages, n_free, page_size, out)
     if r.__class__ is tuple:
         return r
@@ -340,7 +340,8 @@ def attention_decode_q4(q, k_cache, v_cache, block_table=None, seq_lens=None, ma
 
     q `[B,H,1,D]` bfloat16, D 64 or 128.  `block_table` (int32 `[B, max_pages]`) names each sequence's pages; None: batch entry b has
     page b to itself.  `seq_lens` (int32 `[B]`): keys of each sequence.  `max_len`: longest possible sequence (default: what the pages
-    can hold), which decides how the keys are divided.  An empty sequence gives out = 0, lse = -inf."""
+    can hold), which decides how the keys are divided.  An empty sequence gives out = 0, lse = -inf.  A group of more than 16 query heads reads the
+    cache once for each 16."""
     r = _native.attention_decode_q4(q, k_cache, v_cache, block_table, seq_lens, max_len, scale, out, lse, workspace, need_lse)
     return r if r.__class__ is tuple else _done(r, _explain_decode_q4, q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse)
 
