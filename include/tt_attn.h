@@ -295,6 +295,40 @@ typedef struct tt_rotary_desc {
 int tt_rotary(const tt_rotary_desc* desc, const void* q, const void* k, const int32_t* positions, const double* inv_freq,
               const int32_t* axes, int32_t backward, void* q_out, void* k_out, void* stream);
 
+/* ---- norms of heads with rotary positions -----------------------------------------------------
+ * Each query and key head x of D channels divided by its root mean square, times a weight per channel, and turned as by tt_rotary, in
+ * one pass (no counterpart in the reference): r = 1 / sqrt(mean(x^2) + eps), y = weight * r * x, then the first R channels turned (and
+ * times `scale`).  Arithmetic is 32-bit, results are rounded once; sums of squares have to be finite in 32 bits.
+ *   desc, q, k, positions, inv_freq, axes, q_out, k_out   as in tt_rotary
+ *   q_weight, k_weight   [D] each, of weight_dtype (TT_F32 or TT_BF16); k_weight is not read where k is null
+ *   eps                  positive
+ *
+ * tt_norm_rotary_bwd: the gradients for upstream gradients dq, dk (at desc's q_stride, k_stride; results at q_out_stride, k_out_stride, which
+ * may be dq and dk themselves) of the call with inputs q, k (at q_stride, k_stride [3] each).  dq_weight, dk_weight [D] are the sums over all
+ * tokens and heads, of weight_dtype; they repeat to the bit.  dk, k, k_weight, dk_out and dk_weight are all null where there is one tensor
+ * only.  No rows: the weights' gradients are 0.  Outputs must not overlap q, k or anything else.  Workspace: tt_norm_rotary_bwd_workspace_bytes(desc)
+ * bytes (of the current device; 0: no device, or no such head dim), 256-byte aligned, contents ignored. */
+int tt_norm_rotary(const tt_rotary_desc* desc, const void* q, const void* k, const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                   const int32_t* positions, const double* inv_freq, const int32_t* axes, void* q_out, void* k_out, void* stream);
+size_t tt_norm_rotary_bwd_workspace_bytes(const tt_rotary_desc* desc);
+int tt_norm_rotary_bwd(const tt_rotary_desc* desc, const void* dq, const void* dk, const void* q, const void* k, const int64_t* q_stride,
+                       const int64_t* k_stride, const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps, const int32_t* positions,
+                       const double* inv_freq, const int32_t* axes, void* dq_out, void* dk_out, void* dq_weight, void* dk_weight, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* A step's keys and values into a paged 16-bit cache, as tt_attn_decode_paged reads it, with queries and keys turned on the way.
+ * desc: B = 1 and S packed tokens, D 64 or 128; dtype is the inputs' (q, k and v [S, heads, D], v at element strides {token, head}),
+ * outputs and pools are bf16.  With k_weight (and q_weight, where there is q) heads are normed first, as by tt_norm_rotary; both null: not.
+ *   slots    [S] page * page_size + row, as from tt_cache_extend; of a negative one, or one behind the last page, neither key nor value is
+ *            kept.  No two tokens may have one slot (what it then holds is of either, and may be of both).
+ *   q_out    the turned queries; null with q.  k_out: the turned keys once more, for attention over the new tokens themselves, or null.  Either may be
+ *            its input where that is bf16, else outputs and pools overlap nothing
+ *   k_pool, v_pool   [n_pages, Hkv, page_size, D]; other rows keep what they hold */
+int tt_cache_append_rotary(const tt_rotary_desc* desc, const void* q, const void* k, const void* v, const int64_t* v_stride, const int32_t* slots,
+                           const int32_t* positions, const double* inv_freq, const int32_t* axes, const void* q_weight, const void* k_weight,
+                           int32_t weight_dtype, float eps, void* q_out, void* k_out, void* k_pool, void* v_pool, int32_t n_pages, int32_t page_size,
+                           void* stream);
+
 /* ---- row softmax ------------------------------------------------------------------------
  * out[r,:] = softmax(in[r,:]) over `cols`, row maximum subtracted; rows = product of the leading
  * axes.  One launch that reads and writes every element once; replaces SoftmaxForward of

@@ -14,5 +14,6 @@ from .functional import (  # noqa: F401
     check_device_status, softmax_forward, softmax_backward, fc_forward, fc_backward, attention_decode_paged,
     set_backward_deterministic, attention_forward_varlen, attention_backward_varlen,
     CacheStep, cache_extend, cache_release, rotary_frequencies, rotary_forward, rotary_backward,
+    norm_rotary_forward, norm_rotary_backward, cache_append_rotary,
     cache_alloc_q4, cache_append_q4, cache_read_q4, attention_decode_q4,
 )

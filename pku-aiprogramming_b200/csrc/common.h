@@ -145,7 +145,8 @@ enum KernelId {
     K_FWD_TC = 0, K_FWD_SIMT, K_BWD_PREP, K_BWD_DKV, K_BWD_DQ, K_BWD_SIMT_DELTA, K_BWD_SIMT_DQ, K_BWD_SIMT_DKV,
     K_DECODE, K_DECODE_MERGE, K_PROBE, K_SOFTMAX_FWD, K_SOFTMAX_BWD, K_FC_GEMM, K_FC_SIMT, K_FC_COLSUM, K_BWD_FUSED,
     K_BWD_DQ_CONVERT, K_DECODE_GQ, K_FWD_F32, K_BWD_F32, K_BWD_BOTH, K_CACHE_TABLES,
-    K_ROTARY, K_CACHE_APPEND, K_CACHE_READ, K_DECODE_Q4, K_COUNT
+    K_ROTARY, K_CACHE_APPEND, K_CACHE_READ, K_DECODE_Q4, K_NORM_ROTARY, K_NORM_ROTARY_BWD, K_NORM_ROTARY_DW, K_CACHE_APPEND_ROTARY,
+    K_COUNT
 };
 // Scoped around ONE kernel launch: counts it and, when timing is enabled, brackets it with
 // CUDA events on the launching stream.
@@ -300,6 +301,29 @@ struct RotaryArgs {
     int back;
 };
 cudaError_t rotary(const RotaryArgs& a, int bf16, int interleaved, cudaStream_t st);
+
+// --- norms of heads with rotary positions (norm_rotary.cu)
+struct NormRotaryArgs {
+    RotaryArgs r;           // backward: x is the gradient of the result, y that of the input
+    const void* w[2];       // [D] for query and key heads
+    int w_bf16;
+    float eps;
+    // backward: the forward's input, and the weights' gradients
+    const void* in[2];
+    long long in_stride[2][3];
+    void* dw[2];
+    // into a paged cache (w null: no norm): values [S, heads[1], D] at strides {token, head}, and pools of bf16 rows [pages, heads[1], page, D];
+    // y[0] and y[1] are bf16, y[1] null or the keys once more
+    const void* v;
+    long long v_stride[2];
+    const int* slots;
+    void* pool[2];
+    int n_slots, page;
+};
+cudaError_t norm_rotary(const NormRotaryArgs& a, int bf16, int interleaved, cudaStream_t st);
+size_t norm_rotary_backward_workspace(int D);
+cudaError_t norm_rotary_backward(const NormRotaryArgs& a, int bf16, int interleaved, void* workspace, cudaStream_t st);
+cudaError_t cache_append_rotary(const NormRotaryArgs& a, int bf16, int interleaved, cudaStream_t st);
 
 // Builds a 3-D bf16 tensor map over a dense [slices, rows, cols] array, box
 // [1, box_rows, 64] with 128-byte swizzle.  Returns false (and sets `why`) on failure.

@@ -595,60 +595,218 @@ bool heads_arg(const Tensor& t, int64_t* B, int64_t* H, int64_t* S, int64_t (&st
     return fits32(*B) && fits32(*H) && fits32(*S);
 }
 
+// Query and key heads with what turns them.
+struct HeadArgs {
+    tt_rotary_desc d = {};
+    const Tensor *q = nullptr, *k = nullptr, *pos = nullptr, *freq = nullptr, *axes = nullptr;
+    Tensor made[2];
+    const Tensor* out[2] = {nullptr, nullptr};
+    enum { kFits, kNot, kError };
+
+    // q or k may be None, not both
+    int read(PyObject* oq, PyObject* ok, PyObject* opos, PyObject* ofreq, PyObject* oaxes, PyObject* inter, PyObject* scale) {
+        int64_t B = 0, H = 0, S = 0, Bk = 0, Hk = 0, Sk = 0;
+        PyObject* first = oq != Py_None ? oq : ok;
+        if (!THPVariable_Check(first)) return kNot;
+        const Tensor& x = THPVariable_Unpack(first);
+        if (!x.is_cuda() || !float_type(x)) return kNot;
+        if (oq != Py_None) {
+            q = &x;
+            if (!heads_arg(x, &B, &H, &S, d.q_stride)) return kNot;
+        }
+        if (ok != Py_None) {
+            k = on_device(ok, x.scalar_type(), &x);
+            if (!k || k->dim() != x.dim() || !heads_arg(*k, &Bk, &Hk, &Sk, d.k_stride) || (q && (Bk != B || Sk != S)) || k->size(-1) != x.size(-1)) return kNot;
+            B = Bk, S = Sk;
+        }
+        pos = on_device(opos, at::kInt, &x), freq = vector_arg(ofreq, at::kDouble, -1, &x);
+        if (!pos || !freq || pos->dim() < 1 || pos->dim() > x.dim() - 1 || pos->size(-1) != S || (S > 1 && pos->stride(-1) != 1)) return kNot;
+        const int64_t n_axes = pos->dim() > 1 ? pos->size(0) : 1;
+        if (pos->dim() == 3 && pos->size(1) != B) return kNot;
+        if (oaxes != Py_None ? !(axes = vector_arg(oaxes, at::kInt, freq->size(0), &x)) : n_axes != 1) return kNot;   // (rows that nothing would read)
+        d.pos_stride[0] = pos->dim() > 1 ? pos->stride(0) : 0;
+        d.pos_stride[1] = pos->dim() == 3 ? pos->stride(1) : 0;
+        const int interleaved = PyObject_IsTrue(inter);
+        if (interleaved < 0 || !scale_arg(scale, &d.scale)) return kError;
+        if (scale == Py_None) d.scale = 1.f;
+        if (!fits32(n_axes) || !fits32(2 * freq->size(0)) || !fits32(x.size(-1))) return kNot;
+        d.B = (int32_t)B, d.S = (int32_t)S, d.H = (int32_t)H, d.Hkv = (int32_t)Hk, d.D = (int32_t)x.size(-1), d.R = (int32_t)(2 * freq->size(0));
+        d.n_axes = (int32_t)n_axes, d.dtype = tt_type(x), d.interleaved = interleaved;
+        return kFits;
+    }
+    // Results of a type, given (of their input's shape) or new.
+    bool results(PyObject* oq, PyObject* ok, at::ScalarType type) {
+        PyObject* given[2] = {oq, ok};
+        const Tensor* in[2] = {q, k};
+        // Short results, up to 2^19 values (1 MB of bf16), share an allocation: a call 3.9 us up to it, 4.4 beyond.  Long ones have their own, which each gives back
+        // by itself.
+        const int64_t k_at = q ? (q->numel() + 127) / 128 * 128 : 0, all = k ? k_at + k->numel() : 0;
+        if (k && k_at && all <= 1 << 19 && oq == Py_None && ok == Py_None) {
+            const Tensor whole = make({all}, type, *q);
+            made[0] = part_of(whole, 0, q->sizes(), whole.dtype());
+            made[1] = part_of(whole, k_at, k->sizes(), whole.dtype());
+        }
+        for (int i = 0; i < 2; ++i) {
+            if (!in[i]) {
+                if (given[i] != Py_None) return false;
+                continue;
+            }
+            if (given[i] != Py_None) {
+                out[i] = on_device(given[i], type, in[i]);
+                if (!out[i] || !same_shape(*out[i], *in[i])) return false;
+            } else {
+                if (!made[i].defined()) made[i] = make(in[i]->sizes(), type, *in[i]);
+                out[i] = &made[i];
+            }
+            if (!strides_of(*out[i], i ? d.k_out_stride : d.q_out_stride)) return false;
+        }
+        return true;
+    }
+    static bool strides_of(const Tensor& t, int64_t (&stride)[3]) {
+        int64_t B, H, S;
+        return heads_arg(t, &B, &H, &S, stride);
+    }
+    const int32_t* positions() const { return (const int32_t*)ptr(pos); }
+    const double* frequencies() const { return (const double*)ptr(freq); }
+    const int32_t* which() const { return (const int32_t*)ptr(axes); }
+};
+// What read() found that is not kFits.
+#define TT_READ(call)                                   \
+    switch (call) {                                     \
+        case HeadArgs::kNot: Py_RETURN_NONE;            \
+        case HeadArgs::kError: return nullptr;          \
+        default: break;                                 \
+    }
+
 // (q, k, positions, inv_freq, axes, interleaved, scale, backward, out_q, out_k) -> (q, k)
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        if (n != 10 || !THPVariable_Check(a[0])) Py_RETURN_NONE;
-        const Tensor& q = THPVariable_Unpack(a[0]);
-        tt_rotary_desc d = {};
-        int64_t B, H, S, Bk = 0, Hk = 0, Sk = 0;
-        if (!q.is_cuda() || !float_type(q) || !heads_arg(q, &B, &H, &S, d.q_stride)) Py_RETURN_NONE;
-        const Tensor* k = nullptr;
-        if (a[1] != Py_None) {
-            k = on_device(a[1], q.scalar_type(), &q);
-            if (!k || k->dim() != q.dim() || !heads_arg(*k, &Bk, &Hk, &Sk, d.k_stride) || Bk != B || Sk != S || k->size(-1) != q.size(-1)) Py_RETURN_NONE;
-        } else if (a[9] != Py_None) {
-            Py_RETURN_NONE;
-        }
-        const Tensor *pos = on_device(a[2], at::kInt, &q), *freq = vector_arg(a[3], at::kDouble, -1, &q), *axes = nullptr;
-        if (!pos || !freq || pos->dim() < 1 || pos->dim() > q.dim() - 1 || pos->size(-1) != S || (S > 1 && pos->stride(-1) != 1)) Py_RETURN_NONE;
-        const int64_t n_axes = pos->dim() > 1 ? pos->size(0) : 1;
-        if (pos->dim() == 3 && pos->size(1) != B) Py_RETURN_NONE;
-        if (a[4] != Py_None ? !(axes = vector_arg(a[4], at::kInt, freq->size(0), &q)) : n_axes != 1) Py_RETURN_NONE;   // (rows that nothing would read)
-        d.pos_stride[0] = pos->dim() > 1 ? pos->stride(0) : 0;
-        d.pos_stride[1] = pos->dim() == 3 ? pos->stride(1) : 0;
-        const int inter = PyObject_IsTrue(a[5]), back = PyObject_IsTrue(a[7]);
-        if (inter < 0 || back < 0 || !scale_arg(a[6], &d.scale)) return nullptr;
-        if (a[6] == Py_None) d.scale = 1.f;
-        if (!fits32(n_axes) || !fits32(2 * freq->size(0)) || !fits32(q.size(-1))) Py_RETURN_NONE;
-        d.B = (int32_t)B, d.S = (int32_t)S, d.H = (int32_t)H, d.Hkv = (int32_t)Hk, d.D = (int32_t)q.size(-1), d.R = (int32_t)(2 * freq->size(0));
-        d.n_axes = (int32_t)n_axes, d.dtype = tt_type(q), d.interleaved = inter;
-        OnDevice dev(q);
-        Tensor made[2];
-        const Tensor* out[2] = {nullptr, nullptr};
-        // Short results, up to 2^19 values (1 MB of bf16), share an allocation: a call 3.9 us up to it, 4.4 beyond.  Long ones have their own, which each gives back
-        // by itself.
-        const int64_t k_at = (q.numel() + 127) / 128 * 128, all = k ? k_at + k->numel() : 0;
-        if (k && k_at && all <= 1 << 19 && a[8] == Py_None && a[9] == Py_None) {
-            const Tensor whole = make({all}, q.scalar_type(), q);
-            made[0] = part_of(whole, 0, q.sizes(), whole.dtype());
-            made[1] = part_of(whole, k_at, k->sizes(), whole.dtype());
-        }
-        for (int i = 0; i < (k ? 2 : 1); ++i) {
-            const Tensor& x = i ? *k : q;
-            if (a[8 + i] != Py_None) {
-                out[i] = on_device(a[8 + i], q.scalar_type(), &q);
-                if (!out[i] || !same_shape(*out[i], x)) Py_RETURN_NONE;
-            } else {
-                if (!made[i].defined()) made[i] = make_like(x);
-                out[i] = &made[i];
-            }
-            if (!heads_arg(*out[i], &Bk, &Hk, &Sk, i ? d.k_out_stride : d.q_out_stride)) Py_RETURN_NONE;
-        }
-        TT_CALL(rc, tt_rotary(&d, ptr(q), ptr(k), (const int32_t*)ptr(pos), (const double*)ptr(freq), (const int32_t*)ptr(axes), back, ptr(out[0]), ptr(out[1]),
-                              dev.stream));
+        if (n != 10 || a[0] == Py_None) Py_RETURN_NONE;
+        HeadArgs h;
+        TT_READ(h.read(a[0], a[1], a[2], a[3], a[4], a[5], a[6]));
+        const int back = PyObject_IsTrue(a[7]);
+        if (back < 0) return nullptr;
+        OnDevice dev(*h.q);
+        if (!h.results(a[8], a[9], h.q->scalar_type())) Py_RETURN_NONE;
+        TT_CALL(rc, tt_rotary(&h.d, ptr(h.q), ptr(h.k), h.positions(), h.frequencies(), h.which(), back, ptr(h.out[0]), ptr(h.out[1]), dev.stream));
         if (rc != TT_OK) return failed(rc);
-        return pack(wrap_or(a[8], made[0]), wrap_or(a[9], made[1]));
+        return pack(wrap_or(a[8], h.made[0]), wrap_or(a[9], h.made[1]));
+    });
+}
+
+// Weights [D] of the heads, of one type, which is the heads' or float; k's is None where there is no k
+bool weights_arg(PyObject* oq, PyObject* ok, const Tensor& x, bool with_q, bool with_k, const Tensor** wq, const Tensor** wk) {
+    const int64_t D = x.size(-1);
+    auto one = [&](PyObject* o) -> const Tensor* {
+        const Tensor* w = vector_arg(o, at::kFloat, D, &x);
+        return w ? w : vector_arg(o, x.scalar_type(), D, &x);
+    };
+    *wq = *wk = nullptr;
+    if (with_q ? !(*wq = one(oq)) : oq != Py_None) return false;
+    if (with_k ? !(*wk = one(ok)) : ok != Py_None) return false;
+    return !with_q || !with_k || (*wq)->scalar_type() == (*wk)->scalar_type();
+}
+bool eps_arg(PyObject* o, float* eps) {
+    if (o == Py_None) {
+        *eps = 0.f;   // (refused by the call)
+        return true;
+    }
+    return scale_arg(o, eps);
+}
+
+// (q, k, q_weight, k_weight, positions, inv_freq, axes, interleaved, eps, scale, out_q, out_k) -> (q, k)
+PyObject* norm_rotary_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 12 || a[0] == Py_None) Py_RETURN_NONE;
+        HeadArgs h;
+        TT_READ(h.read(a[0], a[1], a[4], a[5], a[6], a[7], a[9]));
+        const Tensor *wq, *wk;
+        float eps;
+        if (!weights_arg(a[2], a[3], *h.q, true, h.k != nullptr, &wq, &wk)) Py_RETURN_NONE;
+        if (!eps_arg(a[8], &eps)) return nullptr;
+        OnDevice dev(*h.q);
+        if (!h.results(a[10], a[11], h.q->scalar_type())) Py_RETURN_NONE;
+        TT_CALL(rc, tt_norm_rotary(&h.d, ptr(h.q), ptr(h.k), ptr(wq), ptr(wk), tt_type(*wq), eps, h.positions(), h.frequencies(), h.which(), ptr(h.out[0]),
+                                   ptr(h.out[1]), dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(wrap_or(a[10], h.made[0]), wrap_or(a[11], h.made[1]));
+    });
+}
+
+// (dq, dk, q, k, q_weight, k_weight, positions, inv_freq, axes, interleaved, eps, scale, out_q, out_k, workspace) -> (dq, dk, dq_weight, dk_weight)
+PyObject* norm_rotary_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 15 || a[0] == Py_None) Py_RETURN_NONE;
+        HeadArgs h;
+        TT_READ(h.read(a[0], a[1], a[6], a[7], a[8], a[9], a[11]));
+        const Tensor *wq, *wk, *x[2] = {nullptr, nullptr}, *g[2] = {h.q, h.k}, *ws = nullptr;
+        int64_t strides[2][3] = {};
+        float eps;
+        for (int i = 0; i < 2; ++i) {
+            if (!g[i]) {
+                if (a[2 + i] != Py_None) Py_RETURN_NONE;
+                continue;
+            }
+            x[i] = on_device(a[2 + i], g[i]->scalar_type(), g[i]);
+            if (!x[i] || !same_shape(*x[i], *g[i]) || !HeadArgs::strides_of(*x[i], strides[i])) Py_RETURN_NONE;
+        }
+        if (!weights_arg(a[4], a[5], *h.q, true, h.k != nullptr, &wq, &wk)) Py_RETURN_NONE;
+        if (!eps_arg(a[10], &eps)) return nullptr;
+        if (a[14] != Py_None && (!THPVariable_Check(a[14]) || !(ws = &THPVariable_Unpack(a[14]))->is_contiguous() || ws->device() != h.q->device())) Py_RETURN_NONE;
+        OnDevice dev(*h.q);
+        if (!h.results(a[12], a[13], h.q->scalar_type())) Py_RETURN_NONE;
+        // both weights' gradients in one allocation
+        const int64_t D = h.q->size(-1), apart = (D + 63) / 64 * 64;
+        const Tensor sums = make({h.k ? apart + D : D}, wq->scalar_type(), *h.q);
+        const Tensor dwq = part_of(sums, 0, {D}, sums.dtype()), dwk = h.k ? part_of(sums, apart, {D}, sums.dtype()) : Tensor();
+        Tensor made;
+        size_t bytes;
+        ws = workspace_arg(ws, tt_norm_rotary_bwd_workspace_bytes(&h.d), 0, *h.q, &made, &bytes);
+        TT_CALL(rc, tt_norm_rotary_bwd(&h.d, ptr(h.q), ptr(h.k), ptr(x[0]), ptr(x[1]), strides[0], strides[1], ptr(wq), ptr(wk), tt_type(*wq), eps, h.positions(),
+                                       h.frequencies(), h.which(), ptr(h.out[0]), ptr(h.out[1]), ptr(dwq), h.k ? ptr(dwk) : nullptr, ptr(ws), bytes, dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(wrap_or(a[12], h.made[0]), wrap_or(a[13], h.made[1]), wrap(dwq), wrap_or(Py_None, dwk));
+    });
+}
+
+// (q, k, v, slots, positions, inv_freq, k_pool, v_pool, axes, interleaved, q_weight, k_weight, eps, scale, out_q, out_k) -> (q,)
+PyObject* cache_append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 16 || a[1] == Py_None) Py_RETURN_NONE;
+        HeadArgs h;
+        TT_READ(h.read(a[0], a[1], a[4], a[5], a[8], a[9], a[13]));
+        const Tensor& k = *h.k;
+        const Tensor *v = on_device(a[2], k.scalar_type(), &k), *slots = vector_arg(a[3], at::kInt, h.d.S, &k);
+        if (k.dim() != 3 || !v || v->dim() != 3 || !same_shape(*v, k) || (v->size(2) > 1 && v->stride(2) != 1) || !slots) Py_RETURN_NONE;
+        const Tensor* pool[2];
+        for (int i = 0; i < 2; ++i) {
+            pool[i] = on_device(a[6 + i], at::kBFloat16, &k);
+            if (!pool[i] || !pool[i]->is_contiguous() || pool[i]->dim() != 4 || pool[i]->size(1) != k.size(1) || pool[i]->size(3) != k.size(2) ||
+                !same_shape(*pool[i], *pool[0]) || !fits32(pool[i]->size(0)) || !fits32(pool[i]->size(2)))
+                Py_RETURN_NONE;
+        }
+        const bool normed = a[11] != Py_None;
+        const Tensor *wq, *wk;
+        float eps;
+        if (!weights_arg(a[10], a[11], k, h.q && normed, normed, &wq, &wk)) Py_RETURN_NONE;
+        if (!eps_arg(a[12], &eps)) return nullptr;
+        OnDevice dev(k);
+        // (the keys once more only where the caller gives a place)
+        const Tensor *all_k = h.k, *also = nullptr;
+        h.k = nullptr;
+        const bool fit = h.results(a[14], Py_None, at::kBFloat16);
+        h.k = all_k;
+        if (!fit) Py_RETURN_NONE;
+        if (a[15] != Py_None) {
+            also = on_device(a[15], at::kBFloat16, &k);
+            if (!also || !same_shape(*also, k) || !HeadArgs::strides_of(*also, h.d.k_out_stride)) Py_RETURN_NONE;
+        }
+        const int64_t vs[2] = {v->stride(0), v->stride(1)};
+        TT_CALL(rc, tt_cache_append_rotary(&h.d, ptr(h.q), ptr(k), ptr(v), vs, (const int32_t*)ptr(slots), h.positions(), h.frequencies(), h.which(), ptr(wq), ptr(wk),
+                                           wk ? tt_type(*wk) : TT_F32, eps, h.out[0] ? ptr(h.out[0]) : nullptr, ptr(also), ptr(pool[0]), ptr(pool[1]),
+                                           (int32_t)pool[0]->size(0), (int32_t)pool[0]->size(2), dev.stream));
+        if (rc != TT_OK) return failed(rc);
+        return pack(wrap_or(a[14], h.made[0]));
     });
 }
 
@@ -778,7 +936,7 @@ PyMethodDef methods[] = {
     TT_METHOD(attention_forward), TT_METHOD(attention_backward), TT_METHOD(attention_forward_varlen),
     TT_METHOD(attention_backward_varlen), TT_METHOD(attention_decode), TT_METHOD(attention_decode_paged),
     TT_METHOD(softmax_forward), TT_METHOD(softmax_backward), TT_METHOD(fc_forward), TT_METHOD(fc_backward), TT_METHOD(cache_extend), TT_METHOD(cache_release),
-    TT_METHOD(rotary), TT_METHOD(cache_append_q4), TT_METHOD(cache_read_q4),
+    TT_METHOD(rotary), TT_METHOD(norm_rotary_forward), TT_METHOD(norm_rotary_backward), TT_METHOD(cache_append_rotary), TT_METHOD(cache_append_q4), TT_METHOD(cache_read_q4),
     TT_METHOD(attention_decode_q4),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ttorch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,23 +1,13 @@
 // Rotary positions on query and key heads, several axes, forward and backward.
 //
-// Pair i of a token turns by p[axis_i] * f_i.  In 32 bits a position of 10^6 leaves 0.03 of a radian of the product, so
-// it is taken in 64, in turns, less its nearest whole number; the rest, at most half a turn, goes through sincospif.
+// Pair i of a token turns by p[axis_i] * f_i (rt_turn).
 //
 // HBM-bound: every value is read and written once.  A CTA takes a few tokens: their R / 2 sines and cosines go to shared memory
 // once (for up to 40 heads that use them), then a thread keeps its place in the head -- up to 16 bytes of one half and their partners
 // in the other, or of neighbours -- and walks over tokens and heads, so an access of a warp is whole rows.
-#include "common.h"
+#include "rotary_parts.cuh"
 
 namespace ttk {
-
-template <typename T> __device__ __forceinline__ float rt_get(T v);
-template <> __device__ __forceinline__ float rt_get(float v) { return v; }
-template <> __device__ __forceinline__ float rt_get(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T rt_put(float v);
-template <> __device__ __forceinline__ float rt_put(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 rt_put(float v) { return __float2bfloat16_rn(v); }
-
-template <typename T, int kV> struct alignas(sizeof(T) * kV) RtVec { T v[kV]; };
 
 constexpr int kRotaryThreads = 256;
 
@@ -41,33 +31,21 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs
     const int half = a.R / 2, tid = threadIdx.y * blockDim.x + threadIdx.x, n_threads = blockDim.x * blockDim.y;
     const unsigned t0 = blockIdx.x * (unsigned)tokens_per_cta, n_tok = (unsigned)a.B * (unsigned)a.S;
     const int here = (int)min((unsigned)tokens_per_cta, n_tok - t0);
-    const unsigned b0 = a.B > 1 ? t0 / (unsigned)a.S : 0;
-    auto place = [&](int t, int* b, int* s) {
-        unsigned x = t0 - b0 * (unsigned)a.S + t, y = b0;
-        while (x >= (unsigned)a.S) {
-            x -= (unsigned)a.S;
-            ++y;
-        }
-        *b = (int)y;
-        *s = (int)x;
-    };
+    const RtPlaces places(t0, a.B, a.S);
     grid_let_next_start();
     grid_wait_for_previous();
     for (int i = tid; i < here * half; i += n_threads) {
         const int t = (int)(((float)i + 0.5f) * per_half), pair = i - t * half;   // i < 2^13: exact
         int b, s;
-        place(t, &b, &s);
+        places.at(t, &b, &s);
         const int axis = a.axes ? min(max(a.axes[pair], 0), a.n_axes - 1) : 0;
         const int p = a.pos[axis * a.pos_axis + b * a.pos_batch + s];
-        const double turns = (double)p * a.inv_freq[pair] * 0.15915494309189533576888;   // / 2 pi
-        float sn, co;
-        sincospif((float)(2.0 * (turns - rint(turns))), &sn, &co);
         const int u = pair / kPairs, e = pair % kPairs;
-        cs[t * half + (kPairs == 1 ? u : 2 * ((e >> 1) * turned + u) + (e & 1))] = make_float2(a.scale * co, a.back ? -a.scale * sn : a.scale * sn);
+        cs[t * half + (kPairs == 1 ? u : 2 * ((e >> 1) * turned + u) + (e & 1))] = rt_turn(p, a.inv_freq[pair], a.scale, a.back);
     }
     for (int i = n_threads - 1 - tid; i < 2 * here; i += n_threads) {
         int b, s;
-        place(i >> 1, &b, &s);
+        places.at(i >> 1, &b, &s);
         const int w = i & 1;
         rows[i] = RtRows<T>{(const T*)a.x[w] + b * a.xs[w][0] + s * a.xs[w][2], (T*)a.y[w] + b * a.ys[w][0] + s * a.ys[w][2]};
     }

@@ -118,6 +118,88 @@ bool rows_meet(const Rows& x, const Rows& y, int D, size_t size) {
     return false;
 }
 
+size_t element(const tt_rotary_desc* d) { return d->dtype == TT_BF16 ? 2 : 4; }
+int rotary_desc_args(const char* who, const tt_rotary_desc* d, bool with_q, bool with_k) {
+    if (!d) return fail(TT_ERR_NULL, "%s: desc is null", who);
+    const int hk = with_k ? d->Hkv : 0;
+    if (d->B < 0 || d->S < 0 || (with_q && d->H < 1) || (with_k && hk < 1)) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d S=%d H=%d Hkv=%d", who, d->B, d->S, d->H, d->Hkv);
+    if (d->D < 2 || d->D > 256 || d->R < 2 || d->R > d->D || d->R % 2)
+        return fail(TT_ERR_BAD_SHAPE, "%s: D=%d must be 2..256 and R=%d even, 2..D", who, d->D, d->R);
+    if (d->n_axes < 1) return fail(TT_ERR_BAD_SHAPE, "%s: n_axes=%d", who, d->n_axes);
+    if (d->dtype != TT_F32 && d->dtype != TT_BF16) return fail(TT_ERR_BAD_DTYPE, "%s: dtype %d unknown", who, d->dtype);
+    if (!std::isfinite(d->scale)) return fail(TT_ERR_BAD_SHAPE, "%s: scale is not finite", who);
+    if ((int64_t)d->B * d->S >= (1LL << 31) || (int64_t)(with_q ? d->H : 0) + hk >= (1LL << 24)) return fail(TT_ERR_BAD_SHAPE, "%s: more than 2^31-1 tokens or 2^24 heads", who);
+    return TT_OK;
+}
+int norm_args(const char* who, const tt_rotary_desc* d, int32_t weight_dtype, float eps) {
+    if (weight_dtype != TT_F32 && weight_dtype != TT_BF16) return fail(TT_ERR_BAD_DTYPE, "%s: weight dtype %d unknown", who, weight_dtype);
+    if (!(eps > 0.f) || !std::isfinite(eps)) return fail(TT_ERR_BAD_SHAPE, "%s: eps must be positive and finite", who);
+    return TT_OK;
+}
+bool in_place(const Rows& x, const Rows& y) {
+    for (int i = 0; i < 3; ++i)
+        if (x.n[i] > 1 && x.st[i] != y.st[i]) return false;
+    return x.span.p == y.span.p;
+}
+// Query and key heads and what becomes of them.
+struct Heads {
+    int n[2][3], count;
+    size_t size;
+    Rows in[2], out[2];
+    Heads(const tt_rotary_desc* d, const void* q, const void* k, const void* q_out, const void* k_out, size_t element)
+        : n{{d->B, d->H, d->S}, {d->B, k ? d->Hkv : 0, d->S}}, count(k ? 2 : 1), size(element),
+          in{{q, d->q_stride, n[0], d->D, element, "q"}, {k, d->k_stride, n[1], d->D, element, "k"}},
+          out{{q_out, d->q_out_stride, n[0], d->D, element, "q_out"}, {k_out, d->k_out_stride, n[1], d->D, element, "k_out"}} {}
+    // An output lies on its own input row by row, or apart from everything.
+    int check(const char* who, const tt_rotary_desc* d) const {
+        for (int i = 0; i < 3; ++i)
+            if (d->q_stride[i] < 0 || d->q_out_stride[i] < 0 || (count > 1 && (d->k_stride[i] < 0 || d->k_out_stride[i] < 0)) || (i < 2 && d->pos_stride[i] < 0))
+                return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
+        if (((uintptr_t)in[0].span.p | (uintptr_t)out[0].span.p | (uintptr_t)in[1].span.p | (uintptr_t)out[1].span.p) % size)
+            return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
+        if (!rows_apart(d->q_out_stride, n[0], d->D) || (count > 1 && !rows_apart(d->k_out_stride, n[1], d->D)))
+            return fail(TT_ERR_BAD_SHAPE, "%s: rows of an output overlap", who);
+        for (int i = 0; i < count; ++i)
+            for (int j = 0; j < count; ++j)
+                if (!(i == j && in_place(out[i], in[j])) && rows_meet(out[i], in[j], d->D, size))
+                    return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in[j].span.name);
+        if (count > 1 && rows_meet(out[0], out[1], d->D, size)) return fail(TT_ERR_BAD_SHAPE, "%s: q_out overlaps k_out", who);
+        return TT_OK;
+    }
+};
+Span positions_span(const tt_rotary_desc* d, const int32_t* positions) {
+    return {positions, (size_t)((d->n_axes - 1) * d->pos_stride[0] + (d->B - 1) * d->pos_stride[1] + d->S) * 4, "positions"};
+}
+int rotary_spans(const char* who, const Heads& h, const tt_rotary_desc* d, const int32_t* positions, const double* inv_freq, const int32_t* axes) {
+    const Span angles[] = {positions_span(d, positions), {inv_freq, (size_t)d->R / 2 * 8, "inv_freq"}, {axes, (size_t)d->R / 2 * 4, "axes"}};
+    for (int i = 0; i < h.count; ++i)
+        for (const Span& x : angles)
+            if (overlap(h.out[i].span, x)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, h.out[i].span.name, x.name);
+    return TT_OK;
+}
+int weight_spans(const char* who, const Heads& h, const tt_rotary_desc* d, const void* q_weight, const void* k_weight, int32_t dtype) {
+    const size_t size = dtype == TT_BF16 ? 2 : 4, w = (size_t)d->D * size;
+    if (((uintptr_t)q_weight | (h.count > 1 ? (uintptr_t)k_weight : 0)) % size) return fail(TT_ERR_BAD_SHAPE, "%s: weights must be multiples of their element size", who);
+    const Span weights[] = {{q_weight, w, "q_weight"}, {h.count > 1 ? k_weight : nullptr, w, "k_weight"}};
+    for (int i = 0; i < h.count; ++i)
+        for (const Span& x : weights)
+            if (overlap(h.out[i].span, x)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, h.out[i].span.name, x.name);
+    return TT_OK;
+}
+RotaryArgs rotary_args(const tt_rotary_desc* d, const void* q, const void* k, const int32_t* positions, const double* inv_freq, const int32_t* axes, void* q_out, void* k_out) {
+    RotaryArgs a = {};
+    a.x[0] = q; a.x[1] = k; a.y[0] = q_out; a.y[1] = k_out;
+    for (int i = 0; i < 3; ++i) {
+        a.xs[0][i] = d->q_stride[i]; a.xs[1][i] = d->k_stride[i];
+        a.ys[0][i] = d->q_out_stride[i]; a.ys[1][i] = d->k_out_stride[i];
+    }
+    a.heads[0] = q ? d->H : 0; a.heads[1] = k ? d->Hkv : 0;
+    a.B = d->B; a.S = d->S; a.D = d->D; a.R = d->R; a.n_axes = d->n_axes;
+    a.pos = positions; a.pos_axis = d->pos_stride[0]; a.pos_batch = d->pos_stride[1];
+    a.inv_freq = inv_freq; a.axes = axes; a.scale = d->scale;
+    return a;
+}
+
 }  // namespace
 }  // namespace ttk
 
@@ -253,58 +335,157 @@ int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cac
 int tt_rotary(const tt_rotary_desc* d, const void* q, const void* k, const int32_t* positions, const double* inv_freq, const int32_t* axes, int32_t backward,
               void* q_out, void* k_out, void* stream) {
     const char* who = "tt_rotary";
-    if (!d) return fail(TT_ERR_NULL, "%s: desc is null", who);
-    const int hk = k ? d->Hkv : 0;
-    if (d->B < 0 || d->S < 0 || d->H < 1 || (k && hk < 1)) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d S=%d H=%d Hkv=%d", who, d->B, d->S, d->H, d->Hkv);
-    if (d->D < 2 || d->D > 256 || d->R < 2 || d->R > d->D || d->R % 2)
-        return fail(TT_ERR_BAD_SHAPE, "%s: D=%d must be 2..256 and R=%d even, 2..D", who, d->D, d->R);
-    if (d->n_axes < 1) return fail(TT_ERR_BAD_SHAPE, "%s: n_axes=%d", who, d->n_axes);
-    if (d->dtype != TT_F32 && d->dtype != TT_BF16) return fail(TT_ERR_BAD_DTYPE, "%s: dtype %d unknown", who, d->dtype);
-    if (!std::isfinite(d->scale)) return fail(TT_ERR_BAD_SHAPE, "%s: scale is not finite", who);
-    if ((int64_t)d->B * d->S >= (1LL << 31) || (int64_t)d->H + hk >= (1LL << 24)) return fail(TT_ERR_BAD_SHAPE, "%s: more than 2^31-1 tokens or 2^24 heads", who);
+    int rc = rotary_desc_args(who, d, true, k != nullptr);
+    if (rc != TT_OK) return rc;
     if ((k == nullptr) != (k_out == nullptr)) return fail(TT_ERR_NULL, "%s: k and k_out go together", who);
     if (d->B == 0 || d->S == 0) return TT_OK;
     if (!q || !q_out || !positions || !inv_freq) return fail(TT_ERR_NULL, "%s: null pointer", who);
-    const size_t size = d->dtype == TT_BF16 ? 2 : 4;
-    const int nq[3] = {d->B, d->H, d->S}, nk[3] = {d->B, hk, d->S};
-    for (int i = 0; i < 3; ++i)
-        if (d->q_stride[i] < 0 || d->q_out_stride[i] < 0 || (k && (d->k_stride[i] < 0 || d->k_out_stride[i] < 0)) || (i < 2 && d->pos_stride[i] < 0))
-            return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
-    if (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
-    if (!rows_apart(d->q_out_stride, nq, d->D) || (k && !rows_apart(d->k_out_stride, nk, d->D)))
-        return fail(TT_ERR_BAD_SHAPE, "%s: rows of an output overlap", who);
-    // An output lies on its own input row by row, or apart from everything.
-    const Rows in[2] = {{q, d->q_stride, nq, d->D, size, "q"}, {k, d->k_stride, nk, d->D, size, "k"}};
-    const Rows out[2] = {{q_out, d->q_out_stride, nq, d->D, size, "q_out"}, {k_out, d->k_out_stride, nk, d->D, size, "k_out"}};
-    auto in_place = [](const Rows& x, const Rows& y) {
-        for (int i = 0; i < 3; ++i)
-            if (x.n[i] > 1 && x.st[i] != y.st[i]) return false;
-        return x.span.p == y.span.p;
-    };
-    for (int i = 0; i < (k ? 2 : 1); ++i)
-        for (int j = 0; j < (k ? 2 : 1); ++j)
-            if (!(i == j && in_place(out[i], in[j])) && rows_meet(out[i], in[j], d->D, size))
-                return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in[j].span.name);
-    if (k && rows_meet(out[0], out[1], d->D, size)) return fail(TT_ERR_BAD_SHAPE, "%s: q_out overlaps k_out", who);
-    const size_t n_pos = (size_t)((d->n_axes - 1) * d->pos_stride[0] + (d->B - 1) * d->pos_stride[1] + d->S);
-    const Span angles[] = {{positions, n_pos * 4, "positions"}, {inv_freq, (size_t)d->R / 2 * 8, "inv_freq"}, {axes, (size_t)d->R / 2 * 4, "axes"}};
-    for (int i = 0; i < (k ? 2 : 1); ++i)
-        for (const Span& in : angles)
-            if (overlap(out[i].span, in)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in.name);
-    const int rc = check_device();
-    if (rc != TT_OK) return rc;
-    RotaryArgs a = {};
-    a.x[0] = q; a.x[1] = k; a.y[0] = q_out; a.y[1] = k_out;
-    for (int i = 0; i < 3; ++i) {
-        a.xs[0][i] = d->q_stride[i]; a.xs[1][i] = d->k_stride[i];
-        a.ys[0][i] = d->q_out_stride[i]; a.ys[1][i] = d->k_out_stride[i];
-    }
-    a.heads[0] = d->H; a.heads[1] = hk;
-    a.B = d->B; a.S = d->S; a.D = d->D; a.R = d->R; a.n_axes = d->n_axes;
-    a.pos = positions; a.pos_axis = d->pos_stride[0]; a.pos_batch = d->pos_stride[1];
-    a.inv_freq = inv_freq; a.axes = axes; a.scale = d->scale; a.back = backward != 0;
+    const Heads h(d, q, k, q_out, k_out, element(d));
+    if ((rc = h.check(who, d)) != TT_OK || (rc = rotary_spans(who, h, d, positions, inv_freq, axes)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
+    RotaryArgs a = rotary_args(d, q, k, positions, inv_freq, axes, q_out, k_out);
+    a.back = backward != 0;
     const cudaError_t e = rotary(a, d->dtype == TT_BF16, d->interleaved != 0, (cudaStream_t)stream);
     return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_rotary: launch");
+}
+
+int tt_norm_rotary(const tt_rotary_desc* d, const void* q, const void* k, const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                   const int32_t* positions, const double* inv_freq, const int32_t* axes, void* q_out, void* k_out, void* stream) {
+    const char* who = "tt_norm_rotary";
+    int rc = rotary_desc_args(who, d, true, k != nullptr);
+    if (rc != TT_OK || (rc = norm_args(who, d, weight_dtype, eps)) != TT_OK) return rc;
+    if ((k == nullptr) != (k_out == nullptr)) return fail(TT_ERR_NULL, "%s: k and k_out go together", who);
+    if (d->B == 0 || d->S == 0) return TT_OK;
+    if (!q || !q_out || !positions || !inv_freq || !q_weight || (k && !k_weight)) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    const Heads h(d, q, k, q_out, k_out, element(d));
+    if ((rc = h.check(who, d)) != TT_OK || (rc = rotary_spans(who, h, d, positions, inv_freq, axes)) != TT_OK) return rc;
+    if ((rc = weight_spans(who, h, d, q_weight, k_weight, weight_dtype)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
+    NormRotaryArgs a = {};
+    a.r = rotary_args(d, q, k, positions, inv_freq, axes, q_out, k_out);
+    a.w[0] = q_weight; a.w[1] = k_weight; a.w_bf16 = weight_dtype == TT_BF16; a.eps = eps;
+    const cudaError_t e = norm_rotary(a, d->dtype == TT_BF16, d->interleaved != 0, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_norm_rotary: launch");
+}
+
+size_t tt_norm_rotary_bwd_workspace_bytes(const tt_rotary_desc* d) {
+    return d && d->D > 0 && d->D <= 256 && check_device() == TT_OK ? norm_rotary_backward_workspace(d->D) : 0;
+}
+
+int tt_norm_rotary_bwd(const tt_rotary_desc* d, const void* dq, const void* dk, const void* q, const void* k, const int64_t* q_stride, const int64_t* k_stride,
+                       const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps, const int32_t* positions, const double* inv_freq,
+                       const int32_t* axes, void* dq_out, void* dk_out, void* dq_weight, void* dk_weight, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "tt_norm_rotary_bwd";
+    const bool two = dk_weight != nullptr;   // (no rows have no address)
+    int rc = rotary_desc_args(who, d, true, two);
+    if (rc != TT_OK || (rc = norm_args(who, d, weight_dtype, eps)) != TT_OK) return rc;
+    const bool empty = d->B == 0 || d->S == 0;
+    if (!dq_weight || (!empty && (!dq || !dq_out || !q || !positions || !inv_freq || !q_weight || !q_stride))) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    if (!empty && ((dk == nullptr) == two || (dk_out == nullptr) == two || (two && (!k || !k_weight || !k_stride))))
+        return fail(TT_ERR_NULL, "%s: dk, k, k_weight, dk_out and dk_weight go together", who);
+    const size_t size = element(d), w_size = weight_dtype == TT_BF16 ? 2 : 4, w = (size_t)d->D * w_size;
+    if (((uintptr_t)dq_weight | (uintptr_t)dk_weight) % w_size) return fail(TT_ERR_BAD_SHAPE, "%s: weights must be multiples of their element size", who);
+    const Span sums[3] = {{dq_weight, w, "dq_weight"}, {dk_weight, w, "dk_weight"}, {workspace, workspace_bytes, "workspace"}};
+    for (int i = 1; i < 3; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(sums[i], sums[j])) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, sums[i].name, sums[j].name);
+    NormRotaryArgs a = {};
+    if (!empty) {
+        const Heads h(d, dq, dk, dq_out, dk_out, size);
+        if ((rc = h.check(who, d)) != TT_OK || (rc = rotary_spans(who, h, d, positions, inv_freq, axes)) != TT_OK) return rc;
+        if ((rc = weight_spans(who, h, d, q_weight, k_weight, weight_dtype)) != TT_OK) return rc;
+        for (int i = 0; i < 3; ++i)
+            if (q_stride[i] < 0 || (two && k_stride[i] < 0)) return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
+        if (((uintptr_t)q | (two ? (uintptr_t)k : 0)) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
+        const int64_t* st[2] = {q_stride, k_stride};
+        const void* x[2] = {q, k};
+        for (int j = 0; j < h.count; ++j) {
+            const Rows in(x[j], st[j], h.n[j], d->D, size, j ? "k" : "q");
+            for (int i = 0; i < h.count; ++i)
+                if (rows_meet(h.out[i], in, d->D, size)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, h.out[i].span.name, in.span.name);
+            for (const Span& y : sums)
+                if (overlap(y, in.span) || overlap(y, h.in[j].span) || overlap(y, h.out[j].span))
+                    return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps the heads or their gradients", who, y.name);
+            for (int i = 0; i < 3; ++i) a.in_stride[j][i] = st[j][i];
+            a.in[j] = x[j];
+        }
+        const Span also[] = {{q_weight, w, "q_weight"}, {two ? k_weight : nullptr, w, "k_weight"}, {inv_freq, (size_t)d->R / 2 * 8, "inv_freq"},
+                             {axes, (size_t)d->R / 2 * 4, "axes"}, positions_span(d, positions)};
+        for (const Span& x_ : also)
+            for (const Span& y : sums)
+                if (overlap(x_, y)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, y.name, x_.name);
+    }
+    if ((rc = check_device()) != TT_OK) return rc;
+    const size_t need = norm_rotary_backward_workspace(d->D);
+    if (!workspace || workspace_bytes < need) return fail(TT_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, workspace_bytes);
+    if ((uintptr_t)workspace & 255) return fail(TT_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+    a.r = rotary_args(d, dq, dk, positions, inv_freq, axes, dq_out, dk_out);
+    a.r.heads[0] = d->H; a.r.heads[1] = two ? d->Hkv : 0;
+    a.r.back = 1;
+    a.w[0] = q_weight; a.w[1] = k_weight; a.w_bf16 = weight_dtype == TT_BF16; a.eps = eps;
+    a.dw[0] = dq_weight; a.dw[1] = dk_weight;
+    const cudaError_t e = norm_rotary_backward(a, d->dtype == TT_BF16, d->interleaved != 0, workspace, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_norm_rotary_bwd: launch");
+}
+
+int tt_cache_append_rotary(const tt_rotary_desc* d, const void* q, const void* k, const void* v, const int64_t* v_stride, const int32_t* slots, const int32_t* positions,
+                           const double* inv_freq, const int32_t* axes, const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps, void* q_out,
+                           void* k_out, void* k_pool, void* v_pool, int32_t n_pages, int32_t page_size, void* stream) {
+    const char* who = "tt_cache_append_rotary";
+    int rc = rotary_desc_args(who, d, q != nullptr, true);
+    if (rc != TT_OK) return rc;
+    const bool normed = k_weight != nullptr;
+    if (normed && (rc = norm_args(who, d, weight_dtype, eps)) != TT_OK) return rc;
+    if (d->B != 1) return fail(TT_ERR_BAD_SHAPE, "%s: B=%d, packed tokens are one batch entry", who, d->B);
+    if (d->D != 64 && d->D != 128) return fail(TT_ERR_UNSUPPORTED, "%s: head dim 64 or 128 only, got %d", who, d->D);
+    if (page_size < 1 || n_pages < 0) return fail(TT_ERR_BAD_SHAPE, "%s: n_pages=%d page_size=%d", who, n_pages, page_size);
+    if ((int64_t)n_pages * page_size >= (1LL << 31)) return fail(TT_ERR_BAD_SHAPE, "%s: pages of %d x %d tokens, at most 2^31 - 1", who, n_pages, page_size);
+    if ((q == nullptr) != (q_out == nullptr)) return fail(TT_ERR_NULL, "%s: q and q_out go together", who);
+    if (q && normed != (q_weight != nullptr)) return fail(TT_ERR_NULL, "%s: q_weight and k_weight go together", who);
+    if (!q) q_weight = nullptr;
+    if (normed && ((uintptr_t)q_weight | (uintptr_t)k_weight) % (weight_dtype == TT_BF16 ? 2 : 4))
+        return fail(TT_ERR_BAD_SHAPE, "%s: weights must be multiples of their element size", who);
+    if (!v_stride) return fail(TT_ERR_NULL, "%s: null strides", who);
+    if (d->S == 0) return TT_OK;
+    if (!k || !v || !slots || !positions || !inv_freq || (n_pages && (!k_pool || !v_pool))) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    const size_t size = element(d);
+    const int64_t vs[3] = {0, v_stride[1], v_stride[0]};
+    const int nk[3] = {1, d->Hkv, d->S}, nq[3] = {1, d->H, d->S};
+    for (int i = 0; i < 3; ++i)
+        if ((q && (d->q_stride[i] < 0 || d->q_out_stride[i] < 0)) || d->k_stride[i] < 0 || (k_out && d->k_out_stride[i] < 0) || vs[i] < 0 || (i < 2 && d->pos_stride[i] < 0))
+            return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % size || ((uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)k_pool | (uintptr_t)v_pool) % 2)
+        return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
+    if ((q && !rows_apart(d->q_out_stride, nq, d->D)) || (k_out && !rows_apart(d->k_out_stride, nk, d->D)))
+        return fail(TT_ERR_BAD_SHAPE, "%s: rows of an output overlap", who);
+    const Rows in[3] = {{q, d->q_stride, nq, d->D, size, "q"}, {k, d->k_stride, nk, d->D, size, "k"}, {v, vs, nk, d->D, size, "v"}};
+    const Rows out[2] = {{q_out, d->q_out_stride, nq, d->D, 2, "q_out"}, {k_out, d->k_out_stride, nk, d->D, 2, "k_out"}};
+    const size_t pool = (size_t)n_pages * d->Hkv * page_size * d->D * 2, w = (size_t)d->D * (weight_dtype == TT_BF16 ? 2 : 4);
+    const Span pools[2] = {{k_pool, pool, "k_pool"}, {v_pool, pool, "v_pool"}};
+    const Span also[] = {positions_span(d, positions), {inv_freq, (size_t)d->R / 2 * 8, "inv_freq"}, {axes, (size_t)d->R / 2 * 4, "axes"},
+                         {slots, (size_t)d->S * 4, "slots"}, {q_weight, w, "q_weight"}, {k_weight, w, "k_weight"}};
+    // Queries and keys may be turned in place, where the types are the same; else outputs lie apart from everything.
+    for (int i = 0; i < 2; ++i) {
+        if (!out[i].span.p) continue;
+        for (int j = 0; j < 3; ++j) {
+            if (!in[j].span.p || (i == j && size == 2 && in_place(out[i], in[j]))) continue;
+            if (size == 2 ? rows_meet(out[i], in[j], d->D, size) : overlap(out[i].span, in[j].span))
+                return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, in[j].span.name);
+        }
+        for (const Span& x : also)
+            if (overlap(out[i].span, x)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, x.name);
+        for (const Span& x : pools)
+            if (overlap(out[i].span, x)) return fail(TT_ERR_BAD_SHAPE, "%s: %s overlaps %s", who, out[i].span.name, x.name);
+    }
+    if (q && k_out && rows_meet(out[0], out[1], d->D, 2)) return fail(TT_ERR_BAD_SHAPE, "%s: q_out overlaps k_out", who);
+    const Span ins[] = {in[0].span, in[1].span, in[2].span};
+    if ((rc = check_overlap(who, pools, 2, ins, 3)) != TT_OK || (rc = check_overlap(who, pools, 2, also, 6)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
+    NormRotaryArgs a = {};
+    a.r = rotary_args(d, q, k, positions, inv_freq, axes, q_out, k_out);
+    a.w[0] = q_weight; a.w[1] = k_weight; a.w_bf16 = weight_dtype == TT_BF16; a.eps = eps;
+    a.v = v; a.v_stride[0] = v_stride[0]; a.v_stride[1] = v_stride[1];
+    a.slots = slots;
+    a.pool[0] = k_pool; a.pool[1] = v_pool; a.n_slots = n_pages * page_size; a.page = page_size;
+    const cudaError_t e = cache_append_rotary(a, d->dtype == TT_BF16, d->interleaved != 0, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_append_rotary: launch");
 }
 
 }  // extern "C"

@@ -402,6 +402,84 @@ def rotary_backward(dq, dk, positions, inv_freq, axes=None, interleaved=False, s
     return r if r.__class__ is tuple else _done(r, _explain_rotary, dq, dk, positions, inv_freq, axes, out_q, out_k)
 
 
+def _explain_weights(x, pairs):
+    seen = None
+    for name, w, wanted in pairs:
+        if not wanted and w is not None:
+            raise ValueError(f"{name} goes with the heads it weights")
+        if wanted and (not isinstance(w, torch.Tensor) or w.dtype not in (x.dtype, torch.float32) or w.device != x.device or tuple(w.shape) != (x.shape[-1],)
+                       or not w.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous vector of {x.shape[-1]}, float32 or of the heads' type, on the heads' device")
+        if wanted and seen is not None and w.dtype != seen:
+            raise ValueError("q_weight and k_weight must have one type")
+        seen = w.dtype if wanted else seen
+
+
+def _explain_norm_rotary(q, k, q_weight, k_weight, positions, inv_freq, axes, out_q, out_k, x=()):
+    if not isinstance(q, torch.Tensor):
+        raise ValueError("q must be a CUDA float32/bfloat16 tensor [T,H,D] or [B,H,S,D]")
+    for name, t, g in x:
+        if (t is None) != (g is None) or (t is not None and (not isinstance(t, torch.Tensor) or not isinstance(g, torch.Tensor) or t.shape != g.shape
+                                                            or t.dtype != g.dtype or t.device != g.device or (t.shape[-1] > 1 and t.stride(-1) != 1))):
+            raise ValueError(f"{name} must have its gradient's shape, type and device, channels next to each other")
+    _explain_weights(q, (("q_weight", q_weight, True), ("k_weight", k_weight, k is not None)))
+    _explain_rotary(q, k, positions, inv_freq, axes, out_q, out_k)
+
+
+def norm_rotary_forward(q, k, q_weight, k_weight, positions, inv_freq, axes=None, interleaved=False, eps=1e-6, scale=None, out_q=None, out_k=None):
+    """Query and key heads normed and turned by their positions in one pass -> (q, k); k (with its weight) may be None.
+
+    Each head is divided by the root of its channels' mean square and `eps`, multiplied by a weight per channel (`[D]`, float32 or of
+    the heads' type) and turned as by `rotary_forward`, whose arguments the others are."""
+    r = _native.norm_rotary_forward(q, k, q_weight, k_weight, positions, inv_freq, axes, interleaved, eps, scale, out_q, out_k)
+    return r if r.__class__ is tuple else _done(r, _explain_norm_rotary, q, k, q_weight, k_weight, positions, inv_freq, axes, out_q, out_k)
+
+
+def norm_rotary_backward(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, axes=None, interleaved=False, eps=1e-6, scale=None, out_q=None,
+                         out_k=None, workspace=None):
+    """(dq, dk, dq_weight, dk_weight) of `norm_rotary_forward` on q, k for upstream gradients `dq`, `dk` of its results.  `out_q`, `out_k` may be
+    `dq`, `dk` themselves."""
+    r = _native.norm_rotary_backward(dq, dk, q, k, q_weight, k_weight, positions, inv_freq, axes, interleaved, eps, scale, out_q, out_k, workspace)
+    return r if r.__class__ is tuple else _done(r, _explain_norm_rotary, dq, dk, q_weight, k_weight, positions, inv_freq, axes, out_q, out_k,
+                                                (("q", q, dq), ("k", k, dk)))
+
+
+def _explain_append_rotary(q, k, v, slots, positions, inv_freq, k_pool, v_pool, axes, q_weight, k_weight, out_q, out_k):
+    for name, t in (("k", k), ("q", q), ("v", v)):
+        if t is None and name == "q":
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DT or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{name} must be a CUDA float32/bfloat16 tensor [T, heads, D] whose channels lie next to each other")
+        if t.dtype != k.dtype or t.device != k.device or t.shape[0] != k.shape[0] or t.shape[2] != k.shape[2]:
+            raise ValueError(f"{name} must have k's type, device, tokens and head dim")
+    if v.shape != k.shape:
+        raise ValueError(f"shape mismatch: k {tuple(k.shape)} v {tuple(v.shape)}")
+    if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int32 or slots.device != k.device or tuple(slots.shape) != (k.shape[0],) or not slots.is_contiguous():
+        raise ValueError(f"slots must be a contiguous int32 vector of {k.shape[0]} on k's device")
+    for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.device != k.device or t.dim() != 4 or not t.is_contiguous() \
+                or t.shape[1] != k.shape[1] or t.shape[3] != k.shape[2] or t.shape != k_pool.shape:
+            raise ValueError(f"{name} must be a contiguous bfloat16 tensor [pages, {k.shape[1]}, page_size, {k.shape[2]}] on k's device")
+    for name, t, x in (("out_q", out_q, q), ("out_k", out_k, k)):
+        if t is not None and (x is None or not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.shape != x.shape or t.device != k.device
+                              or (t.shape[2] > 1 and t.stride(2) != 1)):
+            raise ValueError(f"{name} must be a bfloat16 tensor of its input's shape and device")
+    _explain_weights(k, (("q_weight", q_weight, q is not None and k_weight is not None), ("k_weight", k_weight, k_weight is not None)))
+    _explain_rotary(k, None, positions, inv_freq, axes, None, None)
+
+
+def cache_append_rotary(q, k, v, slots, positions, inv_freq, k_pool, v_pool, axes=None, interleaved=False, q_weight=None, k_weight=None, eps=1e-6,
+                        scale=None, out_q=None, out_k=None):
+    """A step's tokens on their way to `attention_decode_paged`: q turned by its positions -> bfloat16 `[T, H, D]`, and keys (turned) and values
+    written into their slots of the bfloat16 pools `[pages, kv_heads, page_size, D]`, D 64 or 128.
+
+    q `[T, H, D]` (or None), k, v `[T, kv_heads, D]`, float32 or bfloat16, strided; `slots`, `positions` as from `cache_extend`; a slot of -1 is passed
+    over, and none may come twice.  With `q_weight` and `k_weight` heads are normed first, as by `norm_rotary_forward`.  `out_k`: a bfloat16 tensor of k's
+    shape that gets the turned keys too, for attention over the new tokens themselves.  `scale` multiplies queries and keys."""
+    r = _native.cache_append_rotary(q, k, v, slots, positions, inv_freq, k_pool, v_pool, axes, interleaved, q_weight, k_weight, eps, scale, out_q, out_k)
+    return r[0] if r.__class__ is tuple else _done(r, _explain_append_rotary, q, k, v, slots, positions, inv_freq, k_pool, v_pool, axes, q_weight, k_weight, out_q, out_k)
+
+
 def _explain_softmax_forward(x):
     raise ValueError("softmax_forward takes a contiguous float32/bfloat16 CUDA tensor")
 
