@@ -271,6 +271,30 @@ int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cac
                       const int32_t* seq_lens, int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- key/value cache in 8 bits --------------------------------------------------------------
+ * k_cache, v_cache: [n_pages, Hkv, tt_cache_q8_page_bytes(page_size, D)] bytes each, 16-byte aligned; D 64 or 128, page_size a multiple of 16.  A page holds,
+ * for one key/value head, [page_size][D] codes and then [page_size / 16] bytes, up to a multiple of 32.  A code is an 8-bit float (e4m3: largest 448, no
+ * infinities, 0x7f and 0xff NaN); rows 16 j .. 16 j + 15 of a page are a block, and the j-th byte behind the codes stands for its scale 2^(byte - 64), the
+ * exponent held to -40 .. 40.  A value is its code times its block's scale, which bf16 holds exactly.  A cache is below 2^37 bytes, and has less than
+ * 2^31 tokens.
+ *
+ * tt_cache_append_q8: as tt_cache_append_q4, tokens [T, Hkv, D] into their slots.  The tokens of a call that go to one block have to lie next to each
+ * other in it, as those of a sequence do (else what the block then holds is of any of them).  The scale of a block is the smallest with 448 scale >= every
+ * finite |x| that has come to it since its row 0 was last written: a call that brings row 0 begins the block anew, another may raise the scale, and then the
+ * block's other rows are rounded to the new one.  Codes are rounded to the nearest, ties to even, so a value is off by at most 2^-4 of itself, or 2^-10 of the scale
+ * (2^-9, where that was raised) if that is more.  Infinities, and values beyond 448 2^40, become the block's largest value of their sign; NaN stays NaN.
+ *
+ * tt_cache_read_q8: as tt_cache_read_q4.  tt_attn_decode_q8: as tt_attn_decode_q4, D, lengths, tables, groups, outputs and workspace alike (size by
+ * tt_attn_decode_q8_workspace_bytes); NaN among a sequence's keys or values reaches its results. */
+size_t tt_cache_q8_page_bytes(int32_t page_size, int32_t D);   /* 0: not supported */
+int tt_cache_append_q8(const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype, const int64_t* k_stride,
+                       const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages, int32_t page_size, void* stream);
+int tt_cache_read_q8(const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* cu_lens, int32_t B, int32_t Hkv, int32_t D,
+                     int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t total, void* k, void* v, void* stream);
+size_t tt_attn_decode_q8_workspace_bytes(const tt_attn_desc* desc);
+int tt_attn_decode_q8(const tt_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* seq_lens,
+                      int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- rotary positions ------------------------------------------------------------------------
  * Query and key heads turned by their tokens' positions (no counterpart in the reference).  Of a head's D channels the first
  * R form R / 2 pairs; pair i of a token at position p on axis a = axes[i] turns by p * inv_freq[i]:

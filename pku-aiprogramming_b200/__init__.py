@@ -16,4 +16,5 @@ from .functional import (  # noqa: F401
     CacheStep, cache_extend, cache_release, rotary_frequencies, rotary_forward, rotary_backward,
     norm_rotary_forward, norm_rotary_backward, cache_append_rotary,
     cache_alloc_q4, cache_append_q4, cache_read_q4, attention_decode_q4,
+    cache_alloc_q8, cache_append_q8, cache_read_q8, attention_decode_q8,
 )

@@ -66,6 +66,11 @@ SIGNATURES = {
     "tt_cache_read_q4": (c_int, [_P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P, _P]),
     "tt_attn_decode_q4_workspace_bytes": (c_size_t, [_DP]),
     "tt_attn_decode_q4": (c_int, [_DP, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, _P, _P, _P, c_size_t, _P]),
+    "tt_cache_q8_page_bytes": (c_size_t, [c_int32, c_int32]),
+    "tt_cache_append_q8": (c_int, [_P, _P, _P, c_int32, c_int32, c_int32, c_int32, POINTER(c_int64), POINTER(c_int64), _P, _P, c_int32, c_int32, _P]),
+    "tt_cache_read_q8": (c_int, [_P, _P, _P, _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, _P, _P, _P]),
+    "tt_attn_decode_q8_workspace_bytes": (c_size_t, [_DP]),
+    "tt_attn_decode_q8": (c_int, [_DP, _P, _P, _P, _P, _P, c_int32, c_int32, c_int32, _P, _P, _P, c_size_t, _P]),
     "tt_rotary": (c_int, [POINTER(RotaryDesc), _P, _P, _P, _P, _P, c_int32, _P, _P, _P]),
     "tt_norm_rotary": (c_int, [POINTER(RotaryDesc), _P, _P, _P, _P, c_int32, c_float, _P, _P, _P, _P, _P, _P]),
     "tt_norm_rotary_bwd_workspace_bytes": (c_size_t, [POINTER(RotaryDesc)]),

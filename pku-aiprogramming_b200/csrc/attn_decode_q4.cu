@@ -35,6 +35,7 @@
 // issue slots 56 % busy, ALU 47 %, half-precision multiply-adds 29 %, tensor pipe 26 %, at 1.75 GHz (power).  So no pipe bounds it but the order within a warp: it waits
 // on its own arithmetic, and the loads do not run under all of it (without them 80.6 us, the loads alone 67, of 94).
 #include "cache_q4.cuh"
+#include "decode_parts.cuh"
 #include "sm100_ptx.cuh"
 
 namespace ttk {
@@ -49,22 +50,6 @@ constexpr float kSlack = 5.f, kLift = 10.f, kNone = -3e38f;   // (kNone: no scor
 // step goes the way of those that raise the reference, where that is done, with 0 and 1 in its and the factor's place for the code behind.
 constexpr float kFar = 1048576.f;
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void copy16(uint32_t saddr, const void* p) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(saddr), "l"(p) : "memory"); }
 template <int N>
 __device__ __forceinline__ void lds(uint32_t (&w)[N], const unsigned char* p) {
     if (N == 4) {
@@ -113,61 +98,8 @@ struct Slot {
 
 }  // namespace
 
-struct DecodeQ4Args {
-    const __nv_bfloat16* q;
-    const unsigned char *kc, *vc;
-    const int *table, *lens;
-    int B, L, hkv, group, head_tiles, n_pages, page, max_pages;
-    float scale_log2;
+struct DecodeQ4Args : PartsArgs {
     uint32_t k8;    // 0x48004800, see Scale2
-    __nv_bfloat16* out;
-    float* lse;        // may be null
-    // Workspace, unless every slice is one warp's (null then): steps before each batch entry [B + 1] (of one slice), and for every part of a slice that a warp does not have to itself the
-    // normalised rows [part][part_rows][D] and log-sum-exps.  Parts are numbered warp + slice: one of the two grows from each to the next.
-    unsigned* before;
-    float *po, *plse;
-    int part_rows;
-};
-
-// Of `total` steps warp w of `parts` has `per`, one more if it is among the first `rest`.  The host has batch x heads x L / 32 below 2^31, so counts
-// fit 32 bits.
-// At least two to a part where slices have 64 or more on average: the merge then takes longer than the second step; one sequence of 3000
-// and eight heads 8.6 us for 9.1, of 16000 and one head 10.5 for 12.0; but 16 of 100 to 300 10.3 for 9.4, 64 of 10 to 100 11.4 for 10.2.
-struct Q4Shares {
-    unsigned parts, per, rest;
-    __host__ __device__ __forceinline__ Q4Shares(unsigned total, unsigned warps, unsigned slices) {
-        parts = total / 64 < slices ? total : (total + 1) / 2;
-        parts = parts < 1 ? 1 : parts < warps ? parts : warps;
-        per = total / parts;
-        rest = total - per * parts;
-    }
-    __device__ __forceinline__ unsigned begin(unsigned w) const { return w * per + (w < rest ? w : rest); }
-    __device__ __forceinline__ unsigned warp_of(unsigned x) const {
-        const unsigned longer = rest * (per + 1);
-        return x < longer ? x / (per + 1) : rest + (x - longer) / per;
-    }
-};
-
-__device__ __forceinline__ int q4_len(const DecodeQ4Args& a, int b) { return a.lens ? min(max(__ldg(a.lens + b), 0), a.L) : a.L; }
-__device__ __forceinline__ unsigned q4_steps(int len) { return (unsigned)(len + kTile - 1) / kTile; }
-
-// A place in the sequence of steps: the batch entry it is in and where that one's steps begin.
-struct Q4Cursor {
-    int b, len;
-    unsigned begin;
-    __device__ __forceinline__ void to(const DecodeQ4Args& a, unsigned per_b, unsigned x) {   // x >= begin, below the end
-        unsigned n;
-        while (x - begin >= (n = q4_steps(len) * per_b)) {
-            begin += n;
-            len = q4_len(a, ++b);
-        }
-    }
-    // the slice within the batch entry, and the step within the slice
-    __device__ __forceinline__ int slice(unsigned x, int* step) const {
-        const unsigned steps = q4_steps(len), s = (x - begin) / steps;
-        *step = (int)(x - begin - s * steps);
-        return (int)s;
-    }
 };
 
 // What the registers hold.  D = 64, up to eight heads: 140.8 / 112.2 / 113.9 us for 64 sequences of 4096 to 8192 with three / four / five.  D = 128: four
@@ -189,64 +121,15 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
     grid_let_next_start();
     grid_wait_for_previous();
 
-    Q4Cursor now{0, 0, 0};   // of the step at hand
-    unsigned x0;             // the part's first step, and how many it has
+    PartsCursor<kTile> now{0, 0, 0};   // of the step at hand
+    unsigned x0;                       // the part's first step, and how many it has
     int n;
-    if (!a.before) {   // a slice to a warp
-        if (w >= a.B * per_b) return;
-        now.b = w / per_b;
-        now.len = q4_len(a, now.b);
-        n = (int)q4_steps(now.len);
-        x0 = (w - now.b * per_b) * n;   // (with the batch entry's own first step as 0)
-        if (n == 0) {
-            const int slice_b = w - now.b * per_b, h0 = slice_b % a.head_tiles * kHeads, n_heads = min(kHeads, a.group - h0);
-            const long long row0 = ((long long)now.b * a.hkv + slice_b / a.head_tiles) * a.group + h0;
-            for (int i = lane; i < n_heads * (D / 8); i += 32) reinterpret_cast<uint4*>(a.out + row0 * D)[i] = make_uint4(0, 0, 0, 0);
-            if (lane < n_heads && a.lse) a.lse[row0 + lane] = -INFINITY;
-            return;
-        }
-    } else {
-        // the batch's steps, and where this warp's part begins
-        unsigned sum = 0;
-        for (int i = lane; i < a.B; i += 32) sum += q4_steps(q4_len(a, i));
-        const unsigned total = __reduce_add_sync(0xffffffffu, sum) * per_b;
-        const Q4Shares shares(total, w_all, a.B * per_b);
-        if (w >= shares.parts) return;
-        x0 = shares.begin(w);
-        n = (int)(shares.begin(w + 1) - x0);
-        const unsigned y = x0 / per_b;
-        unsigned done = 0;
-        int found = -1;
-        for (int i = 0; i < a.B && (found < 0 || w == 0); i += 32) {
-            const int len = i + lane < a.B ? q4_len(a, i + lane) : 0;
-            unsigned to = q4_steps(len);
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const unsigned x = __shfl_up_sync(0xffffffffu, to, d);
-                if (lane >= d) to += x;
-            }
-            to += done;
-            if (w == 0 && i + lane < a.B) {   // for the merge
-                a.before[i + lane + 1] = to;
-                if (i + lane == 0) a.before[0] = 0;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, to > y);
-            if (found < 0 && past) {
-                const int at = __ffs(past) - 1;
-                found = i + at;
-                now.b = found;
-                now.len = __shfl_sync(0xffffffffu, len, at);
-                now.begin = (__shfl_sync(0xffffffffu, to, at) - q4_steps(now.len)) * per_b;
-            }
-            done = __shfl_sync(0xffffffffu, to, 31);
-        }
-        if (found < 0) return;   // no keys at all
-    }
+    if (!parts_find<kTile, D, kHeads>(a, w, w_all, lane, &now, &x0, &n)) return;
 
     // 16 keys lie in one page.  Lane i looks up where the i-th 16 keys of a batch of 32 are: the first row and its codes, in units of 32 bytes
     // (of which all of these are multiples), or kNowhere.
     constexpr unsigned kNowhere = 0xffffffffu;
-    Q4Cursor ahead = now;
+    PartsCursor<kTile> ahead = now;
     unsigned rows_at, codes_at;
     auto look_up = [&](int sub) {   // sub: the lane's, a multiple of 32 for lane 0
         rows_at = codes_at = kNowhere;
@@ -308,7 +191,7 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
         now.to(a, per_b, x0 + i);
         const int slice_b = now.slice(x0 + i, &step), tile = slice_b % a.head_tiles;
         const long long slice = (long long)now.b * per_b + slice_b;
-        const int h0 = tile * kHeads, n_heads = min(kHeads, a.group - h0), in_slice = (int)q4_steps(now.len), end = min(n, i + in_slice - step);
+        const int h0 = tile * kHeads, n_heads = min(kHeads, a.group - h0), in_slice = (int)parts_steps<kTile>(now.len), end = min(n, i + in_slice - step);
         const bool whole = step == 0 && end - i == in_slice;
         const long long row0 = ((long long)now.b * a.hkv + slice_b / a.head_tiles) * a.group + h0;   // the tile's first query head
 
@@ -583,7 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, q4_ctas_per_sm(D, NT)) attn_decod
 // 30.5 / 37.5, 28 of 512 rows 19.0 / 19.4 / 16.2 / 19.1, 222 of 32 rows 16.9 / 10.7 / 10.1 / 9.9, 1776 of 8 rows 116 / 36 / 24 / 17.5.
 constexpr int kMergeParts = 1024;   // weights held at a time
 template <int D, int kT>
-__global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kernel(const DecodeQ4Args a, int heads, int rows_all, int w_all) {
+__global__ void __launch_bounds__(kT == 32 ? 128 : kT) decode_parts_merge_kernel(const PartsArgs a, int heads, int rows_all, int w_all) {
     constexpr int kLanes = D / 4, kRows = kT / kLanes > 0 ? kT / kLanes : 1, kAhead = 4, kWeights = kT == 32 ? 32 : kMergeParts;
     static_assert(kT % kLanes == 0, "whole rows");
     __shared__ float sm_w[kT == 32 ? 4 : 1][kWeights], sm_o[kT == 32 ? 1 : kRows][D], sm_r[2][kT / 32];
@@ -604,7 +487,7 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kern
         if (tid == 0 && a.lse) a.lse[row] = -INFINITY;
         return;
     }
-    const Q4Shares shares(total, w_all, a.B * per_b);
+    const PartsShares shares(total, w_all, a.B * per_b);
     const unsigned x = first * per_b + slice_b * steps;
     const int w0 = (int)shares.warp_of(x), n = (int)shares.warp_of(x + steps - 1) - w0 + 1;
     if (n == 1) return;
@@ -682,6 +565,23 @@ __global__ void __launch_bounds__(kT == 32 ? 128 : kT) attn_decode_q4_merge_kern
     if (tid == 0 && a.lse) a.lse[row] = den == 0.f ? -INFINITY : top + logf(den);
 }
 
+template <int D, int kT>
+static cudaError_t launch_parts_merge(const PartsArgs& g, const AttnArgs& a, int n_warps, cudaStream_t st) {
+    constexpr int kRows = kT == 32 ? 4 : 1;
+    LaunchScope ls(K_DECODE_MERGE, st);
+    return launch_overlapped(decode_parts_merge_kernel<D, kT>, (unsigned)((a.BH + kRows - 1) / kRows), kT * kRows, 0, st, g, a.H, (int)a.BH, n_warps);
+}
+template <int D>
+cudaError_t decode_parts_merge(const PartsArgs& g, const AttnArgs& a, int n_warps, cudaStream_t st) {
+    // A warp for a row of up to a dozen parts, if all slices were of the greatest length; else as many threads as leave all rows in one wave.
+    if (n_warps <= 12 * (a.BH / a.group) * g.head_tiles) return launch_parts_merge<D, 32>(g, a, n_warps, st);
+    const long long room = sm_count() * 1024LL;
+    if (a.BH * 512 <= room) return launch_parts_merge<D, 512>(g, a, n_warps, st);
+    return a.BH * 256 <= room ? launch_parts_merge<D, 256>(g, a, n_warps, st) : launch_parts_merge<D, 128>(g, a, n_warps, st);
+}
+template cudaError_t decode_parts_merge<64>(const PartsArgs&, const AttnArgs&, int, cudaStream_t);
+template cudaError_t decode_parts_merge<128>(const PartsArgs&, const AttnArgs&, int, cudaStream_t);
+
 // Whether every slice is one warp's, without a workspace and a second kernel: where the steps that a warp then has in a row take less time than the merge. From
 // a graph / as calls, us, for the two kernels: 64 sequences of up to 20 keys, 32 on 8 heads, 4.9 / 5.7 for 7.0 / 8.3, of up to 60 6.1 / 5.6 for 9.4 / 10.0, of up to 100 7.6 / 8.4
 // for 10.2 / 10.4, of up to 250 12.9 / 14.3 for 13.2 / 13.8, of up to 500 22.2 / 24.0 for 15.5 / 16.0; two of 200 8.2 / 8.7 for 7.4 / 8.2.
@@ -690,7 +590,7 @@ static bool q4_whole(const AttnArgs& a) { return a.L <= 4 * kTile; }
 template <int NT>
 static int q4_ctas(const AttnArgs& a, int head_tiles) {
     const long long slices = a.BH / a.group * head_tiles, steps = slices * ((a.L + kTile - 1) / kTile);
-    const Q4Shares shares((unsigned)steps, sm_count() * q4_ctas_per_sm(a.D, NT) * kWarps, (unsigned)slices);
+    const PartsShares shares((unsigned)steps, sm_count() * q4_ctas_per_sm(a.D, NT) * kWarps, (unsigned)slices);
     return (int)((shares.parts + kWarps - 1) / kWarps);
 }
 template <int NT>
@@ -710,12 +610,6 @@ static size_t q4_layout(const AttnArgs& a, DecodeQ4Args* g, void* ws) {
 }
 size_t attn_decode_q4_workspace(const AttnArgs& a) { return a.group <= 8 ? q4_layout<1>(a, nullptr, nullptr) : q4_layout<2>(a, nullptr, nullptr); }
 
-template <int D, int kT>
-static cudaError_t launch_q4_merge(const DecodeQ4Args& g, const AttnArgs& a, int n_warps, cudaStream_t st) {
-    constexpr int kRows = kT == 32 ? 4 : 1;
-    LaunchScope ls(K_DECODE_MERGE, st);
-    return launch_overlapped(attn_decode_q4_merge_kernel<D, kT>, (unsigned)((a.BH + kRows - 1) / kRows), kT * kRows, 0, st, g, a.H, (int)a.BH, n_warps);
-}
 template <int D, int NT>
 static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* table, const int* lens, int max_pages, void* ws, cudaStream_t st) {
     DecodeQ4Args g = {};
@@ -737,12 +631,7 @@ static cudaError_t launch_q4(const AttnArgs& a, const CacheQ4& c, const int* tab
         e = launch_overlapped(attn_decode_q4_kernel<D, NT>, (unsigned)ctas, kWarps * 32, q4_smem<D, NT>(), st, g);
         if (e != cudaSuccess || whole) return e;
     }
-    // A warp for a row of up to a dozen parts, if all slices were of the greatest length; else as many threads as leave all rows in one wave.
-    const int n_warps = ctas * kWarps;
-    if (n_warps <= 12 * (a.BH / a.group) * g.head_tiles) return launch_q4_merge<D, 32>(g, a, n_warps, st);
-    const long long room = sm_count() * 1024LL;
-    if (a.BH * 512 <= room) return launch_q4_merge<D, 512>(g, a, n_warps, st);
-    return a.BH * 256 <= room ? launch_q4_merge<D, 256>(g, a, n_warps, st) : launch_q4_merge<D, 128>(g, a, n_warps, st);
+    return decode_parts_merge<D>(g, a, ctas * kWarps, st);
 }
 cudaError_t attn_decode_q4(const AttnArgs& a, const CacheQ4& c, const int* table, const int* lens, int max_pages, void* ws, cudaStream_t st) {
     if (a.D == 128) return a.group <= 8 ? launch_q4<128, 1>(a, c, table, lens, max_pages, ws, st) : launch_q4<128, 2>(a, c, table, lens, max_pages, ws, st);

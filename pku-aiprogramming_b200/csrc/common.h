@@ -146,7 +146,7 @@ enum KernelId {
     K_DECODE, K_DECODE_MERGE, K_PROBE, K_SOFTMAX_FWD, K_SOFTMAX_BWD, K_FC_GEMM, K_FC_SIMT, K_FC_COLSUM, K_BWD_FUSED,
     K_BWD_DQ_CONVERT, K_DECODE_GQ, K_FWD_F32, K_BWD_F32, K_BWD_BOTH, K_CACHE_TABLES,
     K_ROTARY, K_CACHE_APPEND, K_CACHE_READ, K_DECODE_Q4, K_NORM_ROTARY, K_NORM_ROTARY_BWD, K_NORM_ROTARY_DW, K_CACHE_APPEND_ROTARY,
-    K_COUNT
+    K_CACHE_APPEND_Q8, K_CACHE_READ_Q8, K_DECODE_Q8, K_COUNT
 };
 // Scoped around ONE kernel launch: counts it and, when timing is enabled, brackets it with
 // CUDA events on the launching stream.
@@ -274,10 +274,11 @@ cudaError_t cache_release(const int* table, const int* lens, const unsigned char
                           int free_capacity, int* lens_out, int* n_free_out, cudaStream_t st);
 
 // --- 4-bit key/value cache (cache_q4.cu); D 64 or 128, page_size a multiple of 16; strides in elements {token, head}
-struct CacheQ4 {
+struct CacheView {
     void *k, *v;
     int n_pages, page_size, hkv, D;
 };
+using CacheQ4 = CacheView;
 cudaError_t cache_append_q4(const CacheQ4& c, const void* k, const void* v, const long long (&ks)[2], const long long (&vs)[2], int bf16, const int* slots,
                             int T, cudaStream_t st);
 cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st);
@@ -285,6 +286,14 @@ cudaError_t cache_read_q4(const CacheQ4& c, const int* block_table, const int* c
 // Decode over it (attn_decode_q4.cu): block_table null: one page per batch entry.
 size_t attn_decode_q4_workspace(const AttnArgs& a);
 cudaError_t attn_decode_q4(const AttnArgs& a, const CacheQ4& c, const int* block_table, const int* seq_lens, int max_pages, void* workspace, cudaStream_t st);
+
+// --- 8-bit key/value cache (cache_q8.cu, attn_decode_q8.cu); the same
+using CacheQ8 = CacheView;
+cudaError_t cache_append_q8(const CacheQ8& c, const void* k, const void* v, const long long (&ks)[2], const long long (&vs)[2], int bf16, const int* slots,
+                            int T, cudaStream_t st);
+cudaError_t cache_read_q8(const CacheQ8& c, const int* block_table, const int* cu, int B, int max_pages, int total, void* k, void* v, cudaStream_t st);
+size_t attn_decode_q8_workspace(const AttnArgs& a);
+cudaError_t attn_decode_q8(const AttnArgs& a, const CacheQ8& c, const int* block_table, const int* seq_lens, int max_pages, void* workspace, cudaStream_t st);
 
 // --- rotary positions (rotary.cu)
 struct RotaryArgs {

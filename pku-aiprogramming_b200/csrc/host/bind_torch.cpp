@@ -810,35 +810,51 @@ PyObject* cache_append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// The two pools of a 4-bit cache: contiguous bytes [pages, Hkv, page bytes] of one shape and device.
-bool q4_cache(PyObject* ok, PyObject* ov, const Tensor** k, const Tensor** v) {
+// The two pools of a cache of 4 or 8 bits: contiguous bytes [pages, Hkv, page bytes] of one shape and device.
+bool byte_cache(PyObject* ok, PyObject* ov, const Tensor** k, const Tensor** v) {
     *k = on_device(ok, at::kByte);
     *v = *k ? on_device(ov, at::kByte, *k) : nullptr;
     return *v && (*k)->dim() == 3 && (*k)->is_contiguous() && (*v)->is_contiguous() && same_shape(**k, **v) && fits32((*k)->size(0)) && fits32((*k)->size(1));
 }
+// What differs between the two
+struct CacheCalls {
+    decltype(&tt_cache_q4_page_bytes) page_bytes;
+    decltype(&tt_cache_append_q4) append;
+    decltype(&tt_cache_read_q4) read;
+    decltype(&tt_attn_decode_q4_workspace_bytes) workspace;
+    decltype(&tt_attn_decode_q4) decode;
+};
+constexpr CacheCalls kQ4 = {tt_cache_q4_page_bytes, tt_cache_append_q4, tt_cache_read_q4, tt_attn_decode_q4_workspace_bytes, tt_attn_decode_q4};
+constexpr CacheCalls kQ8 = {tt_cache_q8_page_bytes, tt_cache_append_q8, tt_cache_read_q8, tt_attn_decode_q8_workspace_bytes, tt_attn_decode_q8};
 // tokens of a page of `bytes` at head dim D; 0: no page has that size
-int64_t q4_page_size(int64_t bytes, int64_t D) {
-    if (D != 64 && D != 128) return 0;
-    const int64_t row = D / 2 + D / 32;
-    return bytes > 0 && bytes % (16 * row) == 0 && fits32(bytes) ? bytes / row : 0;
+int64_t page_size_of(const CacheCalls& c, int64_t bytes, int64_t D) {
+    if ((D != 64 && D != 128) || bytes < 1 || !fits32(bytes)) return 0;
+    // 16 tokens more are more bytes, so sizes are found by halving
+    int64_t lo = 0, hi = bytes / (8 * D) + 1;   // in units of 16: a token is D / 2 bytes or more
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        if ((int64_t)c.page_bytes((int32_t)(16 * mid), (int32_t)D) <= bytes) lo = mid;
+        else hi = mid;
+    }
+    return lo && (int64_t)c.page_bytes((int32_t)(16 * lo), (int32_t)D) == bytes ? 16 * lo : 0;
 }
 
 // (k, v, slots, k_cache, v_cache) -> (k_cache, v_cache)
-PyObject* cache_append_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* append_to_cache(const CacheCalls& calls, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const Tensor *kc, *vc;
-        if (n != 5 || !q4_cache(a[3], a[4], &kc, &vc) || !THPVariable_Check(a[0])) Py_RETURN_NONE;
+        if (n != 5 || !byte_cache(a[3], a[4], &kc, &vc) || !THPVariable_Check(a[0])) Py_RETURN_NONE;
         const Tensor& k = THPVariable_Unpack(a[0]);
         const Tensor* v = float_type(k) ? on_device(a[1], k.scalar_type(), kc) : nullptr;
         if (!v || !k.is_cuda() || k.device() != kc->device() || k.dim() != 3 || !same_shape(k, *v) || k.stride(2) != 1 || v->stride(2) != 1 || k.size(1) != kc->size(1) ||
             !fits32(k.size(0)))
             Py_RETURN_NONE;
         const Tensor* slots = vector_arg(a[2], at::kInt, k.size(0), kc);
-        const int64_t page = q4_page_size(kc->size(2), k.size(2));
+        const int64_t page = page_size_of(calls, kc->size(2), k.size(2));
         if (!slots || page == 0) Py_RETURN_NONE;
         const int64_t ks[2] = {k.stride(0), k.stride(1)}, vs[2] = {v->stride(0), v->stride(1)};
         OnDevice dev(*kc);
-        TT_CALL(rc, tt_cache_append_q4(ptr(k), ptr(v), (const int32_t*)ptr(slots), (int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), tt_type(k), ks, vs,
+        TT_CALL(rc, calls.append(ptr(k), ptr(v), (const int32_t*)ptr(slots), (int32_t)k.size(0), (int32_t)k.size(1), (int32_t)k.size(2), tt_type(k), ks, vs,
                                        ptr(kc), ptr(vc), (int32_t)kc->size(0), (int32_t)page, dev.stream));
         if (rc != TT_OK) return failed(rc);
         Py_INCREF(a[3]);
@@ -848,10 +864,10 @@ PyObject* cache_append_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // (k_cache, v_cache, block_table, cu_lens, total, page_size, k, v) -> (k, v)
-PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* read_from_cache(const CacheCalls& calls, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const Tensor *kc, *vc;
-        if (n != 8 || !q4_cache(a[0], a[1], &kc, &vc)) Py_RETURN_NONE;
+        if (n != 8 || !byte_cache(a[0], a[1], &kc, &vc)) Py_RETURN_NONE;
         const Tensor* table = on_device(a[2], at::kInt, kc);
         if (!table || !table->is_contiguous() || table->dim() != 2 || !fits32(table->size(0)) || !fits32(table->size(1))) Py_RETURN_NONE;
         const Tensor* cu = vector_arg(a[3], at::kInt, table->size(0) + 1, kc);
@@ -859,8 +875,9 @@ PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!cu) Py_RETURN_NONE;
         if (!int_arg(a[4], &total) || !int_arg(a[5], &page)) return nullptr;
         if (total < 0 || !fits32(total) || page < 1 || !fits32(page)) Py_RETURN_NONE;
-        const int64_t D = kc->size(2) == page * 34 ? 64 : kc->size(2) == page * 68 ? 128 : 0;
-        if (D == 0 || page % 16) Py_RETURN_NONE;
+        if (page % 16) Py_RETURN_NONE;
+        const int64_t D = page_size_of(calls, kc->size(2), 64) == page ? 64 : page_size_of(calls, kc->size(2), 128) == page ? 128 : 0;
+        if (D == 0) Py_RETURN_NONE;
         OnDevice dev(*kc);
         Tensor made[2];
         const Tensor* out[2];
@@ -879,7 +896,7 @@ PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
                 out[i] = &made[i];
             }
         }
-        TT_CALL(rc, tt_cache_read_q4(ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(cu), (int32_t)table->size(0), (int32_t)kc->size(1), (int32_t)D,
+        TT_CALL(rc, calls.read(ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(cu), (int32_t)table->size(0), (int32_t)kc->size(1), (int32_t)D,
                                      (int32_t)kc->size(0), (int32_t)page, (int32_t)table->size(1), (int32_t)total, ptr(out[0]), ptr(out[1]), dev.stream));
         if (rc != TT_OK) return failed(rc);
         return pack(wrap_or(a[6], made[0]), wrap_or(a[7], made[1]));
@@ -887,13 +904,13 @@ PyObject* cache_read_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // (q, k_cache, v_cache, block_table, seq_lens, max_len, scale, out, lse, workspace, need_lse) -> (out, lse)
-PyObject* attention_decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* decode_cache(const CacheCalls& calls, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const Tensor *kc, *vc;
-        if (n != 11 || !q4_cache(a[1], a[2], &kc, &vc)) Py_RETURN_NONE;
+        if (n != 11 || !byte_cache(a[1], a[2], &kc, &vc)) Py_RETURN_NONE;
         const Tensor* q = on_device(a[0], at::kBFloat16, kc);
         if (!q || !q->is_contiguous() || q->dim() != 4 || q->size(2) != 1) Py_RETURN_NONE;
-        const int64_t B = q->size(0), H = q->size(1), D = q->size(3), hkv = kc->size(1), page = q4_page_size(kc->size(2), D);
+        const int64_t B = q->size(0), H = q->size(1), D = q->size(3), hkv = kc->size(1), page = page_size_of(calls, kc->size(2), D);
         if (hkv < 1 || H % hkv != 0 || page == 0 || !fits32(B) || !fits32(H)) Py_RETURN_NONE;
         const Tensor *table = nullptr, *lens = nullptr;
         int64_t max_pages = 0, L = page;
@@ -922,8 +939,8 @@ PyObject* attention_decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!out) new_out = make_like(*q);
         if (!lse && need_lse) new_lse = make({B, H, 1}, at::kFloat, *q);
         size_t bytes;
-        ws = workspace_arg(ws, tt_attn_decode_q4_workspace_bytes(&d), 0, *q, &made, &bytes);
-        TT_CALL(rc, tt_attn_decode_q4(&d, ptr(q), ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(lens), (int32_t)kc->size(0), (int32_t)page,
+        ws = workspace_arg(ws, calls.workspace(&d), 0, *q, &made, &bytes);
+        TT_CALL(rc, calls.decode(&d, ptr(q), ptr(kc), ptr(vc), (const int32_t*)ptr(table), (const int32_t*)ptr(lens), (int32_t)kc->size(0), (int32_t)page,
                                       (int32_t)max_pages, out ? ptr(out) : ptr(new_out),
                                       (float*)(lse ? ptr(lse) : new_lse.defined() ? ptr(new_lse) : nullptr), ptr(ws), bytes, dev.stream));
         if (rc != TT_OK) return failed(rc);
@@ -931,13 +948,22 @@ PyObject* attention_decode_q4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+#define TT_OF_CACHE(name, body, calls) \
+    PyObject* name(PyObject*, PyObject* const* a, Py_ssize_t n) { return body(calls, a, n); }
+TT_OF_CACHE(cache_append_q4, append_to_cache, kQ4)
+TT_OF_CACHE(cache_read_q4, read_from_cache, kQ4)
+TT_OF_CACHE(attention_decode_q4, decode_cache, kQ4)
+TT_OF_CACHE(cache_append_q8, append_to_cache, kQ8)
+TT_OF_CACHE(cache_read_q8, read_from_cache, kQ8)
+TT_OF_CACHE(attention_decode_q8, decode_cache, kQ8)
+
 #define TT_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     TT_METHOD(attention_forward), TT_METHOD(attention_backward), TT_METHOD(attention_forward_varlen),
     TT_METHOD(attention_backward_varlen), TT_METHOD(attention_decode), TT_METHOD(attention_decode_paged),
     TT_METHOD(softmax_forward), TT_METHOD(softmax_backward), TT_METHOD(fc_forward), TT_METHOD(fc_backward), TT_METHOD(cache_extend), TT_METHOD(cache_release),
     TT_METHOD(rotary), TT_METHOD(norm_rotary_forward), TT_METHOD(norm_rotary_backward), TT_METHOD(cache_append_rotary), TT_METHOD(cache_append_q4), TT_METHOD(cache_read_q4),
-    TT_METHOD(attention_decode_q4),
+    TT_METHOD(attention_decode_q4), TT_METHOD(cache_append_q8), TT_METHOD(cache_read_q8), TT_METHOD(attention_decode_q8),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ttorch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

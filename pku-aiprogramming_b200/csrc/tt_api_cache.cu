@@ -4,6 +4,7 @@
 #include "common.h"
 
 #include <cmath>
+#include <cstdio>
 #include <cstdlib>
 
 namespace ttk {
@@ -38,12 +39,13 @@ int table_args(const char* who, int32_t B, int32_t page_size, int32_t max_pages,
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-int q4_args(const char* who, const void* k_cache, const void* v_cache, int32_t Hkv, int32_t D, int32_t n_pages, int32_t page_size) {
+// page_bytes: of one head's page, 0 where the size is not supported
+int cache_args(const char* who, const void* k_cache, const void* v_cache, int32_t Hkv, int32_t D, int32_t n_pages, int32_t page_size, size_t page_bytes) {
     if (D != 64 && D != 128) return fail(TT_ERR_UNSUPPORTED, "%s: head dim 64 or 128 only, got %d", who, D);
     if (page_size < 16 || page_size % 16) return fail(TT_ERR_BAD_SHAPE, "%s: page_size=%d must be a multiple of 16", who, page_size);
     if (Hkv < 1 || n_pages < 0) return fail(TT_ERR_BAD_SHAPE, "%s: Hkv=%d n_pages=%d", who, Hkv, n_pages);
     if ((int64_t)n_pages * page_size >= (1LL << 31)) return fail(TT_ERR_BAD_SHAPE, "%s: pages of %d x %d tokens, at most 2^31 - 1", who, n_pages, page_size);
-    if ((double)n_pages * Hkv * page_size * (D / 2 + D / 32) >= 137438953472.0) return fail(TT_ERR_BAD_SHAPE, "%s: a cache of 2^37 bytes or more", who);
+    if ((double)n_pages * Hkv * page_bytes >= 137438953472.0) return fail(TT_ERR_BAD_SHAPE, "%s: a cache of 2^37 bytes or more", who);
     if (n_pages && (!k_cache || !v_cache)) return fail(TT_ERR_NULL, "%s: null cache", who);
     if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(TT_ERR_BAD_SHAPE, "%s: the cache must be 16-byte aligned", who);
     return TT_OK;
@@ -200,6 +202,90 @@ RotaryArgs rotary_args(const tt_rotary_desc* d, const void* q, const void* k, co
     return a;
 }
 
+int launch_fail(cudaError_t e, const char* who) {
+    char what[64];
+    snprintf(what, sizeof what, "%s: launch", who);
+    return cuda_fail(e, what);
+}
+
+// What the calls of the two caches have in common; `run` launches.
+int append_to_cache(const char* who, size_t page_bytes, decltype(&cache_append_q4) run, const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype, const int64_t* k_stride,
+                       const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages, int32_t page_size, void* stream) {
+    int rc = cache_args(who, k_cache, v_cache, Hkv, D, n_pages, page_size, page_bytes);
+    if (rc != TT_OK) return rc;
+    if (dtype != TT_F32 && dtype != TT_BF16) return fail(TT_ERR_BAD_DTYPE, "%s: dtype %d unknown", who, dtype);
+    if (T < 0 || (int64_t)T * Hkv >= (1LL << 31)) return fail(TT_ERR_BAD_SHAPE, "%s: T=%d Hkv=%d", who, T, Hkv);
+    if (!k_stride || !v_stride) return fail(TT_ERR_NULL, "%s: null strides", who);
+    if (T && (!k || !v || !slots)) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    const size_t size = dtype == TT_BF16 ? 2 : 4;
+    if (((uintptr_t)k | (uintptr_t)v) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
+    if (k_stride[0] < 0 || k_stride[1] < 0 || v_stride[0] < 0 || v_stride[1] < 0) return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
+    const size_t pool = (size_t)n_pages * Hkv * page_bytes;
+    auto bytes = [&](const int64_t* st) { return T ? (size_t)((T - 1) * st[0] + (Hkv - 1) * st[1] + D) * size : 0; };
+    const Span out[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}}, in[] = {{k, bytes(k_stride), "k"}, {v, bytes(v_stride), "v"}, {slots, (size_t)T * 4, "slots"}};
+    if ((rc = check_overlap(who, out, 2, in, 3)) != TT_OK) return rc;
+    if ((rc = check_device()) != TT_OK || T == 0 || n_pages == 0) return rc;
+    const CacheView c{k_cache, v_cache, n_pages, page_size, Hkv, D};
+    const long long ks[2] = {k_stride[0], k_stride[1]}, vs[2] = {v_stride[0], v_stride[1]};
+    const cudaError_t e = run(c, k, v, ks, vs, dtype == TT_BF16, slots, T, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : launch_fail(e, who);
+}
+
+int read_from_cache(const char* who, size_t page_bytes, decltype(&cache_read_q4) run, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* cu_lens, int32_t B, int32_t Hkv, int32_t D,
+                     int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t total, void* k, void* v, void* stream) {
+    int rc = cache_args(who, k_cache, v_cache, Hkv, D, n_pages, page_size, page_bytes);
+    if (rc != TT_OK) return rc;
+    if (B < 1 || max_pages < 1 || total < 0 || (int64_t)total * Hkv >= (1LL << 31))
+        return fail(TT_ERR_BAD_SHAPE, "%s: B=%d max_pages=%d total=%d Hkv=%d", who, B, max_pages, total, Hkv);
+    if (!block_table || !cu_lens || (total && (!k || !v))) return fail(TT_ERR_NULL, "%s: null pointer", who);
+    if (!aligned16(k) || !aligned16(v)) return fail(TT_ERR_BAD_SHAPE, "%s: k and v must be 16-byte aligned", who);
+    const size_t pool = (size_t)n_pages * Hkv * page_bytes, n = (size_t)total * Hkv * D * 2;
+    const Span out[] = {{k, n, "k"}, {v, n, "v"}};
+    const Span in[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}, {block_table, (size_t)B * max_pages * 4, "block_table"}, {cu_lens, ((size_t)B + 1) * 4, "cu_lens"}};
+    if ((rc = check_overlap(who, out, 2, in, 4)) != TT_OK || (rc = check_device()) != TT_OK || total == 0) return rc;
+    const CacheView c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, Hkv, D};
+    const cudaError_t e = run(c, block_table, cu_lens, B, max_pages, total, k, v, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : launch_fail(e, who);
+}
+
+int resolve_cache(const char* who, const tt_attn_desc* desc, AttnArgs* a) {
+    const int rc = resolve(desc, a, who);
+    if (rc != TT_OK) return rc;
+    if (a->S != 1) return fail(TT_ERR_BAD_SHAPE, "%s: S must be 1, got %d", who, a->S);
+    if (!a->bf16 || (a->D != 64 && a->D != 128)) return fail(TT_ERR_BAD_DTYPE, "%s: bf16 with D = 64 or 128 only (dtype %d, D %d)", who, desc->dtype, a->D);
+    if (a->L > (1 << 30)) return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds 2^30", who, a->L);
+    a->causal = 0;
+    return TT_OK;
+}
+int decode_cache(const char* who, decltype(&tt_cache_q4_page_bytes) page_bytes, decltype(&attn_decode_q4_workspace) need_of, decltype(&attn_decode_q4) run, const tt_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* seq_lens,
+                      int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    AttnArgs a;
+    int rc = resolve_cache(who, desc, &a);
+    if (rc != TT_OK) return rc;
+    const int hkv = desc->H / a.group;
+    if ((rc = cache_args(who, k_cache, v_cache, hkv, a.D, n_pages, page_size, page_bytes(page_size, a.D))) != TT_OK) return rc;
+    if (!q || !out) return fail(TT_ERR_NULL, "%s: q and out must be non-null", who);
+    if (!aligned16(q) || !aligned16(out)) return fail(TT_ERR_BAD_SHAPE, "%s: q and out must be 16-byte aligned", who);
+    if (block_table) {
+        if (max_pages < 1 || (int64_t)page_size * max_pages < a.L)
+            return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds page_size*max_pages=%lld", who, a.L, (long long)page_size * max_pages);
+    } else if (page_size < a.L || n_pages < desc->B) {
+        return fail(TT_ERR_BAD_SHAPE, "%s: without a block table page_size=%d must hold L=%d and n_pages=%d the batch of %d", who, page_size, a.L, n_pages, desc->B);
+    }
+    const size_t need = need_of(a);
+    if (need && (!workspace || workspace_bytes < need)) return fail(TT_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, workspace_bytes);
+    if (need && ((uintptr_t)workspace & 255)) return fail(TT_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
+    const size_t rows = (size_t)a.BH * a.D * 2, pool = (size_t)n_pages * hkv * page_bytes(page_size, a.D);
+    const Span outs[] = {{out, rows, "out"}, {lse, (size_t)a.BH * 4, "lse"}, {workspace, need, "workspace"}};
+    const Span ins[] = {{q, rows, "q"}, {k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}, {seq_lens, (size_t)desc->B * 4, "seq_lens"},
+                        {block_table, block_table ? (size_t)desc->B * max_pages * 4 : 0, "block_table"}};
+    if ((rc = check_overlap(who, outs, 3, ins, 5)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
+    a.q = q; a.out = out; a.lse = lse;
+    const CacheView c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, hkv, a.D};
+    const cudaError_t e = run(a, c, block_table, seq_lens, max_pages, workspace, (cudaStream_t)stream);
+    return e == cudaSuccess ? TT_OK : launch_fail(e, who);
+}
+
 }  // namespace
 }  // namespace ttk
 
@@ -250,86 +336,45 @@ size_t tt_cache_q4_page_bytes(int32_t page_size, int32_t D) {
 
 int tt_cache_append_q4(const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype, const int64_t* k_stride,
                        const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages, int32_t page_size, void* stream) {
-    const char* who = "tt_cache_append_q4";
-    int rc = q4_args(who, k_cache, v_cache, Hkv, D, n_pages, page_size);
-    if (rc != TT_OK) return rc;
-    if (dtype != TT_F32 && dtype != TT_BF16) return fail(TT_ERR_BAD_DTYPE, "%s: dtype %d unknown", who, dtype);
-    if (T < 0 || (int64_t)T * Hkv >= (1LL << 31)) return fail(TT_ERR_BAD_SHAPE, "%s: T=%d Hkv=%d", who, T, Hkv);
-    if (!k_stride || !v_stride) return fail(TT_ERR_NULL, "%s: null strides", who);
-    if (T && (!k || !v || !slots)) return fail(TT_ERR_NULL, "%s: null pointer", who);
-    const size_t size = dtype == TT_BF16 ? 2 : 4;
-    if (((uintptr_t)k | (uintptr_t)v) % size) return fail(TT_ERR_BAD_SHAPE, "%s: pointers must be multiples of the element size", who);
-    if (k_stride[0] < 0 || k_stride[1] < 0 || v_stride[0] < 0 || v_stride[1] < 0) return fail(TT_ERR_BAD_SHAPE, "%s: negative stride", who);
-    const size_t pool = (size_t)n_pages * Hkv * tt_cache_q4_page_bytes(page_size, D);
-    auto bytes = [&](const int64_t* st) { return T ? (size_t)((T - 1) * st[0] + (Hkv - 1) * st[1] + D) * size : 0; };
-    const Span out[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}}, in[] = {{k, bytes(k_stride), "k"}, {v, bytes(v_stride), "v"}, {slots, (size_t)T * 4, "slots"}};
-    if ((rc = check_overlap(who, out, 2, in, 3)) != TT_OK) return rc;
-    if ((rc = check_device()) != TT_OK || T == 0 || n_pages == 0) return rc;
-    const CacheQ4 c{k_cache, v_cache, n_pages, page_size, Hkv, D};
-    const long long ks[2] = {k_stride[0], k_stride[1]}, vs[2] = {v_stride[0], v_stride[1]};
-    const cudaError_t e = cache_append_q4(c, k, v, ks, vs, dtype == TT_BF16, slots, T, (cudaStream_t)stream);
-    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_append_q4: launch");
+    return append_to_cache("tt_cache_append_q4", tt_cache_q4_page_bytes(page_size, D), cache_append_q4, k, v, slots, T, Hkv, D, dtype, k_stride, v_stride, k_cache, v_cache, n_pages, page_size, stream);
 }
 
 int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* cu_lens, int32_t B, int32_t Hkv, int32_t D,
                      int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t total, void* k, void* v, void* stream) {
-    const char* who = "tt_cache_read_q4";
-    int rc = q4_args(who, k_cache, v_cache, Hkv, D, n_pages, page_size);
-    if (rc != TT_OK) return rc;
-    if (B < 1 || max_pages < 1 || total < 0 || (int64_t)total * Hkv >= (1LL << 31))
-        return fail(TT_ERR_BAD_SHAPE, "%s: B=%d max_pages=%d total=%d Hkv=%d", who, B, max_pages, total, Hkv);
-    if (!block_table || !cu_lens || (total && (!k || !v))) return fail(TT_ERR_NULL, "%s: null pointer", who);
-    if (!aligned16(k) || !aligned16(v)) return fail(TT_ERR_BAD_SHAPE, "%s: k and v must be 16-byte aligned", who);
-    const size_t pool = (size_t)n_pages * Hkv * tt_cache_q4_page_bytes(page_size, D), n = (size_t)total * Hkv * D * 2;
-    const Span out[] = {{k, n, "k"}, {v, n, "v"}};
-    const Span in[] = {{k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}, {block_table, (size_t)B * max_pages * 4, "block_table"}, {cu_lens, ((size_t)B + 1) * 4, "cu_lens"}};
-    if ((rc = check_overlap(who, out, 2, in, 4)) != TT_OK || (rc = check_device()) != TT_OK || total == 0) return rc;
-    const CacheQ4 c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, Hkv, D};
-    const cudaError_t e = cache_read_q4(c, block_table, cu_lens, B, max_pages, total, k, v, (cudaStream_t)stream);
-    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_cache_read_q4: launch");
+    return read_from_cache("tt_cache_read_q4", tt_cache_q4_page_bytes(page_size, D), cache_read_q4, k_cache, v_cache, block_table, cu_lens, B, Hkv, D, n_pages, page_size, max_pages, total, k, v, stream);
 }
 
-static int resolve_q4(const char* who, const tt_attn_desc* desc, AttnArgs* a) {
-    const int rc = resolve(desc, a, who);
-    if (rc != TT_OK) return rc;
-    if (a->S != 1) return fail(TT_ERR_BAD_SHAPE, "%s: S must be 1, got %d", who, a->S);
-    if (!a->bf16 || (a->D != 64 && a->D != 128)) return fail(TT_ERR_BAD_DTYPE, "%s: bf16 with D = 64 or 128 only (dtype %d, D %d)", who, desc->dtype, a->D);
-    if (a->L > (1 << 30)) return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds 2^30", who, a->L);
-    a->causal = 0;
-    return TT_OK;
-}
 size_t tt_attn_decode_q4_workspace_bytes(const tt_attn_desc* desc) {
     AttnArgs a;
-    return resolve_q4("tt_attn_decode_q4_workspace_bytes", desc, &a) == TT_OK ? attn_decode_q4_workspace(a) : 0;
+    return resolve_cache("tt_attn_decode_q4_workspace_bytes", desc, &a) == TT_OK ? attn_decode_q4_workspace(a) : 0;
 }
 int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* seq_lens,
                       int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-    const char* who = "tt_attn_decode_q4";
+    return decode_cache("tt_attn_decode_q4", tt_cache_q4_page_bytes, attn_decode_q4_workspace, attn_decode_q4, desc, q, k_cache, v_cache, block_table, seq_lens, n_pages, page_size, max_pages, out, lse, workspace, workspace_bytes, stream);
+}
+
+size_t tt_cache_q8_page_bytes(int32_t page_size, int32_t D) {
+    if ((D != 64 && D != 128) || page_size < 16 || page_size % 16) return 0;
+    return (size_t)page_size * D + (size_t)(page_size / 16 + 31) / 32 * 32;
+}
+
+int tt_cache_append_q8(const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype, const int64_t* k_stride,
+                       const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages, int32_t page_size, void* stream) {
+    return append_to_cache("tt_cache_append_q8", tt_cache_q8_page_bytes(page_size, D), cache_append_q8, k, v, slots, T, Hkv, D, dtype, k_stride, v_stride, k_cache, v_cache, n_pages, page_size, stream);
+}
+
+int tt_cache_read_q8(const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* cu_lens, int32_t B, int32_t Hkv, int32_t D,
+                     int32_t n_pages, int32_t page_size, int32_t max_pages, int32_t total, void* k, void* v, void* stream) {
+    return read_from_cache("tt_cache_read_q8", tt_cache_q8_page_bytes(page_size, D), cache_read_q8, k_cache, v_cache, block_table, cu_lens, B, Hkv, D, n_pages, page_size, max_pages, total, k, v, stream);
+}
+
+size_t tt_attn_decode_q8_workspace_bytes(const tt_attn_desc* desc) {
     AttnArgs a;
-    int rc = resolve_q4(who, desc, &a);
-    if (rc != TT_OK) return rc;
-    const int hkv = desc->H / a.group;
-    if ((rc = q4_args(who, k_cache, v_cache, hkv, a.D, n_pages, page_size)) != TT_OK) return rc;
-    if (!q || !out) return fail(TT_ERR_NULL, "%s: q and out must be non-null", who);
-    if (!aligned16(q) || !aligned16(out)) return fail(TT_ERR_BAD_SHAPE, "%s: q and out must be 16-byte aligned", who);
-    if (block_table) {
-        if (max_pages < 1 || (int64_t)page_size * max_pages < a.L)
-            return fail(TT_ERR_BAD_SHAPE, "%s: L=%d exceeds page_size*max_pages=%lld", who, a.L, (long long)page_size * max_pages);
-    } else if (page_size < a.L || n_pages < desc->B) {
-        return fail(TT_ERR_BAD_SHAPE, "%s: without a block table page_size=%d must hold L=%d and n_pages=%d the batch of %d", who, page_size, a.L, n_pages, desc->B);
-    }
-    const size_t need = attn_decode_q4_workspace(a);
-    if (need && (!workspace || workspace_bytes < need)) return fail(TT_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", who, need, workspace_bytes);
-    if (need && ((uintptr_t)workspace & 255)) return fail(TT_ERR_WORKSPACE, "%s: workspace must be 256-byte aligned", who);
-    const size_t rows = (size_t)a.BH * a.D * 2, pool = (size_t)n_pages * hkv * tt_cache_q4_page_bytes(page_size, a.D);
-    const Span outs[] = {{out, rows, "out"}, {lse, (size_t)a.BH * 4, "lse"}, {workspace, need, "workspace"}};
-    const Span ins[] = {{q, rows, "q"}, {k_cache, pool, "k_cache"}, {v_cache, pool, "v_cache"}, {seq_lens, (size_t)desc->B * 4, "seq_lens"},
-                        {block_table, block_table ? (size_t)desc->B * max_pages * 4 : 0, "block_table"}};
-    if ((rc = check_overlap(who, outs, 3, ins, 5)) != TT_OK || (rc = check_device()) != TT_OK) return rc;
-    a.q = q; a.out = out; a.lse = lse;
-    const CacheQ4 c{const_cast<void*>(k_cache), const_cast<void*>(v_cache), n_pages, page_size, hkv, a.D};
-    const cudaError_t e = attn_decode_q4(a, c, block_table, seq_lens, max_pages, workspace, (cudaStream_t)stream);
-    return e == cudaSuccess ? TT_OK : cuda_fail(e, "tt_attn_decode_q4: launch");
+    return resolve_cache("tt_attn_decode_q8_workspace_bytes", desc, &a) == TT_OK ? attn_decode_q8_workspace(a) : 0;
+}
+int tt_attn_decode_q8(const tt_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* seq_lens,
+                      int32_t n_pages, int32_t page_size, int32_t max_pages, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    return decode_cache("tt_attn_decode_q8", tt_cache_q8_page_bytes, attn_decode_q8_workspace, attn_decode_q8, desc, q, k_cache, v_cache, block_table, seq_lens, n_pages, page_size, max_pages, out, lse, workspace, workspace_bytes, stream);
 }
 
 int tt_rotary(const tt_rotary_desc* d, const void* q, const void* k, const int32_t* positions, const double* inv_freq, const int32_t* axes, int32_t backward,

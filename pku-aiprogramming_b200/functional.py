@@ -243,26 +243,51 @@ def cache_release(block_table, seq_lens, done, free_pages, n_free, page_size, ou
         ("n_free", n_free, 1, (torch.int32,))], out, "B, 1"))
 
 
-def cache_alloc_q4(pages, kv_heads, page_size, head_dim, device="cuda"):
-    """(k_cache, v_cache) of a 4-bit key/value cache: zeroed bytes `[pages, kv_heads, page bytes]`, head dim 64 or 128, pages
-    of a multiple of 16 tokens.  4.25 bits a value: per 32 channels a scale of 8 bits and 4 bits each."""
-    n = int(capi.lib.tt_cache_q4_page_bytes(int(page_size), int(head_dim)))
+def _page_bytes(bits, page_size, head_dim):
+    call = capi.lib.tt_cache_q4_page_bytes if bits == 4 else capi.lib.tt_cache_q8_page_bytes
+    return int(call(int(page_size), int(head_dim)))
+
+
+def _page_tokens(bits, n_bytes, head_dim):
+    """The page size whose pages have that many bytes; 0: none has."""
+    if head_dim not in (64, 128):
+        return 0
+    lo, hi = 0, n_bytes // (8 * head_dim) + 1   # in units of 16
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        lo, hi = (mid, hi) if _page_bytes(bits, 16 * mid, head_dim) <= n_bytes else (lo, mid)
+    return 16 * lo if lo and _page_bytes(bits, 16 * lo, head_dim) == n_bytes else 0
+
+
+def _cache_alloc(bits, pages, kv_heads, page_size, head_dim, device):
+    n = _page_bytes(bits, page_size, head_dim)
     if n == 0:
         raise ValueError(f"page_size {page_size} must be a multiple of 16 and head_dim {head_dim} 64 or 128")
     k = torch.zeros((int(pages), int(kv_heads), n), dtype=torch.uint8, device=device)
     return k, torch.zeros_like(k)
 
 
-def _explain_q4_cache(k_cache, v_cache):
+def cache_alloc_q4(pages, kv_heads, page_size, head_dim, device="cuda"):
+    """(k_cache, v_cache) of a 4-bit key/value cache: zeroed bytes `[pages, kv_heads, page bytes]`, head dim 64 or 128, pages
+    of a multiple of 16 tokens.  4.25 bits a value: per 32 channels a scale of 8 bits and 4 bits each."""
+    return _cache_alloc(4, pages, kv_heads, page_size, head_dim, device)
+
+
+def cache_alloc_q8(pages, kv_heads, page_size, head_dim, device="cuda"):
+    """(k_cache, v_cache) of an 8-bit key/value cache, as `cache_alloc_q4`: 8-bit floats (e4m3) and for every 16 tokens of a head a scale, a power of two."""
+    return _cache_alloc(8, pages, kv_heads, page_size, head_dim, device)
+
+
+def _explain_cache(bits, k_cache, v_cache):
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 3 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous CUDA uint8 tensor [pages, kv_heads, page bytes], see cache_alloc_q4")
+            raise ValueError(f"{name} must be a contiguous CUDA uint8 tensor [pages, kv_heads, page bytes], see cache_alloc_q{bits}")
     if k_cache.shape != v_cache.shape or k_cache.device != v_cache.device:
         raise ValueError("k_cache and v_cache must have one shape and device")
 
 
-def _explain_append_q4(k, v, slots, k_cache, v_cache):
-    _explain_q4_cache(k_cache, v_cache)
+def _explain_cache_append(bits, k, v, slots, k_cache, v_cache):
+    _explain_cache(bits, k_cache, v_cache)
     for name, t in (("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor) or t.dtype not in _DT or t.device != k_cache.device or t.dim() != 3 or t.stride(2) != 1:
             raise ValueError(f"{name} must be a float32/bfloat16 tensor [T, kv_heads, D] on the cache's device, channels next to each other")
@@ -280,11 +305,19 @@ def cache_append_q4(k, v, slots, k_cache, v_cache):
     """New keys and values `[T, kv_heads, D]` (float32 or bfloat16, strided) into a 4-bit cache at `slots` (int32 `[T]`, as from
     `cache_extend`; -1 is passed over, no slot may come twice) -> (k_cache, v_cache), written in place."""
     r = _native.cache_append_q4(k, v, slots, k_cache, v_cache)
-    return r if r.__class__ is tuple else _done(r, _explain_append_q4, k, v, slots, k_cache, v_cache)
+    return r if r.__class__ is tuple else _done(r, _explain_cache_append, 4, k, v, slots, k_cache, v_cache)
 
 
-def _explain_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size):
-    _explain_q4_cache(k_cache, v_cache)
+def cache_append_q8(k, v, slots, k_cache, v_cache):
+    """New keys and values into an 8-bit cache, as `cache_append_q4`.  The tokens of a call that go to one block of 16 rows of a page lie next to each
+    other, as a sequence's do.  A block's scale is the smallest power of two that holds its tokens' largest value; tokens that come later raise
+    it where they have to, and a call that brings the block's first row begins it anew."""
+    r = _native.cache_append_q8(k, v, slots, k_cache, v_cache)
+    return r if r.__class__ is tuple else _done(r, _explain_cache_append, 8, k, v, slots, k_cache, v_cache)
+
+
+def _explain_cache_read(bits, k_cache, v_cache, block_table, cu_lens, total, page_size):
+    _explain_cache(bits, k_cache, v_cache)
     dev = k_cache.device
     if not isinstance(block_table, torch.Tensor) or block_table.dtype != torch.int32 or block_table.device != dev or block_table.dim() != 2 \
             or not block_table.is_contiguous():
@@ -293,7 +326,7 @@ def _explain_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size):
     if not isinstance(cu_lens, torch.Tensor) or cu_lens.dtype != torch.int32 or cu_lens.device != dev or tuple(cu_lens.shape) != (n,) \
             or not cu_lens.is_contiguous():
         raise ValueError(f"cu_lens must be a contiguous int32 vector of {n} cumulative token counts on the cache's device")
-    if int(page_size) < 16 or int(page_size) % 16 or k_cache.shape[2] not in (34 * int(page_size), 68 * int(page_size)):
+    if int(page_size) < 16 or int(page_size) % 16 or int(page_size) not in [_page_tokens(bits, k_cache.shape[2], d) for d in (64, 128)]:
         raise ValueError(f"pages of {k_cache.shape[2]} bytes are not {page_size} tokens (a multiple of 16) of head dim 64 or 128")
     raise ValueError("total must be a 32-bit integer, k and v contiguous bfloat16 [total, kv_heads, D] on the cache's device")
 
@@ -303,11 +336,17 @@ def cache_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size, k=No
     the keys of `attention_forward_varlen` with `cu_k = cu_lens`, for prompt tokens that follow what is cached.  Rows of given
     `k`, `v` from `cu_lens[B]` on stay as they are."""
     r = _native.cache_read_q4(k_cache, v_cache, block_table, cu_lens, total, page_size, k, v)
-    return r if r.__class__ is tuple else _done(r, _explain_read_q4, k_cache, v_cache, block_table, cu_lens, total, page_size)
+    return r if r.__class__ is tuple else _done(r, _explain_cache_read, 4, k_cache, v_cache, block_table, cu_lens, total, page_size)
 
 
-def _explain_decode_q4(q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse):
-    _explain_q4_cache(k_cache, v_cache)
+def cache_read_q8(k_cache, v_cache, block_table, cu_lens, total, page_size, k=None, v=None):
+    """The tokens of an 8-bit cache's sequences as packed bfloat16, as `cache_read_q4`."""
+    r = _native.cache_read_q8(k_cache, v_cache, block_table, cu_lens, total, page_size, k, v)
+    return r if r.__class__ is tuple else _done(r, _explain_cache_read, 8, k_cache, v_cache, block_table, cu_lens, total, page_size)
+
+
+def _explain_cache_decode(bits, q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse):
+    _explain_cache(bits, k_cache, v_cache)
     dev = k_cache.device
     if not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[2] != 1 or q.dtype != torch.bfloat16 or q.device != dev or not q.is_contiguous():
         raise ValueError("q must be a contiguous bfloat16 tensor [B,H,1,D] on the cache's device")
@@ -315,8 +354,8 @@ def _explain_decode_q4(q, k_cache, v_cache, block_table, seq_lens, max_len, out,
     Hkv = k_cache.shape[1]
     if Hkv < 1 or H % Hkv != 0:
         raise ValueError(f"key/value heads {Hkv} must divide query heads {H}")
-    row = D // 2 + D // 32
-    if D not in (64, 128) or k_cache.shape[2] == 0 or k_cache.shape[2] % (16 * row) != 0:
+    page = _page_tokens(bits, k_cache.shape[2], D)
+    if page == 0:
         raise ValueError(f"pages of {k_cache.shape[2]} bytes are not a multiple of 16 tokens of head dim {D} (64 or 128)")
     for name, t, shape in (("block_table", block_table, None), ("seq_lens", seq_lens, (B,))):
         if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous()
@@ -326,7 +365,7 @@ def _explain_decode_q4(q, k_cache, v_cache, block_table, seq_lens, max_len, out,
         raise ValueError("block_table must be [B, max_pages]")
     if block_table is None and k_cache.shape[0] != B:
         raise ValueError("a cache without a block table must have one page per batch entry")
-    longest = k_cache.shape[2] // row * (1 if block_table is None else block_table.shape[1])
+    longest = page * (1 if block_table is None else block_table.shape[1])
     if max_len is not None and int(max_len) > longest:
         raise ValueError(f"max_len exceeds the {longest} keys that a sequence may have")
     for name, t, shape, dtype in (("out", out, q.shape, torch.bfloat16), ("lse", lse, (B, H, 1), torch.float32)):
@@ -343,7 +382,13 @@ def attention_decode_q4(q, k_cache, v_cache, block_table=None, seq_lens=None, ma
     can hold), which decides how the keys are divided.  An empty sequence gives out = 0, lse = -inf.  A group of more than 16 query heads reads the
     cache once for each 16."""
     r = _native.attention_decode_q4(q, k_cache, v_cache, block_table, seq_lens, max_len, scale, out, lse, workspace, need_lse)
-    return r if r.__class__ is tuple else _done(r, _explain_decode_q4, q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse)
+    return r if r.__class__ is tuple else _done(r, _explain_cache_decode, 4, q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse)
+
+
+def attention_decode_q8(q, k_cache, v_cache, block_table=None, seq_lens=None, max_len=None, scale=None, out=None, lse=None, workspace=None, need_lse=True):
+    """Single-query attention over an 8-bit cache (see `cache_alloc_q8`) -> (out, lse), with the arguments of `attention_decode_q4`."""
+    r = _native.attention_decode_q8(q, k_cache, v_cache, block_table, seq_lens, max_len, scale, out, lse, workspace, need_lse)
+    return r if r.__class__ is tuple else _done(r, _explain_cache_decode, 8, q, k_cache, v_cache, block_table, seq_lens, max_len, out, lse)
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, sections=None, cyclic=False, own_ladder=False, device="cuda"):
