@@ -132,9 +132,10 @@ void SoftmaxBackward(const TinyTensor<T>& output, const TinyTensor<T>& grad_outp
 }
 
 namespace {
+// heads [B,H,S,D] with their positions; results at the same strides
 template <typename T>
-void rotate(const char* who, const TinyTensor<T>& x, TinyTensor<T>& y, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
-            const TinyTensor<int>& axes, bool interleaved, float scale, int backward) {
+tt_rotary_desc rotary_desc(const char* who, const TinyTensor<T>& x, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq, const TinyTensor<int>& axes,
+                           bool interleaved, float scale) {
     require_gpu(x, who, "input"); require_gpu(positions, who, "positions"); require_gpu(inv_freq, who, "inv_freq"); require_gpu(axes, who, "axes");
     if (x.shape.size() != 4) throw std::invalid_argument(std::string(who) + ": input must be 4-D [B,H,S,D]");
     const int B = x.shape[0], H = x.shape[1], S = x.shape[2], D = x.shape[3];
@@ -142,8 +143,6 @@ void rotate(const char* who, const TinyTensor<T>& x, TinyTensor<T>& y, const Tin
     if ((p.size() != 2 && p.size() != 3) || p.back() != S || (p.size() == 3 && p[1] != B))
         throw std::invalid_argument(std::string(who) + ": positions must be [axes,S] or [axes,B,S]");
     if (axes.size != inv_freq.size) throw std::invalid_argument(std::string(who) + ": inv_freq and axes must hold one value per pair");
-    if (y.device != "gpu") y.gpu();
-    y.resize(x.shape);
     tt_rotary_desc d = {};
     d.B = B; d.S = S; d.H = H; d.D = D;
     d.R = (int)(2 * inv_freq.size);
@@ -155,9 +154,25 @@ void rotate(const char* who, const TinyTensor<T>& x, TinyTensor<T>& y, const Tin
     for (int i = 0; i < 3; ++i) d.q_stride[i] = d.q_out_stride[i] = stride[i];
     d.pos_stride[0] = p.size() == 3 ? (int64_t)B * S : S;
     d.pos_stride[1] = p.size() == 3 ? S : 0;
+    return d;
+}
+
+template <typename T>
+void rotate(const char* who, const TinyTensor<T>& x, TinyTensor<T>& y, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
+            const TinyTensor<int>& axes, bool interleaved, float scale, int backward) {
+    const tt_rotary_desc d = rotary_desc(who, x, positions, inv_freq, axes, interleaved, scale);
+    if (y.device != "gpu") y.gpu();
+    y.resize(x.shape);
     int rc = tt_rotary(&d, x.p_data, nullptr, positions.p_data, inv_freq.p_data, axes.p_data, backward, y.p_data, nullptr, nullptr);
     if (rc == TT_OK) rc = tt_check_device_status(nullptr);
     raise(rc, who);
+}
+
+template <typename T>
+void check_weight(const char* who, const TinyTensor<T>& input, const TinyTensor<T>& weight) {
+    require_gpu(weight, who, "weight");
+    if (weight.shape.size() != 1 || weight.shape[0] != input.shape[3])
+        throw std::invalid_argument(std::string(who) + ": weight must hold one value per channel of a head");
 }
 }  // namespace
 
@@ -181,6 +196,49 @@ void RotaryBackward(const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input,
 TT_INSTANTIATE_ROTARY(float)
 TT_INSTANTIATE_ROTARY(__nv_bfloat16)
 #undef TT_INSTANTIATE_ROTARY
+
+template <typename T>
+void NormRotaryForward(const TinyTensor<T>& input, const TinyTensor<T>& weight, TinyTensor<T>& output, const TinyTensor<int>& positions,
+                       const TinyTensor<double>& inv_freq, const TinyTensor<int>& axes, bool interleaved, float scale, float eps) {
+    const char* who = "NormRotaryForward";
+    const tt_rotary_desc d = rotary_desc(who, input, positions, inv_freq, axes, interleaved, scale);
+    check_weight(who, input, weight);
+    if (output.device != "gpu") output.gpu();
+    output.resize(input.shape);
+    int rc = tt_norm_rotary(&d, input.p_data, nullptr, weight.p_data, nullptr, d.dtype, eps, positions.p_data, inv_freq.p_data, axes.p_data, output.p_data, nullptr,
+                            nullptr);
+    if (rc == TT_OK) rc = tt_check_device_status(nullptr);
+    raise(rc, who);
+}
+
+template <typename T>
+void NormRotaryBackward(const TinyTensor<T>& input, const TinyTensor<T>& weight, const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input,
+                        TinyTensor<T>& grad_weight, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq, const TinyTensor<int>& axes,
+                        bool interleaved, float scale, float eps) {
+    const char* who = "NormRotaryBackward";
+    const tt_rotary_desc d = rotary_desc(who, input, positions, inv_freq, axes, interleaved, scale);
+    check_weight(who, input, weight);
+    require_gpu(grad_output, who, "grad_output");
+    if (grad_output.shape != input.shape) throw std::invalid_argument(std::string(who) + ": grad_output must have input's shape");
+    for (TinyTensor<T>* t : {&grad_input, &grad_weight})
+        if (t->device != "gpu") t->gpu();
+    grad_input.resize(input.shape);
+    grad_weight.resize(weight.shape);
+    PoolBuffer ws(tt_norm_rotary_bwd_workspace_bytes(&d));
+    int rc = tt_norm_rotary_bwd(&d, grad_output.p_data, nullptr, input.p_data, nullptr, d.q_stride, nullptr, weight.p_data, nullptr, d.dtype, eps, positions.p_data,
+                                inv_freq.p_data, axes.p_data, grad_input.p_data, nullptr, grad_weight.p_data, nullptr, ws.p, ws.bytes, nullptr);
+    if (rc == TT_OK) rc = tt_check_device_status(nullptr);
+    raise(rc, who);
+}
+
+#define TT_INSTANTIATE_NORM_ROTARY(T)                                                                                                                    \
+    template void NormRotaryForward<T>(const TinyTensor<T>&, const TinyTensor<T>&, TinyTensor<T>&, const TinyTensor<int>&, const TinyTensor<double>&,    \
+                                       const TinyTensor<int>&, bool, float, float);                                                                      \
+    template void NormRotaryBackward<T>(const TinyTensor<T>&, const TinyTensor<T>&, const TinyTensor<T>&, TinyTensor<T>&, TinyTensor<T>&,                \
+                                        const TinyTensor<int>&, const TinyTensor<double>&, const TinyTensor<int>&, bool, float, float);
+TT_INSTANTIATE_NORM_ROTARY(float)
+TT_INSTANTIATE_NORM_ROTARY(__nv_bfloat16)
+#undef TT_INSTANTIATE_NORM_ROTARY
 
 namespace {
 template <typename T>

@@ -44,6 +44,16 @@ template <typename T>
 void RotaryBackward(const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq,
                     const TinyTensor<int>& axes, bool interleaved, float scale);
 
+// output = input [B,H,S,D], each head over the root of its channels' mean square and eps, times weight [D], and turned as by RotaryForward.
+template <typename T>
+void NormRotaryForward(const TinyTensor<T>& input, const TinyTensor<T>& weight, TinyTensor<T>& output, const TinyTensor<int>& positions,
+                       const TinyTensor<double>& inv_freq, const TinyTensor<int>& axes, bool interleaved, float scale, float eps);
+// grad_input and grad_weight of sum(output * grad_output); grad_input may be grad_output.
+template <typename T>
+void NormRotaryBackward(const TinyTensor<T>& input, const TinyTensor<T>& weight, const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input,
+                        TinyTensor<T>& grad_weight, const TinyTensor<int>& positions, const TinyTensor<double>& inv_freq, const TinyTensor<int>& axes,
+                        bool interleaved, float scale, float eps);
+
 // output[..., out] = input[..., in] . weight[in, out] + bias, bias of shape [out] or [1] (one value
 // for every output) -- signature and semantics of the reference's FcForward (src/Layers.cu:9-40).
 // T = float (fp32 arithmetic) or __nv_bfloat16 (tcgen05 kernel, fp32 accumulation).

@@ -37,6 +37,16 @@ PYBIND11_MODULE(myLayer, m) {
     m.def("RotaryBackward_bf16", &RotaryBackward<__nv_bfloat16>, py::call_guard<py::gil_scoped_release>(), py::arg("grad_output"),
           py::arg("grad_input"), py::arg("positions"), py::arg("inv_freq"), py::arg("axes"), py::arg("interleaved") = false,
           py::arg("scale") = 1.0f);
+    m.def("NormRotaryForward", &NormRotaryForward<float>, py::call_guard<py::gil_scoped_release>(), py::arg("input"), py::arg("weight"), py::arg("output"),
+          py::arg("positions"), py::arg("inv_freq"), py::arg("axes"), py::arg("interleaved") = false, py::arg("scale") = 1.0f, py::arg("eps") = 1e-6f);
+    m.def("NormRotaryBackward", &NormRotaryBackward<float>, py::call_guard<py::gil_scoped_release>(), py::arg("input"), py::arg("weight"),
+          py::arg("grad_output"), py::arg("grad_input"), py::arg("grad_weight"), py::arg("positions"), py::arg("inv_freq"), py::arg("axes"),
+          py::arg("interleaved") = false, py::arg("scale") = 1.0f, py::arg("eps") = 1e-6f);
+    m.def("NormRotaryForward_bf16", &NormRotaryForward<__nv_bfloat16>, py::call_guard<py::gil_scoped_release>(), py::arg("input"), py::arg("weight"), py::arg("output"),
+          py::arg("positions"), py::arg("inv_freq"), py::arg("axes"), py::arg("interleaved") = false, py::arg("scale") = 1.0f, py::arg("eps") = 1e-6f);
+    m.def("NormRotaryBackward_bf16", &NormRotaryBackward<__nv_bfloat16>, py::call_guard<py::gil_scoped_release>(), py::arg("input"), py::arg("weight"),
+          py::arg("grad_output"), py::arg("grad_input"), py::arg("grad_weight"), py::arg("positions"), py::arg("inv_freq"), py::arg("axes"),
+          py::arg("interleaved") = false, py::arg("scale") = 1.0f, py::arg("eps") = 1e-6f);
     // argument orders of the reference's FcForward / FcBackward (src/bind_Layer.cpp:12-13 there)
     m.def("FcForward", &FcForward<float>, py::call_guard<py::gil_scoped_release>());
     m.def("FcBackward", &FcBackward<float>, py::call_guard<py::gil_scoped_release>());

@@ -9,7 +9,7 @@ from this module gives the same numbers on the CPU (that composition is what the
 the kernels against).
 
 Device-resident nodes: `Tensor(x, device="gpu")` keeps a `myTensor` tensor as the node's data
-instead of a NumPy array, so a chain of device-capable ops (`Attention`, `Rotary`, `Softmax`, `+`, `-`,
+instead of a NumPy array, so a chain of device-capable ops (`Attention`, `Rotary`, `NormRotary`, `Softmax`, `+`, `-`,
 scalar `*`, unary `-`, and the reverse sweep's adjoint sums) never leaves the GPU -- the
 reference's GPU ops go through `get_data()` -> Python list -> `np.array` on every call
 (operators.py:56-58, 511 there).  Ops without a device implementation refuse device inputs
@@ -587,6 +587,58 @@ class Rotary(TensorOp):
 
 def rotary(x, positions, **kwargs):
     return Rotary(positions, **kwargs)(x)
+
+
+class NormRotary(Rotary):
+    """Heads `[B,H,S,D]` divided by the root of their channels' mean square and `eps`, times a weight `[D]`, and turned by their positions, in one
+    pass on the GPU (`myLayer.NormRotaryForward` / `NormRotaryBackward`): queries and keys, each with its weight, ahead of `Attention`.  The other
+    arguments are those of `Rotary`.  Both inputs are NumPy-backed or both device-resident and of one type, as are the gradients."""
+
+    def __init__(self, positions, eps: float = 1e-6, **kwargs):
+        super().__init__(positions, **kwargs)
+        if not 0 < float(eps) < math.inf:
+            raise ValueError("eps must be positive and finite")
+        self.eps = float(eps)
+
+    def _native_of(self, x, w):
+        """(tensor type, forward, backward, whether the inputs stay on the device) for the data of both inputs."""
+        _, ml = _native()
+        resident = _all_or_none_on_device(x, w)
+        T = self._kernels(x)[0]
+        if resident and type(w) is not T:
+            raise TypeError("device-resident heads and weight must share one tensor class")
+        if T.__name__ == "Tensor_bf16":
+            return T, ml.NormRotaryForward_bf16, ml.NormRotaryBackward_bf16, resident
+        return T, ml.NormRotaryForward, ml.NormRotaryBackward, resident
+
+    def compute(self, x, w):
+        T, fwd, _, resident = self._native_of(x, w)
+        tx, tw = (x, w) if resident else (T(np.ascontiguousarray(a, dtype=np.float32), "gpu") for a in (x, w))
+        D = tx.get_shape()[-1]
+        rest = self._saved[D] = self._arguments(D)
+        out = T([1], "gpu")
+        fwd(tx, tw, out, *rest, self.eps)
+        return out if resident else out.numpy().astype(x.dtype, copy=False)
+
+    def gradient(self, out_grad, node):
+        x, w = (i.realize_cached_data() for i in node.inputs)
+        T, _, bwd, resident = self._native_of(x, w)
+        D = node.inputs[0].shape[-1]
+        if D not in self._saved:
+            self._saved[D] = self._arguments(D)
+        g = out_grad.realize_cached_data()
+        if _on_device(g) and type(g) is not T:
+            raise TypeError(f"upstream gradient is {type(g).__name__}, the op ran on {T.__name__}")
+        up = lambda a: a if _on_device(a) else T(np.ascontiguousarray(a, dtype=np.float32), "gpu")
+        gx, gw = T([1], "gpu"), T([1], "gpu")
+        bwd(up(x), up(w), up(g), gx, gw, *self._saved[D], self.eps)
+        if resident:
+            return tuple(Tensor(t, device="gpu", requires_grad=False) for t in (gx, gw))
+        return tuple(Tensor(t.numpy().astype(a.dtype, copy=False), requires_grad=False) for t, a in ((gx, x), (gw, w)))
+
+
+def norm_rotary(x, weight, positions, **kwargs):
+    return NormRotary(positions, **kwargs)(x, weight)
 
 
 class FC(TensorOp):
