@@ -7,10 +7,14 @@
 // units of two accesses of kV values, the two halves of kV pairs (or kV pairs of neighbours, or channels that only are normed); 2^n lanes
 // have a row, so the sums are n shuffles, and the rows of a warp lie next to each other.
 #include "rotary_parts.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ttk {
+using namespace sm100;
 
 constexpr int kHeadThreads = 256;
+constexpr int hd_ctas_per_sm(int units) { return units == 1 ? 4 : 2; }
+constexpr int kBackCtas = 2;   // per SM, of the gradient
 
 // A token's rows of one of the tensors, of head 0: where they come from, where they go, and for keys on their way into a cache a second place.
 template <typename Tin, typename Tout>
@@ -49,72 +53,228 @@ struct HdUnits {
             }
         }
     }
+    // The flags differ among the lanes of a row, which meet in every turn of a loop: they are made unknown to the compiler in each, so that it cannot make
+    // loops of their own for lanes with one and with another.
+    __device__ __forceinline__ void forget() { asm volatile("" : "+r"(has0), "+r"(has1), "+r"(turns)); }
 };
 
-// The table of sines: kV pairs of a unit, two beside each other and then the same two of the next unit, so that what the lanes of a row read at a time is
-// whole banks.
-template <int kV>
-__device__ __forceinline__ int hd_place(int pair, int turned) {
+// Tables in shared memory lie as the lanes of a row read them, 16 bytes of one unit beside the same of the next, so that a read is whole banks.
+// The sines: (cos, sin) of two pairs of a unit, in halves cosines first; kV = 1: of the unit's pair.
+template <int kV, bool kNeighbours>
+__device__ __forceinline__ void hd_put_turn(float* cs, int pair, int turned, float2 f) {
     const int u = pair / kV, e = pair % kV;
-    return kV == 1 ? u : 2 * ((e >> 1) * turned + u) + (e & 1);
+    if (kV == 1) {
+        cs[2 * u] = f.x;
+        cs[2 * u + 1] = f.y;
+    } else {
+        float* at = cs + 4 * ((e >> 1) * turned + u);
+        at[kNeighbours ? 2 * (e & 1) : e & 1] = f.x;
+        at[kNeighbours ? 2 * (e & 1) + 1 : 2 + (e & 1)] = f.y;
+    }
 }
-template <int kV>
-__device__ __forceinline__ void hd_sines(float2* cs, const RotaryArgs& a, const RtPlaces& places, int here, int tid, float per_half) {
-    const int half = a.R / 2, turned = (half + kV - 1) / kV;
-    for (int i = tid; i < here * half; i += kHeadThreads) {
-        const int t = (int)(((float)i + 0.5f) * per_half), pair = i - t * half;   // i < 2^13: exact
+// of a tile's tokens: a thread keeps its pair
+template <int kV, bool kNeighbours>
+__device__ __forceinline__ void hd_sines(float* cs, const RotaryArgs& a, const RtPlaces& places, int here, int tid) {
+    const int half = a.R / 2, turned = (half + kV - 1) / kV, at_once = kHeadThreads / half;   // half is at most 128
+    const int first = tid / half, pair = tid - first * half;
+    if (first >= at_once) return;
+    const int axis = a.axes ? min(max(a.axes[pair], 0), a.n_axes - 1) : 0;
+    const double freq = a.inv_freq[pair];
+    const int* pos = a.pos + axis * a.pos_axis;
+    for (int t = first; t < here; t += at_once) {
         int b, s;
         places.at(t, &b, &s);
-        const int axis = a.axes ? min(max(a.axes[pair], 0), a.n_axes - 1) : 0;
-        const int p = a.pos[axis * a.pos_axis + b * a.pos_batch + s];
-        cs[t * (turned * kV) + hd_place<kV>(pair, turned)] = rt_turn(p, a.inv_freq[pair], a.scale, a.back);
+        hd_put_turn<kV, kNeighbours>(cs + t * (2 * turned * kV), pair, turned, rt_turn(pos[b * a.pos_batch + s], freq, a.scale, a.back));
     }
 }
 // kV pairs of floats turned: (x[0][e], x[1][e]), or neighbours among x[0] and then among x[1]
 template <int kV, bool kNeighbours>
-__device__ __forceinline__ void hd_turn(float (&x)[2][kV], const float2* cs, int u, int turned) {
-    float2 f[kV];
-    if (kV == 1) {
-        f[0] = cs[u];
+__device__ __forceinline__ void hd_turn(float (&x)[2][kV], const float* cs, int u, int turned) {
+    auto turn = [](float& p, float& q, float c, float s) {
+        const float x1 = p, x2 = q;
+        p = x1 * c - x2 * s;
+        q = x2 * c + x1 * s;
+    };
+    if constexpr (kV == 1) {
+        const float2 f = reinterpret_cast<const float2*>(cs)[u];
+        turn(x[0][0], x[1][0], f.x, f.y);
     } else {
 #pragma unroll
         for (int e = 0; e < kV; e += 2) {
-            const float4 z = *reinterpret_cast<const float4*>(cs + 2 * ((e >> 1) * turned + u));
-            f[e] = make_float2(z.x, z.y);
-            f[(e + 1) % kV] = make_float2(z.z, z.w);
+            const float4 z = reinterpret_cast<const float4*>(cs)[(e >> 1) * turned + u];
+            if (kNeighbours) {
+                turn(x[2 * e / kV][2 * e % kV], x[2 * e / kV][2 * e % kV + 1], z.x, z.y);
+                turn(x[(2 * e + 2) / kV][(2 * e + 2) % kV], x[(2 * e + 2) / kV][(2 * e + 2) % kV + 1], z.z, z.w);
+            } else {
+                const uint64_t c = pack_f32x2(z.x, z.y), s = pack_f32x2(z.z, z.w), minus = pack_f32x2(-z.z, -z.w);
+                const uint64_t x1 = pack_f32x2(x[0][e], x[0][e + 1]), x2 = pack_f32x2(x[1][e], x[1][e + 1]);
+                unpack_f32x2(fma_f32x2(x1, c, mul_f32x2(x2, minus)), x[0][e], x[0][e + 1]);
+                unpack_f32x2(fma_f32x2(x2, c, mul_f32x2(x1, s)), x[1][e], x[1][e + 1]);
+            }
         }
     }
-#pragma unroll
-    for (int e = 0; e < kV; ++e) {
-        float &p = kNeighbours && kV > 1 ? x[2 * e / kV][2 * e % kV] : x[0][e], &q = kNeighbours && kV > 1 ? x[2 * e / kV][(2 * e + 1) % kV] : x[1][e];
-        const float x1 = p, x2 = q;
-        p = x1 * f[e].x - x2 * f[e].y;
-        q = x2 * f[e].x + x1 * f[e].y;
+}
+// The weights of a tensor, up to 4 channels of a chunk of a unit at a time; 0 for channels that are not there.
+template <int kV>
+__device__ __forceinline__ void hd_weights(float* ws, const void* w, int bf16, int n_units, int D, int R, bool neighbours, int tid) {
+    constexpr int kQuad = kV < 4 ? kV : 4;
+    const int turned = (R / 2 + kV - 1) / kV;
+    for (int i = tid; i < n_units * 2 * kV; i += kHeadThreads) {
+        const int in = i % kQuad, u = i / kQuad % n_units, m = i / kQuad / n_units, chunk = m / (kV / kQuad), e = m % (kV / kQuad) * kQuad + in;
+        const bool turn = u < turned;
+        const int c0 = !turn ? R + 2 * (u - turned) * kV : neighbours ? 2 * u * kV : u * kV, c = (chunk == 0 ? c0 : turn && !neighbours ? c0 + R / 2 : c0 + kV) + e;
+        const bool there = c < (turn ? R : D);
+        ws[i] = !there ? 0.f : bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[c]) : static_cast<const float*>(w)[c];
     }
 }
-__device__ __forceinline__ float hd_weight(const void* w, int bf16, int c) {
-    return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[c]) : static_cast<const float*>(w)[c];
+template <int kV>
+__device__ __forceinline__ void hd_weight(float (&w)[2][kV], const float* ws, int u, int n_units) {
+    constexpr int kQuad = kV < 4 ? kV : 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < kV; e += kQuad) {
+            const RtVec<float, kQuad> z = reinterpret_cast<const RtVec<float, kQuad>*>(ws)[(i * (kV / kQuad) + e / kQuad) * n_units + u];
+#pragma unroll
+            for (int j = 0; j < kQuad; ++j) w[i][e + j] = z.v[j];
+        }
 }
+// Values of a chunk in floats, and of two of them at a time f(a, b) = a * b, or + c
+template <typename T, int kV>
+__device__ __forceinline__ void hd_floats(float (&x)[kV], const RtVec<T, kV>& v) {
+    if constexpr (sizeof(T) == 2 && kV > 1) {
+        RtVec<uint32_t, kV / 2> w;
+        memcpy(&w, &v, sizeof w);
+#pragma unroll
+        for (int e = 0; e < kV / 2; ++e) {
+            x[2 * e] = __uint_as_float(w.v[e] << 16);
+            x[2 * e + 1] = __uint_as_float(w.v[e] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) x[e] = rt_get(v.v[e]);
+    }
+}
+template <typename T, int kV>
+__device__ __forceinline__ RtVec<T, kV> hd_rounded(const float (&x)[kV]) {
+    RtVec<T, kV> z;
+    if constexpr (sizeof(T) == 2 && kV > 1) {
+#pragma unroll
+        for (int e = 0; e < kV; e += 2) {
+            const __nv_bfloat162 two = __floats2bfloat162_rn(x[e], x[e + 1]);
+            z.v[e] = two.x;
+            z.v[e + 1] = two.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kV; ++e) z.v[e] = rt_put<T>(x[e]);
+    }
+    return z;
+}
+template <int kV>
+__device__ __forceinline__ void hd_mul(float (&y)[kV], const float (&a)[kV], const float (&b)[kV]) {
+    if constexpr (kV == 1) {
+        y[0] = a[0] * b[0];
+    } else {
+#pragma unroll
+        for (int e = 0; e < kV; e += 2) unpack_f32x2(mul_f32x2(pack_f32x2(a[e], a[e + 1]), pack_f32x2(b[e], b[e + 1])), y[e], y[e + 1]);
+    }
+}
+template <int kV>
+__device__ __forceinline__ void hd_mul(float (&y)[kV], const float (&a)[kV], float b) {
+    if constexpr (kV == 1) {
+        y[0] = a[0] * b;
+    } else {
+#pragma unroll
+        for (int e = 0; e < kV; e += 2) unpack_f32x2(mul_f32x2(pack_f32x2(a[e], a[e + 1]), pack_f32x2(b, b)), y[e], y[e + 1]);
+    }
+}
+// y += a b, over the channels into two sums or into one for each
+template <int kV>
+__device__ __forceinline__ void hd_add_products(float (&sum)[2], const float (&a)[kV], const float (&b)[kV]) {
+    if constexpr (kV == 1) {
+        sum[0] = fmaf(a[0], b[0], sum[0]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kV; e += 2)
+            unpack_f32x2(fma_f32x2(pack_f32x2(a[e], a[e + 1]), pack_f32x2(b[e], b[e + 1]), pack_f32x2(sum[0], sum[1])), sum[0], sum[1]);
+    }
+}
+template <int kV>
+__device__ __forceinline__ void hd_fma(float (&y)[kV], const float (&a)[kV], const float (&b)[kV], const float (&c)[kV]) {
+    if constexpr (kV == 1) {
+        y[0] = fmaf(a[0], b[0], c[0]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kV; e += 2)
+            unpack_f32x2(fma_f32x2(pack_f32x2(a[e], a[e + 1]), pack_f32x2(b[e], b[e + 1]), pack_f32x2(c[e], c[e + 1])), y[e], y[e + 1]);
+    }
+}
+template <int kV>
+__device__ __forceinline__ void hd_fma(float (&y)[kV], const float (&a)[kV], float b, const float (&c)[kV]) {
+    float bs[kV];
+#pragma unroll
+    for (int e = 0; e < kV; ++e) bs[e] = b;
+    hd_fma<kV>(y, a, bs, c);
+}
+// What a lane has of a row, as it comes; nothing where there is no row
+template <typename T, int kV, int kUnits>
+struct HdRaw {
+    RtVec<T, kV> v[kUnits][2];
+    template <typename Units>
+    __device__ __forceinline__ void load(const T* x, const Units& units) {
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int e = 0; e < kV; ++e) v[k][i].v[e] = rt_put<T>(0.f);
+                if (x && ((i ? units.has1 : units.has0) >> k & 1)) v[k][i] = *reinterpret_cast<const RtVec<T, kV>*>(x + (i ? units.c1[k] : units.c0[k]));
+            }
+    }
+};
+// A walk of a group of lanes over the rows (token, head) of a tile, as many apart as there are groups.  Every group takes as many turns, some of the last without a row.
+struct HdWalk {
+    int t, h, dt, dh, heads, row, total, apart;
+    __device__ __forceinline__ HdWalk(int group, int groups, int n_heads, int tokens) : heads(n_heads), row(group), total(tokens * n_heads), apart(groups) {
+        t = group / n_heads;
+        h = group - t * n_heads;
+        dt = groups / n_heads;
+        dh = groups - dt * n_heads;
+    }
+    __device__ __forceinline__ int turns() const { return (total + apart - 1) / apart; }
+    __device__ __forceinline__ bool there() const { return row < total; }
+    __device__ __forceinline__ void next() {
+        row += apart;
+        t += dt;
+        h += dh;
+        if (h >= heads) {
+            h -= heads;
+            ++t;
+        }
+    }
+};
 
 // blockDim = kHeadThreads; 2^log_lanes lanes to a row.  kAppend: keys and values go into the pools' rows (a third tensor, which is copied).
 template <typename Tin, typename Tout, int kV, int kUnits, bool kNeighbours, bool kNorm, bool kAppend>
-__global__ void __launch_bounds__(kHeadThreads) heads_kernel(const NormRotaryArgs a, int tokens_per_cta, int log_lanes, float per_half) {
-    using In = RtVec<Tin, kV>;
+__global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kUnits)) heads_kernel(const NormRotaryArgs a, int tokens_per_cta, int log_lanes) {
     using Out = RtVec<Tout, kV>;
     using Rows = typename std::conditional<kAppend, HdRows3<Tin, Tout>, HdRows<Tin, Tout>>::type;
-    constexpr int kTensors = kAppend ? 3 : 2, kAhead = 2;
+    constexpr int kTensors = kAppend ? 3 : 2;
     extern __shared__ float4 sm[];
-    Rows* rows = reinterpret_cast<Rows*>(sm);   // [tokens_per_cta][kTensors]
-    float2* cs = reinterpret_cast<float2*>(rows + kTensors * tokens_per_cta);
     const RotaryArgs& r = a.r;
     const int tid = threadIdx.x, lanes = 1 << log_lanes, lane = tid & (lanes - 1), group = tid >> log_lanes, groups = kHeadThreads >> log_lanes;
+    const int turned = (r.R / 2 + kV - 1) / kV, n_units = lanes * kUnits;
+    Rows* rows = reinterpret_cast<Rows*>(sm);   // [tokens_per_cta][kTensors]
+    float* ws = reinterpret_cast<float*>(rows + kTensors * tokens_per_cta);   // [2][n_units * 2 * kV]
+    float* cs = ws + (kNorm ? 4 * n_units * kV : 0);                          // [tokens_per_cta][2 * turned * kV]
     const unsigned t0 = blockIdx.x * (unsigned)tokens_per_cta, n_tok = (unsigned)r.B * (unsigned)r.S;
-    const int here = (int)min((unsigned)tokens_per_cta, n_tok - t0), turned = (r.R / 2 + kV - 1) / kV;
+    const int here = (int)min((unsigned)tokens_per_cta, n_tok - t0);
     const RtPlaces places(t0, r.B, r.S);
-    const HdUnits<kV, kUnits, kNeighbours> units(lane, lanes, r.D, r.R);
+    const HdUnits<kV, kUnits, kNeighbours> all_units(lane, lanes, r.D, r.R);
     grid_let_next_start();
     grid_wait_for_previous();
-    hd_sines<kV>(cs, r, places, here, tid, per_half);
+    hd_sines<kV, kNeighbours>(cs, r, places, here, tid);
     for (int i = kHeadThreads - 1 - tid; i < kTensors * here; i += kHeadThreads) {
         const int t = i / kTensors, w = i - t * kTensors;
         int b, s;
@@ -138,6 +298,10 @@ __global__ void __launch_bounds__(kHeadThreads) heads_kernel(const NormRotaryArg
             rows[i] = Rows{(const Tin*)r.x[w] + b * r.xs[w][0] + s * r.xs[w][2], (Tout*)r.y[w] + b * r.ys[w][0] + s * r.ys[w][2]};
         }
     }
+    if (kNorm) {
+        for (int w = 0; w < 2; ++w)
+            if (r.heads[w]) hd_weights<kV>(ws + w * (2 * n_units * kV), a.w[w], a.w_bf16, n_units, r.D, r.R, kNeighbours, tid);
+    }
     __syncthreads();
     const float inv_D = 1.f / (float)r.D;
 #pragma unroll 1
@@ -146,84 +310,68 @@ __global__ void __launch_bounds__(kHeadThreads) heads_kernel(const NormRotaryArg
         if (heads == 0) continue;
         const bool moved = kAppend && w == 2;   // as it is
         const long long x_head = moved ? a.v_stride[1] : r.xs[w][1], y_head = kAppend && w > 0 ? (long long)a.page * r.D : r.ys[w][1], also_head = r.ys[1][1];
-        float weight[kUnits][2][kV];
-        if (kNorm && !moved) {
+        const float* weights = ws + w * (2 * n_units * kV);
+        HdWalk at(group, groups, heads, here);
+        const int turns = at.turns();
+        HdRaw<Tin, kV, kUnits> raw, next;
+        auto fetch = [&](HdRaw<Tin, kV, kUnits>& to, const HdWalk& from) { to.load(from.there() ? rows[kTensors * from.t + w].x + from.h * x_head : nullptr, all_units); };
+        fetch(raw, at);
+        for (int turn = 0; turn < turns; ++turn) {
+            HdUnits<kV, kUnits, kNeighbours> units = all_units;
+            units.forget();
+            HdWalk then = at;
+            then.next();
+            fetch(next, then);
+            float x[kUnits][2][kV];
 #pragma unroll
             for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-                for (int e = 0; e < kV; ++e) {
-                    weight[k][0][e] = units.has0 >> k & 1 ? hd_weight(a.w[w], a.w_bf16, units.c0[k] + e) : 0.f;
-                    weight[k][1][e] = units.has1 >> k & 1 ? hd_weight(a.w[w], a.w_bf16, units.c1[k] + e) : 0.f;
-                }
-        }
-        const int total = here * heads, dt = groups / heads, dh = groups - dt * heads;
-        int t = group / heads, h = group - t * heads;
-        for (int base = 0; base < total; base += kAhead * groups) {
-            In v[kAhead][kUnits][2];
-            int at_t[kAhead], at_h[kAhead];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                at_t[j] = base + j * groups + group < total ? t : -1;
-                at_h[j] = h;
-                if (at_t[j] >= 0) {
-                    const Tin* x = rows[kTensors * t + w].x + h * x_head;
-#pragma unroll
-                    for (int k = 0; k < kUnits; ++k) {
-                        if (units.has0 >> k & 1) v[j][k][0] = *reinterpret_cast<const In*>(x + units.c0[k]);
-                        if (units.has1 >> k & 1) v[j][k][1] = *reinterpret_cast<const In*>(x + units.c1[k]);
-                    }
-                }
-                t += dt;
-                h += dh;
-                if (h >= heads) {
-                    h -= heads;
-                    ++t;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                float x[kUnits][2][kV], sum = 0.f;
+                for (int i = 0; i < 2; ++i) hd_floats<Tin, kV>(x[k][i], raw.v[k][i]);
+            if (kNorm && !moved) {
+                float sums[2] = {0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < kV; ++e) {
-                            x[k][i][e] = at_t[j] >= 0 && ((i ? units.has1 : units.has0) >> k & 1) ? rt_get(v[j][k][i].v[e]) : 0.f;
-                            if (kNorm) sum = fmaf(x[k][i][e], x[k][i][e], sum);
-                        }
-                if (kNorm && !moved) {
-                    for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                    const float by = rsqrtf(sum * inv_D + a.eps);
-#pragma unroll
-                    for (int k = 0; k < kUnits; ++k)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int e = 0; e < kV; ++e) x[k][i][e] = x[k][i][e] * by * weight[k][i][e];
-                }
-                if (at_t[j] < 0) continue;
-                const Rows& row = rows[kTensors * at_t[j] + w];
-                Tout* y = row.y ? row.y + at_h[j] * y_head : nullptr;
-                Tout* also = nullptr;
-                if constexpr (kAppend) {
-                    if (row.also) also = row.also + at_h[j] * also_head;
-                }
+                    for (int i = 0; i < 2; ++i) hd_add_products<kV>(sums, x[k][i], x[k][i]);
+                float sum = sums[0] + sums[1];
+                __syncwarp();
+                for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const float by = rsqrtf(sum * inv_D + a.eps);
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k) {
-                    if (!moved && (units.turns >> k & 1)) hd_turn<kV, kNeighbours>(x[k], cs + at_t[j] * (turned * kV), units.at[k], turned);
+                    float wt[2][kV];
+                    hd_weight<kV>(wt, weights, units.at[k], n_units);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        hd_mul<kV>(wt[i], wt[i], by);
+                        hd_mul<kV>(x[k][i], x[k][i], wt[i]);
+                    }
+                }
+            }
+            if (at.there()) {
+                const Rows& row = rows[kTensors * at.t + w];
+                Tout* y = row.y;
+                if (!kAppend || y) y += at.h * y_head;
+                Tout* also = nullptr;
+                if constexpr (kAppend) {
+                    if (row.also) also = row.also + at.h * also_head;
+                }
+                const float* sines = cs + at.t * (2 * turned * kV);
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k) {
+                    if (!moved && (units.turns >> k & 1)) hd_turn<kV, kNeighbours>(x[k], sines, units.at[k], turned);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (!((i ? units.has1 : units.has0) >> k & 1)) continue;
-                        Out z;
-#pragma unroll
-                        for (int e = 0; e < kV; ++e) z.v[e] = rt_put<Tout>(x[k][i][e]);
+                        const Out z = hd_rounded<Tout, kV>(x[k][i]);
                         const int c = i ? units.c1[k] : units.c0[k];
                         if (!kAppend || y) *reinterpret_cast<Out*>(y + c) = z;
                         if (kAppend && also) *reinterpret_cast<Out*>(also + c) = z;
                     }
                 }
             }
+            raw = next;
+            at = then;
         }
     }
 }
@@ -236,38 +384,36 @@ struct alignas(16) HdRowsBack {
     T* y;
 };
 template <typename T, int kV, int kUnits, bool kNeighbours>
-__global__ void __launch_bounds__(kHeadThreads) heads_backward_kernel(const NormRotaryArgs a, int tokens_per_tile, int log_lanes, float per_half, int ctas_q, float* partial) {
-    using Vec = RtVec<T, kV>;
+__global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel(const NormRotaryArgs a, int tokens_per_tile, int log_lanes, int ctas_q, float* partial) {
     using Rows = HdRowsBack<T>;
-    constexpr int kAhead = 2, kWarps = kHeadThreads / 32;
+    using Raw = HdRaw<T, kV, kUnits>;
+    constexpr int kWarps = kHeadThreads / 32;
     extern __shared__ float4 sm[];
-    Rows* rows = reinterpret_cast<Rows*>(sm);   // [tokens_per_tile]
-    float2* cs = reinterpret_cast<float2*>(rows + tokens_per_tile);
     const RotaryArgs& r = a.r;
     const int tid = threadIdx.x, lanes = 1 << log_lanes, lane = tid & (lanes - 1), group = tid >> log_lanes, groups = kHeadThreads >> log_lanes;
+    const int turned = (r.R / 2 + kV - 1) / kV, n_units = lanes * kUnits;
+    Rows* rows = reinterpret_cast<Rows*>(sm);                       // [tokens_per_tile]
+    float* ws = reinterpret_cast<float*>(rows + tokens_per_tile);   // [n_units * 2 * kV]
+    float* cs = ws + 2 * n_units * kV;                              // [tokens_per_tile][2 * turned * kV]
     const int w = (int)blockIdx.x >= ctas_q, cta = (int)blockIdx.x - (w ? ctas_q : 0), n_cta = w ? (int)gridDim.x - ctas_q : ctas_q;
-    const int heads = r.heads[w], turned = (r.R / 2 + kV - 1) / kV;
+    const int heads = r.heads[w];
     const unsigned n_tok = (unsigned)r.B * (unsigned)r.S, tiles = (n_tok + tokens_per_tile - 1) / tokens_per_tile;
-    const HdUnits<kV, kUnits, kNeighbours> units(lane, lanes, r.D, r.R);
-    grid_let_next_start();
-    grid_wait_for_previous();
-    float weight[kUnits][2][kV], dw[kUnits][2][kV];
+    const HdUnits<kV, kUnits, kNeighbours> all_units(lane, lanes, r.D, r.R);
+    const float inv_D = 1.f / (float)r.D;
+    float dw[kUnits][2][kV];
 #pragma unroll
     for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-        for (int e = 0; e < kV; ++e) {
-            weight[k][0][e] = units.has0 >> k & 1 ? hd_weight(a.w[w], a.w_bf16, units.c0[k] + e) : 0.f;
-            weight[k][1][e] = units.has1 >> k & 1 ? hd_weight(a.w[w], a.w_bf16, units.c1[k] + e) : 0.f;
-            dw[k][0][e] = dw[k][1][e] = 0.f;
-        }
-    const float inv_D = 1.f / (float)r.D;
-    const int dt = groups / heads, dh = groups - dt * heads;
+        for (int e = 0; e < kV; ++e) dw[k][0][e] = dw[k][1][e] = 0.f;
+    grid_let_next_start();
+    grid_wait_for_previous();
+    hd_weights<kV>(ws, a.w[w], a.w_bf16, n_units, r.D, r.R, kNeighbours, tid);
     for (unsigned tile = cta; tile < tiles; tile += n_cta) {
         const unsigned t0 = tile * tokens_per_tile;
-        const int here = (int)min((unsigned)tokens_per_tile, n_tok - t0), total = here * heads;
+        const int here = (int)min((unsigned)tokens_per_tile, n_tok - t0);
         const RtPlaces places(t0, r.B, r.S);
         __syncthreads();   // the tile before has been read
-        hd_sines<kV>(cs, r, places, here, tid, per_half);
+        hd_sines<kV, kNeighbours>(cs, r, places, here, tid);
         for (int t = kHeadThreads - 1 - tid; t < here; t += kHeadThreads) {
             int b, s;
             places.at(t, &b, &s);
@@ -275,82 +421,76 @@ __global__ void __launch_bounds__(kHeadThreads) heads_backward_kernel(const Norm
                            (T*)r.y[w] + b * r.ys[w][0] + s * r.ys[w][2]};
         }
         __syncthreads();
-        int t = group / heads, h = group - t * heads;
-        for (int base = 0; base < total; base += kAhead * groups) {
-            Vec vg[kAhead][kUnits][2], vx[kAhead][kUnits][2];
-            int at_t[kAhead], at_h[kAhead];
+        HdWalk at(group, groups, heads, here);
+        const int turns = at.turns();
+        Raw raw_g, raw_x, next_g, next_x;
+        auto fetch = [&](Raw& g, Raw& x, const HdWalk& from) {
+            g.load(from.there() ? rows[from.t].g + from.h * r.xs[w][1] : nullptr, all_units);
+            x.load(from.there() ? rows[from.t].x + from.h * a.in_stride[w][1] : nullptr, all_units);
+        };
+        fetch(raw_g, raw_x, at);
+        for (int turn = 0; turn < turns; ++turn) {
+            HdUnits<kV, kUnits, kNeighbours> units = all_units;
+            units.forget();
+            HdWalk then = at;
+            then.next();
+            fetch(next_g, next_x, then);
+            float g[kUnits][2][kV], x[kUnits][2][kV], squares[2] = {0.f, 0.f}, alongs[2] = {0.f, 0.f};
+            const float* sines = cs + (at.there() ? at.t : 0) * (2 * turned * kV);
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                at_t[j] = base + j * groups + group < total ? t : -1;
-                at_h[j] = h;
-                if (at_t[j] >= 0) {
-                    const T *g = rows[t].g + h * r.xs[w][1], *x = rows[t].x + h * a.in_stride[w][1];
+            for (int k = 0; k < kUnits; ++k) {
+                float wt[2][kV];
+                hd_weight<kV>(wt, ws, units.at[k], n_units);
 #pragma unroll
-                    for (int k = 0; k < kUnits; ++k) {
-                        if (units.has0 >> k & 1) {
-                            vg[j][k][0] = *reinterpret_cast<const Vec*>(g + units.c0[k]);
-                            vx[j][k][0] = *reinterpret_cast<const Vec*>(x + units.c0[k]);
-                        }
-                        if (units.has1 >> k & 1) {
-                            vg[j][k][1] = *reinterpret_cast<const Vec*>(g + units.c1[k]);
-                            vx[j][k][1] = *reinterpret_cast<const Vec*>(x + units.c1[k]);
-                        }
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    hd_floats<T, kV>(g[k][i], raw_g.v[k][i]);
+                    hd_floats<T, kV>(x[k][i], raw_x.v[k][i]);
                 }
-                t += dt;
-                h += dh;
-                if (h >= heads) {
-                    h -= heads;
-                    ++t;
+                if (units.turns >> k & 1) hd_turn<kV, kNeighbours>(g[k], sines, units.at[k], turned);
+                if (!(units.has1 >> k & 1))
+#pragma unroll
+                    for (int e = 0; e < kV; ++e) g[k][1][e] = 0.f;   // (turned by what no pair has)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float h[kV];
+                    hd_mul<kV>(h, g[k][i], wt[i]);
+                    hd_add_products<kV>(squares, x[k][i], x[k][i]);
+                    hd_add_products<kV>(alongs, h, x[k][i]);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                float g[kUnits][2][kV], x[kUnits][2][kV], squares = 0.f, along = 0.f;
+            float square = squares[0] + squares[1], along = alongs[0] + alongs[1];
+            __syncwarp();
+            for (int d = 1; d < lanes; d <<= 1) {
+                square += __shfl_xor_sync(0xffffffffu, square, d);
+                along += __shfl_xor_sync(0xffffffffu, along, d);
+            }
+            const float by = rsqrtf(square * inv_D + a.eps), less = -along * inv_D * by * by;
+            if (at.there()) {
+                T* y = rows[at.t].y + at.h * r.ys[w][1];
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < kV; ++e) {
-                            const bool there = at_t[j] >= 0 && ((i ? units.has1 : units.has0) >> k & 1);
-                            g[k][i][e] = there ? rt_get(vg[j][k][i].v[e]) : 0.f;
-                            x[k][i][e] = there ? rt_get(vx[j][k][i].v[e]) : 0.f;
-                        }
-                    if (at_t[j] >= 0 && (units.turns >> k & 1)) hd_turn<kV, kNeighbours>(g[k], cs + at_t[j] * (turned * kV), units.at[k], turned);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < kV; ++e) {
-                            if (!((i ? units.has1 : units.has0) >> k & 1)) g[k][i][e] = 0.f;   // (turned by what no pair has)
-                            squares = fmaf(x[k][i][e], x[k][i][e], squares);
-                            along = fmaf(g[k][i][e] * weight[k][i][e], x[k][i][e], along);
-                        }
-                }
-                for (int d = 1; d < lanes; d <<= 1) {
-                    squares += __shfl_xor_sync(0xffffffffu, squares, d);
-                    along += __shfl_xor_sync(0xffffffffu, along, d);
-                }
-                const float by = rsqrtf(squares * inv_D + a.eps), less = along * inv_D * by * by;
-                if (at_t[j] < 0) continue;
-                T* y = rows[at_t[j]].y + at_h[j] * r.ys[w][1];
-#pragma unroll
-                for (int k = 0; k < kUnits; ++k)
+                    float wt[2][kV];
+                    hd_weight<kV>(wt, ws, units.at[k], n_units);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (!((i ? units.has1 : units.has0) >> k & 1)) continue;
-                        Vec z;
-#pragma unroll
-                        for (int e = 0; e < kV; ++e) {
-                            dw[k][i][e] = fmaf(g[k][i][e], x[k][i][e] * by, dw[k][i][e]);
-                            z.v[e] = rt_put<T>(by * (g[k][i][e] * weight[k][i][e] - x[k][i][e] * less));
-                        }
-                        *reinterpret_cast<Vec*>(y + (i ? units.c1[k] : units.c0[k])) = z;
+                        float unit[kV], h[kV];
+                        hd_mul<kV>(unit, x[k][i], by);
+                        hd_fma<kV>(dw[k][i], g[k][i], unit, dw[k][i]);
+                        hd_mul<kV>(h, g[k][i], wt[i]);
+                        hd_fma<kV>(h, x[k][i], less, h);
+                        hd_mul<kV>(h, h, by);
+                        *reinterpret_cast<RtVec<T, kV>*>(y + (i ? units.c1[k] : units.c0[k])) = hd_rounded<T, kV>(h);
                     }
+                }
             }
+            raw_g = next_g;
+            raw_x = next_x;
+            at = then;
         }
     }
     // the rows of a warp, then the warps
+    const HdUnits<kV, kUnits, kNeighbours>& units = all_units;
     float* sums = reinterpret_cast<float*>(sm);   // [kWarps][D]
     __syncthreads();
 #pragma unroll
@@ -434,12 +574,12 @@ static cudaError_t launch_heads(const NormRotaryArgs& a, int interleaved, cudaSt
     int log_lanes;
     hd_lanes(hd_units_of_row(a.r.D, a.r.R, kV), kUnits, &log_lanes);
     const int turned = (a.r.R / 2 + kV - 1) / kV, heads = a.r.heads[0] + a.r.heads[1] * (kAppend ? 2 : 1);
-    const size_t token = (size_t)turned * kV * sizeof(float2) + (kAppend ? 3 * 32 : 2 * 16);
+    const size_t token = (size_t)turned * kV * sizeof(float2) + (kAppend ? 3 * 32 : 2 * 16), weights = kNorm ? (size_t)(kUnits << log_lanes) * kV * 16 : 0;
     const long long n_tok = (long long)a.r.B * a.r.S;
-    const int per = hd_tokens(n_tok, heads, kHeadThreads >> log_lanes, token, 3LL * sm_count());
+    const int per = hd_tokens(n_tok, heads, kHeadThreads >> log_lanes, token, (long long)hd_ctas_per_sm(kUnits) * sm_count());
     LaunchScope ls(kAppend ? K_CACHE_APPEND_ROTARY : K_NORM_ROTARY, st);
     auto go = [&](auto kernel) {
-        return launch_overlapped(kernel, (unsigned)((n_tok + per - 1) / per), kHeadThreads, per * token, st, a, per, log_lanes, 2.f / (float)a.r.R);
+        return launch_overlapped(kernel, (unsigned)((n_tok + per - 1) / per), kHeadThreads, weights + per * token, st, a, per, log_lanes);
     };
     return interleaved ? go(heads_kernel<Tin, Tout, kV, kUnits, true, kNorm, kAppend>) : go(heads_kernel<Tin, Tout, kV, kUnits, false, kNorm, kAppend>);
 }
@@ -484,7 +624,6 @@ cudaError_t cache_append_rotary(const NormRotaryArgs& a, int bf16, int interleav
 }
 
 // CTAs of the gradient: what the SMs hold at once, shared out by the heads; fewer where there are not rows for them.
-constexpr int kBackCtas = 2;   // per SM
 static void hd_ctas(const NormRotaryArgs& a, int (&ctas)[2]) {
     const long long n_tok = (long long)a.r.B * a.r.S, all = (long long)sm_count() * kBackCtas, heads = a.r.heads[0] + a.r.heads[1];
     for (int i = 0; i < 2; ++i) {
@@ -508,10 +647,10 @@ static cudaError_t launch_heads_back(const NormRotaryArgs& a, int interleaved, f
     int per = 4 * groups / most;
     const int fits = (int)(27 * 1024 / token);
     per = per > fits ? fits : per < 1 ? 1 : per;
-    const size_t smem = per * token > sums ? per * token : sums;
+    const size_t tables = per * token + (size_t)(kUnits << log_lanes) * kV * 8, smem = tables > sums ? tables : sums;
     LaunchScope ls(K_NORM_ROTARY_BWD, st);
     auto go = [&](auto kernel) {
-        return launch_overlapped(kernel, (unsigned)(ctas[0] + ctas[1]), kHeadThreads, smem, st, a, per, log_lanes, 2.f / (float)a.r.R, ctas[0], partial);
+        return launch_overlapped(kernel, (unsigned)(ctas[0] + ctas[1]), kHeadThreads, smem, st, a, per, log_lanes, ctas[0], partial);
     };
     return interleaved ? go(heads_backward_kernel<T, kV, kUnits, true>) : go(heads_backward_kernel<T, kV, kUnits, false>);
 }
