@@ -13,7 +13,7 @@ namespace ttk {
 using namespace sm100;
 
 constexpr int kHeadThreads = 256;
-constexpr int hd_ctas_per_sm(int units) { return units == 1 ? 4 : 2; }
+constexpr int hd_ctas_per_sm(int kV, int units) { return units > 1 ? 2 : kV == 8 ? 3 : 4; }
 constexpr int kBackCtas = 2;   // per SM, of the gradient
 
 // A token's rows of one of the tensors, of head 0: where they come from, where they go, and for keys on their way into a cache a second place.
@@ -28,34 +28,31 @@ struct alignas(16) HdRows3 {
     Tout *y, *also;
 };
 
-// A lane's units of a row: unit u turns for u < turned, channels c0 .. and c1 .., each there or not.
-template <int kV, int kUnits, bool kNeighbours>
+// A lane's units of a row: unit u turns for u < turned, channels c0 .. and c1 .., each there or not.  kWhole: all are there.
+template <int kV, int kUnits, bool kNeighbours, bool kWhole>
 struct HdUnits {
     int c0[kUnits], c1[kUnits], at[kUnits];
-    unsigned has0, has1, turns;   // a bit per unit
-    __device__ __forceinline__ HdUnits(int lane, int lanes, int D, int R) : has0(0), has1(0), turns(0) {
+    unsigned there[2], turning;   // a bit per unit
+    __device__ __forceinline__ HdUnits(int lane, int lanes, int D, int R) : there{0, 0}, turning(0) {
         const int turned = (R / 2 + kV - 1) / kV;
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
             const int u = lane + k * lanes;
+            const bool turn = u < turned;
             at[k] = u;
-            if (u < turned) {
-                turns |= 1u << k;
-                has0 |= 1u << k;
-                c0[k] = kNeighbours ? 2 * u * kV : u * kV;
-                c1[k] = kNeighbours ? c0[k] + kV : c0[k] + R / 2;
-                if (c1[k] < R) has1 |= 1u << k;
-            } else {
-                c0[k] = R + 2 * (u - turned) * kV;
-                c1[k] = c0[k] + kV;
-                if (c0[k] < D) has0 |= 1u << k;
-                if (c1[k] < D) has1 |= 1u << k;
-            }
+            c0[k] = !turn ? R + 2 * (u - turned) * kV : kNeighbours ? 2 * u * kV : u * kV;
+            c1[k] = turn && !kNeighbours ? c0[k] + R / 2 : c0[k] + kV;
+            if (turn) turning |= 1u << k;
+            if (c0[k] < D) there[0] |= 1u << k;
+            if (c1[k] < (turn ? R : D)) there[1] |= 1u << k;
         }
     }
+    __device__ __forceinline__ int channel(int k, int chunk) const { return chunk ? c1[k] : c0[k]; }
+    __device__ __forceinline__ bool has(int k, int chunk) const { return kWhole || (there[chunk] >> k & 1); }
+    __device__ __forceinline__ bool turns(int k) const { return turning >> k & 1; }
     // The flags differ among the lanes of a row, which meet in every turn of a loop: they are made unknown to the compiler in each, so that it cannot make
     // loops of their own for lanes with one and with another.
-    __device__ __forceinline__ void forget() { asm volatile("" : "+r"(has0), "+r"(has1), "+r"(turns)); }
+    __device__ __forceinline__ void forget() { asm volatile("" : "+r"(there[0]), "+r"(there[1]), "+r"(turning)); }
 };
 
 // Tables in shared memory lie as the lanes of a row read them, 16 bytes of one unit beside the same of the next, so that a read is whole banks.
@@ -114,17 +111,17 @@ __device__ __forceinline__ void hd_turn(float (&x)[2][kV], const float* cs, int 
         }
     }
 }
-// The weights of a tensor, up to 4 channels of a chunk of a unit at a time; 0 for channels that are not there.
-template <int kV>
-__device__ __forceinline__ void hd_weights(float* ws, const void* w, int bf16, int n_units, int D, int R, bool neighbours, int tid) {
+// The weights of a tensor, up to 4 channels of a chunk of a unit at a time.  What no channel has stays as it is.
+template <int kV, bool kNeighbours>
+__device__ __forceinline__ void hd_weights(float* ws, const void* w, int bf16, int n_units, int D, int R, int tid) {
     constexpr int kQuad = kV < 4 ? kV : 4;
     const int turned = (R / 2 + kV - 1) / kV;
-    for (int i = tid; i < n_units * 2 * kV; i += kHeadThreads) {
-        const int in = i % kQuad, u = i / kQuad % n_units, m = i / kQuad / n_units, chunk = m / (kV / kQuad), e = m % (kV / kQuad) * kQuad + in;
-        const bool turn = u < turned;
-        const int c0 = !turn ? R + 2 * (u - turned) * kV : neighbours ? 2 * u * kV : u * kV, c = (chunk == 0 ? c0 : turn && !neighbours ? c0 + R / 2 : c0 + kV) + e;
-        const bool there = c < (turn ? R : D);
-        ws[i] = !there ? 0.f : bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[c]) : static_cast<const float*>(w)[c];
+    for (int c = tid; c < D; c += kHeadThreads) {
+        const bool paired = !kNeighbours && c < R;   // in halves
+        const int in = paired ? (c < R / 2 ? c : c - R / 2) : c < R ? c : c - R;   // (of the chunks, or of those behind R)
+        const int chunk = paired ? c >= R / 2 : in / kV & 1, u = (paired ? in / kV : in / (2 * kV)) + (c < R ? 0 : turned), e = in % kV;
+        ws[((chunk * (kV / kQuad) + e / kQuad) * n_units + u) * kQuad + e % kQuad] =
+            bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[c]) : static_cast<const float*>(w)[c];
     }
 }
 template <int kV>
@@ -217,7 +214,7 @@ __device__ __forceinline__ void hd_fma(float (&y)[kV], const float (&a)[kV], flo
     for (int e = 0; e < kV; ++e) bs[e] = b;
     hd_fma<kV>(y, a, bs, c);
 }
-// What a lane has of a row, as it comes; nothing where there is no row
+// What a lane has of a row, as it comes; 0 for channels that are not there
 template <typename T, int kV, int kUnits>
 struct HdRaw {
     RtVec<T, kV> v[kUnits][2];
@@ -227,13 +224,17 @@ struct HdRaw {
         for (int k = 0; k < kUnits; ++k)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
+                if (units.has(k, i)) {
+                    v[k][i] = *reinterpret_cast<const RtVec<T, kV>*>(x + units.channel(k, i));
+                } else {
 #pragma unroll
-                for (int e = 0; e < kV; ++e) v[k][i].v[e] = rt_put<T>(0.f);
-                if (x && ((i ? units.has1 : units.has0) >> k & 1)) v[k][i] = *reinterpret_cast<const RtVec<T, kV>*>(x + (i ? units.c1[k] : units.c0[k]));
+                    for (int e = 0; e < kV; ++e) v[k][i].v[e] = rt_put<T>(0.f);
+                }
             }
     }
 };
-// A walk of a group of lanes over the rows (token, head) of a tile, as many apart as there are groups.  Every group takes as many turns, some of the last without a row.
+// A walk of a group of lanes over the rows (token, head) of a tile, as many apart as there are groups.  Every group takes as many turns; where there is no row
+// left it takes the tile's first one, for nothing.
 struct HdWalk {
     int t, h, dt, dh, heads, row, total, apart;
     __device__ __forceinline__ HdWalk(int group, int groups, int n_heads, int tokens) : heads(n_heads), row(group), total(tokens * n_heads), apart(groups) {
@@ -241,9 +242,13 @@ struct HdWalk {
         h = group - t * n_heads;
         dt = groups / n_heads;
         dh = groups - dt * n_heads;
+        stay();
     }
     __device__ __forceinline__ int turns() const { return (total + apart - 1) / apart; }
     __device__ __forceinline__ bool there() const { return row < total; }
+    __device__ __forceinline__ void stay() {
+        if (!there()) t = h = 0;
+    }
     __device__ __forceinline__ void next() {
         row += apart;
         t += dt;
@@ -252,82 +257,95 @@ struct HdWalk {
             h -= heads;
             ++t;
         }
+        stay();
     }
 };
+// A CTA's tokens of n: equal shares.
+__device__ __forceinline__ unsigned hd_share(unsigned n, unsigned cta, unsigned ctas) { return (unsigned)((unsigned long long)n * cta / ctas); }
 
-// blockDim = kHeadThreads; 2^log_lanes lanes to a row.  kAppend: keys and values go into the pools' rows (a third tensor, which is copied).
-template <typename Tin, typename Tout, int kV, int kUnits, bool kNeighbours, bool kNorm, bool kAppend>
-__global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kUnits)) heads_kernel(const NormRotaryArgs a, int tokens_per_cta, int log_lanes) {
+// blockDim = kHeadThreads; 2^log_lanes lanes to a row.  A CTA goes through its tokens tile by tile; the next tile's sines are made before the rows of the one at
+// hand.  kAppend: keys and values go into the pools' rows (a third tensor, which is copied).
+template <typename Tin, typename Tout, int kV, int kUnits, bool kNeighbours, bool kNorm, bool kAppend, bool kWhole>
+__global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kV, kUnits)) heads_kernel(const NormRotaryArgs a, int tile_tokens, int log_lanes) {
     using Out = RtVec<Tout, kV>;
+    using Raw = HdRaw<Tin, kV, kUnits>;
     using Rows = typename std::conditional<kAppend, HdRows3<Tin, Tout>, HdRows<Tin, Tout>>::type;
     constexpr int kTensors = kAppend ? 3 : 2;
     extern __shared__ float4 sm[];
     const RotaryArgs& r = a.r;
     const int tid = threadIdx.x, lanes = 1 << log_lanes, lane = tid & (lanes - 1), group = tid >> log_lanes, groups = kHeadThreads >> log_lanes;
-    const int turned = (r.R / 2 + kV - 1) / kV, n_units = lanes * kUnits;
-    Rows* rows = reinterpret_cast<Rows*>(sm);   // [tokens_per_cta][kTensors]
-    float* ws = reinterpret_cast<float*>(rows + kTensors * tokens_per_cta);   // [2][n_units * 2 * kV]
-    float* cs = ws + (kNorm ? 4 * n_units * kV : 0);                          // [tokens_per_cta][2 * turned * kV]
-    const unsigned t0 = blockIdx.x * (unsigned)tokens_per_cta, n_tok = (unsigned)r.B * (unsigned)r.S;
-    const int here = (int)min((unsigned)tokens_per_cta, n_tok - t0);
-    const RtPlaces places(t0, r.B, r.S);
-    const HdUnits<kV, kUnits, kNeighbours> all_units(lane, lanes, r.D, r.R);
+    const int turned = (r.R / 2 + kV - 1) / kV, n_units = lanes * kUnits, tile_sines = tile_tokens * (2 * turned * kV);
+    Rows* all_rows = reinterpret_cast<Rows*>(sm);                                     // [2][tile_tokens][kTensors]
+    float* ws = reinterpret_cast<float*>(all_rows + 2 * kTensors * tile_tokens);      // [2][n_units * 2 * kV]
+    float* all_cs = ws + (kNorm ? 4 * n_units * kV : 0);                              // [2][tile_tokens][2 * turned * kV]
+    const unsigned n_tok = (unsigned)r.B * (unsigned)r.S, first = hd_share(n_tok, blockIdx.x, gridDim.x), last = hd_share(n_tok, blockIdx.x + 1, gridDim.x);
+    const HdUnits<kV, kUnits, kNeighbours, kWhole> all_units(lane, lanes, r.D, r.R);
     grid_let_next_start();
     grid_wait_for_previous();
-    hd_sines<kV, kNeighbours>(cs, r, places, here, tid);
-    for (int i = kHeadThreads - 1 - tid; i < kTensors * here; i += kHeadThreads) {
-        const int t = i / kTensors, w = i - t * kTensors;
-        int b, s;
-        places.at(t, &b, &s);
-        if constexpr (kAppend) {
-            Rows z{};
-            if (w == 0) {
-                z.x = (const Tin*)r.x[0] + s * r.xs[0][2];
-                z.y = (Tout*)r.y[0] + s * r.ys[0][2];
-            } else {
-                z.x = w == 1 ? (const Tin*)r.x[1] + s * r.xs[1][2] : (const Tin*)a.v + s * a.v_stride[0];
-                if (w == 1 && r.y[1]) z.also = (Tout*)r.y[1] + s * r.ys[1][2];
-                const int slot = a.slots[s];
-                if (slot >= 0 && slot < a.n_slots) {
-                    const int page = slot / a.page;
-                    z.y = (Tout*)a.pool[w - 1] + ((long long)page * r.heads[1] * a.page + (slot - page * a.page)) * r.D;
+    auto tile_of = [&](unsigned t0) { return (int)min((unsigned)tile_tokens, last - t0); };
+    auto prepare = [&](unsigned t0, int which) {
+        const int here = tile_of(t0);
+        const RtPlaces places(t0, r.B, r.S);
+        hd_sines<kV, kNeighbours>(all_cs + which * tile_sines, r, places, here, tid);
+        Rows* rows = all_rows + which * (kTensors * tile_tokens);
+        for (int i = kHeadThreads - 1 - tid; i < kTensors * here; i += kHeadThreads) {
+            const int t = i / kTensors, w = i - t * kTensors;
+            int b, s;
+            places.at(t, &b, &s);
+            if constexpr (kAppend) {
+                Rows z{};
+                if (w == 0) {
+                    z.x = (const Tin*)r.x[0] + s * r.xs[0][2];
+                    z.y = (Tout*)r.y[0] + s * r.ys[0][2];
+                } else {
+                    z.x = w == 1 ? (const Tin*)r.x[1] + s * r.xs[1][2] : (const Tin*)a.v + s * a.v_stride[0];
+                    if (w == 1 && r.y[1]) z.also = (Tout*)r.y[1] + s * r.ys[1][2];
+                    const int slot = a.slots[s];
+                    if (slot >= 0 && slot < a.n_slots) {
+                        const int page = slot / a.page;
+                        z.y = (Tout*)a.pool[w - 1] + ((long long)page * r.heads[1] * a.page + (slot - page * a.page)) * r.D;
+                    }
                 }
+                rows[i] = z;
+            } else {
+                rows[i] = Rows{(const Tin*)r.x[w] + b * r.xs[w][0] + s * r.xs[w][2], (Tout*)r.y[w] + b * r.ys[w][0] + s * r.ys[w][2]};
             }
-            rows[i] = z;
-        } else {
-            rows[i] = Rows{(const Tin*)r.x[w] + b * r.xs[w][0] + s * r.xs[w][2], (Tout*)r.y[w] + b * r.ys[w][0] + s * r.ys[w][2]};
         }
-    }
+    };
+    prepare(first, 0);
     if (kNorm) {
+        if (!kWhole) {
+            for (int i = tid; i < 4 * n_units * kV; i += kHeadThreads) ws[i] = 0.f;
+            __syncthreads();
+        }
         for (int w = 0; w < 2; ++w)
-            if (r.heads[w]) hd_weights<kV>(ws + w * (2 * n_units * kV), a.w[w], a.w_bf16, n_units, r.D, r.R, kNeighbours, tid);
+            if (r.heads[w]) hd_weights<kV, kNeighbours>(ws + w * (2 * n_units * kV), a.w[w], a.w_bf16, n_units, r.D, r.R, tid);
     }
     __syncthreads();
     const float inv_D = 1.f / (float)r.D;
-#pragma unroll 1
-    for (int w = 0; w < kTensors; ++w) {
-        const int heads = w < 2 ? r.heads[w] : r.heads[1];
-        if (heads == 0) continue;
-        const bool moved = kAppend && w == 2;   // as it is
-        const long long x_head = moved ? a.v_stride[1] : r.xs[w][1], y_head = kAppend && w > 0 ? (long long)a.page * r.D : r.ys[w][1], also_head = r.ys[1][1];
-        const float* weights = ws + w * (2 * n_units * kV);
-        HdWalk at(group, groups, heads, here);
-        const int turns = at.turns();
-        HdRaw<Tin, kV, kUnits> raw, next;
-        auto fetch = [&](HdRaw<Tin, kV, kUnits>& to, const HdWalk& from) { to.load(from.there() ? rows[kTensors * from.t + w].x + from.h * x_head : nullptr, all_units); };
-        fetch(raw, at);
-        for (int turn = 0; turn < turns; ++turn) {
-            HdUnits<kV, kUnits, kNeighbours> units = all_units;
+    const int up_to_k = r.heads[0], up_to_v = r.heads[0] + r.heads[1], heads = up_to_v + (kAppend ? r.heads[1] : 0);
+    int which = 0;
+    for (unsigned t0 = first; t0 < last; t0 += tile_tokens, which ^= 1) {
+        if (last - t0 > (unsigned)tile_tokens) prepare(t0 + tile_tokens, which ^ 1);
+        const Rows* rows = all_rows + which * (kTensors * tile_tokens);
+        const float* cs = all_cs + which * tile_sines;
+        HdWalk at(group, groups, heads, tile_of(t0));
+        auto tensor = [&](const HdWalk& x) { return x.h < up_to_k ? 0 : !kAppend || x.h < up_to_v ? 1 : 2; };
+        auto fetch = [&](Raw& to, const HdWalk& x) {
+            const int w = tensor(x), h = x.h - (w == 0 ? 0 : w == 1 ? up_to_k : up_to_v);
+            to.load(rows[kTensors * x.t + w].x + h * (kAppend && w == 2 ? a.v_stride[1] : w ? r.xs[1][1] : r.xs[0][1]), all_units);
+        };
+        auto work = [&](const Raw& raw, const HdWalk& x_at) {
+            HdUnits<kV, kUnits, kNeighbours, kWhole> units = all_units;
             units.forget();
-            HdWalk then = at;
-            then.next();
-            fetch(next, then);
+            const int w = tensor(x_at);
+            const bool moved = kAppend && w == 2;   // as it is
             float x[kUnits][2][kV];
 #pragma unroll
             for (int k = 0; k < kUnits; ++k)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) hd_floats<Tin, kV>(x[k][i], raw.v[k][i]);
-            if (kNorm && !moved) {
+            if (kNorm) {
                 float sums[2] = {0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k)
@@ -336,43 +354,59 @@ __global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kUnits)) heads_ke
                 float sum = sums[0] + sums[1];
                 __syncwarp();
                 for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                const float by = rsqrtf(sum * inv_D + a.eps);
+                if (!moved) {
+                    const float by = rsqrtf(sum * inv_D + a.eps);
+                    const float* weights = ws + w * (2 * n_units * kV);
 #pragma unroll
-                for (int k = 0; k < kUnits; ++k) {
-                    float wt[2][kV];
-                    hd_weight<kV>(wt, weights, units.at[k], n_units);
+                    for (int k = 0; k < kUnits; ++k) {
+                        float wt[2][kV];
+                        hd_weight<kV>(wt, weights, units.at[k], n_units);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        hd_mul<kV>(wt[i], wt[i], by);
-                        hd_mul<kV>(x[k][i], x[k][i], wt[i]);
+                        for (int i = 0; i < 2; ++i) {
+                            hd_mul<kV>(wt[i], wt[i], by);
+                            hd_mul<kV>(x[k][i], x[k][i], wt[i]);
+                        }
                     }
                 }
             }
-            if (at.there()) {
-                const Rows& row = rows[kTensors * at.t + w];
+            if (x_at.there()) {
+                const Rows& row = rows[kTensors * x_at.t + w];
+                const int h = x_at.h - (w == 0 ? 0 : w == 1 ? up_to_k : up_to_v);
                 Tout* y = row.y;
-                if (!kAppend || y) y += at.h * y_head;
+                if (!kAppend || y) y += h * (w == 0 ? r.ys[0][1] : kAppend ? (long long)a.page * r.D : r.ys[1][1]);
                 Tout* also = nullptr;
                 if constexpr (kAppend) {
-                    if (row.also) also = row.also + at.h * also_head;
+                    if (row.also) also = row.also + h * r.ys[1][1];
                 }
-                const float* sines = cs + at.t * (2 * turned * kV);
+                const float* sines = cs + x_at.t * (2 * turned * kV);
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k) {
-                    if (!moved && (units.turns >> k & 1)) hd_turn<kV, kNeighbours>(x[k], sines, units.at[k], turned);
+                    if (!moved && units.turns(k)) hd_turn<kV, kNeighbours>(x[k], sines, units.at[k], turned);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        if (!((i ? units.has1 : units.has0) >> k & 1)) continue;
+                        if (!units.has(k, i)) continue;
                         const Out z = hd_rounded<Tout, kV>(x[k][i]);
-                        const int c = i ? units.c1[k] : units.c0[k];
-                        if (!kAppend || y) *reinterpret_cast<Out*>(y + c) = z;
-                        if (kAppend && also) *reinterpret_cast<Out*>(also + c) = z;
+                        if (!kAppend || y) *reinterpret_cast<Out*>(y + units.channel(k, i)) = z;
+                        if (kAppend && also) *reinterpret_cast<Out*>(also + units.channel(k, i)) = z;
                     }
                 }
             }
-            raw = next;
+        };
+        // a row is loaded ahead of the one at hand
+        const int turns = at.turns();
+        Raw one, two;
+        fetch(one, at);
+        for (int turn = 0; turn < turns; turn += 2) {
+            HdWalk then = at;
+            then.next();
+            fetch(two, then);
+            work(one, at);
             at = then;
+            at.next();
+            fetch(one, at);
+            work(two, then);
         }
+        __syncthreads();   // the tables of the next tile are there, those of this one read
     }
 }
 
@@ -383,23 +417,24 @@ struct alignas(16) HdRowsBack {
     const T *g, *x;
     T* y;
 };
-template <typename T, int kV, int kUnits, bool kNeighbours>
-__global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel(const NormRotaryArgs a, int tokens_per_tile, int log_lanes, int ctas_q, float* partial) {
+template <typename T, int kV, int kUnits, bool kNeighbours, bool kWhole>
+__global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel(const NormRotaryArgs a, int tile_tokens, int log_lanes, int ctas_q, float* partial) {
     using Rows = HdRowsBack<T>;
     using Raw = HdRaw<T, kV, kUnits>;
     constexpr int kWarps = kHeadThreads / 32;
     extern __shared__ float4 sm[];
     const RotaryArgs& r = a.r;
     const int tid = threadIdx.x, lanes = 1 << log_lanes, lane = tid & (lanes - 1), group = tid >> log_lanes, groups = kHeadThreads >> log_lanes;
-    const int turned = (r.R / 2 + kV - 1) / kV, n_units = lanes * kUnits;
-    Rows* rows = reinterpret_cast<Rows*>(sm);                       // [tokens_per_tile]
-    float* ws = reinterpret_cast<float*>(rows + tokens_per_tile);   // [n_units * 2 * kV]
-    float* cs = ws + 2 * n_units * kV;                              // [tokens_per_tile][2 * turned * kV]
+    const int turned = (r.R / 2 + kV - 1) / kV, n_units = lanes * kUnits, tile_sines = tile_tokens * (2 * turned * kV);
+    Rows* all_rows = reinterpret_cast<Rows*>(sm);                          // [2][tile_tokens]
+    float* ws = reinterpret_cast<float*>(all_rows + 2 * tile_tokens);      // [n_units * 2 * kV]
+    float* all_cs = ws + 2 * n_units * kV;                                 // [2][tile_tokens][2 * turned * kV]
     const int w = (int)blockIdx.x >= ctas_q, cta = (int)blockIdx.x - (w ? ctas_q : 0), n_cta = w ? (int)gridDim.x - ctas_q : ctas_q;
     const int heads = r.heads[w];
-    const unsigned n_tok = (unsigned)r.B * (unsigned)r.S, tiles = (n_tok + tokens_per_tile - 1) / tokens_per_tile;
-    const HdUnits<kV, kUnits, kNeighbours> all_units(lane, lanes, r.D, r.R);
+    const unsigned n_tok = (unsigned)r.B * (unsigned)r.S, first = hd_share(n_tok, cta, n_cta), last = hd_share(n_tok, cta + 1, n_cta);
+    const HdUnits<kV, kUnits, kNeighbours, kWhole> all_units(lane, lanes, r.D, r.R);
     const float inv_D = 1.f / (float)r.D;
+    const long long g_head = r.xs[w][1], x_head = a.in_stride[w][1], y_head = r.ys[w][1];
     float dw[kUnits][2][kV];
 #pragma unroll
     for (int k = 0; k < kUnits; ++k)
@@ -407,36 +442,40 @@ __global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel
         for (int e = 0; e < kV; ++e) dw[k][0][e] = dw[k][1][e] = 0.f;
     grid_let_next_start();
     grid_wait_for_previous();
-    hd_weights<kV>(ws, a.w[w], a.w_bf16, n_units, r.D, r.R, kNeighbours, tid);
-    for (unsigned tile = cta; tile < tiles; tile += n_cta) {
-        const unsigned t0 = tile * tokens_per_tile;
-        const int here = (int)min((unsigned)tokens_per_tile, n_tok - t0);
+    auto tile_of = [&](unsigned t0) { return (int)min((unsigned)tile_tokens, last - t0); };
+    auto prepare = [&](unsigned t0, int which) {
+        const int here = tile_of(t0);
         const RtPlaces places(t0, r.B, r.S);
-        __syncthreads();   // the tile before has been read
-        hd_sines<kV, kNeighbours>(cs, r, places, here, tid);
+        hd_sines<kV, kNeighbours>(all_cs + which * tile_sines, r, places, here, tid);
         for (int t = kHeadThreads - 1 - tid; t < here; t += kHeadThreads) {
             int b, s;
             places.at(t, &b, &s);
-            rows[t] = Rows{(const T*)r.x[w] + b * r.xs[w][0] + s * r.xs[w][2], (const T*)a.in[w] + b * a.in_stride[w][0] + s * a.in_stride[w][2],
-                           (T*)r.y[w] + b * r.ys[w][0] + s * r.ys[w][2]};
+            all_rows[which * tile_tokens + t] = Rows{(const T*)r.x[w] + b * r.xs[w][0] + s * r.xs[w][2], (const T*)a.in[w] + b * a.in_stride[w][0] + s * a.in_stride[w][2],
+                                                     (T*)r.y[w] + b * r.ys[w][0] + s * r.ys[w][2]};
         }
+    };
+    prepare(first, 0);
+    if (!kWhole) {
+        for (int i = tid; i < 2 * n_units * kV; i += kHeadThreads) ws[i] = 0.f;
         __syncthreads();
-        HdWalk at(group, groups, heads, here);
-        const int turns = at.turns();
-        Raw raw_g, raw_x, next_g, next_x;
+    }
+    hd_weights<kV, kNeighbours>(ws, a.w[w], a.w_bf16, n_units, r.D, r.R, tid);
+    __syncthreads();
+    int which = 0;
+    for (unsigned t0 = first; t0 < last; t0 += tile_tokens, which ^= 1) {
+        if (last - t0 > (unsigned)tile_tokens) prepare(t0 + tile_tokens, which ^ 1);
+        const Rows* rows = all_rows + which * tile_tokens;
+        const float* cs = all_cs + which * tile_sines;
+        HdWalk at(group, groups, heads, tile_of(t0));
         auto fetch = [&](Raw& g, Raw& x, const HdWalk& from) {
-            g.load(from.there() ? rows[from.t].g + from.h * r.xs[w][1] : nullptr, all_units);
-            x.load(from.there() ? rows[from.t].x + from.h * a.in_stride[w][1] : nullptr, all_units);
+            g.load(rows[from.t].g + from.h * g_head, all_units);
+            x.load(rows[from.t].x + from.h * x_head, all_units);
         };
-        fetch(raw_g, raw_x, at);
-        for (int turn = 0; turn < turns; ++turn) {
-            HdUnits<kV, kUnits, kNeighbours> units = all_units;
+        auto work = [&](const Raw& raw_g, const Raw& raw_x, const HdWalk& from) {
+            HdUnits<kV, kUnits, kNeighbours, kWhole> units = all_units;
             units.forget();
-            HdWalk then = at;
-            then.next();
-            fetch(next_g, next_x, then);
             float g[kUnits][2][kV], x[kUnits][2][kV], squares[2] = {0.f, 0.f}, alongs[2] = {0.f, 0.f};
-            const float* sines = cs + (at.there() ? at.t : 0) * (2 * turned * kV);
+            const float* sines = cs + from.t * (2 * turned * kV);
 #pragma unroll
             for (int k = 0; k < kUnits; ++k) {
                 float wt[2][kV];
@@ -446,8 +485,8 @@ __global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel
                     hd_floats<T, kV>(g[k][i], raw_g.v[k][i]);
                     hd_floats<T, kV>(x[k][i], raw_x.v[k][i]);
                 }
-                if (units.turns >> k & 1) hd_turn<kV, kNeighbours>(g[k], sines, units.at[k], turned);
-                if (!(units.has1 >> k & 1))
+                if (units.turns(k)) hd_turn<kV, kNeighbours>(g[k], sines, units.at[k], turned);
+                if (!units.has(k, 1))
 #pragma unroll
                     for (int e = 0; e < kV; ++e) g[k][1][e] = 0.f;   // (turned by what no pair has)
 #pragma unroll
@@ -465,34 +504,43 @@ __global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel
                 along += __shfl_xor_sync(0xffffffffu, along, d);
             }
             const float by = rsqrtf(square * inv_D + a.eps), less = -along * inv_D * by * by;
-            if (at.there()) {
-                T* y = rows[at.t].y + at.h * r.ys[w][1];
+            if (from.there()) {
+                T* y = rows[from.t].y + from.h * y_head;
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k) {
                     float wt[2][kV];
                     hd_weight<kV>(wt, ws, units.at[k], n_units);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        if (!((i ? units.has1 : units.has0) >> k & 1)) continue;
+                        if (!units.has(k, i)) continue;
                         float unit[kV], h[kV];
                         hd_mul<kV>(unit, x[k][i], by);
                         hd_fma<kV>(dw[k][i], g[k][i], unit, dw[k][i]);
                         hd_mul<kV>(h, g[k][i], wt[i]);
                         hd_fma<kV>(h, x[k][i], less, h);
                         hd_mul<kV>(h, h, by);
-                        *reinterpret_cast<RtVec<T, kV>*>(y + (i ? units.c1[k] : units.c0[k])) = hd_rounded<T, kV>(h);
+                        *reinterpret_cast<RtVec<T, kV>*>(y + units.channel(k, i)) = hd_rounded<T, kV>(h);
                     }
                 }
             }
-            raw_g = next_g;
-            raw_x = next_x;
+        };
+        const int turns = at.turns();
+        Raw one[2], two[2];
+        fetch(one[0], one[1], at);
+        for (int turn = 0; turn < turns; turn += 2) {
+            HdWalk then = at;
+            then.next();
+            fetch(two[0], two[1], then);
+            work(one[0], one[1], at);
             at = then;
+            at.next();
+            fetch(one[0], one[1], at);
+            work(two[0], two[1], then);
         }
+        __syncthreads();   // the tables of the next tile are there, those of this one read
     }
     // the rows of a warp, then the warps
-    const HdUnits<kV, kUnits, kNeighbours>& units = all_units;
     float* sums = reinterpret_cast<float*>(sm);   // [kWarps][D]
-    __syncthreads();
 #pragma unroll
     for (int k = 0; k < kUnits; ++k)
 #pragma unroll
@@ -501,7 +549,7 @@ __global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel
             for (int e = 0; e < kV; ++e) {
                 float y = dw[k][i][e];
                 for (int d = lanes; d < 32; d <<= 1) y += __shfl_xor_sync(0xffffffffu, y, d);
-                if ((tid & 31) < lanes && ((i ? units.has1 : units.has0) >> k & 1)) sums[(tid >> 5) * r.D + (i ? units.c1[k] : units.c0[k]) + e] = y;
+                if ((tid & 31) < lanes && all_units.has(k, i)) sums[(tid >> 5) * r.D + all_units.channel(k, i) + e] = y;
             }
     __syncthreads();
     for (int c = tid; c < r.D; c += kHeadThreads) {
@@ -558,13 +606,14 @@ struct HdPlaces {
     int aligned(int most) const { return (int)((bits | most) & (0 - (bits | most))); }
 };
 
-// Tokens per CTA: four rows to each group of lanes, fewer where all CTAs are resident at once then.
-static int hd_tokens(long long n_tok, int heads, int groups, size_t token, long long resident) {
-    const long long one_wave = (n_tok + resident - 1) / resident;
-    long long per = 4LL * groups / heads;
-    if (per > one_wave || 3 * per >= 2 * one_wave) per = one_wave;
-    const long long fits = 27 * 1024 / (long long)token;
-    if (per > fits) per = fits;
+// Whether all of a row's lanes have two whole chunks of it.
+static bool hd_whole(int D, int R, int interleaved, int kV, int n_units) { return n_units * 2 * kV == D && R % (2 * kV) == 0 && (interleaved || R / 2 % kV == 0); }
+// Tokens per tile: rows for eight turns of every group of lanes, as many as the tables of two have room for.
+static int hd_tile(long long n_tok, long long ctas, int heads, int groups, size_t token) {
+    long long per = 8LL * groups / heads;
+    const long long fits = 12 * 1024 / (long long)token, share = (n_tok + ctas - 1) / ctas;
+    per = per > fits ? fits : per;
+    per = per > share ? share : per;
     return per < 1 ? 1 : (int)per;
 }
 
@@ -573,15 +622,17 @@ static cudaError_t launch_heads(const NormRotaryArgs& a, int interleaved, cudaSt
     constexpr int kUnits = hd_units(kV);
     int log_lanes;
     hd_lanes(hd_units_of_row(a.r.D, a.r.R, kV), kUnits, &log_lanes);
-    const int turned = (a.r.R / 2 + kV - 1) / kV, heads = a.r.heads[0] + a.r.heads[1] * (kAppend ? 2 : 1);
-    const size_t token = (size_t)turned * kV * sizeof(float2) + (kAppend ? 3 * 32 : 2 * 16), weights = kNorm ? (size_t)(kUnits << log_lanes) * kV * 16 : 0;
-    const long long n_tok = (long long)a.r.B * a.r.S;
-    const int per = hd_tokens(n_tok, heads, kHeadThreads >> log_lanes, token, (long long)hd_ctas_per_sm(kUnits) * sm_count());
+    const int turned = (a.r.R / 2 + kV - 1) / kV, heads = a.r.heads[0] + a.r.heads[1] * (kAppend ? 2 : 1), n_units = kUnits << log_lanes;
+    const size_t token = (size_t)turned * kV * sizeof(float2) + (kAppend ? 3 * 32 : 2 * 16), weights = kNorm ? (size_t)n_units * kV * 16 : 0;
+    const long long n_tok = (long long)a.r.B * a.r.S, resident = (long long)hd_ctas_per_sm(kV, kUnits) * sm_count(), ctas = n_tok < resident ? n_tok : resident;
+    const int per = hd_tile(n_tok, ctas, heads, kHeadThreads >> log_lanes, token);
     LaunchScope ls(kAppend ? K_CACHE_APPEND_ROTARY : K_NORM_ROTARY, st);
-    auto go = [&](auto kernel) {
-        return launch_overlapped(kernel, (unsigned)((n_tok + per - 1) / per), kHeadThreads, weights + per * token, st, a, per, log_lanes);
-    };
-    return interleaved ? go(heads_kernel<Tin, Tout, kV, kUnits, true, kNorm, kAppend>) : go(heads_kernel<Tin, Tout, kV, kUnits, false, kNorm, kAppend>);
+    auto go = [&](auto kernel) { return launch_overlapped(kernel, (unsigned)ctas, kHeadThreads, weights + 2 * per * token, st, a, per, log_lanes); };
+    if constexpr (kUnits == 1) {
+        if (hd_whole(a.r.D, a.r.R, interleaved, kV, n_units))
+            return interleaved ? go(heads_kernel<Tin, Tout, kV, 1, true, kNorm, kAppend, true>) : go(heads_kernel<Tin, Tout, kV, 1, false, kNorm, kAppend, true>);
+    }
+    return interleaved ? go(heads_kernel<Tin, Tout, kV, kUnits, true, kNorm, kAppend, false>) : go(heads_kernel<Tin, Tout, kV, kUnits, false, kNorm, kAppend, false>);
 }
 template <typename Tin, typename Tout, bool kNorm, bool kAppend, int kV = 16 / sizeof(Tin)>
 static cudaError_t launch_heads_width(const NormRotaryArgs& a, int interleaved, int aligned, cudaStream_t st) {
@@ -641,18 +692,16 @@ static cudaError_t launch_heads_back(const NormRotaryArgs& a, int interleaved, f
     constexpr int kUnits = hd_units(kV);
     int log_lanes;
     hd_lanes(hd_units_of_row(a.r.D, a.r.R, kV), kUnits, &log_lanes);
-    const int turned = (a.r.R / 2 + kV - 1) / kV, groups = kHeadThreads >> log_lanes;
+    const int turned = (a.r.R / 2 + kV - 1) / kV, n_units = kUnits << log_lanes, most = a.r.heads[0] > a.r.heads[1] ? a.r.heads[0] : a.r.heads[1];
     const size_t token = (size_t)turned * kV * sizeof(float2) + sizeof(HdRowsBack<T>), sums = (size_t)kHeadThreads / 32 * a.r.D * sizeof(float);
-    const int most = a.r.heads[0] > a.r.heads[1] ? a.r.heads[0] : a.r.heads[1];
-    int per = 4 * groups / most;
-    const int fits = (int)(27 * 1024 / token);
-    per = per > fits ? fits : per < 1 ? 1 : per;
-    const size_t tables = per * token + (size_t)(kUnits << log_lanes) * kV * 8, smem = tables > sums ? tables : sums;
+    const int per = hd_tile((long long)a.r.B * a.r.S, ctas[0], most, kHeadThreads >> log_lanes, token);
+    const size_t tables = 2 * per * token + (size_t)n_units * kV * 8, smem = tables > sums ? tables : sums;
     LaunchScope ls(K_NORM_ROTARY_BWD, st);
-    auto go = [&](auto kernel) {
-        return launch_overlapped(kernel, (unsigned)(ctas[0] + ctas[1]), kHeadThreads, smem, st, a, per, log_lanes, ctas[0], partial);
-    };
-    return interleaved ? go(heads_backward_kernel<T, kV, kUnits, true>) : go(heads_backward_kernel<T, kV, kUnits, false>);
+    auto go = [&](auto kernel) { return launch_overlapped(kernel, (unsigned)(ctas[0] + ctas[1]), kHeadThreads, smem, st, a, per, log_lanes, ctas[0], partial); };
+    if constexpr (kUnits == 1) {
+        if (hd_whole(a.r.D, a.r.R, interleaved, kV, n_units)) return interleaved ? go(heads_backward_kernel<T, kV, 1, true, true>) : go(heads_backward_kernel<T, kV, 1, false, true>);
+    }
+    return interleaved ? go(heads_backward_kernel<T, kV, kUnits, true, false>) : go(heads_backward_kernel<T, kV, kUnits, false, false>);
 }
 template <typename T, int kV = 16 / sizeof(T)>
 static cudaError_t launch_heads_back_width(const NormRotaryArgs& a, int interleaved, int aligned, float* partial, const int (&ctas)[2], cudaStream_t st) {
