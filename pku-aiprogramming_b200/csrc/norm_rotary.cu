@@ -13,7 +13,7 @@ namespace ttk {
 using namespace sm100;
 
 constexpr int kHeadThreads = 256;
-constexpr int hd_ctas_per_sm(int kV, int units) { return units > 1 ? 2 : kV == 8 ? 3 : 4; }
+constexpr int hd_ctas_per_sm(int units) { return units == 1 ? 3 : 2; }
 constexpr int kBackCtas = 2;   // per SM, of the gradient
 
 // A token's rows of one of the tensors, of head 0: where they come from, where they go, and for keys on their way into a cache a second place.
@@ -103,10 +103,13 @@ __device__ __forceinline__ void hd_turn(float (&x)[2][kV], const float* cs, int 
                 turn(x[2 * e / kV][2 * e % kV], x[2 * e / kV][2 * e % kV + 1], z.x, z.y);
                 turn(x[(2 * e + 2) / kV][(2 * e + 2) % kV], x[(2 * e + 2) / kV][(2 * e + 2) % kV + 1], z.z, z.w);
             } else {
-                const uint64_t c = pack_f32x2(z.x, z.y), s = pack_f32x2(z.z, z.w), minus = pack_f32x2(-z.z, -z.w);
+                const uint64_t c = pack_f32x2(z.x, z.y), s = pack_f32x2(z.z, z.w);
                 const uint64_t x1 = pack_f32x2(x[0][e], x[0][e + 1]), x2 = pack_f32x2(x[1][e], x[1][e + 1]);
-                unpack_f32x2(fma_f32x2(x1, c, mul_f32x2(x2, minus)), x[0][e], x[0][e + 1]);
+                float less[2];   // (there is no packed subtraction, and changing signs is two operations)
+                unpack_f32x2(mul_f32x2(x2, s), less[0], less[1]);
                 unpack_f32x2(fma_f32x2(x2, c, mul_f32x2(x1, s)), x[1][e], x[1][e + 1]);
+                x[0][e] = fmaf(x[0][e], z.x, -less[0]);
+                x[0][e + 1] = fmaf(x[0][e + 1], z.y, -less[1]);
             }
         }
     }
@@ -233,6 +236,13 @@ struct HdRaw {
             }
     }
 };
+// The sum over a row's lanes, 2^n of them.
+__device__ __forceinline__ float hd_sum(float x, int lanes) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1)
+        if (d < lanes) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
 // A walk of a group of lanes over the rows (token, head) of a tile, as many apart as there are groups.  Every group takes as many turns; where there is no row
 // left it takes the tile's first one, for nothing.
 struct HdWalk {
@@ -266,7 +276,7 @@ __device__ __forceinline__ unsigned hd_share(unsigned n, unsigned cta, unsigned 
 // blockDim = kHeadThreads; 2^log_lanes lanes to a row.  A CTA goes through its tokens tile by tile; the next tile's sines are made before the rows of the one at
 // hand.  kAppend: keys and values go into the pools' rows (a third tensor, which is copied).
 template <typename Tin, typename Tout, int kV, int kUnits, bool kNeighbours, bool kNorm, bool kAppend, bool kWhole>
-__global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kV, kUnits)) heads_kernel(const NormRotaryArgs a, int tile_tokens, int log_lanes) {
+__global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kUnits)) heads_kernel(const NormRotaryArgs a, int tile_tokens, int log_lanes) {
     using Out = RtVec<Tout, kV>;
     using Raw = HdRaw<Tin, kV, kUnits>;
     using Rows = typename std::conditional<kAppend, HdRows3<Tin, Tout>, HdRows<Tin, Tout>>::type;
@@ -330,33 +340,41 @@ __global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kV, kUnits)) head
         const Rows* rows = all_rows + which * (kTensors * tile_tokens);
         const float* cs = all_cs + which * tile_sines;
         HdWalk at(group, groups, heads, tile_of(t0));
-        auto tensor = [&](const HdWalk& x) { return x.h < up_to_k ? 0 : !kAppend || x.h < up_to_v ? 1 : 2; };
-        auto fetch = [&](Raw& to, const HdWalk& x) {
-            const int w = tensor(x), h = x.h - (w == 0 ? 0 : w == 1 ? up_to_k : up_to_v);
-            to.load(rows[kTensors * x.t + w].x + h * (kAppend && w == 2 ? a.v_stride[1] : w ? r.xs[1][1] : r.xs[0][1]), all_units);
+        // what is to be done with a row that is on its way
+        struct Job {
+            Raw raw;
+            Tout *y, *also;   // null: nowhere
+            int sines, w;
         };
-        auto work = [&](const Raw& raw, const HdWalk& x_at) {
+        auto fetch = [&](Job& to, const HdWalk& x) {
+            const int w = x.h < up_to_k ? 0 : !kAppend || x.h < up_to_v ? 1 : 2, h = x.h - (w == 0 ? 0 : w == 1 ? up_to_k : up_to_v);
+            const Rows row = rows[kTensors * x.t + w];
+            to.raw.load(row.x + h * (kAppend && w == 2 ? a.v_stride[1] : w ? r.xs[1][1] : r.xs[0][1]), all_units);
+            to.y = x.there() && (!kAppend || row.y) ? row.y + h * (w == 0 ? r.ys[0][1] : kAppend ? (long long)a.page * r.D : r.ys[1][1]) : nullptr;
+            if constexpr (kAppend) to.also = x.there() && row.also ? row.also + h * r.ys[1][1] : nullptr;
+            to.sines = x.t * (2 * turned * kV);
+            to.w = w;
+        };
+        auto work = [&](const Job& job) {
             HdUnits<kV, kUnits, kNeighbours, kWhole> units = all_units;
             units.forget();
-            const int w = tensor(x_at);
-            const bool moved = kAppend && w == 2;   // as it is
+            const bool moved = kAppend && job.w == 2;   // as it is
             float x[kUnits][2][kV];
 #pragma unroll
             for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) hd_floats<Tin, kV>(x[k][i], raw.v[k][i]);
+                for (int i = 0; i < 2; ++i) hd_floats<Tin, kV>(x[k][i], job.raw.v[k][i]);
             if (kNorm) {
                 float sums[2] = {0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) hd_add_products<kV>(sums, x[k][i], x[k][i]);
-                float sum = sums[0] + sums[1];
                 __syncwarp();
-                for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                const float sum = hd_sum(sums[0] + sums[1], lanes);
                 if (!moved) {
                     const float by = rsqrtf(sum * inv_D + a.eps);
-                    const float* weights = ws + w * (2 * n_units * kV);
+                    const float* weights = ws + job.w * (2 * n_units * kV);
 #pragma unroll
                     for (int k = 0; k < kUnits; ++k) {
                         float wt[2][kV];
@@ -369,42 +387,29 @@ __global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kV, kUnits)) head
                     }
                 }
             }
-            if (x_at.there()) {
-                const Rows& row = rows[kTensors * x_at.t + w];
-                const int h = x_at.h - (w == 0 ? 0 : w == 1 ? up_to_k : up_to_v);
-                Tout* y = row.y;
-                if (!kAppend || y) y += h * (w == 0 ? r.ys[0][1] : kAppend ? (long long)a.page * r.D : r.ys[1][1]);
-                Tout* also = nullptr;
-                if constexpr (kAppend) {
-                    if (row.also) also = row.also + h * r.ys[1][1];
-                }
-                const float* sines = cs + x_at.t * (2 * turned * kV);
 #pragma unroll
-                for (int k = 0; k < kUnits; ++k) {
-                    if (!moved && units.turns(k)) hd_turn<kV, kNeighbours>(x[k], sines, units.at[k], turned);
+            for (int k = 0; k < kUnits; ++k) {
+                if (!moved && units.turns(k)) hd_turn<kV, kNeighbours>(x[k], cs + job.sines, units.at[k], turned);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (!units.has(k, i)) continue;
-                        const Out z = hd_rounded<Tout, kV>(x[k][i]);
-                        if (!kAppend || y) *reinterpret_cast<Out*>(y + units.channel(k, i)) = z;
-                        if (kAppend && also) *reinterpret_cast<Out*>(also + units.channel(k, i)) = z;
-                    }
+                for (int i = 0; i < 2; ++i) {
+                    if (!units.has(k, i)) continue;
+                    const Out z = hd_rounded<Tout, kV>(x[k][i]);
+                    if (job.y) *reinterpret_cast<Out*>(job.y + units.channel(k, i)) = z;
+                    if (kAppend && job.also) *reinterpret_cast<Out*>(job.also + units.channel(k, i)) = z;
                 }
             }
         };
         // a row is loaded ahead of the one at hand
         const int turns = at.turns();
-        Raw one, two;
+        Job one, two;
         fetch(one, at);
         for (int turn = 0; turn < turns; turn += 2) {
-            HdWalk then = at;
-            then.next();
-            fetch(two, then);
-            work(one, at);
-            at = then;
+            at.next();
+            fetch(two, at);
+            work(one);
             at.next();
             fetch(one, at);
-            work(two, then);
+            work(two);
         }
         __syncthreads();   // the tables of the next tile are there, those of this one read
     }
@@ -467,23 +472,31 @@ __global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel
         const Rows* rows = all_rows + which * tile_tokens;
         const float* cs = all_cs + which * tile_sines;
         HdWalk at(group, groups, heads, tile_of(t0));
-        auto fetch = [&](Raw& g, Raw& x, const HdWalk& from) {
-            g.load(rows[from.t].g + from.h * g_head, all_units);
-            x.load(rows[from.t].x + from.h * x_head, all_units);
+        struct Job {
+            Raw g, x;
+            T* y;   // null: nowhere
+            int sines;
         };
-        auto work = [&](const Raw& raw_g, const Raw& raw_x, const HdWalk& from) {
+        auto fetch = [&](Job& to, const HdWalk& from) {
+            const Rows row = rows[from.t];
+            to.g.load(row.g + from.h * g_head, all_units);
+            to.x.load(row.x + from.h * x_head, all_units);
+            to.y = from.there() ? row.y + from.h * y_head : nullptr;
+            to.sines = from.t * (2 * turned * kV);
+        };
+        auto work = [&](const Job& job) {
             HdUnits<kV, kUnits, kNeighbours, kWhole> units = all_units;
             units.forget();
             float g[kUnits][2][kV], x[kUnits][2][kV], squares[2] = {0.f, 0.f}, alongs[2] = {0.f, 0.f};
-            const float* sines = cs + from.t * (2 * turned * kV);
+            const float* sines = cs + job.sines;
 #pragma unroll
             for (int k = 0; k < kUnits; ++k) {
                 float wt[2][kV];
                 hd_weight<kV>(wt, ws, units.at[k], n_units);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    hd_floats<T, kV>(g[k][i], raw_g.v[k][i]);
-                    hd_floats<T, kV>(x[k][i], raw_x.v[k][i]);
+                    hd_floats<T, kV>(g[k][i], job.g.v[k][i]);
+                    hd_floats<T, kV>(x[k][i], job.x.v[k][i]);
                 }
                 if (units.turns(k)) hd_turn<kV, kNeighbours>(g[k], sines, units.at[k], turned);
                 if (!units.has(k, 1))
@@ -497,15 +510,10 @@ __global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel
                     hd_add_products<kV>(alongs, h, x[k][i]);
                 }
             }
-            float square = squares[0] + squares[1], along = alongs[0] + alongs[1];
             __syncwarp();
-            for (int d = 1; d < lanes; d <<= 1) {
-                square += __shfl_xor_sync(0xffffffffu, square, d);
-                along += __shfl_xor_sync(0xffffffffu, along, d);
-            }
+            const float square = hd_sum(squares[0] + squares[1], lanes), along = hd_sum(alongs[0] + alongs[1], lanes);
             const float by = rsqrtf(square * inv_D + a.eps), less = -along * inv_D * by * by;
-            if (from.there()) {
-                T* y = rows[from.t].y + from.h * y_head;
+            if (job.y) {
 #pragma unroll
                 for (int k = 0; k < kUnits; ++k) {
                     float wt[2][kV];
@@ -519,28 +527,26 @@ __global__ void __launch_bounds__(kHeadThreads, kBackCtas) heads_backward_kernel
                         hd_mul<kV>(h, g[k][i], wt[i]);
                         hd_fma<kV>(h, x[k][i], less, h);
                         hd_mul<kV>(h, h, by);
-                        *reinterpret_cast<RtVec<T, kV>*>(y + units.channel(k, i)) = hd_rounded<T, kV>(h);
+                        *reinterpret_cast<RtVec<T, kV>*>(job.y + units.channel(k, i)) = hd_rounded<T, kV>(h);
                     }
                 }
             }
         };
         const int turns = at.turns();
-        Raw one[2], two[2];
-        fetch(one[0], one[1], at);
+        Job one, two;
+        fetch(one, at);
         for (int turn = 0; turn < turns; turn += 2) {
-            HdWalk then = at;
-            then.next();
-            fetch(two[0], two[1], then);
-            work(one[0], one[1], at);
-            at = then;
             at.next();
-            fetch(one[0], one[1], at);
-            work(two[0], two[1], then);
+            fetch(two, at);
+            work(one);
+            at.next();
+            fetch(one, at);
+            work(two);
         }
         __syncthreads();   // the tables of the next tile are there, those of this one read
     }
     // the rows of a warp, then the warps
-    float* sums = reinterpret_cast<float*>(sm);   // [kWarps][D]
+    float* sums = reinterpret_cast<float*>(sm);   // [kWarps][D]; (the barrier at a tile's end: the tables have been read)
 #pragma unroll
     for (int k = 0; k < kUnits; ++k)
 #pragma unroll
@@ -608,31 +614,39 @@ struct HdPlaces {
 
 // Whether all of a row's lanes have two whole chunks of it.
 static bool hd_whole(int D, int R, int interleaved, int kV, int n_units) { return n_units * 2 * kV == D && R % (2 * kV) == 0 && (interleaved || R / 2 % kV == 0); }
-// Tokens per tile: rows for eight turns of every group of lanes, as many as the tables of two have room for.
-static int hd_tile(long long n_tok, long long ctas, int heads, int groups, size_t token) {
-    long long per = 8LL * groups / heads;
+// Tokens per tile: rows for so many turns of every group of lanes, as the tables of two have room for.  A tile's first rows are loaded behind a barrier: 16384 tokens of 40
+// heads 73.4 / 69.8 / 67.7 / 66.2 us with 4 / 8 / 14 / 28 turns of one unit, the gradient of 8192 121.5 / 79.2 / 72.5 / 68.6; without norm and with half of the channels
+// turned the forward call takes 58.9 / 60.7 with 14 / 28.
+static int hd_tile(long long n_tok, long long ctas, int turns, int heads, int groups, size_t token) {
+    long long per = (long long)turns * groups / heads;
     const long long fits = 12 * 1024 / (long long)token, share = (n_tok + ctas - 1) / ctas;
     per = per > fits ? fits : per;
     per = per > share ? share : per;
     return per < 1 ? 1 : (int)per;
 }
 
+template <typename Tin, typename Tout, int kV, int kUnits, bool kNorm, bool kAppend, bool kWhole>
+static cudaError_t launch_heads_units(const NormRotaryArgs& a, int interleaved, int log_lanes, cudaStream_t st) {
+    const int turned = (a.r.R / 2 + kV - 1) / kV, heads = a.r.heads[0] + a.r.heads[1] * (kAppend ? 2 : 1), n_units = kUnits << log_lanes;
+    const size_t token = (size_t)turned * kV * sizeof(float2) + (kAppend ? 3 * 32 : 2 * 16), weights = kNorm ? (size_t)n_units * kV * 16 : 0;
+    const long long n_tok = (long long)a.r.B * a.r.S, resident = (long long)hd_ctas_per_sm(kUnits) * sm_count(), ctas = n_tok < resident ? n_tok : resident;
+    const int per = hd_tile(n_tok, ctas, 14, heads, kHeadThreads >> log_lanes, token);
+    LaunchScope ls(kAppend ? K_CACHE_APPEND_ROTARY : K_NORM_ROTARY, st);
+    auto go = [&](auto kernel) { return launch_overlapped(kernel, (unsigned)ctas, kHeadThreads, weights + 2 * per * token, st, a, per, log_lanes); };
+    return interleaved ? go(heads_kernel<Tin, Tout, kV, kUnits, true, kNorm, kAppend, kWhole>) : go(heads_kernel<Tin, Tout, kV, kUnits, false, kNorm, kAppend, kWhole>);
+}
 template <typename Tin, typename Tout, int kV, bool kNorm, bool kAppend>
 static cudaError_t launch_heads(const NormRotaryArgs& a, int interleaved, cudaStream_t st) {
     constexpr int kUnits = hd_units(kV);
     int log_lanes;
-    hd_lanes(hd_units_of_row(a.r.D, a.r.R, kV), kUnits, &log_lanes);
-    const int turned = (a.r.R / 2 + kV - 1) / kV, heads = a.r.heads[0] + a.r.heads[1] * (kAppend ? 2 : 1), n_units = kUnits << log_lanes;
-    const size_t token = (size_t)turned * kV * sizeof(float2) + (kAppend ? 3 * 32 : 2 * 16), weights = kNorm ? (size_t)n_units * kV * 16 : 0;
-    const long long n_tok = (long long)a.r.B * a.r.S, resident = (long long)hd_ctas_per_sm(kV, kUnits) * sm_count(), ctas = n_tok < resident ? n_tok : resident;
-    const int per = hd_tile(n_tok, ctas, heads, kHeadThreads >> log_lanes, token);
-    LaunchScope ls(kAppend ? K_CACHE_APPEND_ROTARY : K_NORM_ROTARY, st);
-    auto go = [&](auto kernel) { return launch_overlapped(kernel, (unsigned)ctas, kHeadThreads, weights + 2 * per * token, st, a, per, log_lanes); };
+    const int units = hd_units_of_row(a.r.D, a.r.R, kV);
+    // Whole rows: two units to a lane, so that what a row costs beside its values is shared by more of them (16384 tokens of 40 heads of 128 bf16 64.2 us for 66.2).
     if constexpr (kUnits == 1) {
-        if (hd_whole(a.r.D, a.r.R, interleaved, kV, n_units))
-            return interleaved ? go(heads_kernel<Tin, Tout, kV, 1, true, kNorm, kAppend, true>) : go(heads_kernel<Tin, Tout, kV, 1, false, kNorm, kAppend, true>);
+        hd_lanes(units, 2, &log_lanes);
+        if (hd_whole(a.r.D, a.r.R, interleaved, kV, 2 << log_lanes)) return launch_heads_units<Tin, Tout, kV, 2, kNorm, kAppend, true>(a, interleaved, log_lanes, st);
     }
-    return interleaved ? go(heads_kernel<Tin, Tout, kV, kUnits, true, kNorm, kAppend, false>) : go(heads_kernel<Tin, Tout, kV, kUnits, false, kNorm, kAppend, false>);
+    hd_lanes(units, kUnits, &log_lanes);
+    return launch_heads_units<Tin, Tout, kV, kUnits, kNorm, kAppend, false>(a, interleaved, log_lanes, st);
 }
 template <typename Tin, typename Tout, bool kNorm, bool kAppend, int kV = 16 / sizeof(Tin)>
 static cudaError_t launch_heads_width(const NormRotaryArgs& a, int interleaved, int aligned, cudaStream_t st) {
@@ -674,16 +688,16 @@ cudaError_t cache_append_rotary(const NormRotaryArgs& a, int bf16, int interleav
     return bf16 ? go(__nv_bfloat16{}) : go(float{});
 }
 
-// CTAs of the gradient: what the SMs hold at once, shared out by the heads; fewer where there are not rows for them.
+// CTAs of the gradient: what the SMs hold at once, shared out by what the rows of the two tensors cost; fewer where there are not tokens for them.  A token's sines, where
+// all channels turn, take as long as five rows: 8192 tokens of 32 and 8 heads 68.2 / 65.4 / 60.6 / 57.6 us if that is taken for 0 / 1 / 3 / 5 rows.
 static void hd_ctas(const NormRotaryArgs& a, int (&ctas)[2]) {
-    const long long n_tok = (long long)a.r.B * a.r.S, all = (long long)sm_count() * kBackCtas, heads = a.r.heads[0] + a.r.heads[1];
-    for (int i = 0; i < 2; ++i) {
-        long long n = (all * a.r.heads[i] + heads / 2) / heads;
-        if (i == 0 && n >= all && a.r.heads[1]) n = all - 1;
-        if (i == 1) n = all - ctas[0];
-        if (n > n_tok) n = n_tok;
-        ctas[i] = !a.r.heads[i] || !n_tok ? 0 : n < 1 ? 1 : (int)n;
-    }
+    const long long n_tok = (long long)a.r.B * a.r.S, all = (long long)sm_count() * kBackCtas, sines = 5LL * a.r.R;
+    const long long cost[2] = {(long long)a.r.heads[0] * a.r.D + sines, a.r.heads[1] ? (long long)a.r.heads[1] * a.r.D + sines : 0};
+    long long q = (all * cost[0] + (cost[0] + cost[1]) / 2) / (cost[0] + cost[1]);
+    if (q >= all && cost[1]) q = all - 1;
+    if (q < 1) q = 1;
+    const long long n[2] = {q, cost[1] ? all - q : 0};
+    for (int i = 0; i < 2; ++i) ctas[i] = (int)(n[i] < n_tok ? n[i] : n_tok);
 }
 size_t norm_rotary_backward_workspace(int D) { return align256((size_t)sm_count() * kBackCtas * D * sizeof(float)); }
 
@@ -694,7 +708,7 @@ static cudaError_t launch_heads_back(const NormRotaryArgs& a, int interleaved, f
     hd_lanes(hd_units_of_row(a.r.D, a.r.R, kV), kUnits, &log_lanes);
     const int turned = (a.r.R / 2 + kV - 1) / kV, n_units = kUnits << log_lanes, most = a.r.heads[0] > a.r.heads[1] ? a.r.heads[0] : a.r.heads[1];
     const size_t token = (size_t)turned * kV * sizeof(float2) + sizeof(HdRowsBack<T>), sums = (size_t)kHeadThreads / 32 * a.r.D * sizeof(float);
-    const int per = hd_tile((long long)a.r.B * a.r.S, ctas[0], most, kHeadThreads >> log_lanes, token);
+    const int per = hd_tile((long long)a.r.B * a.r.S, ctas[0], 28, most, kHeadThreads >> log_lanes, token);
     const size_t tables = 2 * per * token + (size_t)n_units * kV * 8, smem = tables > sums ? tables : sums;
     LaunchScope ls(K_NORM_ROTARY_BWD, st);
     auto go = [&](auto kernel) { return launch_overlapped(kernel, (unsigned)(ctas[0] + ctas[1]), kHeadThreads, smem, st, a, per, log_lanes, ctas[0], partial); };
