@@ -1,6 +1,6 @@
 // Single-query attention over the 8-bit key/value cache: out = softmax(scale q K^T) V, K and V e4m3 codes times 2^e, one e for 16 tokens of a head.
 //
-// HBM-bound: a key and key/value head are 2 D bytes and two 16ths of one.  Codes become halves, exactly, in registers (one conversion for two), which
+// HBM-bound: a key and key/value head are 2 D bytes and two 16ths of one.  Codes become halves, exactly, in registers (a conversion makes two), which
 // go to mma.sync: its accumulators (16 x 8) a group of up to eight query heads fills; tcgen05 would want q in codes too, in several parts, and P.  A warp takes up to
 // 16 query heads; a larger group reads the cache once for each 16.  Both products are m16n8k16 in halves with 32-bit sums, 16 keys of one exponent at a time:
 //   S^T [16 keys x 8 heads] += K [16 keys x 16 channels] Q^T: lane (g, t) of a warp (g = lane / 4, t = lane % 4) has of keys g and g + 8 every fourth
@@ -206,7 +206,9 @@ __global__ void __launch_bounds__(kWarps * 32, q8_ctas_per_sm(D, NT)) attn_decod
                     const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t a0 = q8_halves(x[j] & 0xffffu), a1 = q8_halves(y[j] & 0xffffu), a2 = q8_halves(x[j] >> 16), a3 = q8_halves(y[j] >> 16);
+                        uint32_t a0, a1, a2, a3;
+                        q8_halves(x[j], a0, a2);
+                        q8_halves(y[j], a1, a3);
 #pragma unroll
                         for (int m = 0; m < NT; ++m) {
                             if (c + j == 0) mma_f16_first(s[u][m], a0, a1, a2, a3, qf[m][c * 4 + j][0], qf[m][c * 4 + j][1]);
@@ -327,7 +329,9 @@ __global__ void __launch_bounds__(kWarps * 32, q8_ctas_per_sm(D, NT)) attn_decod
                     for (int half = 0; half < 2; ++half) {
                         const uint32_t sel = half ? 0x7362u : 0x5140u;   // channels 0 and 1, or 2 and 3, of two keys
                         const uint32_t x = __byte_perm(r[0][j], r[1][j], sel), y = __byte_perm(r[2][j], r[3][j], sel);
-                        const uint32_t a0 = q8_halves(x & 0xffffu), a1 = q8_halves(x >> 16), a2 = q8_halves(y & 0xffffu), a3 = q8_halves(y >> 16);
+                        uint32_t a0, a1, a2, a3;
+                        q8_halves(x, a0, a1);
+                        q8_halves(y, a2, a3);
 #pragma unroll
                         for (int m = 0; m < NT; ++m) mma_f16(o[j * 2 + half][m], a0, a1, a2, a3, p[u][m][0], p[u][m][1]);
                     }

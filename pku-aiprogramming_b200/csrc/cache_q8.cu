@@ -88,14 +88,9 @@ __global__ void __launch_bounds__(kQ8Threads) cache_append_q8_kernel(const T* __
                 uint32_t w[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    uint32_t out = 0;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t two = q8_halves(w[m] >> 16 * half & 0xffffu);
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
-                        out |= q8_encode2(f.x * by, f.y * by) << 16 * half;
-                    }
-                    w[m] = out;
+                    float f[4];
+                    q8_floats(w[m], f);
+                    w[m] = q8_encode4(f[0] * by, f[1] * by, f[2] * by, f[3] * by);
                 }
                 *reinterpret_cast<uint4*>(codes + at) = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -108,7 +103,7 @@ __global__ void __launch_bounds__(kQ8Threads) cache_append_q8_kernel(const T* __
                 uint32_t out[kV / 4];
 #pragma unroll
                 for (int m = 0; m < kV / 4; ++m)
-                    out[m] = q8_encode2((float)y[j][4 * m] * by, (float)y[j][4 * m + 1] * by) | q8_encode2((float)y[j][4 * m + 2] * by, (float)y[j][4 * m + 3] * by) << 16;
+                    out[m] = q8_encode4((float)y[j][4 * m] * by, (float)y[j][4 * m + 1] * by, (float)y[j][4 * m + 2] * by, (float)y[j][4 * m + 3] * by);
                 unsigned char* to = codes + (sm_slot[1 + first + r] & (kQ8Block - 1)) * D + col;
                 if (kV == 8) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[kV / 4 - 1]);
                 else *reinterpret_cast<uint32_t*>(to) = out[0];
@@ -194,11 +189,11 @@ __global__ void __launch_bounds__(kQ8Threads) cache_read_q8_kernel(const unsigne
                 const uint32_t in[4] = {x[i][j].x, x[i][j].y, x[i][j].z, x[i][j].w};
                 uint32_t out[8];
 #pragma unroll
-                for (int m = 0; m < 8; ++m) {
-                    const uint32_t two = q8_halves(in[m >> 1] >> 16 * (m & 1) & 0xffffu);
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
-                    const __nv_bfloat162 z = __floats2bfloat162_rn(f.x * by, f.y * by);
-                    out[m] = *reinterpret_cast<const uint32_t*>(&z);
+                for (int m = 0; m < 4; ++m) {
+                    float f[4];
+                    q8_floats(in[m], f);
+                    out[2 * m] = sm100::pack_bf16x2(f[0] * by, f[1] * by);
+                    out[2 * m + 1] = sm100::pack_bf16x2(f[2] * by, f[3] * by);
                 }
                 __nv_bfloat16* p = (j ? v : k) + to;
                 if (kSectors) {
