@@ -11,14 +11,63 @@ namespace ttk {
 
 constexpr int kQ8Threads = 256, kQ8Most = 32;   // tokens that a CTA looks for runs in
 
-// What a row of D values is to a warp: 16 bytes a lane, kRows rows at a time.
+// What a row of D values is to a warp: 16 bytes a lane, kRows rows at a time; a block's are kLoads loads of four registers.  kCtas: as many per SM as hold them; 20,000
+// tokens of 8 heads, us with one CTA fewer and so: bf16 D = 128 24.3, 23.9 (4; 5 take 25.1), D = 64 16.0, 14.9 (5), floats D = 128 58.5, 41.8 (2), D = 64 26.0, 22.1 (3).
 template <typename T, int D>
 struct Q8Rows {
     static constexpr int kV = 16 / sizeof(T), kLanes = D / kV, kRows = 32 / kLanes, kLoads = kQ8Block / kRows;
+    static constexpr int kCtas = sizeof(T) == 2 ? (D == 64 ? 5 : 4) : D == 64 ? 3 : 2;
+};
+
+// 16 bytes of them; 0 where there is no token.
+template <typename T> struct Q8Values;
+template <> struct Q8Values<__nv_bfloat16> {
+    uint32_t w[4];
+    template <bool kWide> __device__ __forceinline__ void load(const __nv_bfloat16* p, bool there) {
+        if (!there) {
+            w[0] = w[1] = w[2] = w[3] = 0;
+        } else if (kWide) {
+            const uint4 r = *reinterpret_cast<const uint4*>(p);
+            w[0] = r.x; w[1] = r.y; w[2] = r.z; w[3] = r.w;
+        } else {
+            const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+    // magnitudes' bits, two in a word: ordered as the values, infinities and NaN above them
+    __device__ __forceinline__ unsigned largest(unsigned top) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+        return top;
+    }
+    static __device__ __forceinline__ unsigned bits(unsigned top) { return max(top << 16, top & 0xffff0000u); }
+};
+template <> struct Q8Values<float> {
+    float x[4];
+    template <bool kWide> __device__ __forceinline__ void load(const float* p, bool there) {
+        if (!there) {
+            x[0] = x[1] = x[2] = x[3] = 0.f;
+        } else if (kWide) {
+            const float4 r = *reinterpret_cast<const float4*>(p);
+            x[0] = r.x; x[1] = r.y; x[2] = r.z; x[3] = r.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ float get(int i) const { return x[i]; }
+    __device__ __forceinline__ unsigned largest(unsigned top) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        return top;
+    }
+    static __device__ __forceinline__ unsigned bits(unsigned top) { return top; }
 };
 
 template <typename T, int D, bool kWide>
-__global__ void __launch_bounds__(kQ8Threads) cache_append_q8_kernel(const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ slots, int n_tok, int tokens_per_cta,
+__global__ void __launch_bounds__(kQ8Threads, Q8Rows<T, D>::kCtas) cache_append_q8_kernel(const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ slots, int n_tok, int tokens_per_cta,
                                                                      int hkv, long long k_tok, long long k_head, long long v_tok, long long v_head, unsigned char* kc,
                                                                      unsigned char* vc, int n_slots, int page) {
     using R = Q8Rows<T, D>;
@@ -53,27 +102,25 @@ __global__ void __launch_bounds__(kQ8Threads) cache_append_q8_kernel(const T* __
         unsigned char *begin = cache + ((long long)at_page * hkv + h) * page_bytes, *codes = begin + (long long)in_page * D, *power = begin + (long long)page * D + in_page / kQ8Block;
         const int was_byte = *power;
         // the run's values, and the largest finite one
-        T y[R::kLoads][kV];
+        Q8Values<T> y[R::kLoads];
         unsigned top = 0;
+        const T* from = x + (t0 + first + row) * tok + h * head + col;
 #pragma unroll
-        for (int j = 0; j < R::kLoads; ++j) {
-            const int r = j * R::kRows + row;
-            if (r < len) {
-                const T* p = x + (t0 + first + r) * tok + h * head + col;
-                if (kWide) {
-                    *reinterpret_cast<uint4*>(y[j]) = *reinterpret_cast<const uint4*>(p);
-                } else {
+        for (int j = 0; j < R::kLoads; ++j, from += R::kRows * tok) y[j].template load<kWide>(from, j * R::kRows + row < len);
 #pragma unroll
-                    for (int e = 0; e < kV; ++e) y[j][e] = p[e];
-                }
+        for (int j = 0; j < R::kLoads; ++j) top = y[j].largest(top);
+        top = __reduce_max_sync(0xffffffffu, Q8Values<T>::bits(top));
+        if (top >= 0x7f800000u) {   // infinities or NaN among them
+            top = 0;
+#pragma unroll
+            for (int j = 0; j < R::kLoads; ++j)
 #pragma unroll
                 for (int e = 0; e < kV; ++e) {
-                    const unsigned bits = __float_as_uint((float)y[j][e]) & 0x7fffffffu;
+                    const unsigned bits = __float_as_uint(y[j].get(e)) & 0x7fffffffu;
                     if (bits < 0x7f800000u) top = max(top, bits);
                 }
-            }
+            top = __reduce_max_sync(0xffffffffu, top);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
         const int mine = lane < len ? sm_slot[1 + first + lane] & (kQ8Block - 1) : -1;   // a token's row of the block
         const unsigned rows = __reduce_or_sync(0xffffffffu, mine >= 0 ? 1u << mine : 0u);
         const bool fresh = rows & 1;
@@ -103,7 +150,7 @@ __global__ void __launch_bounds__(kQ8Threads) cache_append_q8_kernel(const T* __
                 uint32_t out[kV / 4];
 #pragma unroll
                 for (int m = 0; m < kV / 4; ++m)
-                    out[m] = q8_encode4((float)y[j][4 * m] * by, (float)y[j][4 * m + 1] * by, (float)y[j][4 * m + 2] * by, (float)y[j][4 * m + 3] * by);
+                    out[m] = q8_encode4(y[j].get(4 * m) * by, y[j].get(4 * m + 1) * by, y[j].get(4 * m + 2) * by, y[j].get(4 * m + 3) * by);
                 unsigned char* to = codes + (sm_slot[1 + first + r] & (kQ8Block - 1)) * D + col;
                 if (kV == 8) *reinterpret_cast<uint2*>(to) = make_uint2(out[0], out[kV / 4 - 1]);
                 else *reinterpret_cast<uint32_t*>(to) = out[0];
