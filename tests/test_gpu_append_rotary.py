@@ -156,3 +156,20 @@ def test_refusals(tt):
     x = Case(tt, 12, 4, 2, 32, 32, 16, 4)
     with pytest.raises((ValueError, tt.TTError)):
         x.call(tt)
+
+
+def test_pools_beyond_4_gb(tt):
+    """Rows whose places pass 32 bits, in elements and in bytes."""
+    hkv, D, page = 8, 128, 64
+    pages = (1 << 32) // (hkv * D * page) + 30
+    pools = [torch.empty(pages, hkv, page, D, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    T = 70
+    rows = torch.randn(T, 4 + 2 * hkv, D, device="cuda").bfloat16()
+    q, k, v = rows[:, :4], rows[:, 4:4 + hkv], rows[:, 4 + hkv:]
+    slots = torch.cat((torch.arange(40), (pages - 1) * page + torch.arange(30))).int().cuda()
+    freq, _ = tt.rotary_frequencies(D)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    got = tt.cache_append_rotary(q, k, v, slots, pos, freq, *pools)
+    want_q, want_k = tt.rotary_forward(q, k, pos, freq)
+    at = slots.long()
+    assert torch.equal(got, want_q) and torch.equal(pools[0][at // page, :, at % page], want_k) and torch.equal(pools[1][at // page, :, at % page], v)

@@ -94,7 +94,7 @@ class Case:
 @pytest.mark.parametrize("lens,H,hkv,D,page", [
     ([1], 1, 1, 64, 16), ([1], 8, 8, 128, 64), ([1, 2, 15, 16, 17], 4, 2, 128, 16), ([0, 31, 32, 33, 0, 127, 128, 129], 6, 2, 64, 16), ([255, 256, 257, 511, 513], 8, 1, 128, 32),
     ([100, 700], 7, 1, 128, 48), ([333, 5], 9, 1, 128, 64), ([300, 1, 0], 12, 1, 64, 48), ([500, 64], 16, 1, 128, 128), ([400], 17, 1, 128, 16), ([260, 3], 40, 2, 64, 64),
-    ([129], 33, 1, 128, 256), ([0, 31, 32, 33, 0, 127, 128, 5], 40, 2, 64, 16), ([128, 0, 100], 24, 1, 128, 64), ([0, 0], 3, 1, 128, 16), (list(range(97)), 6, 2, 64, 16), ([5001], 32, 8, 128, 64), ([3000, 1, 2999], 5, 1, 64, 80), ([4097], 2, 2, 128, 1024)])
+    ([129], 33, 1, 128, 256), ([1100, 3], 4, 2, 64, 528), ([0, 31, 32, 33, 0, 127, 128, 5], 40, 2, 64, 16), ([128, 0, 100], 24, 1, 128, 64), ([0, 0], 3, 1, 128, 16), (list(range(97)), 6, 2, 64, 16), ([5001], 32, 8, 128, 64), ([3000, 1, 2999], 5, 1, 64, 80), ([4097], 2, 2, 128, 1024)])
 def test_against_64_bits(tt, lens, H, hkv, D, page):
     c = Case(lens, H, hkv, D, page, seed=len(lens) + H)
     a = c.args()

@@ -237,3 +237,52 @@ def test_refusals(tt):
         back(workspace=torch.empty(3, device="cpu"))
     small = torch.empty(16, dtype=torch.uint8, device="cuda")
     back(workspace=small)               # too small: another is made
+
+
+def test_strides_beyond_32_bits(tt):
+    T, H, D, far = 3, 2, 64, 1_200_000_000
+    base = torch.empty(2 * far + H * D, device="cuda", dtype=torch.bfloat16)
+    x = base.as_strided((T, H, D), (far, D, 1))
+    x.copy_(torch.randn(T, H, D, device="cuda"))
+    freq, _ = tt.rotary_frequencies(D)
+    pos, w = torch.arange(T, dtype=torch.int32, device="cuda"), weights(D, torch.float32, 4)
+    near_by = x.contiguous()
+    want, _ = tt.norm_rotary_forward(near_by, None, w, None, pos, freq)
+    assert torch.equal(tt.norm_rotary_forward(x, None, w, None, pos, freq)[0], want)
+    g = torch.randn_like(near_by)
+    a, b = (tt.norm_rotary_backward(g, None, y, None, w, None, pos, freq) for y in (x, near_by))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+    got, _ = tt.norm_rotary_forward(near_by, None, w, None, pos, freq, out_q=x)
+    assert got is x and torch.equal(x, want)
+
+
+def test_neighbouring_memory(tt):
+    """Outputs and workspace end where they end."""
+    import ctypes
+
+    from test_gpu_canary import Guarded
+    for T, H, Hkv, D, R, dtype in ((1, 1, 1, 64, 64, torch.bfloat16), (37, 5, 2, 80, 40, torch.bfloat16), (9, 3, 1, 50, 18, torch.float32), (600, 8, 2, 128, 128, torch.bfloat16)):
+        q, k = (torch.randn(T, h, D, device="cuda").to(dtype) for h in (H, Hkv))
+        freq, _ = tt.rotary_frequencies(R)
+        pos, w = torch.arange(T, dtype=torch.int32, device="cuda"), weights(D, torch.float32, 5)
+        d = tt.capi.RotaryDesc(B=1, S=T, H=H, Hkv=Hkv, D=D, R=R, n_axes=1, dtype=tt.capi.TT_F32, interleaved=0, scale=1.0)
+        need = int(tt.capi.lib.tt_norm_rotary_bwd_workspace_bytes(ctypes.byref(d)))
+        assert need > 0
+        a, b, ws = Guarded((T, H, D), dtype), Guarded((T, Hkv, D), dtype), Guarded((need,), torch.uint8)
+        want = tt.norm_rotary_forward(q, k, w, w, pos, freq)
+        tt.norm_rotary_forward(q, k, w, w, pos, freq, out_q=a.t, out_k=b.t)
+        torch.cuda.synchronize()
+        assert a.intact() and b.intact() and torch.equal(a.t, want[0]) and torch.equal(b.t, want[1])
+        want = tt.norm_rotary_backward(q, k, q + 1, k + 1, w, w, pos, freq)
+        got = tt.norm_rotary_backward(q, k, q + 1, k + 1, w, w, pos, freq, out_q=a.t, out_k=b.t, workspace=ws.t)
+        torch.cuda.synchronize()
+        assert a.intact() and b.intact() and ws.intact() and all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("H,Hkv", [(1, 40), (64, 1), (7, 3)])
+def test_shares_of_the_gradient_s_ctas(tt, H, Hkv):
+    """Tensors of very different numbers of heads, and many more tokens than CTAs."""
+    T, D = 2500, 64
+    q, k = (torch.randn(T, h, D, device="cuda") for h in (H, Hkv))
+    freq, _ = tt.rotary_frequencies(D)
+    check(tt, q, k, torch.arange(T, dtype=torch.int32, device="cuda"), freq)
