@@ -6,6 +6,12 @@
 // HBM-bound: a row is read once, its sum of squares is met by the lanes that hold it, and it is written once.  A row of D channels is
 // units of two accesses of kV values, the two halves of kV pairs (or kV pairs of neighbours, or channels that only are normed); 2^n lanes
 // have a row, so the sums are n shuffles, and the rows of a warp lie next to each other.
+//
+// What keeps it from the memory's rate is instructions: sixteen conversions, products and roundings for 32 bytes of bf16, and a token's sines, exact
+// for any position, which are worth five of its rows.  So sines, weights and places lie in shared memory, made a tile of tokens ahead, each CTA that is resident
+// has an equal share of the tokens, and two rows of a lane are on their way at once.  16384 tokens of 32 + 8 heads of 128 in bf16, all channels
+// turned: 63.4 us, 5.3 TB/s (a copy runs at 6.6); the gradient of 8192 of them 56.4 us, 4.5 TB/s; of 4094 tokens of 8 + 8 heads of
+// 64 floats 15.0 us, 3.4 TB/s; 13,000 tokens turned and written into a cache of pages of 16 58.1 us, 5.5 TB/s; 64 single tokens 4 us, a launch.
 #include "rotary_parts.cuh"
 #include "sm100_ptx.cuh"
 
@@ -13,8 +19,9 @@ namespace ttk {
 using namespace sm100;
 
 constexpr int kHeadThreads = 256;
+// CTAs per SM, as many as hold two rows of a lane in registers: with one unit a lane 3 (4, which spill, take 77 us for 70), with two 2 (3: 87.7 for 65.4).
 constexpr int hd_ctas_per_sm(int units) { return units == 1 ? 3 : 2; }
-constexpr int kBackCtas = 2;   // per SM, of the gradient
+constexpr int kBackCtas = 2;   // of the gradient: 79 us, 3 take 110
 
 // A token's rows of one of the tensors, of head 0: where they come from, where they go, and for keys on their way into a cache a second place.
 template <typename Tin, typename Tout>
@@ -239,7 +246,7 @@ struct HdRaw {
 // The sum over a row's lanes, 2^n of them.
 __device__ __forceinline__ float hd_sum(float x, int lanes) {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1)
+    for (int d = 16; d; d >>= 1)
         if (d < lanes) x += __shfl_xor_sync(0xffffffffu, x, d);
     return x;
 }
@@ -365,26 +372,33 @@ __global__ void __launch_bounds__(kHeadThreads, hd_ctas_per_sm(kUnits)) heads_ke
 #pragma unroll
                 for (int i = 0; i < 2; ++i) hd_floats<Tin, kV>(x[k][i], job.raw.v[k][i]);
             if (kNorm) {
-                float sums[2] = {0.f, 0.f};
+                // unit by unit, and the lanes the farthest first: in one order whether a lane has one unit of a whole row or two
+                float sum = 0.f;
 #pragma unroll
-                for (int k = 0; k < kUnits; ++k)
+                for (int k = 0; k < kUnits; ++k) {
+                    float sums[2] = {0.f, 0.f};
 #pragma unroll
                     for (int i = 0; i < 2; ++i) hd_add_products<kV>(sums, x[k][i], x[k][i]);
+                    sum += sums[0] + sums[1];
+                }
+                // the row times its weights while the lanes meet
+                const float* weights = ws + (moved ? 0 : job.w) * (2 * n_units * kV);
+                float y[kUnits][2][kV];
+#pragma unroll
+                for (int k = 0; k < kUnits; ++k) {
+                    float wt[2][kV];
+                    hd_weight<kV>(wt, weights, units.at[k], n_units);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) hd_mul<kV>(y[k][i], x[k][i], wt[i]);
+                }
                 __syncwarp();
-                const float sum = hd_sum(sums[0] + sums[1], lanes);
+                sum = hd_sum(sum, lanes);
                 if (!moved) {
                     const float by = rsqrtf(sum * inv_D + a.eps);
-                    const float* weights = ws + job.w * (2 * n_units * kV);
 #pragma unroll
-                    for (int k = 0; k < kUnits; ++k) {
-                        float wt[2][kV];
-                        hd_weight<kV>(wt, weights, units.at[k], n_units);
+                    for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            hd_mul<kV>(wt[i], wt[i], by);
-                            hd_mul<kV>(x[k][i], x[k][i], wt[i]);
-                        }
-                    }
+                        for (int i = 0; i < 2; ++i) hd_mul<kV>(x[k][i], y[k][i], by);
                 }
             }
 #pragma unroll
@@ -640,8 +654,16 @@ static cudaError_t launch_heads(const NormRotaryArgs& a, int interleaved, cudaSt
     constexpr int kUnits = hd_units(kV);
     int log_lanes;
     const int units = hd_units_of_row(a.r.D, a.r.R, kV);
-    // Whole rows: two units to a lane, so that what a row costs beside its values is shared by more of them (16384 tokens of 40 heads of 128 bf16 64.2 us for 66.2).
+    // Whole rows: two units to a lane, so that what a row costs beside its values is shared by more of them (TB/s with one unit and two, 20 heads: floats of 128, 64
+    // channels turned, 5.35 and 5.59; bf16 of 256 and 128 5.04 and 5.29).  But bf16 norms of rows of four units, where a warp then has 16 rows, and of few heads that
+    // turn all channels, where the CTAs make sines for longer, have three CTAs per SM, and one unit (64 and 64 4.55 and 4.01, 64 and 16 4.86 and 4.76, 128 and 128 4.87
+    // and 4.50, 256 and 256 4.94 and 4.73; 40 heads of 128 and 128 67.4 us and 65.5).
     if constexpr (kUnits == 1) {
+        if constexpr (sizeof(Tin) == 2 && kNorm && !kAppend) {
+            hd_lanes(units, 1, &log_lanes);
+            if ((units <= 4 || (a.r.heads[0] + a.r.heads[1]) * a.r.D < 32LL * a.r.R) && hd_whole(a.r.D, a.r.R, interleaved, kV, 1 << log_lanes))
+                return launch_heads_units<Tin, Tout, kV, 1, kNorm, kAppend, true>(a, interleaved, log_lanes, st);
+        }
         hd_lanes(units, 2, &log_lanes);
         if (hd_whole(a.r.D, a.r.R, interleaved, kV, 2 << log_lanes)) return launch_heads_units<Tin, Tout, kV, 2, kNorm, kAppend, true>(a, interleaved, log_lanes, st);
     }
