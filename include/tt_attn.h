@@ -285,7 +285,7 @@ int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cac
  * (2^-9, where that was raised) if that is more.  Infinities, and values beyond 448 2^40, become the block's largest value of their sign; NaN stays NaN.
  *
  * tt_cache_read_q8: as tt_cache_read_q4.  tt_attn_decode_q8: as tt_attn_decode_q4, D, lengths, tables, groups, outputs and workspace alike (size by
- * tt_attn_decode_q8_workspace_bytes); NaN among a sequence's keys or values reaches its results. */
+ * tt_attn_decode_q8_workspace_bytes; 0, and NULL, where L is at most 192); NaN among a sequence's keys or values reaches its results. */
 size_t tt_cache_q8_page_bytes(int32_t page_size, int32_t D);   /* 0: not supported */
 int tt_cache_append_q8(const void* k, const void* v, const int32_t* slots, int32_t T, int32_t Hkv, int32_t D, int32_t dtype, const int64_t* k_stride,
                        const int64_t* v_stride, void* k_cache, void* v_cache, int32_t n_pages, int32_t page_size, void* stream);

@@ -16,6 +16,10 @@
 // The keys are shared out among the warps as decode_parts.cuh says; a warp streams its part through a ring of its own in shared memory (cp.async, kDepth steps,
 // on into the next slice's keys where one ends).  In a slot 16 bytes of a row lie where neither product's reads meet in a bank.  No warp waits for another, and
 // results do not depend on timing.
+//
+// Measured: 64 sequences of 4096 to 8192 keys, 32 heads on 8 of 128, 143 us, 5.7 TB/s (a copy runs at 6.6): beyond some 11 us, which are the chain lengths, page, exponents,
+// keys at the start, one step more for some warps than for others, and the merge, a byte costs what it does at 6.2 TB/s.  16 heads on 16 of 64, 0 to 4096 keys,
+// 48 us, 4.1 TB/s; 2 sequences of 120,000 keys, 32 heads on 2, 36 us, 3.6 TB/s of 128 MB.  Issue slots are a third to two fifths busy.
 #include "cache_q8.cuh"
 #include "decode_parts.cuh"
 #include "sm100_ptx.cuh"
@@ -28,6 +32,8 @@ namespace {
 constexpr int kWarps = 4, kTile = 32, kDepth = 3;   // a step of a warp: 32 keys, two blocks of 16
 constexpr float kSlack = 5.f, kLift = 10.f, kNone = -3e38f;   // (kNone: no score yet; above every finite one that counts as such)
 
+// CTAs per SM: what their registers and rings leave room for.  D = 128: 2 (64 sequences of 4096 to 8192 keys, 8 heads, 143 us); 3 need rings of two steps and spill
+// (164; 2 with such rings 148).  CTAs of three warps take 150 us, of two 158.
 constexpr int q8_ctas_per_sm(int D, int NT) { return D == 128 ? 2 : NT == 1 ? 4 : 3; }
 template <int D>
 struct Q8Slot {   // 16 keys: rows of K, rows of V
@@ -379,8 +385,9 @@ __global__ void __launch_bounds__(kWarps * 32, q8_ctas_per_sm(D, NT)) attn_decod
     }
 }
 
-// Whether every slice is one warp's, without a workspace and a second kernel
-static bool q8_whole(const AttnArgs& a) { return a.L <= 4 * kTile; }
+// Whether every slice is one warp's, without a workspace and a second kernel: as long as one sequence takes no longer that way.  us so and in parts, one sequence and 64
+// of 8 heads of 128, 128 keys 6.0 and 7.0, 7.8 and 10.8; 192 keys 7.4 and 7.4, 9.7 and 11.6; 256 keys 8.8 and 7.4, 11.5 and 13.1.
+static bool q8_whole(const AttnArgs& a) { return a.L <= 6 * kTile; }
 // CTAs: what an SM holds at once, fewer where there are not steps for their warps.
 template <int NT>
 static int q8_ctas(const AttnArgs& a, int head_tiles) {

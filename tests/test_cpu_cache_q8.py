@@ -78,7 +78,7 @@ def test_q8_decode_refuses_what_does_not_fit(tt):
     assert need < 1 << 20
     for kw in (dict(out=big), dict(out=_at(big, need - 256)), dict(lse=_at(big, 256)), dict(q=_at(big, 512)), dict(table=_at(big, 512))):
         assert call(**long, kc=k_far, vc=v_far, ws=big, ws_bytes=need, **kw) == c.TT_ERR_BAD_SHAPE and "workspace" in c.last_error(), kw
-    for L, some in ((1, False), (128, False), (129, True)):
+    for L, some in ((1, False), (192, False), (193, True)):
         assert (lib.tt_attn_decode_q8_workspace_bytes(ctypes.byref(c.make_desc(2, 4, 1, L, 64, c.TT_BF16, False, None, Hkv=2))) > 0) == some
     assert call(**long, ws=None) == c.TT_ERR_WORKSPACE and call(**long, ws_bytes=need - 1) == c.TT_ERR_WORKSPACE and call(**long, ws=_at(ws, 64), ws_bytes=need) == c.TT_ERR_WORKSPACE
     if not torch.cuda.is_available():

@@ -106,6 +106,13 @@ def test_against_64_bits(tt, lens, H, hkv, D, page):
     c.check(out2, lse2, 0.3)
 
 
+@pytest.mark.parametrize("D,H,hkv", [(128, 8, 2), (64, 3, 3), (128, 17, 1)])
+@pytest.mark.parametrize("longest", [191, 192, 193, 224])
+def test_around_the_longest_that_a_warp_has_alone(tt, longest, D, H, hkv):
+    c = Case([longest, 0, longest - 30, 1, 129, 16], H, hkv, D, 16, seed=longest)
+    c.check(*tt.attention_decode_q8(**c.args()))
+
+
 @pytest.mark.parametrize("B,H,hkv,D,page", [(3, 8, 2, 128, 64), (2, 4, 4, 64, 512)])
 def test_without_a_block_table(tt, B, H, hkv, D, page):
     c = Case([page] * B, H, hkv, D, page, table=False)
