@@ -629,8 +629,8 @@ struct HdPlaces {
 // Whether all of a row's lanes have two whole chunks of it.
 static bool hd_whole(int D, int R, int interleaved, int kV, int n_units) { return n_units * 2 * kV == D && R % (2 * kV) == 0 && (interleaved || R / 2 % kV == 0); }
 // Tokens per tile: rows for so many turns of every group of lanes, as the tables of two have room for.  A tile's first rows are loaded behind a barrier: 16384 tokens of 40
-// heads 73.4 / 69.8 / 67.7 / 66.2 us with 4 / 8 / 14 / 28 turns of one unit, the gradient of 8192 121.5 / 79.2 / 72.5 / 68.6; without norm and with half of the channels
-// turned the forward call takes 58.9 / 60.7 with 14 / 28.
+// heads 73.4 / 69.8 / 67.7 / 66.2 us with 4 / 8 / 14 / 28 turns of one unit, the gradient of 8192 121.5 / 79.2 / 72.5 / 68.6; of two units, turns of twice the rows, 14: without
+// norm and with half of the channels turned the forward call takes 58.9 / 60.7 with 14 / 28.
 static int hd_tile(long long n_tok, long long ctas, int turns, int heads, int groups, size_t token) {
     long long per = (long long)turns * groups / heads;
     const long long fits = 12 * 1024 / (long long)token, share = (n_tok + ctas - 1) / ctas;
@@ -644,7 +644,7 @@ static cudaError_t launch_heads_units(const NormRotaryArgs& a, int interleaved, 
     const int turned = (a.r.R / 2 + kV - 1) / kV, heads = a.r.heads[0] + a.r.heads[1] * (kAppend ? 2 : 1), n_units = kUnits << log_lanes;
     const size_t token = (size_t)turned * kV * sizeof(float2) + (kAppend ? 3 * 32 : 2 * 16), weights = kNorm ? (size_t)n_units * kV * 16 : 0;
     const long long n_tok = (long long)a.r.B * a.r.S, resident = (long long)hd_ctas_per_sm(kUnits) * sm_count(), ctas = n_tok < resident ? n_tok : resident;
-    const int per = hd_tile(n_tok, ctas, 14, heads, kHeadThreads >> log_lanes, token);
+    const int per = hd_tile(n_tok, ctas, kUnits == 1 ? 28 : 14, heads, kHeadThreads >> log_lanes, token);
     LaunchScope ls(kAppend ? K_CACHE_APPEND_ROTARY : K_NORM_ROTARY, st);
     auto go = [&](auto kernel) { return launch_overlapped(kernel, (unsigned)ctas, kHeadThreads, weights + 2 * per * token, st, a, per, log_lanes); };
     return interleaved ? go(heads_kernel<Tin, Tout, kV, kUnits, true, kNorm, kAppend, kWhole>) : go(heads_kernel<Tin, Tout, kV, kUnits, false, kNorm, kAppend, kWhole>);
@@ -656,7 +656,7 @@ static cudaError_t launch_heads(const NormRotaryArgs& a, int interleaved, cudaSt
     const int units = hd_units_of_row(a.r.D, a.r.R, kV);
     // Whole rows: two units to a lane, so that what a row costs beside its values is shared by more of them (TB/s with one unit and two, 20 heads: floats of 128, 64
     // channels turned, 5.35 and 5.59; bf16 of 256 and 128 5.04 and 5.29).  But bf16 norms of rows of four units, where a warp then has 16 rows, and of few heads that
-    // turn all channels, where the CTAs make sines for longer, have three CTAs per SM, and one unit (64 and 64 4.55 and 4.01, 64 and 16 4.86 and 4.76, 128 and 128 4.87
+    // turn all channels, where the CTAs make sines for longer, have three CTAs per SM, and one unit (64 and 64 4.55 and 4.01, 64 and 16 4.97 and 4.76, 128 and 128 4.87
     // and 4.50, 256 and 256 4.94 and 4.73; 40 heads of 128 and 128 67.4 us and 65.5).
     if constexpr (kUnits == 1) {
         if constexpr (sizeof(Tin) == 2 && kNorm && !kAppend) {
