@@ -696,10 +696,10 @@ cudaError_t cache_append_rotary(const NormRotaryArgs& a, int bf16, int interleav
     const int n[2] = {a.r.S, a.r.heads[1]};
     for (int i = 0; i < 2; ++i) {
         const int m[3] = {1, a.r.heads[i], a.r.S};
+        out.add(a.pool[i], nullptr, nullptr, 0, 2);   // keys' and values', with and without queries
         if (!a.r.heads[i]) continue;
         in.add(a.r.x[i], a.r.xs[i], m, 3, size);
         if (a.r.y[i]) out.add(a.r.y[i], a.r.ys[i], m, 3, 2);
-        out.add(a.pool[i], nullptr, nullptr, 0, 2);
     }
     in.add(a.v, a.v_stride, n, 2, size);
     const int from = in.aligned(16), to = out.aligned(16) * (size / 2), aligned = from < to ? from : to;
