@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32, q8_ctas_per_sm(D, NT)) attn_decod
                         const float to = fmaxf(top_x[m][j], x);
                         f[j] = ex2_approx(top_x[m][j] - to);
                         top_x[m][j] = to;
-                        above[m][j] = to + kSlack;
+                        above[m][j] = __fadd_rd(to, kSlack);   // (beyond 2^24 the nearest may lie above to + kSlack, and a weight then beyond half)
 #pragma unroll
                         for (int c = 0; c < kMT; ++c) {
                             o[c][m][j] *= f[j];
