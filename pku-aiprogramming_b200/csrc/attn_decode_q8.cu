@@ -236,10 +236,11 @@ __global__ void __launch_bounds__(kWarps * 32, q8_ctas_per_sm(D, NT)) attn_decod
                 const float pk = __uint_as_float((pw[u] & 0xffffu) << 23), ev = (float)((int)(pw[u] >> 16) - 127);
 #pragma unroll
                 for (int m = 0; m < NT; ++m) {
-                    const uint64_t by = pack_f32x2(to_log2[m][0] * pk, to_log2[m][1] * pk), more = pack_f32x2(ev, ev);
+                    // (products of codes with half's values are 2^-33 .. 2^31 or 0, so that times the block's power is exact; the two factors' product may be infinite)
+                    const uint64_t by = pack_f32x2(to_log2[m][0], to_log2[m][1]), block = pack_f32x2(pk, pk), more = pack_f32x2(ev, ev);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        x2[u][m][k] = fma_f32x2(pack_f32x2(s[u][m][2 * k], s[u][m][2 * k + 1]), by, more);
+                        x2[u][m][k] = fma_f32x2(mul_f32x2(pack_f32x2(s[u][m][2 * k], s[u][m][2 * k + 1]), block), by, more);
                         unpack_f32x2(x2[u][m][k], s[u][m][2 * k], s[u][m][2 * k + 1]);
                     }
                 }

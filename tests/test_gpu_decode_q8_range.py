@@ -135,3 +135,31 @@ def test_far_scores_in_many_parts(tt, q, one, other, ahead, G):
     assert torch.isfinite(out).all() and (out.abs() <= 448).all()
     assert (out.double().cpu().numpy().min((0, 1, 2)) >= v[:, 0].min(0) - 2).all() and (out.double().cpu().numpy().max((0, 1, 2)) <= v[:, 0].max(0) + 2).all()
     assert (np.abs(lse.double().cpu().numpy() - top) <= 2.0 ** -20 * abs(top) + 6).all()
+
+
+@pytest.mark.parametrize("power", [60, 100, 104, 110, 120, 127])
+@pytest.mark.parametrize("G,D,n", [(1, 64, 50), (8, 128, 700), (16, 128, 100)])
+def test_a_large_query_beside_blocks_of_large_keys(tt, power, G, D, n):
+    """The head's largest value meets zeros only, and some blocks' scale is 2^40 for other channels' sake: scores are 0, though the query's scale times the
+    block's is beyond 32 bits."""
+    c = Case([n, 30], G, 1, D, 16)
+    codes, powers = c.pools[0].parts()
+    codes[..., 0] = 0
+    powers[::2] = 104
+    c.q = torch.zeros(2, G, 1, D)
+    c.q[..., 0] = 2.0 ** power
+    c.q = c.q.bfloat16()
+    c.check(*tt.attention_decode_q8(**c.args()))
+    # and one key that another channel, 2^25 below, meets: with the smallest code of a block of 2^40
+    if power == 110:
+        at = 20
+        c.q[0, :, 0, 1] = 2.0 ** (power - 25)
+        codes[..., 1] = 0
+        codes[c.table[0, at // 16], 0, at % 16, 1] = 1
+        powers[c.table[0, at // 16]] = 104
+        out, lse = tt.attention_decode_q8(**c.args())
+        k, v, _ = c.rows(0)
+        top = 2.0 ** (power - 25) * k[at, 0, 1] * D ** -0.5
+        assert top == 2.0 ** 116 * D ** -0.5
+        assert np.array_equal(out[0, :, 0].double().cpu().numpy(), np.broadcast_to(v[at, 0], (G, D)))
+        assert (np.abs(lse[0, :, 0].double().cpu().numpy() - top) <= 2.0 ** -21 * top).all()
