@@ -436,7 +436,7 @@ def rotary_forward(q, k, positions, inv_freq, axes=None, interleaved=False, scal
     None, see `rotary_frequencies`): channels i and i + R/2, or with `interleaved` 2i and 2i + 1; the other channels are copied.
     positions: int32 `[axes, T]` / `[axes, B, S]` / `[axes, S]`, or `[T]` / `[S]` with one axis; without `axes` there is one, and more
     rows are refused (position ids `[B, S]` are `[1, B, S]` here).  Strided inputs are fine as long
-    as channels lie next to each other; `out_q`, `out_k` may be the inputs themselves.  `scale` (1) multiplies the result."""
+    as channels lie next to each other; `out_q`, `out_k` may be the inputs themselves.  `scale` (1) multiplies the channels that turn."""
     r = _native.rotary(q, k, positions, inv_freq, axes, interleaved, scale, False, out_q, out_k)
     return r if r.__class__ is tuple else _done(r, _explain_rotary, q, k, positions, inv_freq, axes, out_q, out_k)
 
@@ -520,7 +520,7 @@ def cache_append_rotary(q, k, v, slots, positions, inv_freq, k_pool, v_pool, axe
 
     q `[T, H, D]` (or None), k, v `[T, kv_heads, D]`, float32 or bfloat16, strided; `slots`, `positions` as from `cache_extend`; a slot of -1 is passed
     over, and none may come twice.  With `q_weight` and `k_weight` heads are normed first, as by `norm_rotary_forward`.  `out_k`: a bfloat16 tensor of k's
-    shape that gets the turned keys too, for attention over the new tokens themselves.  `scale` multiplies queries and keys."""
+    shape that gets the turned keys too, for attention over the new tokens themselves.  `scale` multiplies the channels that turn."""
     r = _native.cache_append_rotary(q, k, v, slots, positions, inv_freq, k_pool, v_pool, axes, interleaved, q_weight, k_weight, eps, scale, out_q, out_k)
     return r[0] if r.__class__ is tuple else _done(r, _explain_append_rotary, q, k, v, slots, positions, inv_freq, k_pool, v_pool, axes, q_weight, k_weight, out_q, out_k)
 
