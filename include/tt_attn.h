@@ -279,7 +279,8 @@ int tt_attn_decode_q4(const tt_attn_desc* desc, const void* q, const void* k_cac
  * 2^31 tokens.
  *
  * tt_cache_append_q8: as tt_cache_append_q4, tokens [T, Hkv, D] into their slots.  The tokens of a call that go to one block have to lie next to each
- * other in it, as those of a sequence do (else what the block then holds is of any of them).  The scale of a block is the smallest with 448 scale >= every
+ * other in it, none passed over between them, each in a slot of its own, as those of a sequence do; else the block, its scale too, is unspecified until its row 0 is
+ * written again, and other blocks are not concerned.  The scale of a block is the smallest with 448 scale >= every
  * finite |x| that has come to it since its row 0 was last written: a call that brings row 0 begins the block anew, another may raise the scale, and then the
  * block's other rows are rounded to the new one.  Codes are rounded to the nearest, ties to even, so a value is off by at most 2^-4 of itself, or 2^-10 of the scale
  * (2^-9, where that was raised) if that is more.  Infinities, and values beyond 448 2^40, become the block's largest value of their sign; NaN stays NaN.

@@ -310,7 +310,7 @@ def cache_append_q4(k, v, slots, k_cache, v_cache):
 
 def cache_append_q8(k, v, slots, k_cache, v_cache):
     """New keys and values into an 8-bit cache, as `cache_append_q4`.  The tokens of a call that go to one block of 16 rows of a page lie next to each
-    other, as a sequence's do.  A block's scale is the smallest power of two that holds its tokens' largest value; tokens that come later raise
+    other and each has a slot of its own, as a sequence's do (else that block is unspecified).  A block's scale is the smallest power of two that holds its tokens' largest value; tokens that come later raise
     it where they have to, and a call that brings the block's first row begins it anew."""
     r = _native.cache_append_q8(k, v, slots, k_cache, v_cache)
     return r if r.__class__ is tuple else _done(r, _explain_cache_append, 8, k, v, slots, k_cache, v_cache)
