@@ -261,7 +261,9 @@ int tt_cache_read_q4(const void* k_cache, const void* v_cache, const int32_t* bl
  *                  NULL: batch entry b has page b to itself (page_size >= desc->L, n_pages >= B).
  *   seq_lens       [B] or NULL (desc->L each), clamped to 0 .. desc->L; an entry without keys gets out = 0, lse = -inf
  * desc: dtype TT_BF16, S = 1, D 64 or 128, L the longest sequence there may be, at most 2^30; any group H / Hkv.  `lse` may be NULL.
- * q may be of any finite size, as long as scale * q is finite in 32 bits and scores stay below 2^127.
+ * q may be of any finite size, as long as scale * log2 e and scale * q are finite in 32 bits and scores stay below 2^127; its values are taken to multiples of
+ * at most 2^-34 (8 bits: 2^-38) of their head's largest.  Scores and the log-sum-exps by which parts are merged are 32-bit numbers, so a probability may be off by
+ * 2^-21 of the largest score's magnitude, of itself.
  * out, lse and the workspace must not overlap each other or an input, so `out` cannot be `q`.  A group of more than 16 query heads
  * reads the cache once for each 16 of them.
  * Products are exact in what the cache holds; probabilities are rounded to 11 bits, sums are 32-bit.  Results repeat to the bit.

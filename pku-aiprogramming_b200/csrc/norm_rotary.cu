@@ -7,11 +7,13 @@
 // units of two accesses of kV values, the two halves of kV pairs (or kV pairs of neighbours, or channels that only are normed); 2^n lanes
 // have a row, so the sums are n shuffles, and the rows of a warp lie next to each other.
 //
-// What keeps it from the memory's rate is instructions: sixteen conversions, products and roundings for 32 bytes of bf16, and a token's sines, exact
-// for any position, which are worth five of its rows.  So sines, weights and places lie in shared memory, made a tile of tokens ahead, each CTA that is resident
-// has an equal share of the tokens, and two rows of a lane are on their way at once.  16384 tokens of 32 + 8 heads of 128 in bf16, all channels
-// turned: 63.4 us, 5.3 TB/s (a copy runs at 6.6); the gradient of 8192 of them 56.4 us, 4.5 TB/s; of 4094 tokens of 8 + 8 heads of
-// 64 floats 15.0 us, 3.4 TB/s; 13,000 tokens turned and written into a cache of pages of 16 58.1 us, 5.5 TB/s; 64 single tokens 4 us, a launch.
+// Beside the bytes stand sixteen conversions, products and roundings for 32 bytes of bf16, and a token's sines, exact for any position, which are worth five
+// of its rows; fewer of them were faster, though issue slots are half busy (45 %, the gradient 51 %): what is left waits within a row, on its loads, on shared memory
+// and the lanes' sums, on its own arithmetic (1.6, 3.0 and 1.1 cycles an issue, in the gradient 1.8, 1.3 and 1.4), with the 16 or 24 warps per SM that the registers
+// leave.  So sines, weights and places lie in shared memory, made a tile of tokens ahead, each CTA that is resident has an equal share of the tokens, and two rows
+// of a lane are on their way at once.  Replayed from a graph: 16384 tokens of 32 + 8 heads of 128 in bf16, all
+// channels turned, 62.2 us, 5.4 TB/s (a copy runs at 6.6); the gradient of 8192 of them 56.5 us, 4.5 TB/s; of 4094 tokens of 8 + 8 heads of 64 floats 15.0 us, 3.4 TB/s; 13,000
+// tokens turned and written into a cache of pages of 16 58.2 us, 5.5 TB/s; 64 single tokens 4 us, a launch.
 #include "rotary_parts.cuh"
 #include "sm100_ptx.cuh"
 
@@ -19,9 +21,10 @@ namespace ttk {
 using namespace sm100;
 
 constexpr int kHeadThreads = 256;
-// CTAs per SM, as many as hold two rows of a lane in registers: with one unit a lane 3 (4, which spill, take 77 us for 70), with two 2 (3: 87.7 for 65.4).
+// CTAs per SM, as many as hold two rows of a lane in registers.  16384 tokens of 40 heads of 128, all channels turned: with one unit a lane 3, 63.6 us (4, which
+// spill, 69.4), with two 2, 62.2 us (3, which spill, 82.7).
 constexpr int hd_ctas_per_sm(int units) { return units == 1 ? 3 : 2; }
-constexpr int kBackCtas = 2;   // of the gradient: 79 us, 3 take 110
+constexpr int kBackCtas = 2;   // of the gradient: 8192 of those tokens 56.5 us; 3, which spill, 77.7
 
 // A token's rows of one of the tensors, of head 0: where they come from, where they go, and for keys on their way into a cache a second place.
 template <typename Tin, typename Tout>
@@ -629,8 +632,8 @@ struct HdPlaces {
 // Whether all of a row's lanes have two whole chunks of it.
 static bool hd_whole(int D, int R, int interleaved, int kV, int n_units) { return n_units * 2 * kV == D && R % (2 * kV) == 0 && (interleaved || R / 2 % kV == 0); }
 // Tokens per tile: rows for so many turns of every group of lanes, as the tables of two have room for.  A tile's first rows are loaded behind a barrier: 16384 tokens of 40
-// heads 73.4 / 69.8 / 67.7 / 66.2 us with 4 / 8 / 14 / 28 turns of one unit, the gradient of 8192 121.5 / 79.2 / 72.5 / 68.6; of two units, turns of twice the rows, 14: without
-// norm and with half of the channels turned the forward call takes 58.9 / 60.7 with 14 / 28.
+// heads of 128 71.2 / 67.7 / 65.1 / 63.6 us with 4 / 8 / 14 / 28 turns of one unit, the gradient of 8192 88.0 / 61.1 / 59.3 / 56.5.  Of two units, whose turns have twice
+// the rows, 67.6 / 67.5 / 62.0 / 62.0 with 4 / 7 / 14 / 28, and into a cache, half of the channels turned, 60.4 / 58.8 / 58.2 / 59.6: 14.
 static int hd_tile(long long n_tok, long long ctas, int turns, int heads, int groups, size_t token) {
     long long per = (long long)turns * groups / heads;
     const long long fits = 12 * 1024 / (long long)token, share = (n_tok + ctas - 1) / ctas;
@@ -655,9 +658,10 @@ static cudaError_t launch_heads(const NormRotaryArgs& a, int interleaved, cudaSt
     int log_lanes;
     const int units = hd_units_of_row(a.r.D, a.r.R, kV);
     // Whole rows: two units to a lane, so that what a row costs beside its values is shared by more of them (TB/s with one unit and two, 20 heads: floats of 128, 64
-    // channels turned, 5.35 and 5.59; bf16 of 256 and 128 5.04 and 5.29).  But bf16 norms of rows of four units, where a warp then has 16 rows, and of few heads that
-    // turn all channels, where the CTAs make sines for longer, have three CTAs per SM, and one unit (64 and 64 4.55 and 4.01, 64 and 16 4.97 and 4.76, 128 and 128 4.87
-    // and 4.50, 256 and 256 4.94 and 4.73; 40 heads of 128 and 128 67.4 us and 65.5).
+    // channels turned, 5.58 and 5.66, of 64 and 64, where it is otherwise, 5.45 and 5.32; bf16 of 256 and 128 5.24 and 5.40).  But bf16 norms of rows of four units, where
+    // a warp then has 16 rows, and of few heads that turn all channels, where the CTAs make sines for longer, have three CTAs per SM, and one unit (64 and 64 4.59 and 4.06,
+    // 64 and 16 5.03 and 4.92, 128 and 128 4.91 and 4.59, 256 and 256 5.01 and 4.82).  Around the border of 32 heads, all of 128 channels turned, the two are within 2 %:
+    // with one unit and two 24 heads 67.3 and 70.9 us, 28 66.0 and 65.2, 32 65.0 and 65.2, 36 64.3 and 65.5, 40 63.6 and 62.2, 56 62.8 and 60.5.
     if constexpr (kUnits == 1) {
         if constexpr (sizeof(Tin) == 2 && kNorm && !kAppend) {
             hd_lanes(units, 1, &log_lanes);
@@ -711,7 +715,7 @@ cudaError_t cache_append_rotary(const NormRotaryArgs& a, int bf16, int interleav
 }
 
 // CTAs of the gradient: what the SMs hold at once, shared out by what the rows of the two tensors cost; fewer where there are not tokens for them.  A token's sines, where
-// all channels turn, take as long as five rows: 8192 tokens of 32 and 8 heads 68.2 / 65.4 / 60.6 / 57.6 us if that is taken for 0 / 1 / 3 / 5 rows.
+// all channels turn, take as long as five rows: 8192 tokens of 32 and 8 heads 67.2 / 63.7 / 59.0 / 56.5 / 58.2 us if that is taken for 0 / 1 / 3 / 5 / 7 rows.
 static void hd_ctas(const NormRotaryArgs& a, int (&ctas)[2]) {
     const long long n_tok = (long long)a.r.B * a.r.S, all = (long long)sm_count() * kBackCtas, sines = 5LL * a.r.R;
     const long long cost[2] = {(long long)a.r.heads[0] * a.r.D + sines, a.r.heads[1] ? (long long)a.r.heads[1] * a.r.D + sines : 0};
