@@ -97,7 +97,7 @@ def whole_scores(G, D, n, q, one, other, at):
     return c, float(scale)
 
 
-FAR = [  # a key's score (base 2) is that of those before it and 6 or 8 more: the next in 32 bits but two, or the next
+FAR = [  # q's channels, those of all keys but one, that one's, and how much its score (base 2) is ahead: a few of the scores' last bits, or around 5, which raises the reference
     ((2.0 ** 24, 2.0), (1, 1), (1, 4), 6), ((2.0 ** 26, 8.0), (1, 0), (1, 1), 8), ((-2.0 ** 26, 8.0), (1, -1), (1, 0), 8), ((-2.0 ** 27, 16.0), (1, -1), (1, 0), 16),
     ((2.0 ** 10, 1.0), (1, 0), (1, 5), 5), ((2.0 ** 10, 1.0), (1, 0), (1, 6), 6), ((2.0 ** 20, 1.0), (1, 1), (1, 6), 5), ((2.0 ** 30, 128.0), (1, 0), (1, 1), 128)]
 
